@@ -251,6 +251,127 @@ mkv_status mkv_attn_step(mkv_cache *c, int layer, uint32_t first_pos, uint32_t p
 mkv_status mkv_attn_prefill(mkv_cache *c, int layer, uint32_t first_pos, uint32_t pos0, uint32_t ntok,
                             const void *q_dev, int q_is_f16, float *out_dev);
 
+/* ---- rotary positions: a pair (u, w) of a head's first `dims` dims at position p becomes
+ *   m (u cos a - w sin a), m (u sin a + w cos a),   a = p * f_i for pair i
+ * (M/engine.rs:108-114 and W/ops.wgsl:141-162 have the half layout, 64 of 256 dims, base 1e7, without scaling). The other
+ * dims are left as they are. Angles are taken in 64 bits, so that far positions keep theirs; products and sums are f32 and
+ * an f16 result is rounded once.
+ *  - layout: MKV_ROPE_HALF pairs dims (i, i + dims / 2), MKV_ROPE_INTERLEAVED dims (2 i, 2 i + 1).
+ *  - scaling for contexts longer than the trained one, s = factor >= 1: MKV_SCALE_NONE f_i = base^(-2 i / dims);
+ *    MKV_SCALE_LINEAR f_i / s; MKV_SCALE_NTK base * s^(dims / (dims - 2)) in place of base; MKV_SCALE_YARN ("NTK by parts"):
+ *    with r_i = original * f_i / (2 pi) turns over the original context and g = clamp((r_i - slow) / (fast - slow), 0, 1),
+ *    f_i * (g + (1 - g) / s), and m = 0.1 ln s + 1 (m = 1 otherwise). slow and fast of 0 stand for 1 and 32.
+ * A mkv_rope is host data only: it needs no device, and a captured launch carries a copy of it. */
+typedef struct mkv_rope mkv_rope;
+enum { MKV_ROPE_HALF = 0, MKV_ROPE_INTERLEAVED = 1 };
+enum { MKV_SCALE_NONE = 0, MKV_SCALE_LINEAR = 1, MKV_SCALE_NTK = 2, MKV_SCALE_YARN = 3 };
+enum { MKV_ROPE_MAX_DIMS = 256 };
+typedef struct {
+    int32_t dims;    /* rotated dims of a head: even, 2 .. 256 */
+    int32_t layout;  /* MKV_ROPE_HALF, MKV_ROPE_INTERLEAVED */
+    int32_t scaling; /* MKV_SCALE_* */
+    double base;     /* > 1 */
+    double factor;   /* s >= 1; ignored without scaling */
+    double original; /* MKV_SCALE_YARN: tokens of the original context, > 0 */
+    double slow, fast; /* MKV_SCALE_YARN: 0 <= slow < fast, or both 0 */
+} mkv_rope_desc;
+mkv_status mkv_rope_create(const mkv_rope_desc *desc, mkv_rope **out);
+void mkv_rope_destroy(mkv_rope *r);
+/* f_i (radians per position, [dims / 2]) and m as the library uses them */
+mkv_status mkv_rope_freqs(const mkv_rope *r, double *freqs_host, double *m_host);
+/* y = rotated x for ntok tokens of `heads` heads. backward != 0: the transposed map (angles negated, the same m), which takes
+ * the gradient of y to the gradient of x. x and y may be f16 or f32 each, and may be the same memory with the same strides and
+ * type (any other overlap is refused). Strides in elements; 0 = dense ([ntok][heads][head_dim]). A head's dims are contiguous. */
+typedef struct {
+    const void *x_dev;
+    void *y_dev;
+    mkv_fmt x_fmt, y_fmt;
+    uint32_t ntok, heads, head_dim; /* head_dim: dims .. 1024 */
+    int64_t x_token_stride, x_head_stride, y_token_stride, y_head_stride;
+    const int32_t *pos_dev; /* [ntok] */
+    int32_t backward;
+} mkv_rope_rows;
+mkv_status mkv_rope_apply(mkv_ctx *ctx, const mkv_rope *r, const mkv_rope_rows *rows);
+
+/* ---- paged rows: many sequences in one pool of pages. No counterpart in the reference (one conversation, one contiguous
+ * buffer a layer); the rows, formats and the attention's arithmetic are the cache's above.
+ * A page holds page_tokens positions of K and of V of every layer, [page_tokens][kv_heads][head_dim]; position p of a sequence lies
+ * in row p % page_tokens of its page number p / page_tokens. The library keeps which pages a sequence has; a new page is always the
+ * lowest free one. Pages may be shared by sequences that were forked from one another; a row is only ever written to a
+ * page that one sequence has alone (a shared page is copied first: its rows in front of the written one).
+ * Sequences are named by small numbers, which are used again after mkv_seq_free.
+ * ctx = NULL makes a pool of the bookkeeping alone (no device, no rows): mkv_pool_write and mkv_attn_pool check their arguments
+ * and then return MKV_ERR_UNSUPPORTED; all other calls work.
+ * What a call does to the bookkeeping is done when it returns; what it does to rows is enqueued on the ctx's stream. A captured
+ * launch keeps the pages of its capture: replay it only while its sequences are as they were then, and in the order of the ctx's stream
+ * (the calls of a ctx share the scratch of split work). A call that is refused changes nothing. */
+typedef struct mkv_pool mkv_pool;
+typedef struct {
+    mkv_fmt fmt;
+    int32_t n_layers;     /* 1 .. 256 */
+    uint32_t n_pages;     /* n_pages * page_tokens < 2^31 */
+    uint32_t page_tokens; /* 16, 32, 64, 128 or 256 */
+    uint32_t max_seqs;    /* sequences at one time, 1 .. 65536 */
+    uint32_t max_tokens;  /* longest sequence, 1 .. 2^30 */
+    int32_t q_heads, kv_heads, head_dim; /* q_heads a multiple of kv_heads, at most 64 times it; kv_heads 1 .. 64; head_dim 64, 128 or 256 */
+} mkv_pool_desc;
+/* rows [pos, pos + ntok) of a sequence. Attention: first_pos is the first key its tokens see. Ignored by mkv_pool_write. */
+typedef struct {
+    uint32_t seq, first_pos, pos, ntok;
+} mkv_seq_rows;
+mkv_status mkv_pool_create(mkv_ctx *ctx, const mkv_pool_desc *desc, mkv_pool **out);
+void mkv_pool_destroy(mkv_pool *p);
+/* device pointers of a layer's K and V pages, [n_pages][page_tokens][kv_heads][head_dim] */
+mkv_status mkv_pool_buffers(mkv_pool *p, int layer, void **k_dev, void **v_dev);
+uint32_t mkv_pool_free_pages(const mkv_pool *p);
+/* an empty sequence */
+mkv_status mkv_seq_create(mkv_pool *p, uint32_t *seq_out);
+/* n sequences whose first len rows are those of `seq` (len <= its length): on shared pages, or with copy != 0 on pages of their own.
+ * children_host [n]. MKV_ERR_NOMEM when sequences or pages do not suffice. */
+mkv_status mkv_seq_fork(mkv_pool *p, uint32_t seq, uint32_t len, int copy, int n, uint32_t *children_host);
+/* ends n different sequences; pages that no other sequence has are free again */
+mkv_status mkv_seq_free(mkv_pool *p, const uint32_t *seqs_host, int n);
+/* forgets the rows from len on; pages behind them are given back */
+mkv_status mkv_seq_truncate(mkv_pool *p, uint32_t seq, uint32_t len);
+/* declares rows [.., len) of all layers valid without writing them (after the host filled the pages itself): takes the pages that
+ * are missing; len >= the current length. Pages that are shared stay so. */
+mkv_status mkv_seq_set_len(mkv_pool *p, uint32_t seq, uint32_t len);
+uint32_t mkv_seq_len(const mkv_pool *p, uint32_t seq);
+/* *n_out = number of the sequence's pages; the first min(cap, that) of them in pages_host */
+mkv_status mkv_seq_pages(const mkv_pool *p, uint32_t seq, uint32_t *pages_host, uint32_t cap, uint32_t *n_out);
+/* moves pages so that those in use are the lowest, in their order: the pages from that number on go, in ascending order, to the free
+ * ones below it. *moved_out (may be NULL) = pages that moved. */
+mkv_status mkv_pool_compact(mkv_pool *p, uint32_t *moved_out);
+/* New rows of n sequences (each at most once) in one layer, by mkv_append's rule: pos may not lie beyond the rows the layer has;
+ * afterwards the sequence ends at pos + ntok (rows behind are forgotten) and the layer's rows are valid up to there. Takes missing
+ * pages and copies shared ones (all layers) as needed: MKV_ERR_NOMEM, with nothing changed, when they do not suffice.
+ * k, v: f32 or f16 [ntok of all items, in their order][kv_heads][head_dim], token strides in elements (0 = dense).
+ * rope: rotates K at the rows' positions (dims <= head_dim); NULL when K is already rotated. */
+typedef struct {
+    const void *k_dev;
+    const void *v_dev;
+    mkv_fmt fmt;
+    int64_t k_stride, v_stride;
+    const mkv_rope *rope;
+} mkv_pool_rows;
+mkv_status mkv_pool_write(mkv_pool *p, int layer, const mkv_seq_rows *items, int n, const mkv_pool_rows *in);
+/* Attention of n blocks of new tokens over their sequences, each block of any length (one launch for decode steps, drafts and prefill
+ * blocks together): token t of an item sees first_pos <= key <= pos + t, and with a window key > pos + t - window. The rows must be
+ * there (pos + ntok <= the layer's valid rows). A row that sees no key gets zeros.
+ * q, out: the pool's type, [tokens of all items, in their order][q_heads][head_dim], token strides in elements (0 = dense; multiples of
+ * 16 bytes), 16-byte aligned. scale 0 = 1 / sqrt(head_dim). sinks_dev: [q_heads] logits that join the softmax's maximum and sum and
+ * never the output, or NULL. f16 pools: weights are rounded to f16 for the tensor cores (2^-11 of each), everything else is
+ * summed in f32; f32 pools: f32-grade throughout. */
+typedef struct {
+    const void *q_dev;
+    void *out_dev;
+    int64_t q_stride, out_stride;
+    float scale;
+    uint32_t window;
+    const float *sinks_dev;
+} mkv_pool_attn;
+mkv_status mkv_attn_pool(mkv_pool *p, int layer, const mkv_seq_rows *items, int n, const mkv_pool_attn *in);
+
 /* ---- snapshot / restore of the prefix cache ("root"): replaces the KV part of Engine::read_root /
  * write_root (M/engine.rs:782-823). Payload = for each layer in order, K rows [0,p) then V rows [0,p), raw
  * cache bytes (f16 bit patterns or f32), i.e. Root.kv flattened. A shard copies only the rows it holds; its

@@ -39,6 +39,37 @@ class VerifyItem(C.Structure):
                 ("ntok", C.c_uint32), ("q_dev", C.c_void_p), ("out_dev", C.c_void_p)]
 
 
+class RopeDesc(C.Structure):
+    """mkv_rope_desc of include/mechta_kv.h."""
+    _fields_ = [("dims", C.c_int32), ("layout", C.c_int32), ("scaling", C.c_int32), ("base", C.c_double), ("factor", C.c_double),
+                ("original", C.c_double), ("slow", C.c_double), ("fast", C.c_double)]
+
+
+class RopeRows(C.Structure):
+    """mkv_rope_rows of include/mechta_kv.h."""
+    _fields_ = [("x_dev", C.c_void_p), ("y_dev", C.c_void_p), ("x_fmt", C.c_int), ("y_fmt", C.c_int), ("ntok", C.c_uint32),
+                ("heads", C.c_uint32), ("head_dim", C.c_uint32), ("x_token_stride", C.c_int64), ("x_head_stride", C.c_int64),
+                ("y_token_stride", C.c_int64), ("y_head_stride", C.c_int64), ("pos_dev", C.c_void_p), ("backward", C.c_int32)]
+
+
+class PoolDesc(C.Structure):
+    """mkv_pool_desc of include/mechta_kv.h."""
+    _fields_ = [("fmt", C.c_int), ("n_layers", C.c_int32), ("n_pages", C.c_uint32), ("page_tokens", C.c_uint32), ("max_seqs", C.c_uint32),
+                ("max_tokens", C.c_uint32), ("q_heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32)]
+
+
+class PoolRows(C.Structure):
+    """mkv_pool_rows of include/mechta_kv.h."""
+    _fields_ = [("k_dev", C.c_void_p), ("v_dev", C.c_void_p), ("fmt", C.c_int), ("k_stride", C.c_int64), ("v_stride", C.c_int64),
+                ("rope", C.c_void_p)]
+
+
+class PoolAttn(C.Structure):
+    """mkv_pool_attn of include/mechta_kv.h."""
+    _fields_ = [("q_dev", C.c_void_p), ("out_dev", C.c_void_p), ("q_stride", C.c_int64), ("out_stride", C.c_int64), ("scale", C.c_float),
+                ("window", C.c_uint32), ("sinks_dev", C.c_void_p)]
+
+
 def build(force: bool = False) -> str:
     """Compile the library for sm_100a with nvcc (no GPU needed to build)."""
     csrc = os.path.join(_HERE, "csrc")
@@ -99,6 +130,24 @@ _SIGS = {
     "mkv_attn_verify_window": (C.c_int, [C.c_void_p, C.c_int, C.c_uint32, C.c_void_p, C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p]),
     "mkv_attn_step": (C.c_int, [C.c_void_p, C.c_int, C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(StepIn), C.c_void_p, C.c_void_p]),
     "mkv_attn_prefill": (C.c_int, [C.c_void_p, C.c_int, C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p, C.c_int, C.c_void_p]),
+    "mkv_rope_create": (C.c_int, [C.POINTER(RopeDesc), C.POINTER(C.c_void_p)]),
+    "mkv_rope_destroy": (None, [C.c_void_p]),
+    "mkv_rope_freqs": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(C.c_double)]),
+    "mkv_rope_apply": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(RopeRows)]),
+    "mkv_pool_create": (C.c_int, [C.c_void_p, C.POINTER(PoolDesc), C.POINTER(C.c_void_p)]),
+    "mkv_pool_destroy": (None, [C.c_void_p]),
+    "mkv_pool_buffers": (C.c_int, [C.c_void_p, C.c_int, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p)]),
+    "mkv_pool_free_pages": (C.c_uint32, [C.c_void_p]),
+    "mkv_seq_create": (C.c_int, [C.c_void_p, C.POINTER(C.c_uint32)]),
+    "mkv_seq_fork": (C.c_int, [C.c_void_p, C.c_uint32, C.c_uint32, C.c_int, C.c_int, C.c_void_p]),
+    "mkv_seq_free": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int]),
+    "mkv_seq_truncate": (C.c_int, [C.c_void_p, C.c_uint32, C.c_uint32]),
+    "mkv_seq_set_len": (C.c_int, [C.c_void_p, C.c_uint32, C.c_uint32]),
+    "mkv_seq_len": (C.c_uint32, [C.c_void_p, C.c_uint32]),
+    "mkv_seq_pages": (C.c_int, [C.c_void_p, C.c_uint32, C.c_void_p, C.c_uint32, C.POINTER(C.c_uint32)]),
+    "mkv_pool_compact": (C.c_int, [C.c_void_p, C.POINTER(C.c_uint32)]),
+    "mkv_pool_write": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.POINTER(PoolRows)]),
+    "mkv_attn_pool": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.POINTER(PoolAttn)]),
     "mkv_snapshot_bytes": (C.c_size_t, [C.c_void_p, C.c_uint32]),
     "mkv_snapshot": (C.c_int, [C.c_void_p, C.c_uint32, C.c_void_p, C.c_size_t, C.POINTER(C.c_size_t)]),
     "mkv_snapshot_wait": (C.c_int, [C.c_void_p]),

@@ -49,17 +49,17 @@ static EncodeTiledFn encode_tiled() {
     return fn;
 }
 
-// Tensor map of one K or V buffer seen as [rows][512] elements; boxes of 128 bytes x `box_rows` rows with the
+// Tensor map of one K or V buffer seen as [rows][cols] elements; boxes of 128 bytes x `box_rows` rows with the
 // 128-byte swizzle. Rows past the end read as zero.
-static mkv_status make_tensor_map(CUtensorMap *out, mkv_fmt fmt, void *base, uint32_t rows, uint32_t box_rows) {
+mkv_status make_tensor_map(CUtensorMap *out, mkv_fmt fmt, void *base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
     EncodeTiledFn enc = encode_tiled();
     if (!enc) {
         set_error("cuTensorMapEncodeTiled is not available from the driver");
         return MKV_ERR_CUDA;
     }
     const size_t elem = fmt == MKV_F16 ? 2 : 4;
-    cuuint64_t dims[2] = {512, rows};
-    cuuint64_t strides[1] = {512 * elem};
+    cuuint64_t dims[2] = {cols, rows};
+    cuuint64_t strides[1] = {cols * elem};
     cuuint32_t box[2] = {(cuuint32_t)(128 / elem), box_rows};
     cuuint32_t estr[2] = {1, 1};
     CUresult r = enc(out, fmt == MKV_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, base, dims,
@@ -105,6 +105,18 @@ uint32_t Cache::safe_below(uint32_t pos) const {
 static mkv_status use_device(Ctx *ctx) {
     MKV_CUDA(cudaSetDevice(ctx->device));
     return MKV_OK;
+}
+
+DeviceScope::DeviceScope(Ctx *ctx) {
+    if (cudaGetDevice(&before) != cudaSuccess) before = -1;
+    if (before == ctx->device) {
+        before = -1;
+        return;
+    }
+    status = use_device(ctx);
+}
+DeviceScope::~DeviceScope() {
+    if (before >= 0) cudaSetDevice(before);
 }
 
 // Reads and clears the device status word (blocks); nonzero means a kernel gave up on a wait.
@@ -416,6 +428,12 @@ static void ctx_free(Ctx *ctx) {
     delete ctx;
 }
 
+} // extern "C"
+void mkv::ctx_release(Ctx *ctx) {
+    if (--ctx->live_caches == 0 && ctx->closing) ctx_free(ctx);
+}
+extern "C" {
+
 void mkv_ctx_destroy(mkv_ctx *h) {
     Ctx *ctx = reinterpret_cast<Ctx *>(h);
     if (!ctx || ctx->closing) return;
@@ -559,10 +577,10 @@ static mkv_status cache_create_common(mkv_ctx *h, mkv_fmt fmt, int n_layers, uin
     maps.resize(4 * (size_t)n_layers);
     const uint32_t box_rows = fmt == MKV_F16 ? TILE : TILE32;
     for (int l = 0; l < n_layers; l++) {
-        if ((st = make_tensor_map(&maps[2 * l], fmt, c->k[l], capacity, box_rows)) != MKV_OK) return fail(st);
-        if ((st = make_tensor_map(&maps[2 * l + 1], fmt, c->v[l], capacity, box_rows)) != MKV_OK) return fail(st);
-        if ((st = make_tensor_map(&maps[2 * (n_layers + l)], fmt, c->k[l], capacity, PF_TILE)) != MKV_OK) return fail(st);
-        if ((st = make_tensor_map(&maps[2 * (n_layers + l) + 1], fmt, c->v[l], capacity, PF_TILE)) != MKV_OK) return fail(st);
+        if ((st = make_tensor_map(&maps[2 * l], fmt, c->k[l], capacity, ROW, box_rows)) != MKV_OK) return fail(st);
+        if ((st = make_tensor_map(&maps[2 * l + 1], fmt, c->v[l], capacity, ROW, box_rows)) != MKV_OK) return fail(st);
+        if ((st = make_tensor_map(&maps[2 * (n_layers + l)], fmt, c->k[l], capacity, ROW, PF_TILE)) != MKV_OK) return fail(st);
+        if ((st = make_tensor_map(&maps[2 * (n_layers + l) + 1], fmt, c->v[l], capacity, ROW, PF_TILE)) != MKV_OK) return fail(st);
     }
     if (cudaMalloc(&c->maps_dev, maps.size() * sizeof(CUtensorMap)) != cudaSuccess ||
         cudaMalloc(&c->kptrs_dev, n_layers * sizeof(void *)) != cudaSuccess ||
@@ -668,7 +686,7 @@ void mkv_cache_destroy(mkv_cache *h) {
     if (c->ev_snapshot) cudaEventDestroy(c->ev_snapshot);
     Ctx *ctx = c->ctx;
     delete c;
-    if (--ctx->live_caches == 0 && ctx->closing) ctx_free(ctx);
+    ctx_release(ctx);
 }
 
 mkv_status mkv_cache_buffers(mkv_cache *h, int layer, void **k_dev, void **v_dev) {

@@ -143,7 +143,7 @@ struct Ctx {
     int slot_next = 0;
     uint32_t *counters_dev = nullptr;          // [SLOT_ITEMS] arrival counters, zeroed once
     std::vector<uint32_t> counter_base;        // host shadow: value of each counter after the launches so far
-    // lifetime: caches hold a reference; a ctx destroyed while caches live is freed with the last of them
+    // lifetime: caches and pools hold a reference; a ctx destroyed while some live is freed with the last of them
     int live_caches = 0;
     bool closing = false;
 };
@@ -224,6 +224,17 @@ bool verify32_use_tc();
 // plan, and with it the order of its sums, then depends on the call alone, also when the context's first prefill is being captured.
 // Where the memory is not there the context does without for this cache (whole items) and the next cache tries again.
 void prefill_reserve(Ctx *ctx);
+// Makes the ctx's device the current one until the scope's end.
+struct DeviceScope {
+    mkv_status status = MKV_OK;
+    int before = -1; // to go back to, -1: nothing to do
+    explicit DeviceScope(Ctx *ctx);
+    ~DeviceScope();
+};
+// One holder of the ctx (a cache, a pool) less; frees a ctx that was destroyed before its last holder.
+void ctx_release(Ctx *ctx);
+// Tensor map of a [rows][cols] buffer, boxes of 128 bytes x box_rows rows with the 128-byte swizzle.
+mkv_status make_tensor_map(CUtensorMap *out, mkv_fmt fmt, void *base, uint64_t rows, uint64_t cols, uint32_t box_rows);
 // plans the split of the items so that the grid fills the SMs once
 void plan_items(Ctx *ctx, mkv_fmt fmt, VerifyItem *items, int n);
 

@@ -268,6 +268,197 @@ class KvCache:
             pass
 
 
+def _need(ok, text: str) -> None:
+    if not ok:
+        raise MkvError(_lib.ERR_INVALID, text)
+
+
+def _fmt_of(t: torch.Tensor) -> int:
+    _need(t.dtype in (torch.float16, torch.float32), f"{t.dtype}: must be float16 or float32")
+    return _lib.F16 if t.dtype == torch.float16 else _lib.F32
+
+
+def _strides(t: torch.Tensor, what: str) -> tuple[int, int]:
+    """Token and head stride of a [tokens][heads][dims] tensor whose heads are contiguous."""
+    _need(t.dim() == 3 and (t.stride(2) == 1 or t.shape[2] <= 1 or t.numel() == 0), f"{what} must be [tokens][heads][dims] with contiguous dims")
+    return t.stride(0), t.stride(1)
+
+
+class Rope:
+    """Rotary positions (mkv_rope): which dims turn, how they pair, how the frequencies are scaled for long contexts. The defaults
+    are the reference's (engine.rs:108-114); without `ctx` only `freqs` can be asked for."""
+
+    LAYOUTS = {"half": 0, "interleaved": 1}
+    SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+
+    def __init__(self, ctx: KvContext | None, dims: int = 64, base: float = 1e7, layout: str = "half", scaling: str = "none",
+                 factor: float = 1.0, original: float = 0.0, slow: float = 0.0, fast: float = 0.0):
+        self._h = C.c_void_p()
+        _need(layout in self.LAYOUTS, f"layout {layout!r}: one of {sorted(self.LAYOUTS)}")
+        _need(scaling in self.SCALINGS, f"scaling {scaling!r}: one of {sorted(self.SCALINGS)}")
+        self.ctx, self.dims = ctx, int(dims)
+        d = _lib.RopeDesc(self.dims, self.LAYOUTS[layout], self.SCALINGS[scaling], base, factor, original, slow, fast)
+        check(_lib.lib().mkv_rope_create(C.byref(d), C.byref(self._h)))
+
+    def freqs(self) -> tuple[np.ndarray, float]:
+        """Radians per position of each pair, and the factor on cosine and sine."""
+        f, m = np.empty(self.dims // 2), C.c_double()
+        check(_lib.lib().mkv_rope_freqs(self._h, f.ctypes.data_as(C.c_void_p), C.byref(m)))
+        return f, m.value
+
+    def apply(self, x: torch.Tensor, positions: torch.Tensor, out: torch.Tensor, backward: bool = False) -> None:
+        """out = x rotated at `positions` (int32 [tokens]); x, out [tokens][heads][dims], f16 or f32 each, any token and head
+        strides, the same memory allowed. backward: the transposed map, for gradients."""
+        _need(self.ctx is not None, "a Rope without a context does not run")
+        xs, ys = _strides(x, "x"), _strides(out, "out")
+        _need(x.shape == out.shape, f"x is {tuple(x.shape)}, out {tuple(out.shape)}")
+        _need(positions.dtype == torch.int32 and positions.shape == x.shape[:1] and positions.is_contiguous(), "positions must be contiguous int32 [tokens]")
+        n, heads, dim = x.shape
+        _need(all(s > 0 for s, k in zip(xs, (n, heads)) if k > 1), "x may not be broadcast over tokens or heads")
+        _need(all(s > 0 for s, k in zip(ys, (n, heads)) if k > 1), "out may not be broadcast")
+        for t in (x, out, positions):
+            _need(t.device.type == "cuda" and t.device.index == self.ctx.device, f"tensors must be on cuda:{self.ctx.device}")
+        r = _lib.RopeRows(x.data_ptr(), out.data_ptr(), _fmt_of(x), _fmt_of(out), n, heads, dim, xs[0] if n > 1 else 0, xs[1] if heads > 1 else 0,
+                          ys[0] if n > 1 else 0, ys[1] if heads > 1 else 0, positions.data_ptr(), int(backward))
+        check(_lib.lib().mkv_rope_apply(self.ctx._h, self._h, C.byref(r)))
+
+    def close(self) -> None:
+        if self._h:
+            _lib.lib().mkv_rope_destroy(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class KvPool:
+    """Pages for the K and V rows of many sequences (mkv_pool). `items` of write() and attn() are rows of (sequence, first_pos, pos,
+    ntok): a [n][4] uint32 array, or a list of such tuples. Without a context the bookkeeping alone works."""
+
+    def __init__(self, ctx: KvContext | None, fmt: KvFormat, n_layers: int, n_pages: int, page_tokens: int, max_seqs: int, max_tokens: int,
+                 q_heads: int = HQ, kv_heads: int = HKV, head_dim: int = D):
+        self._h = C.c_void_p()
+        self.ctx, self.fmt, self.n_layers, self.n_pages, self.page_tokens = ctx, KvFormat(fmt), n_layers, n_pages, page_tokens
+        self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim
+        for v in (n_pages, page_tokens, max_seqs, max_tokens):
+            _need(0 <= v < 2**32, f"{v} is no size")
+        d = _lib.PoolDesc(int(fmt), n_layers, n_pages, page_tokens, max_seqs, max_tokens, q_heads, kv_heads, head_dim)
+        check(_lib.lib().mkv_pool_create(ctx._h if ctx is not None else None, C.byref(d), C.byref(self._h)))
+
+    # -- bookkeeping
+    @property
+    def free_pages(self) -> int:
+        return int(_lib.lib().mkv_pool_free_pages(self._h))
+
+    def create(self) -> int:
+        """An empty sequence."""
+        s = C.c_uint32()
+        check(_lib.lib().mkv_seq_create(self._h, C.byref(s)))
+        return s.value
+
+    def fork(self, seq: int, length: int | None = None, n: int = 1, copy: bool = False) -> list[int]:
+        """n sequences that begin with the first `length` rows of `seq` (all of them by default), on the same pages or on copies."""
+        _need(0 < n < 2**31, f"fork of {n} sequences")
+        kids = (C.c_uint32 * n)()
+        check(_lib.lib().mkv_seq_fork(self._h, seq, self.length(seq) if length is None else length, int(copy), n, kids))
+        return list(kids)
+
+    def free(self, seqs) -> None:
+        a = np.ascontiguousarray(seqs, np.uint32).reshape(-1)
+        check(_lib.lib().mkv_seq_free(self._h, a.ctypes.data, a.size))
+
+    def truncate(self, seq: int, length: int) -> None:
+        check(_lib.lib().mkv_seq_truncate(self._h, seq, length))
+
+    def set_len(self, seq: int, length: int) -> None:
+        """Declares rows valid that the host fills itself (buffer_tensors), in all layers."""
+        check(_lib.lib().mkv_seq_set_len(self._h, seq, length))
+
+    def length(self, seq: int) -> int:
+        return int(_lib.lib().mkv_seq_len(self._h, seq))
+
+    def pages(self, seq: int) -> np.ndarray:
+        n = C.c_uint32()
+        check(_lib.lib().mkv_seq_pages(self._h, seq, None, 0, C.byref(n)))
+        a = np.empty(n.value, np.uint32)
+        check(_lib.lib().mkv_seq_pages(self._h, seq, a.ctypes.data, a.size, C.byref(n)))
+        return a
+
+    def compact(self) -> int:
+        """Moves the pages in use together; returns how many moved."""
+        n = C.c_uint32()
+        check(_lib.lib().mkv_pool_compact(self._h, C.byref(n)))
+        return n.value
+
+    # -- rows
+    def buffers(self, layer: int) -> tuple[int, int]:
+        k, v = C.c_void_p(), C.c_void_p()
+        check(_lib.lib().mkv_pool_buffers(self._h, layer, C.byref(k), C.byref(v)))
+        return k.value, v.value
+
+    def buffer_tensors(self, layer: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """Zero-copy torch views [n_pages][page_tokens][kv_heads][head_dim] of a layer's K and V pages; a view keeps the pool alive."""
+        shape = (self.n_pages, self.page_tokens, self.kv_heads, self.head_dim)
+        return tuple(_as_tensor(p, self.n_pages * self.page_tokens * self.kv_heads * self.head_dim, self.fmt.torch_dtype, self.ctx.device, self).view(shape)
+                     for p in self.buffers(layer))
+
+    def _rows(self, t: torch.Tensor, heads: int, rows: int, what: str) -> int:
+        """Checks [rows][heads][head_dim] with dense heads; the token stride."""
+        ts, hs = _strides(t, what)
+        _need(tuple(t.shape) == (rows, heads, self.head_dim), f"{what} is {tuple(t.shape)}, the items want {(rows, heads, self.head_dim)}")
+        _need(heads == 1 or hs == self.head_dim or rows == 0, f"{what}: a token's heads must be contiguous")
+        _need(rows <= 1 or ts > 0, f"{what} may not be broadcast")
+        if self.ctx is not None:
+            _need(t.device.type == "cuda" and t.device.index == self.ctx.device, f"{what} must be on cuda:{self.ctx.device}")
+        return ts if rows > 1 else 0
+
+    @staticmethod
+    def _items(items) -> np.ndarray:
+        a = np.ascontiguousarray(items, np.uint32)
+        a = a.reshape(0, 4) if a.size == 0 else a
+        _need(a.ndim == 2 and a.shape[1] == 4, "items are rows of (sequence, first_pos, pos, ntok)")
+        return a
+
+    def write(self, layer: int, items, k: torch.Tensor, v: torch.Tensor, rope: Rope | None = None) -> None:
+        """New rows of the items' sequences in one layer; k, v f32 or f16 [tokens of all items][kv_heads][head_dim]. rope rotates k at
+        the rows' positions."""
+        a = self._items(items)
+        rows = int(a[:, 3].sum(dtype=np.int64))
+        _need(k.dtype == v.dtype, "k and v must have one type")
+        r = _lib.PoolRows(k.data_ptr(), v.data_ptr(), _fmt_of(k), self._rows(k, self.kv_heads, rows, "k"), self._rows(v, self.kv_heads, rows, "v"),
+                          rope._h if rope is not None else None)
+        check(_lib.lib().mkv_pool_write(self._h, layer, a.ctypes.data, len(a), C.byref(r)))
+
+    def attn(self, layer: int, items, q: torch.Tensor, out: torch.Tensor, window: int = 0, sinks: torch.Tensor | None = None,
+             scale: float = 0.0) -> None:
+        """Attention of the items' tokens over their sequences; q, out in the pool's type, [tokens of all items][q_heads][head_dim].
+        scale 0 = 1 / sqrt(head_dim); sinks f32 [q_heads]."""
+        a = self._items(items)
+        rows = int(a[:, 3].sum(dtype=np.int64))
+        _need(q.dtype == out.dtype == self.fmt.torch_dtype, f"q and out must be {self.fmt.torch_dtype}")
+        _need(0 <= window < 2**32, f"window {window}")
+        if sinks is not None:
+            _need(sinks.dtype == torch.float32 and sinks.is_contiguous() and tuple(sinks.shape) == (self.q_heads,), "sinks must be f32 [q_heads]")
+            _need(self.ctx is None or sinks.device == q.device, "sinks must be where q is")
+        r = _lib.PoolAttn(q.data_ptr(), out.data_ptr(), self._rows(q, self.q_heads, rows, "q"), self._rows(out, self.q_heads, rows, "out"), scale,
+                          window, sinks.data_ptr() if sinks is not None else None)
+        check(_lib.lib().mkv_attn_pool(self._h, layer, a.ctypes.data, len(a), C.byref(r)))
+
+    def close(self) -> None:
+        if self._h:
+            _lib.lib().mkv_pool_destroy(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
 class KvExchange:
     """Mailboxes for the peer exchange of shard records (mkv_exchange): every rank's attention kernel stores its
     record into every rank's mailbox over NVLink, no collective call. `gather_handles(my_handle) -> [bytes] * world`
@@ -320,14 +511,15 @@ def read_root_file(path: str, fmt: KvFormat, n_layers: int, pin: bool = True) ->
     return toks, Root(p.value, KvFormat(fmt), n_layers, payload)
 
 
-def _as_tensor(ptr: int, numel: int, dtype, device: int) -> torch.Tensor:
-    """A torch view over device memory owned by the library (no copy)."""
+def _as_tensor(ptr: int, numel: int, dtype, device: int, owner=None) -> torch.Tensor:
+    """A torch view over device memory owned by the library (no copy); the view keeps `owner` alive."""
     itemsize = torch.empty((), dtype=dtype).element_size()
 
     class _Mem:
         pass
 
     m = _Mem()
+    m.owner = owner
     typestr = {torch.float16: "<f2", torch.float32: "<f4", torch.uint8: "|u1"}[dtype]
     m.__cuda_array_interface__ = {"shape": (numel,), "typestr": typestr, "data": (ptr, False), "version": 3,
                                   "strides": (itemsize,)}

@@ -1,6 +1,6 @@
 #!/usr/bin/env python
 """Writes src/lib.rs of the mechta-kv-sys crate from include/mechta_kv.h: one `extern "C"` declaration per entry
-point of the C ABI, the two `#[repr(C)]` structs, the status and format constants.
+point of the C ABI, the `#[repr(C)]` structs, the status and format constants.
 
     python rust/mechta-kv-sys/gen_bindings.py          # rewrites rust/mechta-kv-sys/src/lib.rs
     python rust/mechta-kv-sys/gen_bindings.py --check  # exits 1 if the file on disk differs from what would be written
@@ -19,10 +19,11 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 HEADER = os.path.join(HERE, "..", "..", "include", "mechta_kv.h")
 OUT = os.path.join(HERE, "src", "lib.rs")
 
-SCALARS = {"int": "c_int", "uint32_t": "u32", "int32_t": "i32", "uint64_t": "u64", "size_t": "usize", "float": "f32",
+SCALARS = {"int": "c_int", "uint32_t": "u32", "int32_t": "i32", "uint64_t": "u64", "int64_t": "i64", "size_t": "usize", "float": "f32",
            "double": "f64", "char": "c_char", "void": "c_void", "mkv_status": "mkv_status", "mkv_fmt": "mkv_fmt"}
-OPAQUE = ["mkv_ctx", "mkv_cache", "mkv_exchange"]
-STRUCTS = ["mkv_verify_item", "mkv_step_in"]
+OPAQUE = ["mkv_ctx", "mkv_cache", "mkv_exchange", "mkv_rope", "mkv_pool"]
+STRUCTS = ["mkv_verify_item", "mkv_step_in", "mkv_rope_desc", "mkv_rope_rows", "mkv_pool_desc", "mkv_seq_rows", "mkv_pool_rows",
+           "mkv_pool_attn"]
 
 
 def strip_comments(text: str) -> str:

@@ -30,6 +30,13 @@ pub const MKV_MAX_VERIFY: c_int = 4;
 pub const MKV_REC: c_int = 258;
 pub const MKV_CTX_MIN: c_int = 4096;
 pub const MKV_CTX_MAX: c_int = 262144;
+pub const MKV_ROPE_HALF: c_int = 0;
+pub const MKV_ROPE_INTERLEAVED: c_int = 1;
+pub const MKV_SCALE_NONE: c_int = 0;
+pub const MKV_SCALE_LINEAR: c_int = 1;
+pub const MKV_SCALE_NTK: c_int = 2;
+pub const MKV_SCALE_YARN: c_int = 3;
+pub const MKV_ROPE_MAX_DIMS: c_int = 256;
 
 #[repr(C)]
 pub struct mkv_ctx {
@@ -41,6 +48,14 @@ pub struct mkv_cache {
 }
 #[repr(C)]
 pub struct mkv_exchange {
+    _private: [u8; 0],
+}
+#[repr(C)]
+pub struct mkv_rope {
+    _private: [u8; 0],
+}
+#[repr(C)]
+pub struct mkv_pool {
     _private: [u8; 0],
 }
 
@@ -66,6 +81,83 @@ pub struct mkv_step_in {
     pub k_norm_dev: *const f32,
     pub rope_tab_dev: *const f32,
     pub eps: f32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct mkv_rope_desc {
+    pub dims: i32,
+    pub layout: i32,
+    pub scaling: i32,
+    pub base: f64,
+    pub factor: f64,
+    pub original: f64,
+    pub slow: f64,
+    pub fast: f64,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct mkv_rope_rows {
+    pub x_dev: *const c_void,
+    pub y_dev: *mut c_void,
+    pub x_fmt: mkv_fmt,
+    pub y_fmt: mkv_fmt,
+    pub ntok: u32,
+    pub heads: u32,
+    pub head_dim: u32,
+    pub x_token_stride: i64,
+    pub x_head_stride: i64,
+    pub y_token_stride: i64,
+    pub y_head_stride: i64,
+    pub pos_dev: *const i32,
+    pub backward: i32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct mkv_pool_desc {
+    pub fmt: mkv_fmt,
+    pub n_layers: i32,
+    pub n_pages: u32,
+    pub page_tokens: u32,
+    pub max_seqs: u32,
+    pub max_tokens: u32,
+    pub q_heads: i32,
+    pub kv_heads: i32,
+    pub head_dim: i32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct mkv_seq_rows {
+    pub seq: u32,
+    pub first_pos: u32,
+    pub pos: u32,
+    pub ntok: u32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct mkv_pool_rows {
+    pub k_dev: *const c_void,
+    pub v_dev: *const c_void,
+    pub fmt: mkv_fmt,
+    pub k_stride: i64,
+    pub v_stride: i64,
+    pub rope: *const mkv_rope,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct mkv_pool_attn {
+    pub q_dev: *const c_void,
+    pub out_dev: *mut c_void,
+    pub q_stride: i64,
+    pub out_stride: i64,
+    pub scale: f32,
+    pub window: u32,
+    pub sinks_dev: *const f32,
 }
 
 extern "C" {
@@ -104,6 +196,24 @@ extern "C" {
     pub fn mkv_attn_verify_window(c: *mut mkv_cache, layer: c_int, window: u32, sinks_dev: *const f32, pos: u32, ntok: u32, q_dev: *const f32, out_dev: *mut f32) -> mkv_status;
     pub fn mkv_attn_step(c: *mut mkv_cache, layer: c_int, first_pos: u32, pos: u32, ntok: u32, r#in: *const mkv_step_in, ag_dev: *mut f32, ag16_dev: *mut c_void) -> mkv_status;
     pub fn mkv_attn_prefill(c: *mut mkv_cache, layer: c_int, first_pos: u32, pos0: u32, ntok: u32, q_dev: *const c_void, q_is_f16: c_int, out_dev: *mut f32) -> mkv_status;
+    pub fn mkv_rope_create(desc: *const mkv_rope_desc, out: *mut *mut mkv_rope) -> mkv_status;
+    pub fn mkv_rope_destroy(r: *mut mkv_rope);
+    pub fn mkv_rope_freqs(r: *const mkv_rope, freqs_host: *mut f64, m_host: *mut f64) -> mkv_status;
+    pub fn mkv_rope_apply(ctx: *mut mkv_ctx, r: *const mkv_rope, rows: *const mkv_rope_rows) -> mkv_status;
+    pub fn mkv_pool_create(ctx: *mut mkv_ctx, desc: *const mkv_pool_desc, out: *mut *mut mkv_pool) -> mkv_status;
+    pub fn mkv_pool_destroy(p: *mut mkv_pool);
+    pub fn mkv_pool_buffers(p: *mut mkv_pool, layer: c_int, k_dev: *mut *mut c_void, v_dev: *mut *mut c_void) -> mkv_status;
+    pub fn mkv_pool_free_pages(p: *const mkv_pool) -> u32;
+    pub fn mkv_seq_create(p: *mut mkv_pool, seq_out: *mut u32) -> mkv_status;
+    pub fn mkv_seq_fork(p: *mut mkv_pool, seq: u32, len: u32, copy: c_int, n: c_int, children_host: *mut u32) -> mkv_status;
+    pub fn mkv_seq_free(p: *mut mkv_pool, seqs_host: *const u32, n: c_int) -> mkv_status;
+    pub fn mkv_seq_truncate(p: *mut mkv_pool, seq: u32, len: u32) -> mkv_status;
+    pub fn mkv_seq_set_len(p: *mut mkv_pool, seq: u32, len: u32) -> mkv_status;
+    pub fn mkv_seq_len(p: *const mkv_pool, seq: u32) -> u32;
+    pub fn mkv_seq_pages(p: *const mkv_pool, seq: u32, pages_host: *mut u32, cap: u32, n_out: *mut u32) -> mkv_status;
+    pub fn mkv_pool_compact(p: *mut mkv_pool, moved_out: *mut u32) -> mkv_status;
+    pub fn mkv_pool_write(p: *mut mkv_pool, layer: c_int, items: *const mkv_seq_rows, n: c_int, r#in: *const mkv_pool_rows) -> mkv_status;
+    pub fn mkv_attn_pool(p: *mut mkv_pool, layer: c_int, items: *const mkv_seq_rows, n: c_int, r#in: *const mkv_pool_attn) -> mkv_status;
     pub fn mkv_snapshot_bytes(c: *const mkv_cache, p: u32) -> usize;
     pub fn mkv_snapshot(c: *mut mkv_cache, p: u32, dst_host: *mut c_void, cap: usize, written: *mut usize) -> mkv_status;
     pub fn mkv_snapshot_wait(c: *mut mkv_cache) -> mkv_status;

@@ -1,0 +1,593 @@
+"""The paged operators on the GPU against plain 64-bit implementations: rotary positions, written rows, forks and compaction, attention
+over pages. Needs a B200.
+
+Tolerances follow from the roundings (a half step is eps / 2 of the value): see `attn_bound` and the comments beside each test."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from mechta_b200 import _lib, kv
+
+pytestmark = pytest.mark.gpu
+F16, F32 = kv.KvFormat.F16, kv.KvFormat.F32
+FMTS = [F16, F32]
+HALF_STEP = {torch.float16: 2.0**-11, torch.float32: 2.0**-24}
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    assert torch.cuda.is_available(), "these tests need the GPU"
+    torch.cuda.set_device(0)
+    c = kv.KvContext(0, torch.cuda.current_stream())
+    yield c
+    c.close()
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def randn(g, *shape, dtype=torch.float32):
+    return torch.randn(*shape, device="cuda", generator=g).to(dtype)
+
+
+# ---- rotary positions ----------------------------------------------------------------------------------------------
+
+def rotate64(x, positions, f, m, layout, backward=False):
+    rot = 2 * len(f)
+    a = positions.double()[:, None, None] * torch.from_numpy(np.asarray(f)).cuda()
+    c, s = m * torch.cos(a), m * torch.sin(a) * (-1 if backward else 1)
+    y = x.double().clone()
+    u, w = (x[..., :rot:2].double(), x[..., 1:rot:2].double()) if layout == "interleaved" else (x[..., : rot // 2].double(), x[..., rot // 2: rot].double())
+    p, q = u * c - w * s, u * s + w * c
+    if layout == "interleaved":
+        y[..., :rot:2], y[..., 1:rot:2] = p, q
+    else:
+        y[..., : rot // 2], y[..., rot // 2: rot] = p, q
+    return y
+
+
+def rope_bound(x, rot, m, dtype, layout):
+    """Cosine and sine are off by the f32 rounding of the angle's fraction of a turn (at most pi * 2^-24 * 2 radians) and a few half
+    steps of sincospi and of the factor: under 2^-21 of each product in all with the two products' and the sum's own; then one
+    rounding to the output's type (half a step of the subnormals at least)."""
+    u, w = (x[..., :rot:2], x[..., 1:rot:2]) if layout == "interleaved" else (x[..., : rot // 2], x[..., rot // 2: rot])
+    size = m * (u.double().abs() + w.double().abs())
+    size = size.repeat_interleave(2, -1) if layout == "interleaved" else torch.cat((size, size), -1)
+    size = torch.cat((size, x[..., rot:].double().abs()), -1)
+    return size * (2.0**-21 + HALF_STEP[dtype]) + (2.0**-25 if dtype == torch.float16 else 0.0)
+
+
+@pytest.mark.parametrize("heads,dim,rot,layout", [(16, 256, 64, "half"), (3, 128, 128, "interleaved"), (5, 64, 30, "half"), (2, 80, 36, "interleaved"),
+                                                  (1, 30, 2, "half"), (7, 33, 32, "half"), (2, 256, 256, "half"), (40, 1000, 256, "interleaved")])
+@pytest.mark.parametrize("src,dst", [(torch.float32, torch.float16), (torch.float16, torch.float16), (torch.float32, torch.float32), (torch.float16, torch.float32)])
+def test_rope(ctx, heads, dim, rot, layout, src, dst):
+    g = gen(heads * 1000 + dim)
+    for n, far, scaling in ((1, 5, "none"), (37, 1 << 20, "yarn"), (300, 2**31 - 1, "linear")):
+        rope = kv.Rope(ctx, rot, layout=layout, scaling=scaling, factor=4.0, original=4096)
+        f, m = rope.freqs()
+        x = randn(g, n, heads, dim, dtype=src)
+        pos = torch.randint(-3, far, (n,), device="cuda", generator=g, dtype=torch.int32)
+        for backward in (False, True):
+            out = torch.full((n, heads, dim), math.nan, device="cuda", dtype=dst)
+            rope.apply(x, pos, out, backward=backward)
+            want = rotate64(x, pos, f, m, layout, backward)
+            assert ((out.double() - want).abs() <= rope_bound(x, rot, m, dst, layout)).all(), (n, scaling, backward)
+
+
+def test_rope_in_place_strided_and_gradient(ctx):
+    g = gen(3)
+    rope = kv.Rope(ctx, 64, scaling="yarn", factor=4.0, original=4096)
+    f, m = rope.freqs()
+    qf = randn(g, 5, 16, 512)  # query and gate side by side, as the step's input
+    pos = torch.arange(9000, 9005, device="cuda", dtype=torch.int32)
+    want, gate = rotate64(qf[..., :256], pos, f, m, "half"), qf[..., 256:].clone()
+    bound = rope_bound(qf[..., :256], 64, m, torch.float32, "half")
+    view = qf[..., :256]
+    rope.apply(view, pos, view)
+    assert ((view.double() - want).abs() <= bound).all() and torch.equal(qf[..., 256:], gate)
+    # heads outside tokens, odd addresses and strides: rows of a [heads][tokens][dims + 1] buffer
+    buf = torch.zeros(16, 5, 257, device="cuda")
+    x, y = randn(g, 16, 5, 257)[..., 1:].transpose(0, 1), buf[..., 1:].transpose(0, 1)
+    for layout in ("half", "interleaved"):
+        r = kv.Rope(ctx, 64, layout=layout)
+        r.apply(x, pos, y)
+        assert ((y.double() - rotate64(x, pos, r.freqs()[0], 1.0, layout)).abs() <= rope_bound(x, 64, 1.0, torch.float32, layout)).all()
+    assert not buf[..., 0].any()
+    # <R x, y> = <x, R^T y>, and against differences: the map is linear, so a step in x gives R of the step
+    a, b = randn(g, 5, 4, 64), randn(g, 5, 4, 64)
+    ra, rb = torch.empty_like(a), torch.empty_like(b)
+    rope.apply(a, pos, ra)
+    rope.apply(b, pos, rb, backward=True)
+    lhs, rhs = (ra.double() * b.double()).sum(), (a.double() * rb.double()).sum()
+    assert abs(lhs - rhs) <= 2 * (rope_bound(a, 64, m, torch.float32, "half") * b.double().abs()).sum()
+    d = torch.zeros_like(a)
+    d[2, 1, 40] = 1.0
+    up, down = torch.empty_like(a), torch.empty_like(a)
+    rope.apply(a + d, pos, up)
+    rope.apply(a - d, pos, down)
+    slope = ((up.double() - down.double()) / 2 * b.double()).sum()  # d<R x, b> / dx[2, 1, 40]
+    slack = (2 * rope_bound(a.abs() + d, 64, m, torch.float32, "half") * b.double().abs())[2, 1].sum() + HALF_STEP[torch.float32] * 8
+    assert abs(slope - rb[2, 1, 40].double()) <= slack
+    rope.apply(torch.empty(0, 4, 64, device="cuda"), pos[:0], torch.empty(0, 4, 64, device="cuda"))
+    for bad in ((a, pos[:4], ra), (a, pos.long(), ra), (a, pos, ra[:, :2]), (a.cpu(), pos, ra), (a[:, :1].expand(5, 4, 64), pos, ra), (a, pos, a[:, :, :].flip(0)[:, ::2]),
+                (a.double(), pos, ra), (a, pos, ra[:, :, ::2])):
+        with pytest.raises(_lib.MkvError):
+            rope.apply(*bad)
+
+
+# ---- a pool and its plain twin ---------------------------------------------------------------------------------------
+
+def rows_of(pool, seq, layer=0, upto=None):
+    """K and V rows of a sequence, in order."""
+    pages = torch.from_numpy(pool.pages(seq).astype(np.int64)).cuda()
+    n = pool.length(seq) if upto is None else upto
+    return [t[pages].reshape(-1, pool.kv_heads, pool.head_dim)[:n] for t in pool.buffer_tensors(layer)]
+
+
+def scattered(ctx, fmt, lens, page, seed, layers=1, spare=8, poison=None, heads=(16, 2, 256), longest=None):
+    """A pool whose sequences have N(0, 1) rows on pages that lie among one another's; what no sequence has holds `poison`."""
+    hq, hkv, dim = heads
+    need = sum(-(-n // page) for n in lens) + spare
+    pool = kv.KvPool(ctx, fmt, layers, need, page, len(lens) + 8, longest or max(max(lens), 1) + 600, hq, hkv, dim)
+    g = gen(seed)
+    ids = [pool.create() for _ in lens]
+    for r in range(1, 6):
+        for i, n in zip(ids, lens):
+            pool.set_len(i, n * r // 5)
+    for l in range(layers):
+        for t in pool.buffer_tensors(l):
+            if poison is None:
+                t.normal_(generator=g)
+            else:
+                t.fill_(poison)
+                for i, n in zip(ids, lens):
+                    pages = torch.from_numpy(pool.pages(i).astype(np.int64)).cuda()
+                    data = torch.full((len(pages) * page, hkv, dim), poison, device="cuda", dtype=t.dtype)
+                    data[:n] = randn(g, n, hkv, dim, dtype=t.dtype)
+                    t[pages] = data.view(len(pages), page, hkv, dim)
+    return pool, ids, g
+
+
+# ---- written rows ------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("heads,page,rot,layout,src", [((16, 2, 256), 16, 64, "half", torch.float32), ((32, 4, 128), 64, 128, "interleaved", torch.float16),
+                                                       ((3, 3, 64), 128, 30, "half", torch.float32), ((8, 1, 64), 256, 0, "half", torch.float16),
+                                                       ((16, 2, 256), 32, 54, "interleaved", torch.float32)])
+def test_write(ctx, fmt, heads, page, rot, layout, src):
+    lens = [0, 1, 15, 16, 17, 250, 256, 999]
+    news = [1, 0, 3, 40, 1, 7, 300, 2]
+    pool, ids, g = scattered(ctx, fmt, lens, page, 5, layers=2, spare=60, heads=heads)
+    before = [rows_of(pool, i) for i in ids]
+    other = [t.clone() for t in pool.buffer_tensors(1)]
+    rope = kv.Rope(ctx, rot, layout=layout) if rot else None
+    total = sum(news)
+    wide = torch.zeros(total, 2 * heads[1] + 1, heads[2], device="cuda", dtype=src)  # k and v inside a wider buffer
+    wide.normal_(generator=g)
+    k, v = wide[:, :heads[1]], wide[:, heads[1]:2 * heads[1]]
+    pool.write(0, [(i, 0, n, m) for i, n, m in zip(ids, lens, news)], k, v, rope)
+    at = 0
+    for i, n, m, (k0, v0) in zip(ids, lens, news, before):
+        assert pool.length(i) == n + m
+        k1, v1 = rows_of(pool, i)
+        assert torch.equal(k1[:n], k0) and torch.equal(v1[:n], v0)
+        kn, vn = k[at:at + m], v[at:at + m]
+        assert torch.equal(v1[n:], vn.to(v1.dtype))
+        if rope is None:
+            assert torch.equal(k1[n:], kn.to(k1.dtype))
+        elif m:
+            pos = torch.arange(n, n + m, device="cuda")
+            want, bound = rotate64(kn, pos, rope.freqs()[0], 1.0, layout), rope_bound(kn, rot, 1.0, k1.dtype, layout)
+            assert ((k1[n:].double() - want).abs() <= bound).all()
+        at += m
+    for t, o in zip(pool.buffer_tensors(1), other):
+        assert torch.equal(t, o)
+    pool.close()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_steps_with_rollback_and_copy_on_write(ctx, fmt):
+    """Layers written one after the other, refused drafts overwritten, forks that go their own ways: every sequence keeps its rows."""
+    page, layers = 16, 3
+    pool = kv.KvPool(ctx, fmt, layers, 60, page, 9, 1000)
+    g = gen(8)
+    truth = {}
+    a = pool.create()
+    truth[a] = [[torch.empty(0, 2, 256, device="cuda", dtype=pool.fmt.torch_dtype) for _ in range(2)] for _ in range(layers)]
+
+    def step(plan):  # (sequence, pos, ntok)
+        rows = sum(n for _, _, n in plan)
+        for l in range(layers):
+            k, v = randn(g, rows, 2, 256), randn(g, rows, 2, 256)
+            pool.write(l, [(s, 0, p, n) for s, p, n in plan], k, v)
+            at = 0
+            for s, p, n in plan:
+                for j, x in enumerate((k, v)):
+                    truth[s][l][j] = torch.cat((truth[s][l][j][:p], x[at:at + n].to(pool.fmt.torch_dtype)))
+                at += n
+        verify()
+
+    def verify():
+        for s, t in truth.items():
+            for l in range(layers):
+                for got, want in zip(rows_of(pool, s, l), t[l]):
+                    assert torch.equal(got, want)
+
+    def fork(s, length, n, copy=False):
+        kids = pool.fork(s, length, n, copy)
+        for c in kids:
+            truth[c] = [[x[:length].clone() for x in kv_] for kv_ in truth[s]]
+        return kids
+
+    step([(a, 0, 37)])
+    step([(a, 37, 4)])
+    step([(a, 39, 4)])          # two of the four were accepted
+    b, c = fork(a, 41, 2)
+    free = pool.free_pages
+    step([(b, 41, 1), (a, 43, 4), (c, 41, 3)])  # c is the last on the page that all three had: two copies
+    assert pool.free_pages == free - 2
+    step([(b, 30, 2)])          # back into a page that is shared: rows 32.. of b are gone, 16..29 copied
+    d = fork(c, 44, 1, copy=True)[0]
+    step([(d, 44, 30), (c, 44, 1)])
+    # with no free page a write that needs one is refused and changes nothing
+    hold = pool.create()
+    pool.set_len(hold, pool.free_pages * page)
+    assert pool.free_pages == 0
+    e = fork(d, 74, 1)[0]
+    k = randn(g, 2, 2, 256)
+    for plan in ([(e, 0, 74, 1), (c, 0, 45, 1)], [(c, 0, 45, 1), (e, 0, 74, 1)]):
+        with pytest.raises(_lib.MkvError) as err:
+            pool.write(0, plan, k, k)
+        assert err.value.status == _lib.ERR_NOMEM
+    verify()
+    # d and e share every page: when both write, one needs a page; d gives its part up first
+    pool.truncate(d, 64)
+    truth[d] = [[x[:64] for x in kv_] for kv_ in truth[d]]
+    step([(e, 74, 1)])
+    pool.free([hold, a])
+    del truth[a]
+    moved = pool.compact()
+    assert moved > 0
+    verify()
+    assert pool.compact() == 0
+    step([(b, 32, 40), (e, 75, 1), (c, 45, 2)])
+    pool.close()
+
+
+@pytest.mark.parametrize("fmt,page,length,layers", [(F16, 16, 100, 3), (F32, 256, 700, 2), (F16, 64, 9001, 10), (F32, 32, 6000, 1)])
+def test_copies_and_compaction(ctx, fmt, page, length, layers):
+    """More pages than one launch lists, holes in between; rows behind the last page's stay as they were."""
+    m = -(-length // page)
+    pool, ids, g = scattered(ctx, fmt, [length, length // 3, 40], page, 11, layers=layers, spare=4 * m)
+    want = [[t.clone() for t in rows_of(pool, ids[0], l)] for l in range(layers)]
+    tails = [[t.clone() for t in pool.buffer_tensors(l)] for l in range(layers)]
+    twin = pool.fork(ids[0], copy=True)[0]
+    assert not set(pool.pages(twin)) & set(pool.pages(ids[0]))
+    last = int(pool.pages(twin)[-1])
+    for l in range(layers):
+        for t, o in zip(pool.buffer_tensors(l), tails[l]):
+            if length % page:
+                assert torch.equal(t[last, length % page:], o[last, length % page:])
+    kids = pool.fork(twin, length // 2, 2)
+    pool.free([ids[0], ids[2]])
+    assert pool.compact() > 0
+    used = {int(p) for s in [twin, ids[1], *kids] for p in pool.pages(s)}
+    assert used == set(range(len(used))) and pool.free_pages == pool.n_pages - len(used)
+    for l in range(layers):
+        for s, n in [(twin, length)] + [(c, length // 2) for c in kids]:
+            for got, w in zip(rows_of(pool, s, l), want[l]):
+                assert torch.equal(got, w[:n])
+    pool.close()
+
+
+# ---- attention -----------------------------------------------------------------------------------------------------------
+
+def attn64(pool, items, q, window=0, sinks=None, scale=None, layer=0):
+    """From the formula, in 64 bits: the outputs, and what their tolerance is made of: sum of weight * |v|, sum of |q k| * scale at its
+    largest, the largest |v| among the keys seen."""
+    group = pool.q_heads // pool.kv_heads
+    scale = scale or pool.head_dim**-0.5
+    outs, mags, qks, tops, at = [], [], [], [], 0
+    for s, first, pos, n in items:
+        if n == 0:
+            continue
+        k, v = rows_of(pool, s, layer, pos + n)
+        k, v, x = k.double().transpose(0, 1), v.double().transpose(0, 1), q[at:at + n].double().transpose(0, 1)
+        at += n
+        k, v = k.repeat_interleave(group, 0), v.repeat_interleave(group, 0)
+        key, tok = torch.arange(pos + n, device="cuda")[None], torch.arange(pos, pos + n, device="cuda")[:, None]
+        seen = (key <= tok) & (key >= first)
+        if window:
+            seen &= key > tok - window
+        score = (x @ k.transpose(1, 2)) * scale
+        score = torch.where(seen, score, torch.tensor(-math.inf, dtype=torch.float64, device="cuda"))
+        top = score.amax(-1, keepdim=True)
+        if sinks is not None:
+            top = torch.maximum(top, sinks.double()[:, None, None])
+        top = torch.where(torch.isinf(top), torch.zeros_like(top), top)
+        w = torch.exp(score - top)
+        total = w.sum(-1, keepdim=True)
+        if sinks is not None:
+            total = total + torch.exp(sinks.double()[:, None, None] - top)
+        w = torch.where(seen.any(-1)[None, :, None], w / total, torch.zeros_like(w))
+        # (a masked row's infinities and NaN do not count)
+        clean = torch.where(seen.any(0)[None, :, None], v, torch.zeros_like(v))
+        outs.append((w @ clean).transpose(0, 1))
+        mags.append((w @ clean.abs()).transpose(0, 1))
+        qk = torch.where(seen, (x.abs() @ k.abs().transpose(1, 2)) * scale, torch.zeros_like(score))
+        qks.append(qk.amax(-1, keepdim=True).transpose(0, 1))
+        tops.append((clean.abs().amax((1, 2))[:, None, None].expand(-1, n, 1) * (pos + n)).transpose(0, 1))
+    return torch.cat(outs), torch.cat(mags), torch.cat(qks), torch.cat(tops)
+
+
+def attn_bound(fmt, out, mag, qk, top):
+    """f16: a weight is rounded to f16 (2^-11 of it, or half a subnormal step, 2^-25, against a largest weight of at least 1), the output
+    once more; f32 sums and exponentials in between. A score is off by its f32 sums: at most 2^-20 of sum |q k| here (the tensor
+    core's sums of 16 truncate: 16 steps of 2^-24 each), and a weight by as much, twice (sum and weight). f32: the products are
+    split into f16 parts of 11 bits each (2^-22 is left out), weights likewise."""
+    exponent = 2 * qk * 2.0**-20 + 2.0**-20
+    if fmt == F16:
+        return mag * (2.0**-11 * 1.03 + exponent) + out.abs() * 2.0**-11 + top * 2.0**-25 + 2.0**-25
+    return mag * (2.0**-20 + exponent) + 1e-30
+
+
+def run_attn(pool, items, q, **kw):
+    out = torch.full_like(q, math.nan)
+    pool.attn(0, items, q, out, **kw)
+    return out
+
+
+def check_attn(pool, items, q, **kw):
+    got = run_attn(pool, items, q, **kw)
+    want, mag, qk, top = attn64(pool, items, q, **kw)
+    off = (got.double() - want).abs()
+    bound = attn_bound(pool.fmt, want, mag, qk, top)
+    assert (off <= bound).all(), f"worst {float((off / bound).nan_to_num(1e9).max()):.3g} of the bound, {int((~(off <= bound)).sum())} values"
+    return got
+
+
+GEOMETRIES = [(16, 2, 256), (32, 4, 128), (4, 4, 64), (12, 4, 128), (5, 1, 256), (64, 1, 64), (40, 2, 64), (128, 2, 128)]
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("heads", GEOMETRIES)
+def test_attention_layouts(ctx, fmt, heads):
+    """Decode steps, drafts and blocks together, over every head layout; pages that end inside a tile."""
+    lens = [1, 2, 16, 63, 64, 65, 127, 128, 129, 200, 513, 1000]
+    news = [1, 2, 3, 1, 64, 4, 127, 1, 5, 33, 17, 300]
+    for page in (16, 128):
+        pool, ids, g = scattered(ctx, fmt, lens, page, sum(heads) + page, heads=heads)
+        q = randn(g, sum(news), heads[0], heads[2], dtype=pool.fmt.torch_dtype)
+        check_attn(pool, [(i, 0, n - m, m) for i, n, m in zip(ids, lens, news)], q)
+        pool.close()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("length,ntok", [(1, 1), (5, 3), (128, 128), (129, 1), (384, 129), (2000, 1), (3001, 4), (2500, 700)])
+def test_attention_lengths(ctx, fmt, page, length, ntok):
+    pool, ids, g = scattered(ctx, fmt, [length], page, length + page)
+    q = randn(g, ntok, 16, 256, dtype=pool.fmt.torch_dtype)
+    check_attn(pool, [(ids[0], 0, length - ntok, ntok)], q)
+    pool.close()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("heads", [(16, 2, 256), (32, 4, 128), (6, 2, 64)])
+@pytest.mark.parametrize("window,first", [(1, 0), (7, 0), (100, 0), (513, 0), (129, 700), (0, 650), (2**32 - 1, 0), (0, 900), (300, 2**32 - 1)])
+def test_attention_windows_sinks_and_empty_rows(ctx, fmt, heads, window, first):
+    """first_pos behind the first tokens, or behind all: rows that see nothing are zero, whatever the sinks."""
+    lens, news = [820, 33, 1400], [150, 33, 2]
+    pool, ids, g = scattered(ctx, fmt, lens, 32, window % 1000 + first % 1000, heads=heads)
+    q = randn(g, sum(news), heads[0], heads[2], dtype=pool.fmt.torch_dtype)
+    items = [(i, first if j != 1 else 0, n - m, m) for j, (i, n, m) in enumerate(zip(ids, lens, news))]
+    for sinks in (None, 3.0 * randn(g, heads[0]), torch.full((heads[0],), -math.inf, device="cuda")):
+        got = check_attn(pool, items, q, window=window, sinks=sinks)
+        if first >= 1400:
+            assert not got[:150].any() and not got[183:].any()
+    pool.close()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_attention_scales_and_extreme_scores(ctx, fmt):
+    """Peaked and flat softmaxes, a maximum that keeps rising along the keys, scores whose exponentials would overflow."""
+    pool, ids, g = scattered(ctx, fmt, [1500], 64, 77)
+    q = randn(g, 9, 16, 256, dtype=pool.fmt.torch_dtype)
+    items = [(ids[0], 0, 1491, 9)]
+    for scale in (1e-6, 0.02, 1.0, 20.0):
+        check_attn(pool, items, q, scale=scale)
+    k, _ = pool.buffer_tensors(0)
+    pages = torch.from_numpy(pool.pages(ids[0]).astype(np.int64)).cuda()
+    ramp = torch.linspace(-8, 8, len(pages) * 64, device="cuda").view(len(pages), 64, 1, 1)
+    k[pages] = (ramp * torch.ones_like(k[pages]) * 0.25).to(k.dtype)
+    q.fill_(0.5)
+    for sign in (1, -1):
+        check_attn(pool, items, q * sign, scale=1.0)
+    pool.close()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("poison", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("heads", [(16, 2, 256), (12, 4, 128), (4, 4, 64)])
+def test_what_no_row_sees_stays_out(ctx, fmt, poison, heads):
+    """NaN and infinities in free pages, behind the last row, in front of first_pos and of the window, and in rows of later tokens."""
+    lens, news = [1, 70, 300, 515], [1, 3, 40, 130]
+    pool, ids, g = scattered(ctx, fmt, lens, 32, 5, poison=poison, heads=heads)
+    q = randn(g, sum(news), heads[0], heads[2], dtype=pool.fmt.torch_dtype)
+    items = [(i, 0, n - m, m) for i, n, m in zip(ids, lens, news)]
+    check_attn(pool, items, q)
+    k, v = pool.buffer_tensors(0)
+
+    def place(s, p):
+        return int(pool.pages(ids[s])[p // 32]), p % 32
+
+    for p in (0, 3, 100):  # in front of first_pos = 101
+        k[place(3, p)] = poison
+        v[place(3, p)] = poison
+    items[3] = (ids[3], 101, 385, 130)
+    check_attn(pool, items, q)
+    check_attn(pool, items, q, window=50)
+    # the rows of token 7 of the third block and of token 60 of the fourth: earlier tokens do not see them
+    clean = run_attn(pool, items, q)
+    for s, p in ((2, 267), (3, 445)):
+        k[place(s, p)] = poison
+        v[place(s, p)] = poison
+    got = run_attn(pool, items, q)
+    assert torch.equal(got[:4 + 7], clean[:4 + 7]) and torch.equal(got[44:44 + 60], clean[44:44 + 60])
+    assert not torch.isfinite(got[4 + 7:44]).any() and not torch.isfinite(got[44 + 60:]).any()
+    # with a finite K row the one bad value of V reaches its dim alone, and only rows that see it
+    k[place(3, 445)], v[place(3, 445)] = 0.25, 0.5
+    v[place(3, 445)][0, 5] = poison
+    k[place(2, 267)], v[place(2, 267)] = 0.25, 0.5
+    got = run_attn(pool, items, q, window=30)
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    bad[44 + 60:44 + 90, : heads[0] // heads[1], 5] = True
+    assert torch.equal(~torch.isfinite(got), bad)
+    want, mag, qk, top = attn64(pool, items[:3], q[:44], window=30)
+    assert ((got[:44].double() - want).abs() <= attn_bound(fmt, want, mag, qk, top)).all()
+    v[place(3, 445)][0, 5] = 0.5
+    want, mag, qk, top = attn64(pool, items, q, window=30)
+    assert ((got.double() - want).abs() <= attn_bound(fmt, want, mag, qk, top))[~bad].all()
+    pool.close()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_attention_strides_shared_prefix_and_many_items(ctx, fmt):
+    """q inside a wider buffer; forks that share pages; more sequences than one launch takes; the rows around an output stay."""
+    pool, ids, g = scattered(ctx, fmt, [777], 16, 9, spare=600, longest=1500)
+    kids = [ids[0]]
+    pool.close()
+    pool = kv.KvPool(ctx, fmt, 1, 900, 16, 700, 1500)
+    for t in pool.buffer_tensors(0):
+        t.normal_(generator=g)
+    a = pool.create()
+    pool.set_len(a, 777)
+    kids = pool.fork(a, n=600)
+    k = randn(g, 600, 2, 256)
+    for _ in range(2):  # (each child its own last page)
+        pool.write(0, [(c, 0, 776, 1) for c in kids[:100]], k[:100], k[:100].flip(0))
+    items = [(c, 0, 770 + i % 7, 1 + (i % 3 if i % 7 < 5 else 0)) for i, c in enumerate(kids)]
+    total = sum(n for *_, n in items)
+    dt = pool.fmt.torch_dtype
+    wide = randn(g, total, 17, 256, dtype=dt)
+    q = wide[:, 1:]
+    room = torch.full((total + 2, 18, 256), 7.0, device="cuda", dtype=dt)
+    pool.attn(0, items, q, room[1:-1, :16])
+    want, mag, qk, top = attn64(pool, items, q)
+    assert ((room[1:-1, :16].double() - want).abs() <= attn_bound(fmt, want, mag, qk, top)).all()
+    assert (room[:, 16:] == 7.0).all() and (room[0] == 7.0).all() and (room[-1] == 7.0).all()
+    out = torch.full((0, 16, 256), 1.0, device="cuda", dtype=dt)
+    pool.attn(0, [], out, out)
+    pool.attn(0, [(a, 0, 5, 0)], out, out)
+    pool.close()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_the_same_call_gives_the_same_bits(ctx, fmt):
+    pool, ids, g = scattered(ctx, fmt, [5000, 40, 900], 64, 21)
+    q = randn(g, 40, 16, 256, dtype=pool.fmt.torch_dtype)
+    items = [(ids[0], 0, 4998, 2), (ids[1], 0, 39, 1), (ids[2], 0, 863, 37)]
+    first = run_attn(pool, items, q)
+    for _ in range(20):
+        assert torch.equal(run_attn(pool, items, q), first)
+    pool.close()
+
+
+# ---- the operators together ----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_serving_run(ctx, fmt):
+    """A prompt in blocks, samples forked from it, decode steps with rotated queries and rows, a session that ends, compaction: every
+    output against the rows as a plain program would have kept them."""
+    g, layers, page = gen(31), 2, 32
+    dt = kv.KvFormat(fmt).torch_dtype
+    pool = kv.KvPool(ctx, fmt, layers, 120, page, 8, 2000)
+    rope = kv.Rope(ctx, 64, layout="half", scaling="yarn", factor=4.0, original=512)
+
+    def step(plan):  # (sequence, pos, ntok)
+        rows = sum(n for *_, n in plan)
+        items = np.array([(s, 0, p, n) for s, p, n in plan], np.uint32)
+        pos = torch.cat([torch.arange(p, p + n, device="cuda", dtype=torch.int32) for _, p, n in plan])
+        for l in range(layers):
+            x, k, v = randn(g, rows, 16, 512), randn(g, rows, 2, 256), randn(g, rows, 2, 256)
+            q, out = torch.empty(rows, 16, 256, device="cuda", dtype=dt), torch.empty(rows, 16, 256, device="cuda", dtype=dt)
+            rope.apply(x[..., :256], pos, q)
+            pool.write(l, items, k, v, rope)
+            pool.attn(l, items, q, out)
+            want, mag, qk, top = attn64(pool, items.tolist(), q, layer=l)
+            assert ((out.double() - want).abs() <= attn_bound(fmt, want, mag, qk, top)).all()
+
+    a, z = pool.create(), pool.create()
+    step([(a, 0, 300), (z, 0, 70)])
+    step([(a, 300, 211), (z, 70, 1)])
+    kids = pool.fork(a, n=3)
+    step([(c, 511, 1) for c in kids] + [(z, 71, 4)])
+    step([(z, 73, 4), (kids[1], 512, 4)])
+    pool.free([a, kids[0]])
+    assert pool.compact() > 0
+    step([(kids[2], 512, 2), (z, 77, 1), (kids[1], 514, 3)])
+    pool.close()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_captured_step_replays(ctx, fmt):
+    """A captured rotation, write and attention, replayed with other inputs in the same memory; eager calls of the pool in between."""
+    stream = torch.cuda.Stream()
+    c2 = kv.KvContext(0, stream)
+    with torch.cuda.stream(stream):
+        pool, ids, g = scattered(c2, fmt, [3000, 100], 64, 41)
+        dt = pool.fmt.torch_dtype
+        rope = kv.Rope(c2)
+        items = np.array([(ids[0], 0, 3000, 2), (ids[1], 0, 100, 2)], np.uint32)
+        pos = torch.tensor([3000, 3001, 100, 101], device="cuda", dtype=torch.int32)
+        x, k, v = randn(g, 4, 16, 256), randn(g, 4, 2, 256), randn(g, 4, 2, 256)
+        q, out = torch.empty(4, 16, 256, device="cuda", dtype=dt), torch.empty(4, 16, 256, device="cuda", dtype=dt)
+
+        def step():
+            rope.apply(x, pos, q)
+            pool.write(0, items, k, v, rope)
+            pool.attn(0, items, q, out)
+
+        graph = torch.cuda.CUDAGraph()
+        stream.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            step()
+        for i in range(3):
+            for t in (x, k, v):
+                t.normal_(generator=g)
+            out.fill_(math.nan)
+            graph.replay()
+            replayed = out.clone()
+            step()
+            assert torch.equal(out, replayed)
+            want, mag, qk, top = attn64(pool, items.tolist(), q)
+            assert ((replayed.double() - want).abs() <= attn_bound(fmt, want, mag, qk, top)).all()
+        stream.synchronize()
+        del graph
+        pool.close()
+    c2.close()
+
+
+def test_context_outlives_and_launches_count(ctx):
+    c2 = kv.KvContext(0, torch.cuda.current_stream())
+    pool = kv.KvPool(c2, F16, 1, 8, 16, 2, 100)
+    a = pool.create()
+    n0 = c2.launches
+    pool.write(0, [(a, 0, 0, 20)], torch.ones(20, 2, 256, device="cuda"), torch.ones(20, 2, 256, device="cuda"))
+    assert c2.launches == n0 + 2  # the page table, the rows
+    view = pool.buffer_tensors(0)[0]
+    c2.close()  # the pool keeps it alive
+    q = torch.ones(20, 16, 256, device="cuda", dtype=torch.float16)
+    out = torch.empty_like(q)
+    pool.attn(0, [(a, 0, 0, 20)], q, out)
+    assert (out == 1).all()
+    del pool
+    assert float(view[0].float().sum()) == 16 * 512
+    with pytest.raises(_lib.MkvError) as e:
+        kv.KvPool(ctx, F16, 256, 2**24, 64, 1, 1000)  # 256 TB
+    assert e.value.status == _lib.ERR_NOMEM
