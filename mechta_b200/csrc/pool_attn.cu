@@ -2,7 +2,7 @@
 //   out_t = sum_k e^(s_k - M) v_k / (sum_k e^(s_k - M) + e^(sink - M)),  s_k = scale q_t . k_k, over the keys the token sees
 // One block of eight warps for one query head of one token; a warp takes every eighth key, keeps its own running maximum and sum, and
 // the eight meet in shared memory.
-#include "pool.cuh"
+#include "pool_plan.cuh"
 #include "ptx.cuh"
 
 namespace mkv {
@@ -92,7 +92,169 @@ __global__ void __launch_bounds__(256) pool_attn_kernel(const __grid_constant__ 
     }
 }
 
-mkv_status pool_attn_setup(Pool *) { return MKV_OK; }
+// ---- the plan of a launch ------------------------------------------------------------------------------------------
+bool pool_plan(const Pool *p, const mkv_seq_rows *items, int n, int &i, uint32_t &rows, uint32_t window, uint32_t keys, PoolPlan &plan, MergeList &merge) {
+    plan.nseq = 0;
+    plan.kv_heads = (uint32_t)p->desc.kv_heads;
+    plan.group = (uint32_t)(p->desc.q_heads / p->desc.kv_heads);
+    plan.block = 128u / plan.group;
+    plan.window = window;
+    plan.total = 0;
+    for (; i < n && plan.nseq < PLAN_SEQS; i++) {
+        if (items[i].ntok == 0u) continue;
+        PlanSeq &s = plan.seq[plan.nseq];
+        s = {items[i].seq * p->book.max_pages, items[i].first_pos, items[i].pos, items[i].ntok, rows};
+        uint64_t tiles = plan.total;
+        for (uint32_t b = 0; b * plan.block < s.ntok; b++) tiles += (uint64_t)plan.kv_heads * plan_item(s, window, plan.block, b, keys).tiles;
+        if (tiles > 0x7fffffffull && plan.nseq > 0u) break; // (one sequence alone stays below: mkv_attn_pool refuses more)
+        plan.total = (uint32_t)tiles;
+        plan.nseq++;
+        rows += s.ntok;
+    }
+    if (plan.nseq == 0u) return false;
+    const uint32_t sms = std::min<uint32_t>((uint32_t)p->ctx->sm_count, PLAN_CTAS);
+    plan.len = (plan.total + sms - 1u) / sms;
+    plan.ctas = (plan.total + plan.len - 1u) / plan.len;
+    merge.n = 0;
+    merge.group = plan.group;
+    uint32_t base = 0, c = 0;
+    for (uint32_t q = 0; q < plan.nseq; q++)
+        for (uint32_t b = 0; b * plan.block < plan.seq[q].ntok; b++) {
+            const PlanItem it = plan_item(plan.seq[q], window, plan.block, b, keys);
+            for (; c < plan.ctas && c * plan.len < base + it.tiles * plan.kv_heads; c++) {
+                const uint32_t h = (c * plan.len - base) / it.tiles, t = (c * plan.len - base) % it.tiles;
+                plan.start[c] = {(uint16_t)q, (uint16_t)h, b, t};
+                if (t > 0u && t <= plan.len) // the item's first cut: it begins in the CTA in front
+                    merge.item[merge.n++] = {plan.seq[q].row + it.tok0, h * plan.group, it.ntok, (uint16_t)(c - 1u),
+                                             (uint16_t)((it.tiles - t + plan.len - 1u) / plan.len + 1u)};
+            }
+            base += it.tiles * plan.kv_heads;
+        }
+    return true;
+}
+
+// ---- the merge of split items --------------------------------------------------------------------------------------
+// out = sum_s e^(m_s - M) O_s / (sum_s e^(m_s - M) l_s + e^(sink - M)) over an item's parts. A few dozen L2 accesses of a thread one after
+// the other are all there is to it, so the parts of a row are spread over up to 16 groups of threads, which meet in shared memory.
+struct MergeArgs {
+    const float *scratch, *sinks;
+    void *out;
+    int64_t out_stride;
+    uint32_t groups; // of a row
+};
+template <class T, int DIM>
+__global__ void __launch_bounds__(1024) pool_merge_kernel(const __grid_constant__ MergeList list, const __grid_constant__ MergeArgs g) {
+    constexpr uint32_t L = DIM / 4; // threads of a row's dims
+    __shared__ float4 acc_s[1024];
+    __shared__ float2 ml_s[1024 / L];
+    ptx::pdl_wait();
+    ptx::pdl_launch_dependents();
+    const MergeItem &it = list.item[blockIdx.y];
+    const uint32_t d = threadIdx.x % L, slot = threadIdx.x / L, grp = slot % g.groups, rpb = blockDim.x / L / g.groups;
+    const uint32_t row = blockIdx.x * rpb + slot / g.groups, parts = it.parts;
+    const bool real = row < it.ntok * list.group;
+    float M = NEG_BIG, l = 0.0f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    bool seen = true;
+    for (uint32_t s0 = grp; real && s0 < parts; s0 += 4u * g.groups) {
+        float2 ml[4];
+        float4 v[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; k++) {
+            const uint32_t s = s0 + k * g.groups;
+            const float *ps = g.scratch + part_slot(it.cta0 + min(s, parts - 1u), s == 0u ? 1u : 0u) * part_floats(DIM);
+            ml[k] = s < parts ? __ldcg(reinterpret_cast<const float2 *>(ps + 128u * DIM + 2u * row)) : make_float2(NEG_BIG, 0.0f);
+            v[k] = s < parts ? __ldcg(reinterpret_cast<const float4 *>(ps + (size_t)row * DIM + 4u * d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        const float mx = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x));
+        if (mx > M) {
+            const float f = M > NEG_TEST ? exp2f(M - mx) : 0.0f;
+            l *= f;
+            acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+            M = mx;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            seen = seen && ml[k].y >= 0.0f; // (-1: the row sees no key of the item; the sum of NaN weights is NaN and goes on)
+            if (ml[k].y != ml[k].y) seen = true;
+            const float e = ml[k].x > NEG_TEST ? exp2f(ml[k].x - M) : 0.0f;
+            if (e == 0.0f && ml[k].y == ml[k].y) continue;
+            l = fmaf(e, ml[k].y, l);
+            acc.x = fmaf(e, v[k].x, acc.x);
+            acc.y = fmaf(e, v[k].y, acc.y);
+            acc.z = fmaf(e, v[k].z, acc.z);
+            acc.w = fmaf(e, v[k].w, acc.w);
+        }
+    }
+    acc_s[threadIdx.x] = acc;
+    if (d == 0u) ml_s[slot] = make_float2(M, seen ? l : -1.0f);
+    __syncthreads();
+    if (grp != 0u || !real) return;
+    const uint32_t head = it.head + row % list.group;
+    const float sink = g.sinks ? g.sinks[head] * 1.4426950408889634f : NEG_BIG;
+    float Mr = sink;
+    for (uint32_t k = 0; k < g.groups; k++) Mr = fmaxf(Mr, ml_s[slot + k].x);
+    float den = sink > NEG_TEST ? exp2f(sink - Mr) : 0.0f;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    seen = true;
+    for (uint32_t k = 0; k < g.groups; k++) {
+        const float2 ml = ml_s[slot + k];
+        if (ml.y < 0.0f) seen = false;
+        const float e = ml.x > NEG_TEST ? exp2f(ml.x - Mr) : 0.0f;
+        if (e == 0.0f && ml.y == ml.y) continue;
+        const float4 a = acc_s[threadIdx.x + k * L];
+        den = fmaf(e, ml.y, den);
+        y.x = fmaf(e, a.x, y.x);
+        y.y = fmaf(e, a.y, y.y);
+        y.z = fmaf(e, a.z, y.z);
+        y.w = fmaf(e, a.w, y.w);
+    }
+    const float inv = 1.0f / den;
+    y = seen ? make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f);
+    T *dst = static_cast<T *>(g.out) + (int64_t)(it.row + row / list.group) * g.out_stride + (size_t)head * DIM + 4u * d;
+    if constexpr (sizeof(T) == 2) {
+        const __half2 a = __floats2half2_rn(y.x, y.y), b = __floats2half2_rn(y.z, y.w);
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+    } else {
+        *reinterpret_cast<float4 *>(dst) = y;
+    }
+}
+
+template <class T, int DIM> static mkv_status launch_merge(Pool *p, const MergeList &list, const PoolAttn &a) {
+    uint32_t parts = 0, rows = 0;
+    for (uint32_t i = 0; i < list.n; i++) {
+        parts = std::max<uint32_t>(parts, list.item[i].parts);
+        rows = std::max(rows, list.item[i].ntok * list.group);
+    }
+    const uint32_t threads = parts > 4u ? 1024u : 256u, slots = threads / (DIM / 4);
+    MergeArgs g = {p->scratch, a.sinks, a.out, a.out_stride, 1u};
+    while (g.groups < slots && g.groups < 16u && 4u * g.groups < parts) g.groups *= 2u;
+    const uint32_t rpb = slots / g.groups;
+    PdlLaunch l(p->ctx, dim3((rows + rpb - 1u) / rpb, list.n), threads);
+    MKV_CUDA(cudaLaunchKernelEx(&l.cfg, pool_merge_kernel<T, DIM>, list, g));
+    p->ctx->launches++;
+    return MKV_OK;
+}
+mkv_status launch_pool_merge(Pool *p, const MergeList &list, const PoolAttn &a) {
+    if (list.n == 0u) return MKV_OK;
+    const bool f16 = p->desc.fmt == MKV_F16;
+    switch (p->desc.head_dim) {
+    case 64: return f16 ? launch_merge<__half, 64>(p, list, a) : launch_merge<float, 64>(p, list, a);
+    case 128: return f16 ? launch_merge<__half, 128>(p, list, a) : launch_merge<float, 128>(p, list, a);
+    default: return f16 ? launch_merge<__half, 256>(p, list, a) : launch_merge<float, 256>(p, list, a);
+    }
+}
+
+mkv_status pool_attn_setup(Pool *p) {
+    if (p->desc.fmt != MKV_F16) return MKV_OK;
+    const size_t bytes = 2u * (size_t)std::min<uint32_t>((uint32_t)p->ctx->sm_count, PLAN_CTAS) * part_floats((uint32_t)p->desc.head_dim) * sizeof(float);
+    if (cudaMalloc(reinterpret_cast<void **>(&p->scratch), bytes) != cudaSuccess) {
+        cudaGetLastError();
+        set_error("out of device memory for %zu bytes of scratch", bytes);
+        return MKV_ERR_NOMEM;
+    }
+    return pool_attn_f16_setup(p);
+}
 
 template <class T> static mkv_status launch_dim(Pool *p, const AttnItems &it, const AttnArgs &g, uint32_t rows) {
     PdlLaunch l(p->ctx, dim3(rows, (unsigned)p->desc.q_heads), 256);
@@ -106,6 +268,17 @@ template <class T> static mkv_status launch_dim(Pool *p, const AttnItems &it, co
 }
 
 mkv_status launch_pool_attn(Pool *p, int layer, const mkv_seq_rows *items, int n, const PoolAttn &a) {
+    if (p->desc.fmt == MKV_F16) {
+        PoolPlan plan;
+        MergeList merge;
+        uint32_t rows = 0;
+        for (int i = 0; pool_plan(p, items, n, i, rows, a.window, 128u, plan, merge);) {
+            mkv_status st = launch_pool_attn_f16(p, layer, plan, a);
+            if (st == MKV_OK) st = launch_pool_merge(p, merge, a);
+            if (st != MKV_OK) return st;
+        }
+        return MKV_OK;
+    }
     AttnArgs g;
     g.q = a.q;
     g.out = a.out;
@@ -135,7 +308,7 @@ mkv_status launch_pool_attn(Pool *p, int layer, const mkv_seq_rows *items, int n
                 it.n++;
             }
         if (it.n == 0u) break;
-        const mkv_status st = p->desc.fmt == MKV_F16 ? launch_dim<__half>(p, it, g, it.row[it.n]) : launch_dim<float>(p, it, g, it.row[it.n]);
+        const mkv_status st = launch_dim<float>(p, it, g, it.row[it.n]);
         if (st != MKV_OK) return st;
         g.row0 += it.row[it.n];
     }
