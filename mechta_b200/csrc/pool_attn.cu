@@ -93,43 +93,63 @@ __global__ void __launch_bounds__(256) pool_attn_kernel(const __grid_constant__ 
 }
 
 // ---- the plan of a launch ------------------------------------------------------------------------------------------
-bool pool_plan(const Pool *p, const mkv_seq_rows *items, int n, int &i, uint32_t &rows, uint32_t window, uint32_t keys, PoolPlan &plan, MergeList &merge) {
+// Cuts the items into ranges of cost `budget`: true if the GPU's CTAs suffice.
+static bool plan_cut(PoolPlan &plan, MergeList &merge, const PlanCost &cost, uint32_t most, uint64_t budget) {
+    plan.ctas = 0;
+    merge.n = 0;
+    merge.group = plan.group;
+    uint64_t left = 0; // of the current CTA's budget
+    for (uint32_t q = 0; q < plan.nseq; q++)
+        for (uint32_t b = 0; b * plan.block < plan.seq[q].ntok; b++) {
+            const PlanItem it = plan_item(plan.seq[q], plan.window, plan.block, b, cost.keys);
+            for (uint32_t h = 0; h < plan.kv_heads; h++) {
+                uint32_t at = 0, parts = 0, cta0 = 0;
+                while (at < it.tiles) {
+                    // the rest of the item whole, or a part that is worth a segment, or a CTA of its own
+                    const uint64_t rest = it.tiles - at;
+                    if (plan.ctas == 0u || (left < rest + cost.segment && left < 2u * cost.segment + 1u)) {
+                        if (plan.ctas == most) return false;
+                        plan.start[plan.ctas++] = {(uint16_t)q, (uint16_t)h, b, at, 0u};
+                        left = budget;
+                    }
+                    const uint64_t room = left > cost.segment ? left - cost.segment : 1u;
+                    const uint32_t n = (uint32_t)std::min<uint64_t>(rest, room);
+                    plan.start[plan.ctas - 1u].tiles += n;
+                    if (parts++ == 0u) cta0 = plan.ctas - 1u;
+                    left -= std::min<uint64_t>(left, n + cost.segment);
+                    at += n;
+                    if (at < it.tiles) left = 0; // (a CTA has one part that does not end its item)
+                }
+                if (parts > 1u) merge.item[merge.n++] = {plan.seq[q].row + it.tok0, h * plan.group, it.ntok, (uint16_t)cta0, (uint16_t)parts};
+            }
+        }
+    return true;
+}
+
+bool pool_plan(const Pool *p, const mkv_seq_rows *items, int n, int &i, uint32_t &rows, uint32_t window, const PlanCost &cost, PoolPlan &plan, MergeList &merge) {
     plan.nseq = 0;
     plan.kv_heads = (uint32_t)p->desc.kv_heads;
     plan.group = (uint32_t)(p->desc.q_heads / p->desc.kv_heads);
     plan.block = 128u / plan.group;
     plan.window = window;
-    plan.total = 0;
+    uint64_t total = 0, count = 0;
     for (; i < n && plan.nseq < PLAN_SEQS; i++) {
         if (items[i].ntok == 0u) continue;
         PlanSeq &s = plan.seq[plan.nseq];
         s = {items[i].seq * p->book.max_pages, items[i].first_pos, items[i].pos, items[i].ntok, rows};
-        uint64_t tiles = plan.total;
-        for (uint32_t b = 0; b * plan.block < s.ntok; b++) tiles += (uint64_t)plan.kv_heads * plan_item(s, window, plan.block, b, keys).tiles;
-        if (tiles > 0x7fffffffull && plan.nseq > 0u) break; // (one sequence alone stays below: mkv_attn_pool refuses more)
-        plan.total = (uint32_t)tiles;
+        uint64_t tiles = 0, blocks = 0;
+        for (; blocks * plan.block < s.ntok; blocks++) tiles += plan_item(s, window, plan.block, (uint32_t)blocks, cost.keys).tiles;
+        if (total + tiles * plan.kv_heads > 0x7fffffffull && plan.nseq > 0u) break; // (one sequence alone stays below: mkv_attn_pool refuses more)
+        total += tiles * plan.kv_heads;
+        count += blocks * plan.kv_heads;
         plan.nseq++;
         rows += s.ntok;
     }
     if (plan.nseq == 0u) return false;
     const uint32_t sms = std::min<uint32_t>((uint32_t)p->ctx->sm_count, PLAN_CTAS);
-    plan.len = (plan.total + sms - 1u) / sms;
-    plan.ctas = (plan.total + plan.len - 1u) / plan.len;
-    merge.n = 0;
-    merge.group = plan.group;
-    uint32_t base = 0, c = 0;
-    for (uint32_t q = 0; q < plan.nseq; q++)
-        for (uint32_t b = 0; b * plan.block < plan.seq[q].ntok; b++) {
-            const PlanItem it = plan_item(plan.seq[q], window, plan.block, b, keys);
-            for (; c < plan.ctas && c * plan.len < base + it.tiles * plan.kv_heads; c++) {
-                const uint32_t h = (c * plan.len - base) / it.tiles, t = (c * plan.len - base) % it.tiles;
-                plan.start[c] = {(uint16_t)q, (uint16_t)h, b, t};
-                if (t > 0u && t <= plan.len) // the item's first cut: it begins in the CTA in front
-                    merge.item[merge.n++] = {plan.seq[q].row + it.tok0, h * plan.group, it.ntok, (uint16_t)(c - 1u),
-                                             (uint16_t)((it.tiles - t + plan.len - 1u) / plan.len + 1u)};
-            }
-            base += it.tiles * plan.kv_heads;
-        }
+    // the least that could do, and a little more as often as it takes
+    uint64_t budget = std::max<uint64_t>((total + count * cost.segment + sms - 1u) / sms, cost.segment + 1u);
+    while (!plan_cut(plan, merge, cost, sms, budget)) budget += budget / 32u + 1u;
     return true;
 }
 
@@ -272,7 +292,7 @@ mkv_status launch_pool_attn(Pool *p, int layer, const mkv_seq_rows *items, int n
         PoolPlan plan;
         MergeList merge;
         uint32_t rows = 0;
-        for (int i = 0; pool_plan(p, items, n, i, rows, a.window, 128u, plan, merge);) {
+        for (int i = 0; pool_plan(p, items, n, i, rows, a.window, {128u, 2u}, plan, merge);) {
             mkv_status st = launch_pool_attn_f16(p, layer, plan, a);
             if (st == MKV_OK) st = launch_pool_merge(p, merge, a);
             if (st != MKV_OK) return st;

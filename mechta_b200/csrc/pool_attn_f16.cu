@@ -7,20 +7,25 @@
 //   P = e^(S - reference maximum) as f16, back into the columns of S
 //   O += P V    A = P (tensor memory), B = the V tile as TMA left it (N-major)
 // One pass: the reference maximum of a row moves only when a tile exceeds it by more than 8 (then O is rescaled; weights stay
-// below e^8, far from f16's end), the sum is kept in f32. Two S buffers: the tensor cores compute the scores of a tile while the
-// one in front is in softmax. TMEM: O = columns 0 .. DIM - 1, S = 256 .. 383 and 384 .. 511.
+// below e^8, far from f16's end), sums are kept in f32. TMEM: O = columns 0 .. DIM - 1, then two (DIM = 256) or three S buffers of 128
+// columns, so that the scores of the next tiles are there when a tile's softmax begins.
 //
-// K and V come in units of 128 keys x 128 dims (32 KB; 64 dims: 16 KB) through one ring, in the order of their use
-// K0 K1 V0 K2 V1 ..; a unit is filled by one TMA box for each page (or half page of 256) and 64 dims, issued by as many lanes, each of
-// which looks its page up a tile ahead. Boxes without a key that the item's tokens see are not read.
+// Two threads share a row, 64 of a tile's keys each. Scores and outputs are issued by a warp each: the tensor cores hold no more than two
+// or three products in advance, so what one issuing thread does between two groups of products would cost their time.
+//
+// K and V come in units of 32 KB (K: 128 keys x 128 dims, V: 64 keys x 256 dims; heads of 128: whole tiles; of 64: whole tiles of 16 KB)
+// through one ring, in the order of their use K0 K1 V0 K2 V1 ..; a unit is filled by one TMA box for each page (at most 64 or 128 rows)
+// and 64 dims, issued by as many lanes, which look their pages up a tile ahead. Boxes without a key that the item's tokens see are not
+// read.
 //
 // Masked keys: their scores are replaced, so nothing in a K row that a token does not see matters. Their weights are zero, but zero
 // times an infinity or NaN is not: V rows outside the item's keys are zeroed in shared memory (first and last tile), and those that
 // only some of its tokens see are searched; one that is not finite is zeroed too and its share added to the rows that see it
 // with ordinary arithmetic.
 //
-// Roles (320 threads): warp 0 = TMA producer, warp 1 = MMA issuer (one thread) and TMEM owner, warps 2..9 = softmax, two threads per
-// row (64 of a tile's keys each). Every wait is bounded; TMEM is freed on every path.
+// Roles (384 threads, three warpgroups whose register budgets are set with setmaxnreg): warp 0 = TMA producer, warp 1 = issues S = Q K^T
+// and owns the TMEM, warp 2 = issues O += P V (warp 3 idle), warps 4..11 = softmax. Every wait is bounded; TMEM is
+// freed on every path.
 #include "pool_plan.cuh"
 #include "ptx.cuh"
 
@@ -28,23 +33,28 @@ namespace mkv {
 using namespace ptx;
 
 constexpr uint32_t PA_KEYS = 128;
-constexpr int PA_THREADS = 320;
+constexpr int PA_THREADS = 384;
+constexpr uint32_t PA_SOFTMAX_TID0 = 128;
 constexpr long long PA_WAIT_LIMIT = 2000000000ll;
 constexpr float PA_LOG2E = 1.4426950408889634f;
 constexpr float PA_LAZY2 = 8.0f * PA_LOG2E;
-constexpr uint32_t PA_COL_S = 256;
 
 template <int DIM> struct PaSizes {
     static constexpr uint32_t UNIT_DIMS = DIM < 128 ? DIM : 128;
     static constexpr uint32_t NUN = DIM / UNIT_DIMS;             // units of a K or V tile
     static constexpr uint32_t BOXES = UNIT_DIMS / 64;            // 64-dim boxes of a unit
-    static constexpr uint32_t BOX = PA_KEYS * 128;               // bytes of one, [128 keys][64 dims]
+    static constexpr uint32_t BOX = PA_KEYS * 128;               // bytes of one of K, [128 keys][64 dims]
+    static constexpr uint32_t V_KEYS = PA_KEYS / NUN;            // a unit of V has all dims of so many keys
+    static constexpr uint32_t V_BOX = V_KEYS * 128;              // [V_KEYS][64 dims]
     static constexpr uint32_t UNIT = BOXES * BOX;
     static constexpr uint32_t NST = DIM == 256 ? 5 : DIM == 128 ? 6 : 12;
     static constexpr uint32_t OFF_RING = (DIM / 64) * 16384;     // behind Q: [DIM / 64][128 rows][64 dims]
+    static constexpr uint32_t NBUF = DIM == 256 ? 2 : 3;         // S buffers
+    static constexpr uint32_t LEAD = NBUF - 1;                   // tiles that the scores are ahead of the outputs
+    static constexpr uint32_t COL_S = 512 - NBUF * 128;          // behind O
     static constexpr uint32_t OFF_RED = OFF_RING + NST * UNIT;   // [2 halves][128 rows] floats
     static constexpr uint32_t OFF_BAR = OFF_RED + 1024;
-    static constexpr uint32_t NBAR = 2 * NST + 6;                // full[NST], empty[NST], s_full[2], p_full[2], pv_done, q_full
+    static constexpr uint32_t NBAR = 2 * NST + 3 * NBUF + 1;     // full[NST], empty[NST], s_full[NBUF], p_full[NBUF], pv_done[NBUF], q_full
     static constexpr uint32_t OFF_MISC = OFF_BAR + NBAR * 8;
     static constexpr uint32_t SMEM = OFF_MISC + 64 + 1024;
     static_assert(SMEM <= 232448, "shared memory");
@@ -53,7 +63,8 @@ template <int DIM> struct PaSizes {
 struct PaShared {
     uint32_t tmem_base;
     volatile uint32_t abort;
-    uint32_t bad[2][4]; // [tile parity]: keys of the tile whose V row is not finite and that not every token sees
+    volatile uint32_t keep; // 1 + the tile whose products are added to O although it is its segment's first
+    uint32_t bad[2][4];     // [tile parity]: keys of the tile whose V row is not finite and that not every token sees
 };
 
 struct PaArgs {
@@ -61,6 +72,7 @@ struct PaArgs {
     __half *out;
     int64_t q_stride, out_stride;
     const uint32_t *pages;
+    const char *kpages;
     const char *vpages;
     const float *sinks;
     float *scratch;
@@ -70,14 +82,53 @@ struct PaArgs {
     uint32_t page_shift;
 };
 
-__device__ __forceinline__ bool pa_wait(uint32_t bar, uint32_t parity, PaShared *sh, uint32_t *status) {
-    if (sh->abort) return false;
-    if (mbar_wait_bounded(bar, parity, PA_WAIT_LIMIT)) return true;
+// Waits for a phase, for a bounded time; false when the time runs out or another thread has given up. The first try is all there is to
+// it when the phase is there.
+__device__ __forceinline__ bool pa_wait_long(uint32_t bar, uint32_t parity, PaShared *sh, uint32_t *status) {
+    const long long t0 = clock64();
+    for (;;) {
+        if (sh->abort) return false;
+#pragma unroll 1
+        for (int i = 0; i < 64; i++)
+            if (mbar_try_wait(bar, parity)) return true;
+        if (clock64() - t0 > PA_WAIT_LIMIT) break;
+    }
     sh->abort = 1;
     atomicOr(status, DEV_ERR_WAIT_TIMEOUT);
     return false;
 }
+__device__ __forceinline__ bool pa_wait(uint32_t bar, uint32_t parity, PaShared *sh, uint32_t *status) {
+    return mbar_try_wait(bar, parity) || pa_wait_long(bar, parity, sh, status);
+}
+// A place of a ring of N and the parity of its current use
+template <uint32_t N> struct PaRing {
+    uint32_t s = 0, turn = 0;
+    __device__ __forceinline__ void next(uint32_t d = 1u) { // d <= N
+        s += d;
+        if (s >= N) {
+            s -= N;
+            turn ^= 1u;
+        }
+    }
+};
 __device__ __forceinline__ bool half2_not_finite(uint32_t w) { return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u; }
+
+// The tiles of a CTA's segments as one stream.
+struct TileStream {
+    PlanWalk walk;
+    PlanSegment sg;
+    uint32_t tile;
+    bool more;
+    __device__ __forceinline__ TileStream(const PoolPlan &plan) : walk(plan, blockIdx.x, PA_KEYS) { step(); }
+    __device__ __forceinline__ void step() {
+        more = walk.next(sg);
+        tile = sg.a;
+    }
+    __device__ __forceinline__ bool first() const { return tile == sg.a; }
+    __device__ __forceinline__ void next() {
+        if (++tile == sg.b) step();
+    }
+};
 
 template <int DIM>
 __global__ void __launch_bounds__(PA_THREADS, 1)
@@ -89,19 +140,20 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     uint8_t *smem = smem_raw + (smem_base - smem_u32(smem_raw));
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t ring = smem_base + Z::OFF_RING, bar0 = smem_base + Z::OFF_BAR;
-    const uint32_t bar_full = bar0, bar_empty = bar0 + 8u * Z::NST, bar_s_full = bar0 + 16u * Z::NST, bar_p_full = bar_s_full + 16u;
-    const uint32_t bar_pv_done = bar_p_full + 16u, bar_q_full = bar_pv_done + 8u;
+    const uint32_t bar_full = bar0, bar_empty = bar0 + 8u * Z::NST, bar_s_full = bar0 + 16u * Z::NST, bar_p_full = bar_s_full + 8u * Z::NBUF;
+    const uint32_t bar_pv_done = bar_p_full + 8u * Z::NBUF, bar_q_full = bar_pv_done + 8u * Z::NBUF;
     PaShared *sh = reinterpret_cast<PaShared *>(smem + Z::OFF_MISC);
 
     if (tid == 0) {
         for (uint32_t s = 0; s < 2u * Z::NST; s++) mbar_init(bar0 + 8u * s, 1);
-        for (uint32_t s = 0; s < 2u; s++) {
+        for (uint32_t s = 0; s < Z::NBUF; s++) {
             mbar_init(bar_s_full + 8u * s, 1);
             mbar_init(bar_p_full + 8u * s, 8); // one arrival per softmax warp
+            mbar_init(bar_pv_done + 8u * s, 1);
         }
-        mbar_init(bar_pv_done, 1);
         mbar_init(bar_q_full, 8);
         sh->abort = 0;
+        sh->keep = 0;
         for (int i = 0; i < 8; i++) sh->bad[i >> 2][i & 3] = 0;
         fence_barrier_init();
         fence_proxy_async();
@@ -114,146 +166,187 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     pdl_wait(); // nothing global is touched before the kernel in front has finished
     pdl_launch_dependents();
 
-    // The units of a segment of n tiles in ring order: K0, then K(j + 1) and V(j) for each j. u counts units, g_ tiles, both across the
-    // CTA's segments.
+    // The units of the CTA's T tiles in ring order, whatever segment they belong to: K(0) .. K(LEAD - 1), then K(t + LEAD) and V(t) for
+    // each t. In front of K(t) are t + max(t - LEAD, 0) tiles of K and V, in front of V(t) min(t + LEAD + 1, T) + t.
+    if (warp < 4u) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 0) {
         // ---------------- TMA producer ----------------
-        const uint32_t page_tokens = 1u << g.page_shift, box_rows = min(page_tokens, PA_KEYS), nrb = PA_KEYS / box_rows;
-        const uint32_t rb = lane % nrb, cb = lane / nrb; // this lane's row box and 64-dim box of a unit
+        const uint32_t page_tokens = 1u << g.page_shift, box_rows = min(page_tokens, Z::V_KEYS), nrb = PA_KEYS / box_rows, nrbv = Z::V_KEYS / box_rows;
+        const uint32_t rb = lane % nrb, cb = lane / nrb, rbv = lane % nrbv, cbv = lane / nrbv; // this lane's row box and 64-dim box of a unit
+        PaRing<Z::NST> at;
         uint32_t u = 0;
-        PlanWalk walk(plan, blockIdx.x, PA_KEYS);
-        PlanSegment sg;
-        bool ok = true;
-        while (ok && walk.next(sg)) {
-            const PlanItem &it = sg.it;
-            const uint32_t *pages = g.pages + plan.seq[sg.seq].table;
-            // the row in the pool of the lane's row box of a tile, ~0u where no token of the item sees a key of it
-            auto look_up = [&](uint32_t j) -> uint32_t {
-                const uint32_t key = (it.tile0 + j) * PA_KEYS + rb * box_rows;
-                if (cb >= Z::BOXES || j >= sg.b || key + box_rows <= it.lo || key >= it.hi) return ~0u;
-                return (__ldg(pages + (key >> g.page_shift)) << g.page_shift) + (key & (page_tokens - 1u));
-            };
-            auto load = [&](const CUtensorMap *map, uint32_t row) -> bool { // the units of one K or V tile
+        TileStream ts(plan);
+        struct Tile {
+            uint32_t row; // in the pool, of this lane's row box of K; ~0u where no token of the item sees a key of it
+            int x;        // first column of the head
+            bool is;
+        };
+        auto look_up = [&]() -> Tile { // the stream's tile; the stream moves on
+            Tile t = {~0u, 0, ts.more};
+            if (!ts.more) return t;
+            const PlanItem &it = ts.sg.it;
+            const uint32_t key = (it.tile0 + ts.tile) * PA_KEYS + rb * box_rows;
+            if (lane < nrb * Z::BOXES && key + box_rows > it.lo && key < it.hi)
+                t.row = (__ldg(g.pages + plan.seq[ts.sg.seq].table + (key >> g.page_shift)) << g.page_shift) + (key & (page_tokens - 1u));
+            t.x = (int)(ts.sg.kvh * DIM);
+            ts.next();
+            return t;
+        };
+        auto load = [&](bool v, const Tile &t) -> bool { // the units of one K or V tile
 #pragma unroll
-                for (uint32_t h = 0; h < Z::NUN; h++, u++) {
-                    const uint32_t s = u % Z::NST, bar = bar_full + 8u * s;
-                    if (u >= Z::NST && !__all_sync(0xffffffffu, pa_wait(bar_empty + 8u * s, ((u / Z::NST) - 1u) & 1u, sh, g.status))) return false;
-                    const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, row != ~0u));
-                    if (lane == 0) mbar_expect_tx(bar, boxes * box_rows * 128u);
-                    __syncwarp();
-                    if (row != ~0u)
-                        tma_load_2d(ring + s * Z::UNIT + cb * Z::BOX + rb * box_rows * 128u, map, (int)(sg.kvh * DIM + h * Z::UNIT_DIMS + cb * 64u), (int)row, bar);
-                }
-                return true;
-            };
-            uint32_t row = look_up(sg.a), ahead = look_up(sg.a + 1u);
-            ok = load(&kmap, row);
-            for (uint32_t j = sg.a; ok && j < sg.b; j++) {
-                const uint32_t later = look_up(j + 2u);
-                if (j + 1u < sg.b) ok = load(&kmap, ahead);
-                ok = ok && load(&vmap, row);
-                row = ahead;
-                ahead = later;
+            for (uint32_t h = 0; h < Z::NUN; h++, u++, at.next()) {
+                const uint32_t s = at.s, bar = bar_full + 8u * s;
+                // V: the lane has another row box; a lane of K holds its row
+                const uint32_t of_v = __shfl_sync(0xffffffffu, t.row, h * nrbv + rbv), row = !v ? t.row : cbv < DIM / 64u ? of_v : ~0u;
+                const uint32_t dst = ring + s * Z::UNIT + (v ? cbv * Z::V_BOX + rbv * box_rows * 128u : cb * Z::BOX + rb * box_rows * 128u);
+                const int x = t.x + (int)(v ? cbv * 64u : h * Z::UNIT_DIMS + cb * 64u);
+                if (u >= Z::NST && !__all_sync(0xffffffffu, pa_wait(bar_empty + 8u * s, at.turn ^ 1u, sh, g.status))) return false;
+                const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, row != ~0u));
+                if (lane == 0) mbar_expect_tx(bar, boxes * box_rows * 128u);
+                __syncwarp();
+                if (row != ~0u) tma_load_2d(dst, v ? &vmap : &kmap, x, (int)row, bar);
             }
+            return true;
+        };
+        Tile next[Z::LEAD + 2]; // tiles t .. t + LEAD + 1: a page is looked up a tile before it is wanted
+        bool ok = true;
+#pragma unroll
+        for (uint32_t i = 0; i <= Z::LEAD; i++) {
+            next[i] = look_up();
+            if (i < Z::LEAD && next[i].is) ok = ok && load(false, next[i]);
+        }
+        while (ok && next[0].is) {
+            next[Z::LEAD + 1] = look_up();
+            if (next[Z::LEAD].is) ok = load(false, next[Z::LEAD]);
+            ok = ok && load(true, next[0]);
+#pragma unroll
+            for (uint32_t i = 0; i <= Z::LEAD; i++) next[i] = next[i + 1];
         }
     } else if (warp == 1) {
-        // ---------------- MMA issuer ----------------
+        // ---------------- S = Q K^T ----------------
         if (lane == 0) {
-            constexpr uint32_t IDESC_QK = tc_idesc_f16(128, 128, false);
-            constexpr uint32_t IDESC_PV = tc_idesc_f16(128, Z::UNIT_DIMS, true);
-            uint32_t u = 0, gt = 0, nseg = 0;
-            auto qk = [&](uint32_t t) -> bool { // S = Q K^T of tile t
-#pragma unroll
-                for (uint32_t h = 0; h < Z::NUN; h++, u++) {
-                    const uint32_t s = u % Z::NST;
-                    if (!pa_wait(bar_full + 8u * s, (u / Z::NST) & 1u, sh, g.status)) return false;
-                    tc_fence_after();
-#pragma unroll
-                    for (uint32_t ks = 0; ks < Z::UNIT_DIMS / 16u; ks++) {
-                        const uint64_t a = tc_desc_sw128(smem_base + (h * Z::BOXES + (ks >> 2)) * 16384u + (ks & 3u) * 32u, 16, 1024);
-                        const uint64_t b = tc_desc_sw128(ring + s * Z::UNIT + (ks >> 2) * Z::BOX + (ks & 3u) * 32u, 16, 1024);
-                        tc_mma_f16(tmem + PA_COL_S + 128u * (t & 1u), a, b, IDESC_QK, (h > 0 || ks > 0) ? 1u : 0u);
-                    }
-                    tc_commit(bar_empty + 8u * s);
-                }
-                tc_commit(bar_s_full + 8u * (t & 1u));
-                return true;
-            };
-            PlanWalk walk(plan, blockIdx.x, PA_KEYS);
-            PlanSegment sg;
+            constexpr uint32_t IDESC = tc_idesc_f16(128, 128, false);
+            const uint64_t q_desc = tc_desc_sw128(smem_base, 16, 1024), k_desc = tc_desc_sw128(ring, 16, 1024);
+            PaRing<Z::NST> at;
+            PaRing<Z::NBUF> buf;
+            uint32_t nseg = 0;
             bool ok = true;
-            while (ok && walk.next(sg)) {
-                if (!(ok = pa_wait(bar_q_full, nseg & 1u, sh, g.status))) break;
-                tc_fence_after();
-                nseg++;
-                const uint32_t n = sg.b - sg.a;
-                if (!(ok = qk(gt))) break;
-                for (uint32_t j = 0; j < n; j++, gt++) {
-                    if (j + 1u < n && !(ok = qk(gt + 1u))) break; // the next tile's scores while this one is in softmax
-                    if (!(ok = pa_wait(bar_p_full + 8u * (gt & 1u), (gt >> 1) & 1u, sh, g.status))) break;
-                    tc_fence_after();
-                    const uint32_t p = tmem + PA_COL_S + 128u * (gt & 1u);
-#pragma unroll
-                    for (uint32_t h = 0; h < Z::NUN; h++, u++) {
-                        const uint32_t s = u % Z::NST;
-                        if (!(ok = pa_wait(bar_full + 8u * s, (u / Z::NST) & 1u, sh, g.status))) break;
-                        tc_fence_after();
-#pragma unroll
-                        for (uint32_t ks = 0; ks < 8u; ks++) { // 16 keys an MMA
-                            const uint64_t b = tc_desc_sw128(ring + s * Z::UNIT + ks * 2048u, Z::BOX, 1024);
-                            tc_mma_f16_ta(tmem + h * Z::UNIT_DIMS, p + 64u * (ks >> 2) + 8u * (ks & 3u), b, IDESC_PV, (j > 0 || ks > 0) ? 1u : 0u);
-                        }
-                        tc_commit(bar_empty + 8u * s);
-                    }
-                    if (!ok) break;
-                    tc_commit(bar_pv_done);
+            TileStream ts(plan);
+            for (uint32_t t = 0; ok && ts.more; t++) {
+                if (ts.first()) { // the segment's Q is in shared memory
+                    ok = pa_wait(bar_q_full, nseg & 1u, sh, g.status);
+                    nseg++;
                 }
+                // the buffer's weights have been multiplied
+                if (t >= Z::NBUF) ok = ok && pa_wait(bar_pv_done + 8u * buf.s, buf.turn ^ 1u, sh, g.status);
+                const uint32_t d = tmem + Z::COL_S + 128u * buf.s;
+#pragma unroll
+                for (uint32_t h = 0; h < Z::NUN; h++) {
+                    ok = ok && pa_wait(bar_full + 8u * at.s, at.turn, sh, g.status);
+                    tc_fence_after();
+                    const uint64_t kd = k_desc + at.s * (Z::UNIT >> 4);
+#pragma unroll
+                    for (uint32_t ks = 0; ks < Z::UNIT_DIMS / 16u; ks++)
+                        tc_mma_f16(d, q_desc + (((h * Z::BOXES + (ks >> 2)) * 16384u + (ks & 3u) * 32u) >> 4), kd + (((ks >> 2) * Z::BOX + (ks & 3u) * 32u) >> 4),
+                                   IDESC, (h > 0 || ks > 0) ? 1u : 0u);
+                    tc_commit(bar_empty + 8u * at.s);
+                    at.next();
+                }
+                tc_commit(bar_s_full + 8u * buf.s);
+                buf.next();
+                if (t + 1u > Z::LEAD) at.next(Z::NUN); // over a tile of V
+                ts.next();
             }
         }
-    } else {
+    } else if (warp == 2) {
+        // ---------------- O += P V ----------------
+        if (lane == 0) {
+            constexpr uint32_t IDESC = tc_idesc_f16(128, DIM, true);
+            const uint64_t v_desc = tc_desc_sw128(ring, Z::V_BOX, 1024);
+            const uint32_t total = plan.start[blockIdx.x].tiles;
+            PaRing<Z::NST> at;
+            at.next(min(Z::LEAD + 1u, total) * Z::NUN); // over the first tiles of K
+            PaRing<Z::NBUF> buf;
+            bool ok = true;
+            TileStream ts(plan);
+            for (uint32_t t = 0; ok && ts.more; t++) {
+                ok = pa_wait(bar_p_full + 8u * buf.s, buf.turn, sh, g.status);
+                tc_fence_after();
+                const bool over = ts.first() && sh->keep != t + 1u; // the segment's first products overwrite O
+                const uint32_t p = tmem + Z::COL_S + 128u * buf.s;
+#pragma unroll
+                for (uint32_t h = 0; h < Z::NUN; h++) {
+                    ok = ok && pa_wait(bar_full + 8u * at.s, at.turn, sh, g.status);
+                    tc_fence_after();
+                    const uint64_t vd = v_desc + at.s * (Z::UNIT >> 4);
+#pragma unroll
+                    for (uint32_t ks = 0; ks < Z::V_KEYS / 16u; ks++) { // 16 keys an MMA
+                        const uint32_t k16 = h * (Z::V_KEYS / 16u) + ks;
+                        tc_mma_f16_ta(tmem, p + 64u * (k16 >> 2) + 8u * (k16 & 3u), vd + ((ks * 2048u) >> 4), IDESC, (!over || k16 > 0) ? 1u : 0u);
+                    }
+                    tc_commit(bar_empty + 8u * at.s);
+                    at.next();
+                }
+                tc_commit(bar_pv_done + 8u * buf.s);
+                buf.next();
+                if (t + Z::LEAD + 1u < total) at.next(Z::NUN); // over a tile of K
+                ts.next();
+            }
+        }
+    } else if (warp >= 4u) {
         // ---------------- softmax: two threads per row (TMEM lane), 64 keys of a tile and half of the dims of O each ----------------
-        const uint32_t q4 = warp & 3u, half = (warp - 2u) >> 2;
-        const uint32_t row = 32u * q4 + lane; // the TMEM lanes this warp may access
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;"); // 128 x 72 + 256 x 216 = the launch's 384 x 168
+        const uint32_t q4 = warp & 3u, half = (warp - 4u) >> 2;
+        const uint32_t row = 32u * q4 + lane, st = tid - PA_SOFTMAX_TID0; // row: the TMEM lanes this warp may access
         const uint32_t lane_addr = (32u * q4) << 16;
-        constexpr uint32_t HD = DIM / 2;      // dims of O of a thread
+        constexpr uint32_t HD = DIM / 2; // dims of Q and O of a thread
         float *red = reinterpret_cast<float *>(smem + Z::OFF_RED);
-        const uint32_t group = plan.group, tok = row / group, head = row % group;
+        const uint32_t group = plan.group, tok = row / group, head = row - tok * group, bar_pair = 1u + q4;
         auto arrive = [&](uint32_t bar) { // one arrival per warp, after all its lanes
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
         };
-        // The products of tile t have completed. A parity tells a phase from its neighbours only, and the tile in front need not have been
-        // waited for yet.
-        auto wait_pv = [&](uint32_t t) {
-            if (t > 0u) pa_wait(bar_pv_done, (t - 1u) & 1u, sh, g.status);
-            pa_wait(bar_pv_done, t & 1u, sh, g.status);
+        auto wait = [&](uint32_t bar, uint32_t parity) {
+            pa_wait(bar, parity, sh, g.status);
             __syncwarp();
             tc_fence_after();
         };
-        // Q rows of this warp, half of the dims, to shared memory; rows beyond the block as zeros where the warp has rows of it.
-        auto load_q = [&](const PlanSegment &sg) {
-            constexpr uint32_t CPR = DIM / 16; // 16-byte chunks of a half row
-            constexpr uint32_t RPI = 32 / CPR; // rows of one access of the warp
+        // The products of tile t have completed; for tiles since the newest scores that this warp has waited for. (A parity tells a phase from
+        // its neighbours only; those scores were computed behind the products of NBUF tiles earlier.)
+        auto wait_pv = [&](uint32_t t) { wait(bar_pv_done + 8u * (t % Z::NBUF), (t / Z::NBUF) & 1u); };
+        auto wait_s = [&](uint32_t t) { wait(bar_s_full + 8u * (t % Z::NBUF), (t / Z::NBUF) & 1u); };
+        // Q rows of this quarter, half of the dims; rows beyond the block as zeros where the quarter has rows of it. Fetched while the scores of
+        // the segment in front are still being computed, put into shared memory once they are.
+        constexpr uint32_t CPR = DIM / 16; // 16-byte chunks of a half row
+        constexpr uint32_t RPI = 32 / CPR; // rows of one access of the warp
+        uint4 qv[CPR];
+        auto fetch_q = [&](const PlanSegment &sg) {
             const uint32_t rows = sg.it.ntok * group;
-            if (32u * q4 < rows) {
-                const __half *src = g.q + (int64_t)(plan.seq[sg.seq].row + sg.it.tok0) * g.q_stride + (size_t)sg.kvh * group * DIM;
+            const __half *src = g.q + (int64_t)(plan.seq[sg.seq].row + sg.it.tok0) * g.q_stride + (size_t)sg.kvh * group * DIM + (half * CPR + lane % CPR) * 8u;
+#pragma unroll
+            for (uint32_t i = 0; i < CPR; i++) {
+                const uint32_t r = 32u * q4 + i * RPI + lane / CPR, t = r / group;
+                qv[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (r < rows) qv[i] = __ldg(reinterpret_cast<const uint4 *>(src + (int64_t)t * g.q_stride + (r - t * group) * DIM));
+            }
+        };
+        auto put_q = [&](const PlanSegment &sg) {
+            if (32u * q4 < sg.it.ntok * group) {
                 const uint32_t c = half * CPR + lane % CPR; // chunk of the row
-#pragma unroll 8
-                for (uint32_t i = 0; i < CPR; i++) {
-                    const uint32_t r = 32u * q4 + i * RPI + lane / CPR, t = r / group;
-                    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                    if (r < rows) v = __ldg(reinterpret_cast<const uint4 *>(src + (int64_t)t * g.q_stride + (r - t * group) * DIM + c * 8u));
-                    *reinterpret_cast<uint4 *>(smem + (c >> 3) * 16384u + swz128(r, c & 7u)) = v;
-                }
+#pragma unroll
+                for (uint32_t i = 0; i < CPR; i++)
+                    *reinterpret_cast<uint4 *>(smem + (c >> 3) * 16384u + swz128(32u * q4 + i * RPI + lane / CPR, c & 7u)) = qv[i];
             }
             fence_proxy_async();
             arrive(bar_q_full);
         };
-        uint32_t gt = 0, u = 0;
+        const uint32_t total = plan.start[blockIdx.x].tiles;
+        uint32_t t0 = 0; // the segment's first tile
         PlanWalk walk(plan, blockIdx.x, PA_KEYS);
         PlanSegment sg, nx;
         bool more = walk.next(sg);
-        if (more) load_q(sg);
+        fetch_q(sg);
+        put_q(sg);
         // A wait that runs out makes all later ones return at once; the warps go through the same barriers all the same, so that none waits
         // for one that has left.
         while (more) {
@@ -264,82 +357,78 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             const bool real = row < rows;
             const uint32_t vis = real ? sq.pos + it.tok0 + tok + 1u : 0u; // this row sees klo <= key < vis
             const uint32_t klo = real ? plan_lowest(sq, plan.window, it.tok0 + tok) : 0u;
-            float m_ref = NEG_BIG, l_run = 0.0f; // l_run: this thread's 64 keys of every tile only
-            const uint32_t n = sg.b - sg.a;
-            for (uint32_t j = 0; j < n; j++, gt++) {
-                const uint32_t key0 = (it.tile0 + sg.a + j) * PA_KEYS, s_col = tmem + lane_addr + PA_COL_S + 128u * (gt & 1u);
-                // units in front of this tile's V: K(0 .. min(j + 1, n - 1)) and V(0 .. j - 1)
-                const uint32_t uv = u + (min(j + 2u, n) + j) * Z::NUN;
+            float m_ref = NEG_BIG, l = 0.0f; // l: this thread's keys only
+            const uint32_t end = t0 + (sg.b - sg.a);
+            more = walk.next(nx);
+            for (uint32_t t = t0; t < end; t++) {
+                const uint32_t key0 = (it.tile0 + sg.a + (t - t0)) * PA_KEYS, s_col = tmem + lane_addr + Z::COL_S + 128u * (t % Z::NBUF) + 64u * half;
                 const bool edge = key0 < it.all_lo || key0 + PA_KEYS > it.all_hi; // some row does not see some key
-                pa_wait(bar_s_full + 8u * (gt & 1u), (gt >> 1) & 1u, sh, g.status);
-                __syncwarp();
-                tc_fence_after();
+                const bool last = t + 1u == end && more;
+                if (last) fetch_q(nx);
+                wait_s(t);
+                if (last) put_q(nx); // the segment's scores are all there: its Q may go
                 bool bad_any = false;
-                uint32_t bad[4] = {0u, 0u, 0u, 0u};
-                if (edge) { // (the same for all eight warps)
-                    for (uint32_t h = 0; h < Z::NUN; h++) pa_wait(bar_full + 8u * ((uv + h) % Z::NST), ((uv + h) / Z::NST) & 1u, sh, g.status);
-                    __syncwarp();
-                    const uint32_t st = tid - 64u;
-                    for (uint32_t idx = st; idx < PA_KEYS * (DIM / 8u); idx += 256u) {
-                        const uint32_t r = idx / (DIM / 8u), c = idx % (DIM / 8u), key = key0 + r; // chunk of 8 dims of key r
-                        const uint32_t unit = (uv + c / (Z::UNIT_DIMS / 8u)) % Z::NST, uc = c % (Z::UNIT_DIMS / 8u);
-                        uint4 *at = reinterpret_cast<uint4 *>(smem + Z::OFF_RING + unit * Z::UNIT + (uc >> 3) * Z::BOX + swz128(r, uc & 7u));
-                        if (key < it.lo || key >= it.hi) *at = make_uint4(0u, 0u, 0u, 0u);
-                        else if (key < it.all_lo || key >= it.all_hi) {
-                            const uint4 v = *at;
-                            if (half2_not_finite(v.x) || half2_not_finite(v.y) || half2_not_finite(v.z) || half2_not_finite(v.w)) atomicOr(&sh->bad[gt & 1u][r >> 5], 1u << (r & 31u));
-                        }
+                if (edge) { // (the same for the eight warps)
+                    const uint32_t uv = (min(t + Z::LEAD + 1u, total) + t) * Z::NUN; // units in front of this tile's V
+                    // The unit that a slot held before must be known to have come. Those of K(t) and in front have; with fewer than three tiles
+                    // of slots that may be one of V(t - 1).
+                    if (Z::NST < 3u * Z::NUN && t > 0u) wait_pv(t - 1u);
+                    for (uint32_t h = 0; h < Z::NUN; h++) wait(bar_full + 8u * ((uv + h) % Z::NST), ((uv + h) / Z::NST) & 1u);
+                    auto v_chunk = [&](uint32_t r, uint32_t c) { // 8 dims of key r
+                        const uint32_t unit = (uv + r / Z::V_KEYS) % Z::NST;
+                        return reinterpret_cast<uint4 *>(smem + Z::OFF_RING + unit * Z::UNIT + (c >> 3) * Z::V_BOX + swz128(r % Z::V_KEYS, c & 7u));
+                    };
+                    // rows of the tile: [0, z0) and [z1, 128) are outside the item's keys; [z0, p0) and [p1, z1) are not seen by all
+                    auto in_tile = [&](uint32_t key) { return key > key0 ? min(key - key0, PA_KEYS) : 0u; };
+                    const uint32_t z0 = in_tile(it.lo), z1 = in_tile(it.hi), p0 = max(z0, min(z1, in_tile(it.all_lo))), p1 = max(p0, min(z1, in_tile(it.all_hi)));
+                    for (uint32_t idx = st; idx < (z0 + PA_KEYS - z1) * (DIM / 8u); idx += 256u) {
+                        const uint32_t r = idx / (DIM / 8u);
+                        *v_chunk(r < z0 ? r : r - z0 + z1, idx % (DIM / 8u)) = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    for (uint32_t idx = st; idx < (p0 - z0 + z1 - p1) * (DIM / 8u); idx += 256u) {
+                        const uint32_t i = idx / (DIM / 8u), r = i < p0 - z0 ? z0 + i : i - (p0 - z0) + p1;
+                        const uint4 v = *v_chunk(r, idx % (DIM / 8u));
+                        if (half2_not_finite(v.x) || half2_not_finite(v.y) || half2_not_finite(v.z) || half2_not_finite(v.w))
+                            atomicOr(&sh->bad[t & 1u][r >> 5], 1u << (r & 31u));
                     }
                     if (it.ntok > 1u) { // (else all its rows see the same keys)
                         named_bar_sync(5, 256);
-#pragma unroll
-                        for (int i = 0; i < 4; i++) bad[i] = sh->bad[gt & 1u][i];
-                        bad_any = (bad[0] | bad[1] | bad[2] | bad[3]) != 0u;
-                        if (bad_any) {
-                            for (uint32_t idx = st; idx < PA_KEYS * (DIM / 8u); idx += 256u) {
-                                const uint32_t r = idx / (DIM / 8u), c = idx % (DIM / 8u);
-                                const uint32_t unit = (uv + c / (Z::UNIT_DIMS / 8u)) % Z::NST, uc = c % (Z::UNIT_DIMS / 8u);
-                                if (bad[r >> 5] >> (r & 31u) & 1u)
-                                    *reinterpret_cast<uint4 *>(smem + Z::OFF_RING + unit * Z::UNIT + (uc >> 3) * Z::BOX + swz128(r, uc & 7u)) = make_uint4(0u, 0u, 0u, 0u);
-                            }
-                            named_bar_sync(5, 256); // all have read bad[]
-                            if (st < 4u) sh->bad[gt & 1u][st] = 0u; // (read again two tiles on, behind this tile's p_full)
+                        bad_any = (sh->bad[t & 1u][0] | sh->bad[t & 1u][1] | sh->bad[t & 1u][2] | sh->bad[t & 1u][3]) != 0u;
+                        for (uint32_t idx = st; bad_any && idx < PA_KEYS * (DIM / 8u); idx += 256u) {
+                            const uint32_t r = idx / (DIM / 8u);
+                            if (sh->bad[t & 1u][r >> 5] >> (r & 31u) & 1u) *v_chunk(r, idx % (DIM / 8u)) = make_uint4(0u, 0u, 0u, 0u);
                         }
                     }
                     fence_proxy_async();
                 }
-                uint32_t sr[2][32];
-                float cf = 1.0f;
                 if (active) {
-                    tmem_ld32(s_col + 64u * half, sr[0]);
-                    tmem_ld32(s_col + 64u * half + 32u, sr[1]);
+                    uint32_t sr[2][32];
+                    tmem_ld32(s_col, sr[0]);
+                    tmem_ld32(s_col + 32u, sr[1]);
                     tmem_wait_ld();
-                    const uint32_t key_base = key0 + 64u * half;
                     // work in base-2 exponents: e^(s scale - m) = 2^(s C - m2), C = scale log2(e)
                     float mt[4] = {NEG_BIG, NEG_BIG, NEG_BIG, NEG_BIG};
                     if (edge) {
+                        __syncwarp(); // (a branch: most tiles have no masked keys)
+                        const uint32_t k = key0 + 64u * half;
 #pragma unroll
                         for (int h = 0; h < 2; h++)
 #pragma unroll
-                            for (int c = 0; c < 32; c++) {
-                                const uint32_t key = key_base + 32u * h + c;
-                                const float v = (key >= klo && key < vis) ? __uint_as_float(sr[h][c]) : -INFINITY;
-                                sr[h][c] = __float_as_uint(v);
-                                mt[c & 3] = fmaxf(mt[c & 3], v);
-                            }
-                    } else {
-#pragma unroll
-                        for (int h = 0; h < 2; h++)
-#pragma unroll
-                            for (int c = 0; c < 32; c++) mt[c & 3] = fmaxf(mt[c & 3], __uint_as_float(sr[h][c]));
+                            for (int c = 0; c < 32; c++)
+                                if (k + 32u * h + c < klo || k + 32u * h + c >= vis) sr[h][c] = 0xff800000u; // -infinity
                     }
-                    float mx = fmaxf(fmaxf(mt[0], mt[1]), fmaxf(mt[2], mt[3]));
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int c = 0; c < 32; c += 2) mt[(c >> 1) & 3] = max3(mt[(c >> 1) & 3], __uint_as_float(sr[h][c]), __uint_as_float(sr[h][c + 1]));
+                    float mx = max3(fmaxf(mt[0], mt[1]), mt[2], mt[3]);
                     mx = mx > NEG_TEST ? mx * g.scale2 : NEG_BIG; // this half row's tile maximum as a base-2 exponent
-                    // The reference maximum moves for the first valid tile or when the tile exceeds it by more than 8. The two warps that
+                    // The reference maximum moves for the first tile with a key and when the tile exceeds it by more than 8. The two warps that
                     // share these 32 rows vote; only then they exchange maxima.
-                    if (pair_bar_or(1u + q4, mx > NEG_TEST && (m_ref < NEG_TEST || mx > m_ref + PA_LAZY2))) {
+                    float cf = 1.0f;
+                    if (pair_bar_or(bar_pair, mx > NEG_TEST && (m_ref < NEG_TEST || mx > m_ref + PA_LAZY2))) {
                         red[128u * half + row] = mx;
-                        pair_bar_sync(1u + q4);
+                        pair_bar_sync(bar_pair);
                         mx = fmaxf(mx, red[128u * (half ^ 1u) + row]);
                         if (mx > NEG_TEST && (m_ref < NEG_TEST || mx > m_ref + PA_LAZY2)) {
                             const float m_new = fmaxf(m_ref, mx);
@@ -348,83 +437,70 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                         }
                     }
                     const float neg_m = m_ref > NEG_TEST ? -m_ref : 0.0f;
-                    float sum[2] = {0.0f, 0.0f};
-                    uint32_t ph[32]; // 64 weights as f16 pairs
+                    const uint64_t c2 = pack2(g.scale2, g.scale2), m2 = pack2(neg_m, neg_m);
+                    uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
-                    for (int h = 0; h < 2; h++)
+                    for (int h = 0; h < 2; h++) {
+                        uint32_t ph[16]; // 32 weights as f16 pairs
 #pragma unroll
                         for (int c = 0; c < 32; c += 2) {
-                            float w0, w1;
-                            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w0) : "f"(fmaf(__uint_as_float(sr[h][c]), g.scale2, neg_m)));
-                            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w1) : "f"(fmaf(__uint_as_float(sr[h][c + 1]), g.scale2, neg_m)));
-                            sum[0] += w0;
-                            sum[1] += w1;
-                            if (edge) { // kept for the rows of V that are added by hand
-                                sr[h][c] = __float_as_uint(w0);
-                                sr[h][c + 1] = __float_as_uint(w1);
-                            }
-                            const __half2 hp = __floats2half2_rn(w0, w1);
-                            ph[16 * h + (c >> 1)] = *reinterpret_cast<const uint32_t *>(&hp);
+                            float x0, x1;
+                            unpack2(fma2(pack2(__uint_as_float(sr[h][c]), __uint_as_float(sr[h][c + 1])), c2, m2), x0, x1);
+                            x0 = ex2(x0);
+                            x1 = ex2(x1);
+                            sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], pack2(x0, x1));
+                            const __half2 hp = __floats2half2_rn(x0, x1);
+                            ph[c >> 1] = *reinterpret_cast<const uint32_t *>(&hp);
                         }
-                    l_run = l_run * cf + (sum[0] + sum[1]);
-                    tmem_st32(s_col + 64u * half, ph);
-                    if (j > 0 && __any_sync(0xffffffffu, cf != 1.0f)) { // rescale this warp's rows and dims of O (rare)
-                        wait_pv(gt - 1u);
+                        tmem_st16(s_col + 16u * h, ph);
+                    }
+                    float s0, s1;
+                    unpack2(add2(sum[0], sum[1]), s0, s1);
+                    l = l * cf + (s0 + s1);
+                    const bool moved = t > t0 && __any_sync(0xffffffffu, cf != 1.0f);
+                    if (moved || bad_any) { // this warp's rows of O (rare)
+                        if (t > t0) wait_pv(t - 1u);
 #pragma unroll 1
-                        for (uint32_t c0 = 0; c0 < HD; c0 += 32u) {
+                        for (uint32_t c0 = HD * half; c0 < HD * half + HD; c0 += 32u) {
                             uint32_t orow[32];
-                            tmem_ld32(tmem + lane_addr + HD * half + c0, orow);
-                            tmem_wait_ld();
+                            if (t > t0) {
+                                tmem_ld32(tmem + lane_addr + c0, orow);
+                                tmem_wait_ld();
+                            }
 #pragma unroll
-                            for (int c = 0; c < 32; c++) orow[c] = __float_as_uint(__uint_as_float(orow[c]) * cf);
-                            tmem_st32(tmem + lane_addr + HD * half + c0, orow);
+                            for (int c = 0; c < 32; c++) orow[c] = t > t0 ? __float_as_uint(__uint_as_float(orow[c]) * cf) : 0u;
+                            // rows of V that are not finite, zero in shared memory: w v for the tokens that see them
+                            for (uint32_t r = 0; bad_any && r < PA_KEYS; r++) {
+                                const uint32_t key = key0 + r;
+                                if (!(sh->bad[t & 1u][r >> 5] >> (r & 31u) & 1u) || !real || key < klo || key >= vis) continue;
+                                const size_t page = g.pages[sq.table + (key >> g.page_shift)], off = key & ((1u << g.page_shift) - 1u);
+                                const __half *v = reinterpret_cast<const __half *>(g.vpages + ((page << g.page_shift) + off) * g.row_bytes) + (size_t)sg.kvh * DIM + c0;
+                                const __half *k = reinterpret_cast<const __half *>(g.kpages + ((page << g.page_shift) + off) * g.row_bytes) + (size_t)sg.kvh * DIM;
+                                const __half *q = g.q + (int64_t)(sq.row + it.tok0 + tok) * g.q_stride + (size_t)(sg.kvh * group + head) * DIM;
+                                float s = 0.0f;
+                                for (int d = 0; d < DIM; d++) s = fmaf(__half2float(q[d]), __half2float(k[d]), s);
+                                const float w = exp2f(fmaf(s, g.scale2, neg_m));
+#pragma unroll
+                                for (int c = 0; c < 32; c++) orow[c] = __float_as_uint(fmaf(w, __half2float(v[c]), __uint_as_float(orow[c])));
+                            }
+                            tmem_st32(tmem + lane_addr + c0, orow);
                         }
                     }
                     tmem_wait_st();
                 }
-                tc_fence_before();
-                arrive(bar_p_full + 8u * (gt & 1u));
-                if (bad_any) { // rows of V that are not finite: w v for the tokens that see them, added once the tile's products are there
-                    wait_pv(gt);
-                    for (uint32_t r = 0; r < PA_KEYS; r++) {
-                        if (!(bad[r >> 5] >> (r & 31u) & 1u) || !active) continue;
-                        if ((r >> 6) == half) {
-                            float w = 0.0f;
-#pragma unroll
-                            for (uint32_t c = 0; c < 64u; c++)
-                                if (c == (r & 63u)) w = __uint_as_float(sr[c >> 5][c & 31u]);
-                            red[row] = w;
-                        }
-                        pair_bar_sync(1u + q4);
-                        const float w = red[row];
-                        const uint32_t key = key0 + r;
-                        const bool sees = real && key >= klo && key < vis;
-                        const size_t at = ((size_t)g.pages[sq.table + (key >> g.page_shift)] << g.page_shift) + (key & ((1u << g.page_shift) - 1u));
-                        const __half *v = reinterpret_cast<const __half *>(g.vpages + at * g.row_bytes) + (size_t)sg.kvh * DIM + HD * half;
-#pragma unroll 1
-                        for (uint32_t c0 = 0; c0 < HD; c0 += 32u) {
-                            uint32_t orow[32];
-                            tmem_ld32(tmem + lane_addr + HD * half + c0, orow);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int c = 0; c < 32; c++)
-                                if (sees) orow[c] = __float_as_uint(fmaf(w, __half2float(v[c0 + c]), __uint_as_float(orow[c])));
-                            tmem_st32(tmem + lane_addr + HD * half + c0, orow);
-                        }
-                        tmem_wait_st();
-                        pair_bar_sync(1u + q4); // red[] is free again
-                    }
-                    tc_fence_before();
+                if (bad_any) {
+                    named_bar_sync(5, 256);
+                    if (st < 4u) sh->bad[t & 1u][st] = 0u; // (used again two tiles on, behind this tile's p_full)
+                    if (t == t0 && st == 0u) sh->keep = t + 1u; // what was put into O stays
                 }
+                tc_fence_before();
+                arrive(bar_p_full + 8u * (t % Z::NBUF));
             }
-            // ---------------- end of the segment: all its MMAs have completed ----------------
-            u += 2u * n * Z::NUN;
-            wait_pv(gt - 1u);
-            more = walk.next(nx);
-            if (more) load_q(nx); // the next segment's first scores are computed while this one's epilogue runs
+            // ---------------- end of the segment ----------------
+            wait_pv(end - 1u); // (the next segment's first scores are computed meanwhile)
             if (active) {
-                red[128u * half + row] = l_run;
-                pair_bar_sync(1u + q4);
+                red[128u * half + row] = l;
+                pair_bar_sync(bar_pair);
                 const float l_all = red[row] + red[128u + row];
                 const bool seen = real && klo < vis;
                 if (sg.whole) {
@@ -468,8 +544,9 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                     }
                 }
                 tc_fence_before();
-                pair_bar_sync(1u + q4); // red[] is free for the next segment
+                pair_bar_sync(bar_pair); // O and red[] are free for the next segment
             }
+            t0 = end;
             sg = nx;
         }
     }
@@ -502,6 +579,7 @@ mkv_status launch_pool_attn_f16(Pool *p, int layer, const PoolPlan &plan, const 
     g.q_stride = a.q_stride;
     g.out_stride = a.out_stride;
     g.pages = p->table;
+    g.kpages = p->layer_ptr(layer, 0);
     g.vpages = p->layer_ptr(layer, 1);
     g.sinks = a.sinks;
     g.scratch = p->scratch;
@@ -521,7 +599,7 @@ mkv_status pool_attn_f16_setup(Pool *p) {
     MKV_CUDA(cudaFuncSetAttribute(pool_attn_f16_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PaSizes<128>::SMEM));
     MKV_CUDA(cudaFuncSetAttribute(pool_attn_f16_kernel<256>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PaSizes<256>::SMEM));
     const uint64_t rows = (uint64_t)p->desc.n_pages * p->desc.page_tokens, cols = (uint64_t)p->desc.kv_heads * (uint64_t)p->desc.head_dim;
-    const uint32_t box_rows = std::min(p->desc.page_tokens, PA_KEYS);
+    const uint32_t box_rows = std::min(p->desc.page_tokens, p->desc.head_dim == 256 ? PaSizes<256>::V_KEYS : PA_KEYS);
     p->maps.resize(2 * (size_t)p->desc.n_layers);
     for (int l = 0; l < p->desc.n_layers; l++)
         for (int kv = 0; kv < 2; kv++) {

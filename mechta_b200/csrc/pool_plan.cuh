@@ -2,10 +2,11 @@
 //
 // An item is one KV head and a block of up to `block` tokens of a sequence (all query heads of the KV head for each: the rows of a
 // product); its work is the tiles of TILE_KEYS keys from the first key that any of its tokens sees to the last. The items of all sequences
-// (sequence by sequence, block by block, KV head by KV head) are laid end to end and cut into equal ranges of tiles, one a CTA, so that
-// decode steps over long histories and long blocks over short ones fill the GPU alike. A CTA's range is a few segments; a segment that
-// covers its whole item writes the output, another its un-normalised part, and the parts are merged in the order of their keys: sums do
-// not depend on timing.
+// (sequence by sequence, block by block, KV head by KV head) are laid end to end and cut into ranges of about the same cost, one a CTA,
+// so that decode steps over long histories and long blocks over short ones fill the GPU alike. A CTA's range is a few segments, each of
+// which costs as much as `segment` tiles beside its tiles (queries, the first tile's latency, outputs); a segment that covers its whole
+// item writes the output, another its un-normalised part, and the parts are merged in the order of their keys: sums do not depend on
+// timing.
 #pragma once
 #include "pool.cuh"
 
@@ -17,12 +18,12 @@ constexpr uint32_t PLAN_CTAS = 160;
 struct PlanSeq {
     uint32_t table, first, pos, ntok, row; // first entry of the page table; first key seen; ...; packed tokens in front
 };
-struct PlanStart { // where a CTA's range begins
+struct PlanStart { // where a CTA's range begins, and how many tiles it has
     uint16_t seq, kvh;
-    uint32_t block, tile; // tile: of the item
+    uint32_t block, tile, tiles; // tile: of the item
 };
 struct PoolPlan {
-    uint32_t nseq, ctas, len, total; // tiles of a range, of all items
+    uint32_t nseq, ctas;
     uint32_t kv_heads, group, block, window;
     PlanSeq seq[PLAN_SEQS];
     PlanStart start[PLAN_CTAS];
@@ -70,7 +71,7 @@ struct PlanWalk {
         kvh = s.kvh;
         block = s.block;
         tile = s.tile;
-        left = plan.total - cta * plan.len < plan.len ? plan.total - cta * plan.len : plan.len;
+        left = s.tiles;
     }
     __host__ __device__ __forceinline__ bool next(PlanSegment &s) {
         if (left == 0u) return false;
@@ -107,7 +108,11 @@ struct MergeList {
 
 // Plans one launch over the items [i, n) that it takes (i is moved on); rows: packed tokens in front of them, moved on too.
 // Returns false when no item with tokens is left.
-bool pool_plan(const Pool *p, const mkv_seq_rows *items, int n, int &i, uint32_t &rows, uint32_t window, uint32_t keys, PoolPlan &plan, MergeList &merge);
+struct PlanCost {
+    uint32_t keys;    // of a tile
+    uint32_t segment; // in tiles
+};
+bool pool_plan(const Pool *p, const mkv_seq_rows *items, int n, int &i, uint32_t &rows, uint32_t window, const PlanCost &cost, PoolPlan &plan, MergeList &merge);
 
 // The floats of a part in scratch memory: [128 rows][dim], then [128 rows][maximum, sum]; two parts a CTA
 __host__ __device__ inline size_t part_floats(uint32_t dim) { return 128u * (size_t)(dim + 2u); }
