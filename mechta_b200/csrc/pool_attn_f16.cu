@@ -23,8 +23,8 @@
 // only some of its tokens see are searched; one that is not finite is zeroed too and its share added to the rows that see it
 // with ordinary arithmetic.
 //
-// Roles (384 threads, three warpgroups whose register budgets are set with setmaxnreg): warp 0 = TMA producer, warp 1 = issues S = Q K^T
-// and owns the TMEM, warp 2 = issues O += P V (warp 3 idle), warps 4..11 = softmax. Every wait is bounded; TMEM is
+// Roles (384 threads, three warpgroups whose register budgets are set with setmaxnreg): warps 0 and 3 = TMA producers, warp 1 = issues
+// S = Q K^T and owns the TMEM, warp 2 = issues O += P V, warps 4..11 = softmax. Every wait is bounded; TMEM is
 // freed on every path.
 #include "pool_plan.cuh"
 #include "ptx.cuh"
@@ -168,59 +168,59 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
 
     // The units of the CTA's T tiles in ring order, whatever segment they belong to: K(0) .. K(LEAD - 1), then K(t + LEAD) and V(t) for
     // each t. In front of K(t) are t + max(t - LEAD, 0) tiles of K and V, in front of V(t) min(t + LEAD + 1, T) + t.
-    if (warp < 4u) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp == 0) {
-        // ---------------- TMA producer ----------------
-        const uint32_t page_tokens = 1u << g.page_shift, box_rows = min(page_tokens, Z::V_KEYS), nrb = PA_KEYS / box_rows, nrbv = Z::V_KEYS / box_rows;
-        const uint32_t rb = lane % nrb, cb = lane / nrb, rbv = lane % nrbv, cbv = lane / nrbv; // this lane's row box and 64-dim box of a unit
+    if (warp < 4u) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0 || warp == 3u) {
+        // ---------------- TMA producers: warp 0 loads K, warp 3 V (a page of 16 tokens is 2 KB a box: one warp issues too slowly) ----------------
+        const bool v = warp == 3u;
+        const uint32_t page_tokens = 1u << g.page_shift, box_rows = min(page_tokens, Z::V_KEYS); // of a box; a unit has 128 / box_rows or V_KEYS / box_rows
+        const uint32_t nrb = (v ? Z::V_KEYS : PA_KEYS) / box_rows, rb = lane % nrb, cb = lane / nrb; // this lane's row box and 64-dim box of a unit
+        const bool mine = cb < (v ? DIM / 64u : Z::BOXES);
+        const CUtensorMap *map = v ? &vmap : &kmap;
+        const uint32_t total = plan.start[blockIdx.x].tiles;
         PaRing<Z::NST> at;
-        uint32_t u = 0;
+        uint32_t u = 0; // units of K and V so far
+        if (v) {
+            u = min(Z::LEAD + 1u, total) * Z::NUN; // over the first tiles of K
+            at.next(u);
+        }
         TileStream ts(plan);
         struct Tile {
-            uint32_t row; // in the pool, of this lane's row box of K; ~0u where no token of the item sees a key of it
-            int x;        // first column of the head
-            bool is;
+            uint32_t row[Z::NUN]; // in the pool, of this lane's row box of each unit; ~0u where no token of the item sees a key of it
+            int x;                // first column of the head
         };
-        auto look_up = [&]() -> Tile { // the stream's tile; the stream moves on
-            Tile t = {~0u, 0, ts.more};
-            if (!ts.more) return t;
+        auto look_up = [&]() -> Tile { // the stream's tile, if there is one; the stream moves on
+            Tile t;
             const PlanItem &it = ts.sg.it;
-            const uint32_t key = (it.tile0 + ts.tile) * PA_KEYS + rb * box_rows;
-            if (lane < nrb * Z::BOXES && key + box_rows > it.lo && key < it.hi)
-                t.row = (__ldg(g.pages + plan.seq[ts.sg.seq].table + (key >> g.page_shift)) << g.page_shift) + (key & (page_tokens - 1u));
-            t.x = (int)(ts.sg.kvh * DIM);
-            ts.next();
+            const uint32_t *pages = g.pages + plan.seq[ts.sg.seq].table;
+#pragma unroll
+            for (uint32_t h = 0; h < Z::NUN; h++) {
+                const uint32_t key = (it.tile0 + ts.tile) * PA_KEYS + (v ? h * Z::V_KEYS : 0u) + rb * box_rows;
+                t.row[h] = ~0u;
+                if (ts.more && mine && key + box_rows > it.lo && key < it.hi) t.row[h] = (__ldg(pages + (key >> g.page_shift)) << g.page_shift) + (key & (page_tokens - 1u));
+            }
+            t.x = (int)(ts.sg.kvh * DIM + cb * 64u);
+            if (ts.more) ts.next();
             return t;
         };
-        auto load = [&](bool v, const Tile &t) -> bool { // the units of one K or V tile
+        Tile cur = look_up(); // a page is looked up a tile before it is wanted
+        bool ok = true;
+        for (uint32_t t = 0; ok && t < total; t++) {
+            const Tile ahead = look_up();
 #pragma unroll
             for (uint32_t h = 0; h < Z::NUN; h++, u++, at.next()) {
-                const uint32_t s = at.s, bar = bar_full + 8u * s;
-                // V: the lane has another row box; a lane of K holds its row
-                const uint32_t of_v = __shfl_sync(0xffffffffu, t.row, h * nrbv + rbv), row = !v ? t.row : cbv < DIM / 64u ? of_v : ~0u;
-                const uint32_t dst = ring + s * Z::UNIT + (v ? cbv * Z::V_BOX + rbv * box_rows * 128u : cb * Z::BOX + rb * box_rows * 128u);
-                const int x = t.x + (int)(v ? cbv * 64u : h * Z::UNIT_DIMS + cb * 64u);
-                if (u >= Z::NST && !__all_sync(0xffffffffu, pa_wait(bar_empty + 8u * s, at.turn ^ 1u, sh, g.status))) return false;
+                const uint32_t bar = bar_full + 8u * at.s, row = cur.row[h];
+                if (u >= Z::NST && !(ok = ok && __all_sync(0xffffffffu, pa_wait(bar_empty + 8u * at.s, at.turn ^ 1u, sh, g.status)))) break;
                 const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, row != ~0u));
                 if (lane == 0) mbar_expect_tx(bar, boxes * box_rows * 128u);
                 __syncwarp();
-                if (row != ~0u) tma_load_2d(dst, v ? &vmap : &kmap, x, (int)row, bar);
+                if (row != ~0u)
+                    tma_load_2d(ring + at.s * Z::UNIT + cb * (v ? Z::V_BOX : Z::BOX) + rb * box_rows * 128u, map, cur.x + (v ? 0 : (int)(h * Z::UNIT_DIMS)), (int)row, bar);
             }
-            return true;
-        };
-        Tile next[Z::LEAD + 2]; // tiles t .. t + LEAD + 1: a page is looked up a tile before it is wanted
-        bool ok = true;
-#pragma unroll
-        for (uint32_t i = 0; i <= Z::LEAD; i++) {
-            next[i] = look_up();
-            if (i < Z::LEAD && next[i].is) ok = ok && load(false, next[i]);
-        }
-        while (ok && next[0].is) {
-            next[Z::LEAD + 1] = look_up();
-            if (next[Z::LEAD].is) ok = load(false, next[Z::LEAD]);
-            ok = ok && load(true, next[0]);
-#pragma unroll
-            for (uint32_t i = 0; i <= Z::LEAD; i++) next[i] = next[i + 1];
+            cur = ahead;
+            if (v ? t + Z::LEAD + 1u < total : t + 1u > Z::LEAD) { // over the other's tile
+                at.next(Z::NUN);
+                u += Z::NUN;
+            }
         }
     } else if (warp == 1) {
         // ---------------- S = Q K^T ----------------
@@ -295,7 +295,7 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         }
     } else if (warp >= 4u) {
         // ---------------- softmax: two threads per row (TMEM lane), 64 keys of a tile and half of the dims of O each ----------------
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;"); // 128 x 72 + 256 x 216 = the launch's 384 x 168
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;"); // 128 x 56 + 256 x 224 = the launch's 384 x 168
         const uint32_t q4 = warp & 3u, half = (warp - 4u) >> 2;
         const uint32_t row = 32u * q4 + lane, st = tid - PA_SOFTMAX_TID0; // row: the TMEM lanes this warp may access
         const uint32_t lane_addr = (32u * q4) << 16;
@@ -314,28 +314,30 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         // The products of tile t have completed; for tiles since the newest scores that this warp has waited for. (A parity tells a phase from
         // its neighbours only; those scores were computed behind the products of NBUF tiles earlier.)
         auto wait_pv = [&](uint32_t t) { wait(bar_pv_done + 8u * (t % Z::NBUF), (t / Z::NBUF) & 1u); };
-        auto wait_s = [&](uint32_t t) { wait(bar_s_full + 8u * (t % Z::NBUF), (t / Z::NBUF) & 1u); };
-        // Q rows of this quarter, half of the dims; rows beyond the block as zeros where the quarter has rows of it. Fetched while the scores of
-        // the segment in front are still being computed, put into shared memory once they are.
-        constexpr uint32_t CPR = DIM / 16; // 16-byte chunks of a half row
-        constexpr uint32_t RPI = 32 / CPR; // rows of one access of the warp
-        uint4 qv[CPR];
-        auto fetch_q = [&](const PlanSegment &sg) {
+        // Q rows of this quarter, half of the dims; rows beyond the block as zeros where the quarter has rows of it. The first rows are fetched
+        // while the scores of the segment in front are still being computed; all go to shared memory once they are.
+        constexpr uint32_t CPR = DIM / 16;              // 16-byte chunks of a half row
+        constexpr uint32_t RPI = 32 / CPR;              // rows of one access of the warp
+        constexpr uint32_t QB = CPR < 8u ? CPR : 8u;    // accesses of a batch
+        uint4 qv[QB];
+        auto fetch_q = [&](const PlanSegment &sg, uint32_t b) {
             const uint32_t rows = sg.it.ntok * group;
             const __half *src = g.q + (int64_t)(plan.seq[sg.seq].row + sg.it.tok0) * g.q_stride + (size_t)sg.kvh * group * DIM + (half * CPR + lane % CPR) * 8u;
 #pragma unroll
-            for (uint32_t i = 0; i < CPR; i++) {
-                const uint32_t r = 32u * q4 + i * RPI + lane / CPR, t = r / group;
+            for (uint32_t i = 0; i < QB; i++) {
+                const uint32_t r = 32u * q4 + (b * QB + i) * RPI + lane / CPR, t = r / group;
                 qv[i] = make_uint4(0u, 0u, 0u, 0u);
                 if (r < rows) qv[i] = __ldg(reinterpret_cast<const uint4 *>(src + (int64_t)t * g.q_stride + (r - t * group) * DIM));
             }
         };
-        auto put_q = [&](const PlanSegment &sg) {
-            if (32u * q4 < sg.it.ntok * group) {
-                const uint32_t c = half * CPR + lane % CPR; // chunk of the row
+        auto put_q = [&](const PlanSegment &sg) { // the first batch has been fetched
+            const uint32_t c = half * CPR + lane % CPR; // chunk of the row
+#pragma unroll 1
+            for (uint32_t b = 0; b < CPR / QB && 32u * q4 < sg.it.ntok * group; b++) {
+                if (b > 0u) fetch_q(sg, b);
 #pragma unroll
-                for (uint32_t i = 0; i < CPR; i++)
-                    *reinterpret_cast<uint4 *>(smem + (c >> 3) * 16384u + swz128(32u * q4 + i * RPI + lane / CPR, c & 7u)) = qv[i];
+                for (uint32_t i = 0; i < QB; i++)
+                    *reinterpret_cast<uint4 *>(smem + (c >> 3) * 16384u + swz128(32u * q4 + (b * QB + i) * RPI + lane / CPR, c & 7u)) = qv[i];
             }
             fence_proxy_async();
             arrive(bar_q_full);
@@ -345,8 +347,18 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         PlanWalk walk(plan, blockIdx.x, PA_KEYS);
         PlanSegment sg, nx;
         bool more = walk.next(sg);
-        fetch_q(sg);
+        fetch_q(sg, 0);
         put_q(sg);
+        // The weights of a tile are handed over (finish) when the loads of the next tile's scores are on their way, if those are there.
+        PaRing<Z::NBUF> buf;
+        uint32_t owed = 0; // the p_full barrier of a tile whose weights are not handed over yet
+        auto finish = [&]() {
+            if (owed == 0u) return;
+            tmem_wait_st();
+            tc_fence_before();
+            arrive(owed);
+            owed = 0;
+        };
         // A wait that runs out makes all later ones return at once; the warps go through the same barriers all the same, so that none waits
         // for one that has left.
         while (more) {
@@ -360,12 +372,23 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             float m_ref = NEG_BIG, l = 0.0f; // l: this thread's keys only
             const uint32_t end = t0 + (sg.b - sg.a);
             more = walk.next(nx);
-            for (uint32_t t = t0; t < end; t++) {
-                const uint32_t key0 = (it.tile0 + sg.a + (t - t0)) * PA_KEYS, s_col = tmem + lane_addr + Z::COL_S + 128u * (t % Z::NBUF) + 64u * half;
+            for (uint32_t t = t0; t < end; t++, buf.next()) {
+                const uint32_t key0 = (it.tile0 + sg.a + (t - t0)) * PA_KEYS, s_col = tmem + lane_addr + Z::COL_S + 128u * buf.s + 64u * half;
                 const bool edge = key0 < it.all_lo || key0 + PA_KEYS > it.all_hi; // some row does not see some key
                 const bool last = t + 1u == end && more;
-                if (last) fetch_q(nx);
-                wait_s(t);
+                if (last) fetch_q(nx, 0);
+                const uint32_t bar_s = bar_s_full + 8u * buf.s;
+                if (!__all_sync(0xffffffffu, mbar_test(bar_s, buf.turn))) {
+                    finish();
+                    wait(bar_s, buf.turn);
+                }
+                tc_fence_after();
+                uint32_t sr[2][32];
+                if (active) {
+                    tmem_ld32(s_col, sr[0]);
+                    tmem_ld32(s_col + 32u, sr[1]);
+                }
+                finish();
                 if (last) put_q(nx); // the segment's scores are all there: its Q may go
                 bool bad_any = false;
                 if (edge) { // (the same for the eight warps)
@@ -402,9 +425,6 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                     fence_proxy_async();
                 }
                 if (active) {
-                    uint32_t sr[2][32];
-                    tmem_ld32(s_col, sr[0]);
-                    tmem_ld32(s_col + 32u, sr[1]);
                     tmem_wait_ld();
                     // work in base-2 exponents: e^(s scale - m) = 2^(s C - m2), C = scale log2(e)
                     float mt[4] = {NEG_BIG, NEG_BIG, NEG_BIG, NEG_BIG};
@@ -486,16 +506,15 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                             tmem_st32(tmem + lane_addr + c0, orow);
                         }
                     }
-                    tmem_wait_st();
                 }
                 if (bad_any) {
                     named_bar_sync(5, 256);
                     if (st < 4u) sh->bad[t & 1u][st] = 0u; // (used again two tiles on, behind this tile's p_full)
                     if (t == t0 && st == 0u) sh->keep = t + 1u; // what was put into O stays
                 }
-                tc_fence_before();
-                arrive(bar_p_full + 8u * (t % Z::NBUF));
+                owed = bar_p_full + 8u * buf.s;
             }
+            finish();
             // ---------------- end of the segment ----------------
             wait_pv(end - 1u); // (the next segment's first scores are computed meanwhile)
             if (active) {
