@@ -474,8 +474,10 @@ mkv_status mkv_attn_pool(mkv_pool *h, int layer, const mkv_seq_rows *items, int 
     if (st != MKV_OK) return st;
     for (int i = 0; i < n; i++) {
         if ((st = p->book.need(items[i].seq)) != MKV_OK) return st;
-        // tiles of the launch are counted in 31 bits: an item's blocks of at least one token, times its KV heads, times its tiles
-        if (((uint64_t)items[i].ntok * (uint64_t)p->desc.q_heads / 64u + (uint64_t)p->desc.kv_heads) * (((uint64_t)items[i].pos + items[i].ntok) / 128u + 2u) > 0x7fffffffull) {
+        // tiles of the launch are counted in 31 bits: an item's blocks (of 128 rows and keys, f32 64) times its KV heads times its tiles
+        const uint64_t side = p->desc.fmt == MKV_F16 ? 128u : 64u;
+        if (((uint64_t)items[i].ntok * (uint64_t)p->desc.q_heads / (side / 2u) + (uint64_t)p->desc.kv_heads) *
+                (((uint64_t)items[i].pos + items[i].ntok) / side + 2u) > 0x7fffffffull) {
             set_error("item %d: %u tokens at %u are too many for one call", i, items[i].ntok, items[i].pos);
             return MKV_ERR_INVALID;
         }

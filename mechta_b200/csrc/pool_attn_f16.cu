@@ -39,7 +39,7 @@ constexpr long long PA_WAIT_LIMIT = 2000000000ll;
 constexpr float PA_LOG2E = 1.4426950408889634f;
 constexpr float PA_LAZY2 = 8.0f * PA_LOG2E;
 
-template <int DIM> struct PaSizes {
+template <int DIM> struct PaSizes { // (the tensor maps' boxes go by V_KEYS)
     static constexpr uint32_t UNIT_DIMS = DIM < 128 ? DIM : 128;
     static constexpr uint32_t NUN = DIM / UNIT_DIMS;             // units of a K or V tile
     static constexpr uint32_t BOXES = UNIT_DIMS / 64;            // 64-dim boxes of a unit
@@ -145,7 +145,10 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     PaShared *sh = reinterpret_cast<PaShared *>(smem + Z::OFF_MISC);
 
     if (tid == 0) {
-        for (uint32_t s = 0; s < 2u * Z::NST; s++) mbar_init(bar0 + 8u * s, 1);
+        for (uint32_t s = 0; s < Z::NST; s++) {
+            mbar_init(bar_full + 8u * s, 2); // one arrival per producer
+            mbar_init(bar_empty + 8u * s, 1);
+        }
         for (uint32_t s = 0; s < Z::NBUF; s++) {
             mbar_init(bar_s_full + 8u * s, 1);
             mbar_init(bar_p_full + 8u * s, 8); // one arrival per softmax warp
@@ -170,57 +173,63 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     // each t. In front of K(t) are t + max(t - LEAD, 0) tiles of K and V, in front of V(t) min(t + LEAD + 1, T) + t.
     if (warp < 4u) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0 || warp == 3u) {
-        // ---------------- TMA producers: warp 0 loads K, warp 3 V (a page of 16 tokens is 2 KB a box: one warp issues too slowly) ----------------
-        const bool v = warp == 3u;
-        const uint32_t page_tokens = 1u << g.page_shift, box_rows = min(page_tokens, Z::V_KEYS); // of a box; a unit has 128 / box_rows or V_KEYS / box_rows
-        const uint32_t nrb = (v ? Z::V_KEYS : PA_KEYS) / box_rows, rb = lane % nrb, cb = lane / nrb; // this lane's row box and 64-dim box of a unit
-        const bool mine = cb < (v ? DIM / 64u : Z::BOXES);
-        const CUtensorMap *map = v ? &vmap : &kmap;
-        const uint32_t total = plan.start[blockIdx.x].tiles;
+        // ---------------- TMA producers: every other box of each unit (a page of 16 tokens is 2 KB a box: one warp issues too slowly) ----------------
+        // Both go through all units in order: a parity tells a phase from its neighbours only, so whoever waits for a slot has to have
+        // waited for its uses before.
+        const uint32_t page_tokens = 1u << g.page_shift, box_rows = min(page_tokens, Z::V_KEYS), nrb = PA_KEYS / box_rows, nrbv = Z::V_KEYS / box_rows;
+        const uint32_t box = 2u * lane + (warp == 0 ? 0u : 1u), rb = box % nrb, cb = box / nrb, rbv = box % nrbv, cbv = box / nrbv; // this lane's of a unit of K, of V
         PaRing<Z::NST> at;
-        uint32_t u = 0; // units of K and V so far
-        if (v) {
-            u = min(Z::LEAD + 1u, total) * Z::NUN; // over the first tiles of K
-            at.next(u);
-        }
+        uint32_t u = 0;
         TileStream ts(plan);
         struct Tile {
-            uint32_t row[Z::NUN]; // in the pool, of this lane's row box of each unit; ~0u where no token of the item sees a key of it
-            int x;                // first column of the head
+            uint32_t k_row, v_row[Z::NUN]; // in the pool, of this lane's boxes; ~0u where no token of the item sees a key of it
+            int x;                         // first column of the head
+            bool is;
         };
-        auto look_up = [&]() -> Tile { // the stream's tile, if there is one; the stream moves on
+        auto look_up = [&]() -> Tile { // the stream's tile; the stream moves on
             Tile t;
+            t.is = ts.more;
             const PlanItem &it = ts.sg.it;
+            const uint32_t key0 = (it.tile0 + ts.tile) * PA_KEYS;
             const uint32_t *pages = g.pages + plan.seq[ts.sg.seq].table;
+            auto row = [&](bool mine, uint32_t key) {
+                if (!mine || key + box_rows <= it.lo || key >= it.hi) return ~0u;
+                return (__ldg(pages + (key >> g.page_shift)) << g.page_shift) + (key & (page_tokens - 1u));
+            };
+            t.k_row = row(t.is && cb < Z::BOXES, key0 + rb * box_rows);
 #pragma unroll
-            for (uint32_t h = 0; h < Z::NUN; h++) {
-                const uint32_t key = (it.tile0 + ts.tile) * PA_KEYS + (v ? h * Z::V_KEYS : 0u) + rb * box_rows;
-                t.row[h] = ~0u;
-                if (ts.more && mine && key + box_rows > it.lo && key < it.hi) t.row[h] = (__ldg(pages + (key >> g.page_shift)) << g.page_shift) + (key & (page_tokens - 1u));
-            }
-            t.x = (int)(ts.sg.kvh * DIM + cb * 64u);
-            if (ts.more) ts.next();
+            for (uint32_t h = 0; h < Z::NUN; h++) t.v_row[h] = row(t.is && cbv < DIM / 64u, key0 + h * Z::V_KEYS + rbv * box_rows);
+            t.x = (int)(ts.sg.kvh * DIM);
+            if (t.is) ts.next();
             return t;
         };
-        Tile cur = look_up(); // a page is looked up a tile before it is wanted
-        bool ok = true;
-        for (uint32_t t = 0; ok && t < total; t++) {
-            const Tile ahead = look_up();
+        auto load = [&](bool v, const Tile &t) -> bool { // the units of one K or V tile
 #pragma unroll
             for (uint32_t h = 0; h < Z::NUN; h++, u++, at.next()) {
-                const uint32_t bar = bar_full + 8u * at.s, row = cur.row[h];
-                if (u >= Z::NST && !(ok = ok && __all_sync(0xffffffffu, pa_wait(bar_empty + 8u * at.s, at.turn ^ 1u, sh, g.status)))) break;
+                const uint32_t bar = bar_full + 8u * at.s, row = v ? t.v_row[h] : t.k_row;
+                if (u >= Z::NST && !__all_sync(0xffffffffu, pa_wait(bar_empty + 8u * at.s, at.turn ^ 1u, sh, g.status))) return false;
                 const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, row != ~0u));
                 if (lane == 0) mbar_expect_tx(bar, boxes * box_rows * 128u);
                 __syncwarp();
                 if (row != ~0u)
-                    tma_load_2d(ring + at.s * Z::UNIT + cb * (v ? Z::V_BOX : Z::BOX) + rb * box_rows * 128u, map, cur.x + (v ? 0 : (int)(h * Z::UNIT_DIMS)), (int)row, bar);
+                    tma_load_2d(ring + at.s * Z::UNIT + (v ? cbv * Z::V_BOX + rbv * box_rows * 128u : cb * Z::BOX + rb * box_rows * 128u), v ? &vmap : &kmap,
+                                t.x + (int)(v ? cbv * 64u : h * Z::UNIT_DIMS + cb * 64u), (int)row, bar);
             }
-            cur = ahead;
-            if (v ? t + Z::LEAD + 1u < total : t + 1u > Z::LEAD) { // over the other's tile
-                at.next(Z::NUN);
-                u += Z::NUN;
-            }
+            return true;
+        };
+        Tile next[Z::LEAD + 2]; // tiles t .. t + LEAD + 1: a page is looked up a tile before it is wanted
+        bool ok = true;
+#pragma unroll
+        for (uint32_t i = 0; i <= Z::LEAD; i++) {
+            next[i] = look_up();
+            if (i < Z::LEAD && next[i].is) ok = ok && load(false, next[i]);
+        }
+        while (ok && next[0].is) {
+            next[Z::LEAD + 1] = look_up();
+            if (next[Z::LEAD].is) ok = load(false, next[Z::LEAD]);
+            ok = ok && load(true, next[0]);
+#pragma unroll
+            for (uint32_t i = 0; i <= Z::LEAD; i++) next[i] = next[i + 1];
         }
     } else if (warp == 1) {
         // ---------------- S = Q K^T ----------------
@@ -613,18 +622,10 @@ mkv_status launch_pool_attn_f16(Pool *p, int layer, const PoolPlan &plan, const 
     }
 }
 
-mkv_status pool_attn_f16_setup(Pool *p) {
+mkv_status pool_attn_f16_setup(Pool *) {
     MKV_CUDA(cudaFuncSetAttribute(pool_attn_f16_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PaSizes<64>::SMEM));
     MKV_CUDA(cudaFuncSetAttribute(pool_attn_f16_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PaSizes<128>::SMEM));
     MKV_CUDA(cudaFuncSetAttribute(pool_attn_f16_kernel<256>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PaSizes<256>::SMEM));
-    const uint64_t rows = (uint64_t)p->desc.n_pages * p->desc.page_tokens, cols = (uint64_t)p->desc.kv_heads * (uint64_t)p->desc.head_dim;
-    const uint32_t box_rows = std::min(p->desc.page_tokens, p->desc.head_dim == 256 ? PaSizes<256>::V_KEYS : PA_KEYS);
-    p->maps.resize(2 * (size_t)p->desc.n_layers);
-    for (int l = 0; l < p->desc.n_layers; l++)
-        for (int kv = 0; kv < 2; kv++) {
-            const mkv_status st = make_tensor_map(&p->maps[2 * (size_t)l + (size_t)kv], MKV_F16, p->layer_ptr(l, kv), rows, cols, box_rows);
-            if (st != MKV_OK) return st;
-        }
     return MKV_OK;
 }
 

@@ -1,0 +1,718 @@
+// Attention of blocks of new tokens over f32 pages on the 5th-generation tensor cores, with f32-grade arithmetic.
+//   out_t = sum_k e^(s_k - M) v_k / (sum_k e^(s_k - M) + e^(sink - M)),  s_k = scale q_t . k_k
+//
+// Every f32 operand is scaled by a power of two and split into two f16 values, hi = f16(x), lo = f16(x - hi): 22 bits. An item is up
+// to 64 rows (the query heads of one KV head for 64 / group tokens, row = token * group + head); the 128 rows of a product are the
+// rows' hi parts and, 64 further, their lo parts, so that two products with the hi and the lo tile give all four partial products:
+//   S'[r], S'[64 + r]   = (Q hi, Q lo) (K hi + K lo)^T      A = Q' (tensor memory), B = the converted K tile (K-major)
+//   O'[r], O'[64 + r]   = (P hi, P lo) (V hi + V lo)        A = P' (shared memory), B = the converted V tile (N-major)
+// and a score or an output is the sum of two rows. The tensor core's f32 sums truncate, so a long chain of them drifts (2^-24 a step,
+// all in one direction): the O' of every tile of 64 keys starts from zero and is folded into O in registers with a rounded FMA, which
+// also takes the rescale by the running maximum and the scale of the V tile.
+//
+// Conversion in place: TMA brings a tile as blocks of [64 keys][32 dims] (rows of 128 bytes, 128-byte swizzle); two lanes read the 256
+// bytes that a key has in two neighbouring blocks and write its 64 hi values into the first block's row and its 64 lo values into the
+// second's, so a tile needs no second buffer. The scale of a tile (K and V each their own) is the one in front's as long as the
+// tile's largest finite value then lies in [2^8, 2^15); otherwise the tile is converted once more, from global memory, with its own
+// scale: no f32 value overflows, and what is lost of a value is 2^-23 of it, or 2^-33 of the tile's
+// largest. Values that are not finite are zero in the
+// operands; their keys are noted, and the softmax threads add their share with ordinary arithmetic for the rows that see them. Keys
+// that no token of the item sees are zero as well, whatever lies in their rows.
+//
+// Bound by HBM for few rows (a 64-key tile of 256 dims is 128 KB, 5,600 clocks of an SM's share of 6.4 TB/s, and about 2,600 of
+// products), by the chain softmax - products - fold for long blocks.
+//
+// Roles (512 threads, four warpgroups whose register budgets are set with setmaxnreg): warps 0 and 3 = TMA producers, warp 1 =
+// issues S' and owns the TMEM, warp 2 = issues O', warps 4..7 = converters, warps 8..15 = softmax and owners of O: two threads per TMEM
+// lane, 32 of a tile's keys and half of the dims each. TMEM: O' = columns 0 .. DIM - 1, S' = 256 .. 319 and 320 .. 383, Q' = 384 ...
+// Every wait is bounded; TMEM is freed on every path.
+#include "pool_plan.cuh"
+#include "ptx.cuh"
+
+namespace mkv {
+using namespace ptx;
+
+constexpr uint32_t PF_KEYS32 = 64, PF_ROWS32 = 64;
+constexpr int PB_THREADS = 512;
+constexpr uint32_t PB_CONV_TID0 = 128, PB_SOFT_TID0 = 256;
+constexpr long long PB_WAIT_LIMIT = 2000000000ll;
+constexpr float PB_LOG2E = 1.4426950408889634f;
+constexpr uint32_t PB_COL_S = 256, PB_COL_Q = 384;
+constexpr uint32_t PB_BLK = 8192;          // [64 keys][32 dims] f32, then [64 keys][64 dims] f16
+constexpr uint32_t PB_UNIT = 2 * PB_BLK;   // 64 dims of a tile
+constexpr uint32_t PB_NST = 12;            // units of the ring: a multiple of a tile's, so that a tile lies in one piece
+constexpr uint32_t PB_OFF_P = PB_NST * PB_UNIT; // P' [128 rows][64 keys] f16; also where S'[64 + r] changes hands
+constexpr uint32_t PB_OFF_RED = PB_OFF_P + 16384; // [2 halves][64 rows] floats, [64 rows] rescale factors, [64 rows] reference maxima
+constexpr uint32_t PB_OFF_BAR = PB_OFF_RED + 1024;
+constexpr uint32_t PB_NBAR = 3 * PB_NST + 7; // full[NST], empty[NST], conv[NST], s_full[2], s_free[2], p_full, pv_done, q_full
+constexpr uint32_t PB_OFF_MISC = PB_OFF_BAR + PB_NBAR * 8;
+constexpr uint32_t PB_NOTES = 16;          // tiles whose scale and notes are kept: more than the ring holds
+
+struct PbShared {
+    uint32_t tmem_base;
+    volatile uint32_t abort;
+    uint32_t amax[4];                 // of each converter warp
+    float unscale[2][PB_NOTES];       // [K, V][tile]
+    uint16_t odd[2][PB_NOTES][4];     // keys with a value that is not finite, 16 of each converter warp
+};
+constexpr uint32_t PB_SMEM = PB_OFF_MISC + sizeof(PbShared) + 1024;
+static_assert(PB_SMEM <= 232448, "shared memory");
+
+struct PbArgs {
+    const float *q;
+    float *out;
+    int64_t q_stride, out_stride;
+    const uint32_t *pages;
+    const float *kpages, *vpages;
+    const float *sinks;
+    float *scratch;
+    uint32_t *status;
+    size_t row_floats;
+    float scale2; // scale * log2(e)
+    uint32_t page_shift;
+};
+
+__device__ __forceinline__ bool pb_wait(uint32_t bar, uint32_t parity, PbShared *sh, uint32_t *status) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+    for (;;) {
+        if (sh->abort) return false;
+#pragma unroll 1
+        for (int i = 0; i < 64; i++)
+            if (mbar_try_wait(bar, parity)) return true;
+        if (clock64() - t0 > PB_WAIT_LIMIT) break;
+    }
+    sh->abort = 1;
+    atomicOr(status, DEV_ERR_WAIT_TIMEOUT);
+    return false;
+}
+// A place of a ring of N and the parity of its current use
+template <uint32_t N> struct PbRing {
+    uint32_t s = 0, turn = 0;
+    __device__ __forceinline__ void next(uint32_t d = 1u) { // d <= N
+        s += d;
+        if (s >= N) {
+            s -= N;
+            turn ^= 1u;
+        }
+    }
+};
+// The tiles of a CTA's segments as one stream
+struct PbStream {
+    PlanWalk walk;
+    PlanSegment sg;
+    uint32_t tile;
+    bool more;
+    __device__ __forceinline__ PbStream(const PoolPlan &plan) : walk(plan, blockIdx.x, PF_KEYS32) { step(); }
+    __device__ __forceinline__ void step() {
+        more = walk.next(sg);
+        tile = sg.a;
+    }
+    __device__ __forceinline__ bool first() const { return tile == sg.a; }
+    __device__ __forceinline__ void next() {
+        if (++tile == sg.b) step();
+    }
+};
+__device__ __forceinline__ bool is_finite_bits(uint32_t b) { return (b & 0x7f800000u) != 0x7f800000u; }
+// The power of two that brings `amax` (its bits; finite) to [2^13, 2^14)
+__device__ __forceinline__ uint32_t scale_bits(uint32_t amax) {
+    const int e = (int)(amax >> 23) - 127;
+    return (uint32_t)(min(13 - e, 126) + 127) << 23;
+}
+// 2 x 8 values to their hi and lo parts
+__device__ __forceinline__ void split8(const float (&x)[8], uint4 &hi, uint4 &lo) {
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const __half2 a = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        const float2 f = __half22float2(a);
+        const __half2 b = __floats2half2_rn(x[2 * i] - f.x, x[2 * i + 1] - f.y);
+        h[i] = *reinterpret_cast<const uint32_t *>(&a);
+        l[i] = *reinterpret_cast<const uint32_t *>(&b);
+    }
+    hi = make_uint4(h[0], h[1], h[2], h[3]);
+    lo = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
+template <int DIM>
+__global__ void __launch_bounds__(PB_THREADS, 1)
+pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PoolPlan plan,
+                     const __grid_constant__ PbArgs g) {
+    constexpr uint32_t NU = DIM / 64; // units of a tile
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *smem = smem_raw + (smem_base - smem_u32(smem_raw));
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    const uint32_t bar0 = smem_base + PB_OFF_BAR;
+    const uint32_t bar_full = bar0, bar_empty = bar0 + 8u * PB_NST, bar_conv = bar0 + 16u * PB_NST, bar_s_full = bar0 + 24u * PB_NST;
+    const uint32_t bar_s_free = bar_s_full + 16u, bar_p_full = bar_s_free + 16u, bar_pv_done = bar_p_full + 8u, bar_q_full = bar_pv_done + 8u;
+    PbShared *sh = reinterpret_cast<PbShared *>(smem + PB_OFF_MISC);
+
+    if (tid == 0) {
+        for (uint32_t s = 0; s < PB_NST; s++) {
+            mbar_init(bar_full + 8u * s, 2); // one arrival per producer
+            mbar_init(bar_empty + 8u * s, 1);
+            mbar_init(bar_conv + 8u * s, 4); // one arrival per converter warp
+        }
+        for (uint32_t s = 0; s < 2u; s++) {
+            mbar_init(bar_s_full + 8u * s, 1);
+            mbar_init(bar_s_free + 8u * s, 8); // one arrival per softmax warp
+        }
+        mbar_init(bar_p_full, 8);
+        mbar_init(bar_pv_done, 1);
+        mbar_init(bar_q_full, 8);
+        sh->abort = 0;
+        fence_barrier_init();
+        fence_proxy_async();
+    }
+    if (warp == 1) tmem_alloc(smem_base + PB_OFF_MISC, 512); // writes sh->tmem_base
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh->tmem_base, total = plan.start[blockIdx.x].tiles;
+    pdl_wait(); // nothing global is touched before the kernel in front has finished
+    pdl_launch_dependents();
+
+    // The units of the CTA's T tiles in ring order, whatever segment they belong to: K(0), then K(t + 1) and V(t) for each t. In front of
+    // K(t) are t + max(t - 1, 0) tiles of K and V, in front of V(t) min(t + 2, T) + t.
+    if (warp < 4u) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        if (warp == 0 || warp == 3u) {
+            // ---------------- TMA producers: every other box of each unit ----------------
+            // Both go through all units in order: a parity tells a phase from its neighbours only, so whoever waits for a slot has to have
+            // waited for its uses before.
+            const uint32_t page_tokens = 1u << g.page_shift, box_rows = min(page_tokens, PF_KEYS32), nrb = PF_KEYS32 / box_rows;
+            const uint32_t box = 2u * lane + (warp == 0 ? 0u : 1u), rb = box % nrb, cb = box / nrb; // this lane's row box and 32-dim box of a unit
+            PbRing<PB_NST> at;
+            uint32_t u = 0;
+            PbStream ts(plan);
+            struct Tile {
+                uint32_t row; // in the pool, of this lane's box; ~0u where no token of the item sees a key of it
+                int x;        // first column of the head
+                bool is;
+            };
+            auto look_up = [&]() -> Tile { // the stream's tile; the stream moves on
+                Tile t = {~0u, (int)(ts.sg.kvh * DIM + cb * 32u), ts.more};
+                const PlanItem &it = ts.sg.it;
+                const uint32_t key = (it.tile0 + ts.tile) * PF_KEYS32 + rb * box_rows;
+                if (t.is && cb < 2u && key + box_rows > it.lo && key < it.hi)
+                    t.row = (__ldg(g.pages + plan.seq[ts.sg.seq].table + (key >> g.page_shift)) << g.page_shift) + (key & (page_tokens - 1u));
+                if (t.is) ts.next();
+                return t;
+            };
+            auto load = [&](const CUtensorMap *map, const Tile &t) -> bool { // the units of one K or V tile
+                const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, t.row != ~0u));
+#pragma unroll 1
+                for (uint32_t h = 0; h < NU; h++, u++, at.next()) {
+                    const uint32_t bar = bar_full + 8u * at.s;
+                    if (u >= PB_NST && !__all_sync(0xffffffffu, pb_wait(bar_empty + 8u * at.s, at.turn ^ 1u, sh, g.status))) return false;
+                    if (lane == 0) mbar_expect_tx(bar, boxes * box_rows * 128u);
+                    __syncwarp();
+                    if (t.row != ~0u)
+                        tma_load_2d(smem_base + at.s * PB_UNIT + cb * PB_BLK + rb * box_rows * 128u, map, t.x + (int)(64u * h), (int)t.row, bar);
+                }
+                return true;
+            };
+            Tile cur = look_up(), ahead = look_up();
+            bool ok = load(&kmap, cur);
+            while (ok && cur.is) {
+                const Tile later = look_up(); // (its page is there when its turn comes)
+                if (ahead.is) ok = load(&kmap, ahead);
+                ok = ok && load(&vmap, cur);
+                cur = ahead;
+                ahead = later;
+            }
+        } else if (warp == 1) {
+            // ---------------- S' = Q' (K hi + K lo)^T ----------------
+            if (lane == 0) {
+                constexpr uint32_t IDESC = tc_idesc_f16(128, 64, false);
+                const uint64_t k_desc = tc_desc_sw128(smem_base, 16, 1024);
+                PbRing<PB_NST> at;
+                uint32_t nseg = 0;
+                bool ok = true;
+                PbStream ts(plan);
+                for (uint32_t t = 0; ok && ts.more; t++) {
+                    if (ts.first()) { // the segment's Q' is in tensor memory
+                        ok = pb_wait(bar_q_full, nseg & 1u, sh, g.status);
+                        nseg++;
+                    }
+                    if (t >= 2u) ok = ok && pb_wait(bar_s_free + 8u * (t & 1u), ((t >> 1) - 1u) & 1u, sh, g.status);
+                    const uint32_t d = tmem + PB_COL_S + 64u * (t & 1u);
+#pragma unroll
+                    for (uint32_t h = 0; h < NU; h++) {
+                        ok = ok && pb_wait(bar_conv + 8u * at.s, at.turn, sh, g.status);
+                        tc_fence_after();
+                        const uint64_t kd = k_desc + at.s * (PB_UNIT >> 4);
+#pragma unroll
+                        for (uint32_t ks = 0; ks < 8u; ks++) // 16 dims an MMA, hi and lo
+                            tc_mma_f16_ta(d, tmem + PB_COL_Q + 32u * h + 8u * (ks >> 1), kd + (((ks & 1u) * PB_BLK + (ks >> 1) * 32u) >> 4), IDESC,
+                                          (h > 0 || ks > 0) ? 1u : 0u);
+                        tc_commit(bar_empty + 8u * at.s);
+                        at.next();
+                    }
+                    tc_commit(bar_s_full + 8u * (t & 1u));
+                    if (t > 0u) at.next(NU); // over a tile of V
+                    ts.next();
+                }
+            }
+        } else {
+            // ---------------- O' = P' (V hi + V lo) ----------------
+            if (lane == 0) {
+                constexpr uint32_t IDESC = tc_idesc_f16(128, DIM, true);
+                const uint64_t v_desc = tc_desc_sw128(smem_base, PB_UNIT, 1024), p_desc = tc_desc_sw128(smem_base + PB_OFF_P, 16, 1024);
+                PbRing<PB_NST> at;
+                at.next(min(2u, total) * NU);
+                bool ok = true;
+                for (uint32_t t = 0; ok && t < total; t++) {
+                    const uint32_t s0 = at.s;
+#pragma unroll
+                    for (uint32_t h = 0; h < NU; h++, at.next()) ok = ok && pb_wait(bar_conv + 8u * at.s, at.turn, sh, g.status);
+                    ok = ok && pb_wait(bar_p_full, t & 1u, sh, g.status);
+                    tc_fence_after();
+                    const uint64_t vd = v_desc + s0 * (PB_UNIT >> 4);
+#pragma unroll
+                    for (uint32_t ks = 0; ks < 8u; ks++) // 16 keys an MMA, hi and lo
+                        tc_mma_f16(tmem, p_desc + (((ks >> 1) * 32u) >> 4), vd + (((ks & 1u) * PB_BLK + (ks >> 1) * 2048u) >> 4), IDESC, ks > 0 ? 1u : 0u);
+#pragma unroll
+                    for (uint32_t h = 0; h < NU; h++) tc_commit(bar_empty + 8u * (s0 + h));
+                    tc_commit(bar_pv_done);
+                    if (t + 2u < total) at.next(NU); // over a tile of K
+                }
+            }
+        }
+    } else if (warp < 8u) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        // ---------------- converters: a warp has 16 keys of every unit, a lane one of a key's two blocks ----------------
+        const uint32_t cw = warp - 4u, key_in = 16u * cw + (lane >> 1), j = lane & 1u;
+        PbRing<PB_NST> at;
+        struct Tile {
+            uint32_t key0, lo, hi, table, kvh;
+        };
+        PbStream ts(plan);
+        auto take = [&]() -> Tile { // the stream's tile; the stream moves on
+            const PlanItem &it = ts.sg.it;
+            const Tile t = {(it.tile0 + ts.tile) * PF_KEYS32, it.lo, it.hi, plan.seq[ts.sg.seq].table, ts.sg.kvh};
+            ts.next();
+            return t;
+        };
+        float k_scale = 1.0f, v_scale = 1.0f;
+        auto convert = [&](bool v, const Tile &tl, uint32_t note) {
+            const uint32_t key = tl.key0 + key_in;
+            const bool in = key >= tl.lo && key < tl.hi;
+            const PbRing<PB_NST> begin = at;
+            uint32_t amax = 0u;
+            bool odd = false;
+            float s = v ? v_scale : k_scale;
+            auto put = [&](uint32_t slot, uint32_t (&w)[8][4], bool look) { // 32 values of this lane to hi and lo
+                uint8_t *u = smem + slot * PB_UNIT;
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; i++)
+#pragma unroll
+                    for (uint32_t e = 0; e < 4u; e++) {
+                        const bool fine = is_finite_bits(w[i][e]);
+                        if (look) {
+                            odd = odd || !fine;
+                            amax = max(amax, fine ? w[i][e] & 0x7fffffffu : 0u);
+                        }
+                        w[i][e] = fine ? __float_as_uint(__uint_as_float(w[i][e]) * s) : 0u;
+                    }
+#pragma unroll
+                for (uint32_t c = 0; c < 4u; c++) { // 8 values: a 16-byte chunk of hi, one of lo
+                    float x[8];
+#pragma unroll
+                    for (uint32_t e = 0; e < 8u; e++) x[e] = __uint_as_float(w[2 * c + (e >> 2)][e & 3u]);
+                    uint4 hi, lo;
+                    split8(x, hi, lo);
+                    *reinterpret_cast<uint4 *>(u + swz128(key_in, 4u * j + c)) = hi;
+                    *reinterpret_cast<uint4 *>(u + PB_BLK + swz128(key_in, 4u * j + c)) = lo;
+                }
+            };
+#pragma unroll 1
+            for (uint32_t h = 0; h < NU; h++, at.next()) {
+                pb_wait(bar_full + 8u * at.s, at.turn, sh, g.status);
+                __syncwarp();
+                const uint8_t *u = smem + at.s * PB_UNIT + j * PB_BLK;
+                uint32_t w[8][4];
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; i++) { // (the two blocks' lanes in another order, so that they meet no bank together)
+                    const uint4 a = *reinterpret_cast<const uint4 *>(u + swz128(key_in, i ^ (4u * j)));
+                    const bool ok = in;
+                    w[i][0] = ok ? a.x : 0u; w[i][1] = ok ? a.y : 0u; w[i][2] = ok ? a.z : 0u; w[i][3] = ok ? a.w : 0u;
+                }
+                if (j) { // back into order
+#pragma unroll
+                    for (uint32_t i = 0; i < 4u; i++)
+#pragma unroll
+                        for (uint32_t e = 0; e < 4u; e++) {
+                            const uint32_t x = w[i][e];
+                            w[i][e] = w[i + 4u][e];
+                            w[i + 4u][e] = x;
+                        }
+                }
+                __syncwarp(); // both lanes of a key have read its rows
+                put(at.s, w, true);
+            }
+            // the tile's largest value and the keys with values that are not finite
+            amax = __reduce_max_sync(0xffffffffu, amax);
+            const uint32_t odds = __ballot_sync(0xffffffffu, odd);
+            if (lane == 0) {
+                sh->amax[cw] = amax;
+                uint32_t m = 0u;
+                for (uint32_t i = 0; i < 16u; i++) m |= (odds >> (2u * i) & 3u) ? 1u << i : 0u;
+                sh->odd[v ? 1 : 0][note % PB_NOTES][cw] = (uint16_t)m;
+            }
+            named_bar_sync(3, 128);
+            amax = max(max(sh->amax[0], sh->amax[1]), max(sh->amax[2], sh->amax[3]));
+            const float big = __uint_as_float(amax) * s;
+            if (amax != 0u && !(big >= 256.0f && big < 32768.0f)) { // once more, from global memory, with the tile's own scale
+                s = __uint_as_float(scale_bits(amax));
+                (v ? v_scale : k_scale) = s;
+                PbRing<PB_NST> a2 = begin;
+                const float *src = v ? g.vpages : g.kpages;
+                if (in) {
+                    const size_t page = __ldg(g.pages + tl.table + (key >> g.page_shift));
+                    src += ((page << g.page_shift) + (key & ((1u << g.page_shift) - 1u))) * g.row_floats + (size_t)tl.kvh * DIM + 32u * j;
+                }
+#pragma unroll 1
+                for (uint32_t h = 0; h < NU; h++, a2.next()) {
+                    uint32_t w[8][4];
+#pragma unroll
+                    for (uint32_t i = 0; i < 8u; i++) {
+                        uint4 a = make_uint4(0u, 0u, 0u, 0u);
+                        if (in) a = *reinterpret_cast<const uint4 *>(src + 64u * h + 4u * i);
+                        w[i][0] = a.x; w[i][1] = a.y; w[i][2] = a.z; w[i][3] = a.w;
+                    }
+                    put(a2.s, w, false);
+                }
+            }
+            if (cw == 0u && lane == 0) sh->unscale[v ? 1 : 0][note % PB_NOTES] = 1.0f / s;
+            named_bar_sync(3, 128); // amax[] has been read
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+                PbRing<PB_NST> a2 = begin;
+                for (uint32_t h = 0; h < NU; h++, a2.next()) mbar_arrive(bar_conv + 8u * a2.s);
+            }
+        };
+        // A wait that runs out makes all later ones return at once; the warps go through the same barriers all the same.
+        Tile cur = take();
+        convert(false, cur, 0u);
+        for (uint32_t t = 0; t < total; t++) {
+            const Tile ahead = ts.more ? take() : cur;
+            if (t + 1u < total) convert(false, ahead, t + 1u);
+            convert(true, cur, t);
+            cur = ahead;
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;"); // 128 x 48 + 128 x 80 + 256 x 192 = the launch's 512 x 128
+        // ---------------- softmax ----------------
+        const uint32_t q4 = warp & 3u, half = (warp - 8u) >> 2;
+        const uint32_t lane_addr = (32u * q4) << 16;
+        const bool hi = q4 < 2u;                             // this lane has a row's hi parts, else its lo parts
+        const uint32_t row = 32u * (q4 & 1u) + lane;         // the row, 0 .. 63
+        const uint32_t bar_group = 1u + (q4 & 1u);           // the four warps that have these 32 rows
+        constexpr uint32_t HD = DIM / 2;                     // dims of Q' and O of a thread
+        float *red = reinterpret_cast<float *>(smem + PB_OFF_RED), *cf_s = red + 128;
+        const uint32_t group = plan.group, tok = row / group, head = row - tok * group;
+        auto arrive = [&](uint32_t bar) { // one arrival per warp, after all its lanes
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
+        auto wait = [&](uint32_t bar, uint32_t parity) {
+            pb_wait(bar, parity, sh, g.status);
+            __syncwarp();
+            tc_fence_after();
+        };
+        // where a thread of row r and this half has its 32 scores or weights in the P' buffer: chunk c of 8 (0..3 in row r, 4..7 in row 64 + r)
+        auto p_chunk = [&](uint32_t c) { return smem + PB_OFF_P + swz128(row + (c >> 2) * 64u, 4u * half + (c & 3u)); };
+        // Q' of a segment: the row's hi or lo parts, half of the dims, scaled by a power of two of the row's own
+        auto load_q = [&](const PlanSegment &sg) -> float {
+            const uint32_t rows = sg.it.ntok * group;
+            float unscale = 1.0f;
+            if (32u * (q4 & 1u) < rows) {
+                const float *src = g.q + (int64_t)(plan.seq[sg.seq].row + sg.it.tok0 + tok) * g.q_stride + (size_t)(sg.kvh * group + head) * DIM + HD * half;
+                const bool real = row < rows;
+                uint32_t amax = 0u;
+                if (real)
+#pragma unroll 4
+                    for (uint32_t d = 0; d < HD; d += 4u) {
+                        const uint4 a = __ldg(reinterpret_cast<const uint4 *>(src + d));
+#pragma unroll
+                        for (uint32_t e = 0; e < 4u; e++) {
+                            const uint32_t b = e == 0 ? a.x : e == 1 ? a.y : e == 2 ? a.z : a.w;
+                            if (is_finite_bits(b)) amax = max(amax, b & 0x7fffffffu);
+                        }
+                    }
+                red[64u * half + row] = __uint_as_float(amax); // (hi and lo threads write the same)
+                named_bar_sync(bar_group, 128);
+                amax = max(__float_as_uint(red[row]), __float_as_uint(red[64u + row]));
+                const float s = amax ? __uint_as_float(scale_bits(amax)) : 1.0f;
+                unscale = 1.0f / s;
+#pragma unroll 1
+                for (uint32_t d = 0; d < HD; d += 32u) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (uint32_t i = 0; i < 8u; i++) {
+                        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (real) a = __ldg(reinterpret_cast<const float4 *>(src + d + 4u * i));
+                        const float x[4] = {a.x * s, a.y * s, a.z * s, a.w * s};
+#pragma unroll
+                        for (uint32_t e = 0; e < 4u; e += 2u) {
+                            __half2 h = __floats2half2_rn(x[e], x[e + 1]);
+                            if (!hi) {
+                                const float2 f = __half22float2(h);
+                                h = __floats2half2_rn(isfinite(f.x) ? x[e] - f.x : 0.0f, isfinite(f.y) ? x[e + 1] - f.y : 0.0f);
+                            }
+                            w[2 * i + (e >> 1)] = *reinterpret_cast<const uint32_t *>(&h);
+                        }
+                    }
+                    tmem_st16(tmem + lane_addr + PB_COL_Q + (HD * half + d) / 2u, w);
+                }
+                tmem_wait_st();
+                named_bar_sync(bar_group, 128); // red[] is free
+            }
+            tc_fence_before();
+            arrive(bar_q_full);
+            return unscale;
+        };
+        // score of a key by ordinary arithmetic, for keys that have values that are not finite
+        auto plain_score = [&](const float *q, const float *k) {
+            float s = 0.0f;
+#pragma unroll 1
+            for (int d = 0; d < DIM; d++) s = fmaf(q[d], k[d], s);
+            return s * g.scale2;
+        };
+        float O[HD];
+        uint32_t t0 = 0; // the segment's first tile
+        PlanWalk walk(plan, blockIdx.x, PF_KEYS32);
+        PlanSegment sg, nx;
+        bool more = walk.next(sg);
+        float q_unscale = load_q(sg), q_next = 1.0f;
+        while (more) {
+            const PlanItem it = sg.it;
+            const PlanSeq &sq = plan.seq[sg.seq];
+            const uint32_t rows = it.ntok * group;
+            const bool active = 32u * (q4 & 1u) < rows; // (the same for the four warps of these rows)
+            const bool real = row < rows;
+            const uint32_t vis = real ? sq.pos + it.tok0 + tok + 1u : 0u; // this row sees klo <= key < vis
+            const uint32_t klo = real ? plan_lowest(sq, plan.window, it.tok0 + tok) : 0u;
+            const float *q_row = g.q + (int64_t)(sq.row + it.tok0 + (real ? tok : 0u)) * g.q_stride + (size_t)(sg.kvh * group + head) * DIM;
+            auto k_row = [&](const float *base, uint32_t key) {
+                const size_t page = g.pages[sq.table + (key >> g.page_shift)];
+                return base + ((page << g.page_shift) + (key & ((1u << g.page_shift) - 1u))) * g.row_floats + (size_t)sg.kvh * DIM;
+            };
+            float m = NEG_BIG, l = 0.0f, cf = 0.0f;
+            const uint32_t end = t0 + (sg.b - sg.a);
+#pragma unroll
+            for (uint32_t d = 0; d < HD; d++) O[d] = 0.0f;
+            // O = O * cf + O' of tile t (its weights are against m, as cf is)
+            auto fold = [&](uint32_t t) {
+                wait(bar_pv_done, t & 1u);
+                const uint64_t odd = *reinterpret_cast<const uint64_t *>(sh->odd[1][t % PB_NOTES]);
+                if (odd != 0ull && hi) { // values of V that are not finite: w v for the rows that see them, added to O' where it lies (rare)
+#pragma unroll 1
+                    for (uint32_t c0 = 0; c0 < HD; c0 += 32u) {
+                        uint32_t o[32];
+                        tmem_ld32(tmem + lane_addr + HD * half + c0, o);
+                        tmem_wait_ld();
+#pragma unroll 1
+                        for (uint32_t r = 0; r < PF_KEYS32; r++) {
+                            const uint32_t key = (it.tile0 + sg.a + (t - t0)) * PF_KEYS32 + r;
+                            if (!(odd >> r & 1ull) || key < klo || key >= vis) continue;
+                            const float w = exp2f(plain_score(q_row, k_row(g.kpages, key)) - m);
+                            const float *v = k_row(g.vpages, key) + HD * half + c0;
+#pragma unroll
+                            for (uint32_t c = 0; c < 32u; c++)
+                                if (!is_finite_bits(__float_as_uint(v[c]))) o[c] = __float_as_uint(__uint_as_float(o[c]) + w * v[c]);
+                        }
+                        tmem_st32(tmem + lane_addr + HD * half + c0, o);
+                    }
+                    tmem_wait_st();
+                }
+                const float us = sh->unscale[1][t % PB_NOTES] * 0.00006103515625f; // P' carries 2^14
+#pragma unroll
+                for (uint32_t c0 = 0; c0 < HD; c0 += 32u) {
+                    uint32_t o[32];
+                    tmem_ld32(tmem + lane_addr + HD * half + c0, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (uint32_t c = 0; c < 32u; c++) O[c0 + c] = fmaf(O[c0 + c], cf, __uint_as_float(o[c]) * us);
+                }
+            };
+            for (uint32_t t = t0; t < end; t++) {
+                const uint32_t key0 = (it.tile0 + sg.a + (t - t0)) * PF_KEYS32;
+                if (t > t0) { // (in front of the scores, so that the registers suffice; also: P' of the tile in front has been multiplied)
+                    if (active) fold(t - 1u);
+                    else wait(bar_pv_done, (t - 1u) & 1u);
+                }
+                wait(bar_s_full + 8u * (t & 1u), (t >> 1) & 1u);
+                uint32_t sr[32];
+                if (active) {
+                    tmem_ld32(tmem + lane_addr + PB_COL_S + 64u * (t & 1u) + 32u * half, sr);
+                    tmem_wait_ld();
+                }
+                tc_fence_before();
+                arrive(bar_s_free + 8u * (t & 1u));
+                if (active) {
+                    if (!hi)
+#pragma unroll
+                        for (uint32_t c = 0; c < 8u; c++) *reinterpret_cast<uint4 *>(p_chunk(c)) = make_uint4(sr[4 * c], sr[4 * c + 1], sr[4 * c + 2], sr[4 * c + 3]);
+                    named_bar_sync(bar_group, 128);
+                    if (hi) {
+                        const float f = g.scale2 * (q_unscale * sh->unscale[0][t % PB_NOTES]);
+                        float mx = NEG_BIG;
+                        const uint32_t k0 = key0 + 32u * half;
+#pragma unroll
+                        for (uint32_t c = 0; c < 8u; c++) {
+                            const float4 x = *reinterpret_cast<const float4 *>(p_chunk(c));
+                            sr[4 * c] = __float_as_uint((__uint_as_float(sr[4 * c]) + x.x) * f);
+                            sr[4 * c + 1] = __float_as_uint((__uint_as_float(sr[4 * c + 1]) + x.y) * f);
+                            sr[4 * c + 2] = __float_as_uint((__uint_as_float(sr[4 * c + 2]) + x.z) * f);
+                            sr[4 * c + 3] = __float_as_uint((__uint_as_float(sr[4 * c + 3]) + x.w) * f);
+                        }
+                        const uint32_t odd = *reinterpret_cast<const uint32_t *>(&sh->odd[0][t % PB_NOTES][2u * half]);
+#pragma unroll 1
+                        for (uint32_t left = odd; left != 0u; left &= left - 1u) { // keys with values that are not finite (rare)
+                            const uint32_t r = (uint32_t)__ffs((int)left) - 1u;
+                            if (k0 + r < klo || k0 + r >= vis) continue;
+                            const uint32_t x = __float_as_uint(plain_score(q_row, k_row(g.kpages, k0 + r)));
+#pragma unroll
+                            for (uint32_t c = 0; c < 32u; c++)
+                                if (c == r) sr[c] = x;
+                        }
+                        if (key0 < it.all_lo || key0 + PF_KEYS32 > it.all_hi || !real)
+#pragma unroll
+                            for (uint32_t c = 0; c < 32u; c++)
+                                if (k0 + c < klo || k0 + c >= vis) sr[c] = 0xff800000u; // -infinity
+#pragma unroll
+                        for (uint32_t c = 0; c < 32u; c += 2u) mx = max3(mx, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+                        red[64u * half + row] = mx;
+                    }
+                    named_bar_sync(bar_group, 128);
+                    if (hi) {
+                        const float m_new = max3(m, red[row], red[64u + row]);
+                        cf = m > NEG_TEST ? exp2f(m - m_new) : 0.0f; // (O and l are zero until the first key)
+                        m = m_new;
+                        if (half == 0u) cf_s[row] = cf;
+                        const float neg_m = m > NEG_TEST ? -m : 0.0f;
+                        float sum = 0.0f;
+#pragma unroll
+                        for (uint32_t c = 0; c < 4u; c++) {
+                            float x[8];
+#pragma unroll
+                            for (uint32_t e = 0; e < 8u; e++) {
+                                x[e] = exp2f(__uint_as_float(sr[8 * c + e]) + neg_m);
+                                sum += x[e];
+                                x[e] *= 16384.0f; // 2^14: f16's smallest step is then 2^-38 of the largest weight
+                            }
+                            uint4 a, b;
+                            split8(x, a, b);
+                            *reinterpret_cast<uint4 *>(p_chunk(c)) = a;
+                            *reinterpret_cast<uint4 *>(p_chunk(4u + c)) = b;
+                        }
+                        l = fmaf(l, cf, sum);
+                        fence_proxy_async();
+                    }
+                    named_bar_sync(bar_group, 128);
+                    if (!hi) cf = cf_s[row];
+                }
+                arrive(bar_p_full);
+            }
+            // ---------------- end of the segment ----------------
+            more = walk.next(nx);
+            if (more) q_next = load_q(nx); // the segment's scores were all there: its Q' may go
+            if (active) {
+                fold(end - 1u);
+                if (hi) red[64u * half + row] = l;
+                named_bar_sync(bar_group, 128); // (P' is free too: its last products have completed)
+                const float l_all = red[row] + red[64u + row];
+                const bool seen = real && klo < vis;
+                float inv = 0.0f;
+                float *dst = nullptr;
+                if (sg.whole) {
+                    float den = l_all;
+                    if (g.sinks && real) den += exp2f(g.sinks[sg.kvh * group + head] * PB_LOG2E - (m > NEG_TEST ? m : 0.0f));
+                    inv = 1.0f / den;
+                    dst = g.out + (int64_t)(sq.row + it.tok0 + tok) * g.out_stride + (size_t)(sg.kvh * group + head) * DIM + HD * half;
+                } else { // a part: maximum, sum and O as they are, for the merge
+                    float *ps = g.scratch + part_slot(blockIdx.x, sg.part) * part_floats(DIM);
+                    inv = 1.0f;
+                    dst = ps + (size_t)row * DIM + HD * half;
+                    if (hi && half == 0u && real) *reinterpret_cast<float2 *>(ps + 128u * DIM + 2u * row) = make_float2(m, seen ? l_all : -1.0f);
+                }
+#pragma unroll
+                for (uint32_t c0 = 0; c0 < HD; c0 += 32u) { // the row's hi and lo parts meet, 32 dims at a time
+                    if (!hi)
+#pragma unroll
+                        for (uint32_t c = 0; c < 8u; c++) *reinterpret_cast<float4 *>(p_chunk(c)) = make_float4(O[c0 + 4 * c], O[c0 + 4 * c + 1], O[c0 + 4 * c + 2], O[c0 + 4 * c + 3]);
+                    named_bar_sync(bar_group, 128);
+                    if (hi && real)
+#pragma unroll
+                        for (uint32_t c = 0; c < 8u; c++) {
+                            const float4 x = *reinterpret_cast<const float4 *>(p_chunk(c));
+                            *reinterpret_cast<float4 *>(dst + c0 + 4u * c) =
+                                seen ? make_float4((O[c0 + 4 * c] + x.x) * inv, (O[c0 + 4 * c + 1] + x.y) * inv, (O[c0 + 4 * c + 2] + x.z) * inv, (O[c0 + 4 * c + 3] + x.w) * inv)
+                                     : make_float4(0.f, 0.f, 0.f, 0.f);
+                        }
+                    named_bar_sync(bar_group, 128);
+                }
+            } else {
+                wait(bar_pv_done, (end - 1u) & 1u);
+            }
+            q_unscale = q_next;
+            t0 = end;
+            sg = nx;
+        }
+    }
+
+    // ---------------- teardown ----------------
+    tc_fence_before();
+    __syncwarp();
+    if (sh->abort) { // a wait ran out somewhere: give copies already issued into this CTA's shared memory time to land
+        const long long t0 = clock64();
+        while (clock64() - t0 < 200000000ll) __nanosleep(1000);
+    }
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <int DIM> static mkv_status launch_dim(Pool *p, int layer, const PoolPlan &plan, const PbArgs &g) {
+    PdlLaunch l(p->ctx, dim3(plan.ctas), PB_THREADS, PB_SMEM);
+    MKV_CUDA(cudaLaunchKernelEx(&l.cfg, pool_attn_f32_kernel<DIM>, p->maps[2 * (size_t)layer], p->maps[2 * (size_t)layer + 1], plan, g));
+    p->ctx->launches++;
+    return MKV_OK;
+}
+
+mkv_status launch_pool_attn_f32(Pool *p, int layer, const PoolPlan &plan, const PoolAttn &a) {
+    PbArgs g;
+    g.q = static_cast<const float *>(a.q);
+    g.out = static_cast<float *>(a.out);
+    g.q_stride = a.q_stride;
+    g.out_stride = a.out_stride;
+    g.pages = p->table;
+    g.kpages = reinterpret_cast<const float *>(p->layer_ptr(layer, 0));
+    g.vpages = reinterpret_cast<const float *>(p->layer_ptr(layer, 1));
+    g.sinks = a.sinks;
+    g.scratch = p->scratch;
+    g.status = p->ctx->dev_status;
+    g.row_floats = p->row_bytes / sizeof(float);
+    g.scale2 = a.scale * PB_LOG2E;
+    g.page_shift = (uint32_t)__builtin_ctz(p->desc.page_tokens);
+    switch (p->desc.head_dim) {
+    case 64: return launch_dim<64>(p, layer, plan, g);
+    case 128: return launch_dim<128>(p, layer, plan, g);
+    default: return launch_dim<256>(p, layer, plan, g);
+    }
+}
+
+mkv_status pool_attn_f32_setup(Pool *) {
+    MKV_CUDA(cudaFuncSetAttribute(pool_attn_f32_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PB_SMEM));
+    MKV_CUDA(cudaFuncSetAttribute(pool_attn_f32_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PB_SMEM));
+    MKV_CUDA(cudaFuncSetAttribute(pool_attn_f32_kernel<256>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PB_SMEM));
+    return MKV_OK;
+}
+
+} // namespace mkv

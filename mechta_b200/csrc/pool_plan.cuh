@@ -1,7 +1,7 @@
 // How the attention over paged rows is cut into work, shared by its kernels and the kernel that merges split work.
 //
 // An item is one KV head and a block of up to `block` tokens of a sequence (all query heads of the KV head for each: the rows of a
-// product); its work is the tiles of TILE_KEYS keys from the first key that any of its tokens sees to the last. The items of all sequences
+// product); its work is the tiles of 128 (f16) or 64 (f32) keys from the first key that any of its tokens sees to the last. The items of all sequences
 // (sequence by sequence, block by block, KV head by KV head) are laid end to end and cut into ranges of about the same cost, one a CTA,
 // so that decode steps over long histories and long blocks over short ones fill the GPU alike. A CTA's range is a few segments, each of
 // which costs as much as `segment` tiles beside its tiles (queries, the first tile's latency, outputs); a segment that covers its whole
@@ -109,6 +109,7 @@ struct MergeList {
 // Plans one launch over the items [i, n) that it takes (i is moved on); rows: packed tokens in front of them, moved on too.
 // Returns false when no item with tokens is left.
 struct PlanCost {
+    uint32_t rows;    // of an item: query heads of a KV head times tokens
     uint32_t keys;    // of a tile
     uint32_t segment; // in tiles
 };
@@ -119,7 +120,9 @@ __host__ __device__ inline size_t part_floats(uint32_t dim) { return 128u * (siz
 __host__ __device__ inline size_t part_slot(uint32_t cta, uint32_t part) { return 2u * (size_t)cta + part; }
 
 mkv_status launch_pool_merge(Pool *p, const MergeList &merge, const PoolAttn &a);
-mkv_status pool_attn_f16_setup(Pool *p);
+mkv_status pool_attn_f16_setup(Pool *);
 mkv_status launch_pool_attn_f16(Pool *p, int layer, const PoolPlan &plan, const PoolAttn &a);
+mkv_status pool_attn_f32_setup(Pool *);
+mkv_status launch_pool_attn_f32(Pool *p, int layer, const PoolPlan &plan, const PoolAttn &a);
 
 } // namespace mkv

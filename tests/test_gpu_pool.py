@@ -289,7 +289,7 @@ def test_copies_and_compaction(ctx, fmt, page, length, layers):
 
 def attn64(pool, items, q, window=0, sinks=None, scale=None, layer=0):
     """From the formula, in 64 bits: the outputs, and what their tolerance is made of: sum of weight * |v|, sum of |q k| * scale at its
-    largest, the largest |v| among the keys seen."""
+    largest, the largest |v| among the keys seen, the number of keys."""
     group = pool.q_heads // pool.kv_heads
     scale = scale or pool.head_dim**-0.5
     outs, mags, qks, tops, at = [], [], [], [], 0
@@ -321,19 +321,22 @@ def attn64(pool, items, q, window=0, sinks=None, scale=None, layer=0):
         mags.append((w @ clean.abs()).transpose(0, 1))
         qk = torch.where(seen, (x.abs() @ k.abs().transpose(1, 2)) * scale, torch.zeros_like(score))
         qks.append(qk.amax(-1, keepdim=True).transpose(0, 1))
-        tops.append((clean.abs().amax((1, 2))[:, None, None].expand(-1, n, 1) * (pos + n)).transpose(0, 1))
-    return torch.cat(outs), torch.cat(mags), torch.cat(qks), torch.cat(tops)
+        tops.append(torch.stack((clean.abs().amax((1, 2))[:, None, None].expand(-1, n, 1), torch.full((len(k), n, 1), float(pos + n), device="cuda",
+                                                                                                      dtype=torch.float64))).transpose(1, 2))
+    return torch.cat(outs), torch.cat(mags), torch.cat(qks), torch.cat(tops, 1)
 
 
 def attn_bound(fmt, out, mag, qk, top):
     """f16: a weight is rounded to f16 (2^-11 of it, or half a subnormal step, 2^-25, against a largest weight of at least 1), the output
     once more; f32 sums and exponentials in between. A score is off by its f32 sums: at most 2^-20 of sum |q k| here (the tensor
-    core's sums of 16 truncate: 16 steps of 2^-24 each), and a weight by as much, twice (sum and weight). f32: the products are
-    split into f16 parts of 11 bits each (2^-22 is left out), weights likewise."""
+    core's sums of 16 truncate: 16 steps of 2^-24 each), and a weight by as much, twice (sum and weight). f32: operands are
+    split into two f16 parts (2^-23 of a value is left out, or half a subnormal step, 2^-25, where the largest of a tile of 64 keys is
+    at least 2^8: 2^-33 of that largest), weights likewise; weights sum to at most 1."""
+    top, keys = top
     exponent = 2 * qk * 2.0**-20 + 2.0**-20
     if fmt == F16:
-        return mag * (2.0**-11 * 1.03 + exponent) + out.abs() * 2.0**-11 + top * 2.0**-25 + 2.0**-25
-    return mag * (2.0**-20 + exponent) + 1e-30
+        return mag * (2.0**-11 * 1.03 + exponent) + out.abs() * 2.0**-11 + top * keys * 2.0**-25 + 2.0**-25
+    return mag * (2.0**-20 + exponent) + top * 2.0**-33 + 1e-30
 
 
 def run_attn(pool, items, q, **kw):
