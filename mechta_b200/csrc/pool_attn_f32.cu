@@ -32,9 +32,8 @@
 namespace mkv {
 using namespace ptx;
 
-constexpr uint32_t PF_KEYS32 = 64, PF_ROWS32 = 64;
+constexpr uint32_t PF_KEYS32 = 64;
 constexpr int PB_THREADS = 512;
-constexpr uint32_t PB_CONV_TID0 = 128, PB_SOFT_TID0 = 256;
 constexpr long long PB_WAIT_LIMIT = 2000000000ll;
 constexpr float PB_LOG2E = 1.4426950408889634f;
 constexpr uint32_t PB_COL_S = 256, PB_COL_Q = 384;
@@ -119,14 +118,19 @@ __device__ __forceinline__ uint32_t scale_bits(uint32_t amax) {
     const int e = (int)(amax >> 23) - 127;
     return (uint32_t)(min(13 - e, 126) + 127) << 23;
 }
-// 2 x 8 values to their hi and lo parts
-__device__ __forceinline__ void split8(const float (&x)[8], uint4 &hi, uint4 &lo) {
+// 8 values, times s, to their hi and lo parts
+__device__ __forceinline__ void split8(const float (&x)[8], float s, uint4 &hi, uint4 &lo) {
     uint32_t h[4], l[4];
+    const uint64_t s2 = pack2(s, s);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const __half2 a = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        const uint64_t x2 = pack2(x[2 * i], x[2 * i + 1]);
+        float y0, y1;
+        unpack2(mul2(x2, s2), y0, y1);
+        const __half2 a = __floats2half2_rn(y0, y1);
         const float2 f = __half22float2(a);
-        const __half2 b = __floats2half2_rn(x[2 * i] - f.x, x[2 * i + 1] - f.y);
+        unpack2(fma2(x2, s2, pack2(-f.x, -f.y)), y0, y1);
+        const __half2 b = __floats2half2_rn(y0, y1);
         h[i] = *reinterpret_cast<const uint32_t *>(&a);
         l[i] = *reinterpret_cast<const uint32_t *>(&b);
     }
@@ -281,7 +285,7 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             }
         }
     } else if (warp < 8u) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         // ---------------- converters: a warp has 16 keys of every unit, a lane one of a key's two blocks ----------------
         const uint32_t cw = warp - 4u, key_in = 16u * cw + (lane >> 1), j = lane & 1u;
         PbRing<PB_NST> at;
@@ -298,33 +302,31 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         float k_scale = 1.0f, v_scale = 1.0f;
         auto convert = [&](bool v, const Tile &tl, uint32_t note) {
             const uint32_t key = tl.key0 + key_in;
-            const bool in = key >= tl.lo && key < tl.hi;
+            const bool in = key >= tl.lo && key < tl.hi, whole = tl.key0 >= tl.lo && tl.key0 + PF_KEYS32 <= tl.hi;
             const PbRing<PB_NST> begin = at;
-            uint32_t amax = 0u;
-            bool odd = false;
+            float amax = 0.0f;
+            bool odd = false; // a value of this lane's is not finite
             float s = v ? v_scale : k_scale;
-            auto put = [&](uint32_t slot, uint32_t (&w)[8][4], bool look) { // 32 values of this lane to hi and lo
+            // 32 values of this lane, x[i] = chunk i ^ 4 j of 4, to hi and lo
+            auto put = [&](uint32_t slot, float4 (&x)[8]) {
                 uint8_t *u = smem + slot * PB_UNIT;
 #pragma unroll
-                for (uint32_t i = 0; i < 8u; i++)
-#pragma unroll
-                    for (uint32_t e = 0; e < 4u; e++) {
-                        const bool fine = is_finite_bits(w[i][e]);
-                        if (look) {
-                            odd = odd || !fine;
-                            amax = max(amax, fine ? w[i][e] & 0x7fffffffu : 0u);
-                        }
-                        w[i][e] = fine ? __float_as_uint(__uint_as_float(w[i][e]) * s) : 0u;
-                    }
-#pragma unroll
-                for (uint32_t c = 0; c < 4u; c++) { // 8 values: a 16-byte chunk of hi, one of lo
-                    float x[8];
-#pragma unroll
-                    for (uint32_t e = 0; e < 8u; e++) x[e] = __uint_as_float(w[2 * c + (e >> 2)][e & 3u]);
+                for (uint32_t i = 0; i < 8u; i += 2u) {
+                    const float y[8] = {x[i].x, x[i].y, x[i].z, x[i].w, x[i + 1].x, x[i + 1].y, x[i + 1].z, x[i + 1].w};
                     uint4 hi, lo;
-                    split8(x, hi, lo);
-                    *reinterpret_cast<uint4 *>(u + swz128(key_in, 4u * j + c)) = hi;
-                    *reinterpret_cast<uint4 *>(u + PB_BLK + swz128(key_in, 4u * j + c)) = lo;
+                    split8(y, s, hi, lo);
+                    const uint32_t at_row = swz128(key_in, 4u * j + ((i ^ (4u * j)) >> 1));
+                    *reinterpret_cast<uint4 *>(u + at_row) = hi;
+                    *reinterpret_cast<uint4 *>(u + PB_BLK + at_row) = lo;
+                }
+            };
+            auto fix = [&](float4 (&x)[8]) { // values that are not finite to zero (rare)
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; i++) {
+                    float *e = &x[i].x;
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        if (!is_finite_bits(__float_as_uint(e[k]))) e[k] = 0.0f;
                 }
             };
 #pragma unroll 1
@@ -332,61 +334,68 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 pb_wait(bar_full + 8u * at.s, at.turn, sh, g.status);
                 __syncwarp();
                 const uint8_t *u = smem + at.s * PB_UNIT + j * PB_BLK;
-                uint32_t w[8][4];
+                float4 x[8];
 #pragma unroll
-                for (uint32_t i = 0; i < 8u; i++) { // (the two blocks' lanes in another order, so that they meet no bank together)
-                    const uint4 a = *reinterpret_cast<const uint4 *>(u + swz128(key_in, i ^ (4u * j)));
-                    const bool ok = in;
-                    w[i][0] = ok ? a.x : 0u; w[i][1] = ok ? a.y : 0u; w[i][2] = ok ? a.z : 0u; w[i][3] = ok ? a.w : 0u;
+                for (uint32_t i = 0; i < 8u; i++) x[i] = *reinterpret_cast<const float4 *>(u + swz128(key_in, i ^ (4u * j))); // (so that a key's two lanes meet no bank together)
+                if (!whole && !in) // (keys that no token of the item sees)
+#pragma unroll
+                    for (uint32_t i = 0; i < 8u; i++) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                uint64_t z = 0ull; // 0 * x is a NaN where x is not finite
+                float top = 0.0f;
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; i++) {
+                    top = max3(top, fabsf(x[i].x), fabsf(x[i].y));
+                    top = max3(top, fabsf(x[i].z), fabsf(x[i].w));
+                    z = fma2(pack2(x[i].x, x[i].y), 0ull, z);
+                    z = fma2(pack2(x[i].z, x[i].w), 0ull, z);
                 }
-                if (j) { // back into order
+                float z0, z1;
+                unpack2(z, z0, z1);
+                if (__any_sync(0xffffffffu, z0 + z1 != 0.0f)) { // (also: both lanes of a key have read its rows)
+                    if (z0 + z1 != 0.0f) odd = true;
+                    fix(x);
+                    top = 0.0f;
 #pragma unroll
-                    for (uint32_t i = 0; i < 4u; i++)
-#pragma unroll
-                        for (uint32_t e = 0; e < 4u; e++) {
-                            const uint32_t x = w[i][e];
-                            w[i][e] = w[i + 4u][e];
-                            w[i + 4u][e] = x;
-                        }
+                    for (uint32_t i = 0; i < 8u; i++) top = fmaxf(top, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
                 }
-                __syncwarp(); // both lanes of a key have read its rows
-                put(at.s, w, true);
+                amax = fmaxf(amax, top);
+                put(at.s, x);
             }
-            // the tile's largest value and the keys with values that are not finite
-            amax = __reduce_max_sync(0xffffffffu, amax);
+            // The scale fits if each warp's largest value lies well inside f16's range under it; otherwise all look for the tile's largest.
+            amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
+            if (named_bar_or(3, 128, amax != 0.0f && !(amax * s >= 256.0f && amax * s < 32768.0f))) {
+                if (lane == 0) sh->amax[cw] = __float_as_uint(amax);
+                named_bar_sync(3, 128);
+                const uint32_t most = max(max(sh->amax[0], sh->amax[1]), max(sh->amax[2], sh->amax[3]));
+                const float big = __uint_as_float(most) * s;
+                if (!(big >= 256.0f && big < 32768.0f)) { // once more, from global memory, with the tile's own scale
+                    s = __uint_as_float(scale_bits(most));
+                    (v ? v_scale : k_scale) = s;
+                    PbRing<PB_NST> a2 = begin;
+                    const float *src = v ? g.vpages : g.kpages;
+                    if (in) {
+                        const size_t page = __ldg(g.pages + tl.table + (key >> g.page_shift));
+                        src += ((page << g.page_shift) + (key & ((1u << g.page_shift) - 1u))) * g.row_floats + (size_t)tl.kvh * DIM + 32u * j;
+                    }
+#pragma unroll 1
+                    for (uint32_t h = 0; h < NU; h++, a2.next()) {
+                        float4 x[8];
+#pragma unroll
+                        for (uint32_t i = 0; i < 8u; i++) x[i] = in ? *reinterpret_cast<const float4 *>(src + 64u * h + 4u * (i ^ (4u * j))) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        fix(x);
+                        put(a2.s, x);
+                    }
+                }
+                named_bar_sync(3, 128); // amax[] has been read
+            }
             const uint32_t odds = __ballot_sync(0xffffffffu, odd);
             if (lane == 0) {
-                sh->amax[cw] = amax;
                 uint32_t m = 0u;
-                for (uint32_t i = 0; i < 16u; i++) m |= (odds >> (2u * i) & 3u) ? 1u << i : 0u;
+                if (odds)
+                    for (uint32_t i = 0; i < 16u; i++) m |= (odds >> (2u * i) & 3u) ? 1u << i : 0u;
                 sh->odd[v ? 1 : 0][note % PB_NOTES][cw] = (uint16_t)m;
+                if (cw == 0u) sh->unscale[v ? 1 : 0][note % PB_NOTES] = 1.0f / s;
             }
-            named_bar_sync(3, 128);
-            amax = max(max(sh->amax[0], sh->amax[1]), max(sh->amax[2], sh->amax[3]));
-            const float big = __uint_as_float(amax) * s;
-            if (amax != 0u && !(big >= 256.0f && big < 32768.0f)) { // once more, from global memory, with the tile's own scale
-                s = __uint_as_float(scale_bits(amax));
-                (v ? v_scale : k_scale) = s;
-                PbRing<PB_NST> a2 = begin;
-                const float *src = v ? g.vpages : g.kpages;
-                if (in) {
-                    const size_t page = __ldg(g.pages + tl.table + (key >> g.page_shift));
-                    src += ((page << g.page_shift) + (key & ((1u << g.page_shift) - 1u))) * g.row_floats + (size_t)tl.kvh * DIM + 32u * j;
-                }
-#pragma unroll 1
-                for (uint32_t h = 0; h < NU; h++, a2.next()) {
-                    uint32_t w[8][4];
-#pragma unroll
-                    for (uint32_t i = 0; i < 8u; i++) {
-                        uint4 a = make_uint4(0u, 0u, 0u, 0u);
-                        if (in) a = *reinterpret_cast<const uint4 *>(src + 64u * h + 4u * i);
-                        w[i][0] = a.x; w[i][1] = a.y; w[i][2] = a.z; w[i][3] = a.w;
-                    }
-                    put(a2.s, w, false);
-                }
-            }
-            if (cw == 0u && lane == 0) sh->unscale[v ? 1 : 0][note % PB_NOTES] = 1.0f / s;
-            named_bar_sync(3, 128); // amax[] has been read
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
@@ -404,7 +413,7 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             cur = ahead;
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;"); // 128 x 48 + 128 x 80 + 256 x 192 = the launch's 512 x 128
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;"); // 128 x 48 + 128 x 64 + 256 x 200 = the launch's 512 x 128
         // ---------------- softmax ----------------
         const uint32_t q4 = warp & 3u, half = (warp - 8u) >> 2;
         const uint32_t lane_addr = (32u * q4) << 16;
@@ -546,48 +555,65 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                     else wait(bar_pv_done, (t - 1u) & 1u);
                 }
                 wait(bar_s_full + 8u * (t & 1u), (t >> 1) & 1u);
-                uint32_t sr[32];
+                // The half row's 32 scores stay in the P' buffer (keys 8 c .. 8 c + 3 in chunk c, the next four in chunk 4 + c, where their weights go
+                // in the end): the registers are O's.
+                const uint32_t s_col = tmem + lane_addr + PB_COL_S + 64u * (t & 1u) + 32u * half;
+                auto s_chunk = [&](uint32_t g4) { return p_chunk((g4 >> 1) + 4u * (g4 & 1u)); };
                 if (active) {
-                    tmem_ld32(tmem + lane_addr + PB_COL_S + 64u * (t & 1u) + 32u * half, sr);
-                    tmem_wait_ld();
+                    if (!hi) {
+                        uint32_t w[32];
+                        tmem_ld32(s_col, w);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (uint32_t c = 0; c < 8u; c++) *reinterpret_cast<uint4 *>(s_chunk(c)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+                    }
+                    named_bar_sync(bar_group, 128);
+                    if (hi) {
+                        const float f = g.scale2 * (q_unscale * sh->unscale[0][t % PB_NOTES]);
+                        const uint32_t k0 = key0 + 32u * half, odd = *reinterpret_cast<const uint32_t *>(&sh->odd[0][t % PB_NOTES][2u * half]);
+                        const bool edge = key0 < it.all_lo || key0 + PF_KEYS32 > it.all_hi || !real;
+                        // the keys of this half that the row sees, a bit each; not those with values that are not finite
+                        uint32_t see = 0xffffffffu;
+                        if (edge) {
+                            const uint32_t a = klo > k0 ? min(klo - k0, 32u) : 0u, e = vis > k0 ? min(vis - k0, 32u) : 0u;
+                            see = (uint32_t)((1ull << e) - 1ull) & ~(uint32_t)((1ull << a) - 1ull);
+                        }
+                        const uint32_t plain = see & odd;
+                        see &= ~odd;
+                        float mx = NEG_BIG;
+#pragma unroll
+                        for (uint32_t h = 0; h < 2u; h++) {
+                            uint32_t w[16];
+                            tmem_ld16(s_col + 16u * h, w);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (uint32_t c = 0; c < 4u; c++) {
+                                float4 x = *reinterpret_cast<const float4 *>(s_chunk(4u * h + c));
+                                x.x = (__uint_as_float(w[4 * c]) + x.x) * f;
+                                x.y = (__uint_as_float(w[4 * c + 1]) + x.y) * f;
+                                x.z = (__uint_as_float(w[4 * c + 2]) + x.z) * f;
+                                x.w = (__uint_as_float(w[4 * c + 3]) + x.w) * f;
+                                if (see != 0xffffffffu) {
+                                    const uint32_t b = see >> (16u * h + 4u * c);
+                                    x = make_float4(b & 1u ? x.x : -INFINITY, b & 2u ? x.y : -INFINITY, b & 4u ? x.z : -INFINITY, b & 8u ? x.w : -INFINITY);
+                                }
+                                mx = max3(max3(mx, x.x, x.y), x.z, x.w);
+                                *reinterpret_cast<float4 *>(s_chunk(4u * h + c)) = x;
+                            }
+                        }
+#pragma unroll 1
+                        for (uint32_t left = plain; left != 0u; left &= left - 1u) { // (rare)
+                            const uint32_t r = (uint32_t)__ffs((int)left) - 1u;
+                            const float x = plain_score(q_row, k_row(g.kpages, k0 + r));
+                            mx = fmaxf(mx, x);
+                            reinterpret_cast<float *>(s_chunk(r >> 2))[r & 3u] = x;
+                        }
+                        red[64u * half + row] = mx;
+                    }
                 }
                 tc_fence_before();
                 arrive(bar_s_free + 8u * (t & 1u));
                 if (active) {
-                    if (!hi)
-#pragma unroll
-                        for (uint32_t c = 0; c < 8u; c++) *reinterpret_cast<uint4 *>(p_chunk(c)) = make_uint4(sr[4 * c], sr[4 * c + 1], sr[4 * c + 2], sr[4 * c + 3]);
-                    named_bar_sync(bar_group, 128);
-                    if (hi) {
-                        const float f = g.scale2 * (q_unscale * sh->unscale[0][t % PB_NOTES]);
-                        float mx = NEG_BIG;
-                        const uint32_t k0 = key0 + 32u * half;
-#pragma unroll
-                        for (uint32_t c = 0; c < 8u; c++) {
-                            const float4 x = *reinterpret_cast<const float4 *>(p_chunk(c));
-                            sr[4 * c] = __float_as_uint((__uint_as_float(sr[4 * c]) + x.x) * f);
-                            sr[4 * c + 1] = __float_as_uint((__uint_as_float(sr[4 * c + 1]) + x.y) * f);
-                            sr[4 * c + 2] = __float_as_uint((__uint_as_float(sr[4 * c + 2]) + x.z) * f);
-                            sr[4 * c + 3] = __float_as_uint((__uint_as_float(sr[4 * c + 3]) + x.w) * f);
-                        }
-                        const uint32_t odd = *reinterpret_cast<const uint32_t *>(&sh->odd[0][t % PB_NOTES][2u * half]);
-#pragma unroll 1
-                        for (uint32_t left = odd; left != 0u; left &= left - 1u) { // keys with values that are not finite (rare)
-                            const uint32_t r = (uint32_t)__ffs((int)left) - 1u;
-                            if (k0 + r < klo || k0 + r >= vis) continue;
-                            const uint32_t x = __float_as_uint(plain_score(q_row, k_row(g.kpages, k0 + r)));
-#pragma unroll
-                            for (uint32_t c = 0; c < 32u; c++)
-                                if (c == r) sr[c] = x;
-                        }
-                        if (key0 < it.all_lo || key0 + PF_KEYS32 > it.all_hi || !real)
-#pragma unroll
-                            for (uint32_t c = 0; c < 32u; c++)
-                                if (k0 + c < klo || k0 + c >= vis) sr[c] = 0xff800000u; // -infinity
-#pragma unroll
-                        for (uint32_t c = 0; c < 32u; c += 2u) mx = max3(mx, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
-                        red[64u * half + row] = mx;
-                    }
                     named_bar_sync(bar_group, 128);
                     if (hi) {
                         const float m_new = max3(m, red[row], red[64u + row]);
@@ -598,15 +624,15 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                         float sum = 0.0f;
 #pragma unroll
                         for (uint32_t c = 0; c < 4u; c++) {
-                            float x[8];
+                            const float4 u = *reinterpret_cast<const float4 *>(p_chunk(c)), v = *reinterpret_cast<const float4 *>(p_chunk(4u + c));
+                            float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
                             for (uint32_t e = 0; e < 8u; e++) {
-                                x[e] = exp2f(__uint_as_float(sr[8 * c + e]) + neg_m);
+                                x[e] = ex2(x[e] + neg_m);
                                 sum += x[e];
-                                x[e] *= 16384.0f; // 2^14: f16's smallest step is then 2^-38 of the largest weight
                             }
                             uint4 a, b;
-                            split8(x, a, b);
+                            split8(x, 16384.0f, a, b); // 2^14: f16's smallest step is then 2^-38 of the largest weight
                             *reinterpret_cast<uint4 *>(p_chunk(c)) = a;
                             *reinterpret_cast<uint4 *>(p_chunk(4u + c)) = b;
                         }
