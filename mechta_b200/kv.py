@@ -274,14 +274,24 @@ def _need(ok, text: str) -> None:
 
 
 def _fmt_of(t: torch.Tensor) -> int:
-    _need(t.dtype in (torch.float16, torch.float32), f"{t.dtype}: must be float16 or float32")
-    return _lib.F16 if t.dtype == torch.float16 else _lib.F32
+    if t.dtype is torch.float16:
+        return _lib.F16
+    _need(t.dtype is torch.float32, f"{t.dtype}: must be float16 or float32")
+    return _lib.F32
 
 
-def _strides(t: torch.Tensor, what: str) -> tuple[int, int]:
-    """Token and head stride of a [tokens][heads][dims] tensor whose heads are contiguous."""
-    _need(t.dim() == 3 and (t.stride(2) == 1 or t.shape[2] <= 1 or t.numel() == 0), f"{what} must be [tokens][heads][dims] with contiguous dims")
-    return t.stride(0), t.stride(1)
+def _block(t: torch.Tensor, device: int, what: str) -> tuple[tuple, int, int]:
+    """Shape, token and head stride (0 where there is one token or head) of a [tokens][heads][dims] tensor on `device` whose dims are
+    contiguous and whose tokens and heads are not broadcast."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or (stride[2] != 1 and shape[2] > 1 and 0 not in shape):
+        _need(False, f"{what} must be [tokens][heads][dims] with contiguous dims")
+    ts, hs = (stride[0] if shape[0] > 1 else 0), (stride[1] if shape[1] > 1 else 0)
+    if (shape[0] > 1 and ts <= 0) or (shape[1] > 1 and hs <= 0):
+        _need(False, f"{what} may not be broadcast")
+    if device >= 0 and t.get_device() != device:
+        _need(False, f"{what} must be on cuda:{device}")
+    return shape, ts, hs
 
 
 class Rope:
@@ -299,6 +309,7 @@ class Rope:
         self.ctx, self.dims = ctx, int(dims)
         d = _lib.RopeDesc(self.dims, self.LAYOUTS[layout], self.SCALINGS[scaling], base, factor, original, slow, fast)
         check(_lib.lib().mkv_rope_create(C.byref(d), C.byref(self._h)))
+        self._apply = _lib.lib().mkv_rope_apply
 
     def freqs(self) -> tuple[np.ndarray, float]:
         """Radians per position of each pair, and the factor on cosine and sine."""
@@ -309,18 +320,17 @@ class Rope:
     def apply(self, x: torch.Tensor, positions: torch.Tensor, out: torch.Tensor, backward: bool = False) -> None:
         """out = x rotated at `positions` (int32 [tokens]); x, out [tokens][heads][dims], f16 or f32 each, any token and head
         strides, the same memory allowed. backward: the transposed map, for gradients."""
-        _need(self.ctx is not None, "a Rope without a context does not run")
-        xs, ys = _strides(x, "x"), _strides(out, "out")
-        _need(x.shape == out.shape, f"x is {tuple(x.shape)}, out {tuple(out.shape)}")
-        _need(positions.dtype == torch.int32 and positions.shape == x.shape[:1] and positions.is_contiguous(), "positions must be contiguous int32 [tokens]")
-        n, heads, dim = x.shape
-        _need(all(s > 0 for s, k in zip(xs, (n, heads)) if k > 1), "x may not be broadcast over tokens or heads")
-        _need(all(s > 0 for s, k in zip(ys, (n, heads)) if k > 1), "out may not be broadcast")
-        for t in (x, out, positions):
-            _need(t.device.type == "cuda" and t.device.index == self.ctx.device, f"tensors must be on cuda:{self.ctx.device}")
-        r = _lib.RopeRows(x.data_ptr(), out.data_ptr(), _fmt_of(x), _fmt_of(out), n, heads, dim, xs[0] if n > 1 else 0, xs[1] if heads > 1 else 0,
-                          ys[0] if n > 1 else 0, ys[1] if heads > 1 else 0, positions.data_ptr(), int(backward))
-        check(_lib.lib().mkv_rope_apply(self.ctx._h, self._h, C.byref(r)))
+        ctx = self.ctx
+        _need(ctx is not None, "a Rope without a context does not run")
+        shape, xt, xh = _block(x, ctx.device, "x")
+        out_shape, yt, yh = _block(out, ctx.device, "out")
+        if shape != out_shape:
+            _need(False, f"x is {tuple(shape)}, out {tuple(out_shape)}")
+        n, heads, dim = shape
+        if positions.dtype is not torch.int32 or positions.shape != (n,) or not positions.is_contiguous() or positions.get_device() != ctx.device:
+            _need(False, f"positions must be contiguous int32 [tokens] on cuda:{ctx.device}")
+        r = _lib.RopeRows(x.data_ptr(), out.data_ptr(), _fmt_of(x), _fmt_of(out), n, heads, dim, xt, xh, yt, yh, positions.data_ptr(), backward)
+        check(self._apply(ctx._h, self._h, C.byref(r)))
 
     def close(self) -> None:
         if self._h:
@@ -346,7 +356,10 @@ class KvPool:
         for v in (n_pages, page_tokens, max_seqs, max_tokens):
             _need(0 <= v < 2**32, f"{v} is no size")
         d = _lib.PoolDesc(int(fmt), n_layers, n_pages, page_tokens, max_seqs, max_tokens, q_heads, kv_heads, head_dim)
-        check(_lib.lib().mkv_pool_create(ctx._h if ctx is not None else None, C.byref(d), C.byref(self._h)))
+        L = _lib.lib()
+        check(L.mkv_pool_create(ctx._h if ctx is not None else None, C.byref(d), C.byref(self._h)))
+        self._dtype, self._device = self.fmt.torch_dtype, ctx.device if ctx is not None else -1
+        self._write, self._attn = L.mkv_pool_write, L.mkv_attn_pool
 
     # -- bookkeeping
     @property
@@ -406,46 +419,52 @@ class KvPool:
                      for p in self.buffers(layer))
 
     def _rows(self, t: torch.Tensor, heads: int, rows: int, what: str) -> int:
-        """Checks [rows][heads][head_dim] with dense heads; the token stride."""
-        ts, hs = _strides(t, what)
-        _need(tuple(t.shape) == (rows, heads, self.head_dim), f"{what} is {tuple(t.shape)}, the items want {(rows, heads, self.head_dim)}")
-        _need(heads == 1 or hs == self.head_dim or rows == 0, f"{what}: a token's heads must be contiguous")
-        _need(rows <= 1 or ts > 0, f"{what} may not be broadcast")
-        if self.ctx is not None:
-            _need(t.device.type == "cuda" and t.device.index == self.ctx.device, f"{what} must be on cuda:{self.ctx.device}")
-        return ts if rows > 1 else 0
+        """Checks [rows][heads][head_dim] with dense heads; the token stride (0 for one token)."""
+        shape, ts, hs = _block(t, self._device, what)
+        if shape != (rows, heads, self.head_dim):
+            _need(False, f"{what} is {tuple(shape)}, the items want {(rows, heads, self.head_dim)}")
+        if heads > 1 and rows > 0 and hs != self.head_dim:
+            _need(False, f"{what}: a token's heads must be contiguous")
+        return ts
 
     @staticmethod
-    def _items(items) -> np.ndarray:
-        a = np.ascontiguousarray(items, np.uint32)
-        a = a.reshape(0, 4) if a.size == 0 else a
-        _need(a.ndim == 2 and a.shape[1] == 4, "items are rows of (sequence, first_pos, pos, ntok)")
-        return a
+    def _items(items) -> tuple[np.ndarray, int, int, int]:
+        """The items as an array, its address, their number, their tokens."""
+        a = items
+        if not (type(a) is np.ndarray and a.dtype == np.uint32 and a.flags.c_contiguous):
+            a = np.ascontiguousarray(items, np.uint32)
+        if a.ndim != 2 or a.shape[1] != 4:
+            _need(a.size == 0, "items are rows of (sequence, first_pos, pos, ntok)")
+            a = a.reshape(0, 4)
+        n = len(a)
+        rows = sum(a[:, 3].tolist()) if n <= 64 else int(a[:, 3].sum(dtype=np.int64))
+        return a, a.__array_interface__["data"][0], n, rows
 
     def write(self, layer: int, items, k: torch.Tensor, v: torch.Tensor, rope: Rope | None = None) -> None:
         """New rows of the items' sequences in one layer; k, v f32 or f16 [tokens of all items][kv_heads][head_dim]. rope rotates k at
         the rows' positions."""
-        a = self._items(items)
-        rows = int(a[:, 3].sum(dtype=np.int64))
-        _need(k.dtype == v.dtype, "k and v must have one type")
+        a, at, n, rows = self._items(items)
+        if k.dtype is not v.dtype:
+            _need(False, "k and v must have one type")
         r = _lib.PoolRows(k.data_ptr(), v.data_ptr(), _fmt_of(k), self._rows(k, self.kv_heads, rows, "k"), self._rows(v, self.kv_heads, rows, "v"),
                           rope._h if rope is not None else None)
-        check(_lib.lib().mkv_pool_write(self._h, layer, a.ctypes.data, len(a), C.byref(r)))
+        check(self._write(self._h, layer, at, n, C.byref(r)))
 
     def attn(self, layer: int, items, q: torch.Tensor, out: torch.Tensor, window: int = 0, sinks: torch.Tensor | None = None,
              scale: float = 0.0) -> None:
         """Attention of the items' tokens over their sequences; q, out in the pool's type, [tokens of all items][q_heads][head_dim].
         scale 0 = 1 / sqrt(head_dim); sinks f32 [q_heads]."""
-        a = self._items(items)
-        rows = int(a[:, 3].sum(dtype=np.int64))
-        _need(q.dtype == out.dtype == self.fmt.torch_dtype, f"q and out must be {self.fmt.torch_dtype}")
-        _need(0 <= window < 2**32, f"window {window}")
+        a, at, n, rows = self._items(items)
+        if q.dtype is not self._dtype or out.dtype is not self._dtype:
+            _need(False, f"q and out must be {self._dtype}")
+        if not 0 <= window < 2**32:
+            _need(False, f"window {window}")
         if sinks is not None:
-            _need(sinks.dtype == torch.float32 and sinks.is_contiguous() and tuple(sinks.shape) == (self.q_heads,), "sinks must be f32 [q_heads]")
-            _need(self.ctx is None or sinks.device == q.device, "sinks must be where q is")
+            _need(sinks.dtype is torch.float32 and sinks.is_contiguous() and sinks.shape == (self.q_heads,), "sinks must be f32 [q_heads]")
+            _need(sinks.get_device() == self._device, "sinks must be where the pool is")
         r = _lib.PoolAttn(q.data_ptr(), out.data_ptr(), self._rows(q, self.q_heads, rows, "q"), self._rows(out, self.q_heads, rows, "out"), scale,
                           window, sinks.data_ptr() if sinks is not None else None)
-        check(_lib.lib().mkv_attn_pool(self._h, layer, a.ctypes.data, len(a), C.byref(r)))
+        check(self._attn(self._h, layer, at, n, C.byref(r)))
 
     def close(self) -> None:
         if self._h:
