@@ -5,7 +5,7 @@
 #include <stdint.h>
 
 #include <algorithm>
-#include <unordered_map>
+#include <new>
 #include <vector>
 
 #include "../../include/mechta_kv.h"
@@ -36,12 +36,15 @@ class FreeSet {
     }
     uint32_t size() const { return count; }
     bool has(uint32_t x) const { return bits[x / 64u] >> (x % 64u) & 1u; }
-    uint32_t take() { // (not when empty)
+    uint32_t lowest() { // (not when empty)
         while (!bits[low]) low++;
-        const uint32_t b = (uint32_t)__builtin_ctzll(bits[low]);
+        return (uint32_t)(low * 64u) + (uint32_t)__builtin_ctzll(bits[low]);
+    }
+    uint32_t take() { // (not when empty)
+        const uint32_t x = lowest();
         bits[low] &= bits[low] - 1ull;
         count--;
-        return (uint32_t)(low * 64u + b);
+        return x;
     }
     void take(uint32_t x) {
         bits[x / 64u] &= ~(1ull << (x % 64u));
@@ -89,8 +92,9 @@ class PageBook {
             set_error("all %u sequences are in use", max_seqs);
             return MKV_ERR_NOMEM;
         }
-        std::vector<uint32_t> written((size_t)n_layers, 0u);
-        open(*out = free_seqs.take(), 0u, written);
+        const uint32_t c = free_seqs.lowest();
+        seqs[c].written.assign((size_t)n_layers, 0u); // (what may fail for want of memory comes first)
+        open(*out = free_seqs.take(), 0u);
         return MKV_OK;
     }
 
@@ -110,32 +114,32 @@ class PageBook {
             set_error("fork of %d sequences: %u sequences and %u pages are free", n, free_seqs.size(), free_pages.size());
             return MKV_ERR_NOMEM;
         }
-        // all that may fail for want of memory comes first
-        std::vector<std::vector<uint32_t>> pages((size_t)n), written((size_t)n);
-        for (int i = 0; i < n; i++) {
-            pages[i].assign(seqs[s].pages.begin(), seqs[s].pages.begin() + np);
-            written[i] = seqs[s].written;
-            for (uint32_t &w : written[i]) w = std::min(w, len);
+        // All that may fail for want of memory comes first; a sequence keeps its vectors' room for the next one of its number.
+        for (uint32_t i = 0, c = free_seqs.lowest(); i < (uint32_t)n; i++, c++) {
+            while (!free_seqs.has(c)) c++;
+            seqs[c].pages.reserve(np);
+            seqs[c].written.assign((size_t)n_layers, 0u);
         }
         ops.reserve(ops.size() + (size_t)n * (copy ? np : 1u));
         if (copy) copies.reserve(copies.size() + (size_t)n * np);
+        const std::vector<uint32_t> &pages = seqs[s].pages;
         for (int i = 0; i < n; i++) {
             const uint32_t c = children[i] = free_seqs.take();
-            open(c, len, written[i]);
-            seqs[c].pages.swap(pages[i]);
-            for (uint32_t j = 0; j < np; j++) {
-                uint32_t &p = seqs[c].pages[j];
-                if (copy) {
-                    const uint32_t d = take_page();
-                    copies.push_back({p, d, std::min(page, len - j * page)});
-                    p = d;
-                    entry(c, j, d);
-                } else {
-                    refs[p]++;
-                }
+            open(c, len);
+            for (int l = 0; l < n_layers; l++) seqs[c].written[(size_t)l] = std::min(seqs[s].written[(size_t)l], len);
+            if (!copy) {
+                seqs[c].pages.assign(pages.begin(), pages.begin() + np);
+                if (np > 0u) ops.push_back({c * max_pages, s * max_pages, np | TableOp::COPY});
+                continue;
             }
-            if (!copy && np > 0u) ops.push_back({c * max_pages, s * max_pages, np | TableOp::COPY});
+            for (uint32_t j = 0; j < np; j++) {
+                const uint32_t d = take_page();
+                copies.push_back({pages[j], d, std::min(page, len - j * page)});
+                seqs[c].pages.push_back(d);
+                entry(c, j, d);
+            }
         }
+        for (uint32_t j = 0; !copy && j < np; j++) refs[pages[j]] += (uint32_t)n;
         return MKV_OK;
     }
 
@@ -197,40 +201,12 @@ class PageBook {
     mkv_status write(int layer, const mkv_seq_rows *items, int n, bool dry) {
         clock++;
         uint64_t fresh = 0;
-        std::unordered_map<uint32_t, uint32_t> left; // pages that items of this call leave to their other holders
-        for (int i = 0; i < n; i++) {
-            const mkv_seq_rows &it = items[i];
-            mkv_status st = need(it.seq);
-            if (st != MKV_OK) return st;
-            Seq &s = seqs[it.seq];
-            if (s.stamp == clock) {
-                set_error("sequence %u is named twice", it.seq);
-                return MKV_ERR_INVALID;
-            }
-            s.stamp = clock;
-            const uint64_t end = (uint64_t)it.pos + it.ntok;
-            if (end > max_tokens) {
-                set_error("rows [%u, %llu) do not fit a sequence of %llu", it.pos, (unsigned long long)end, (unsigned long long)max_tokens);
-                return MKV_ERR_CAPACITY;
-            }
-            if (it.pos > s.written[(size_t)layer]) {
-                set_error("sequence %u has %u rows in layer %d: a write at %u would leave a gap", it.seq, s.written[(size_t)layer], layer, it.pos);
-                return MKV_ERR_STATE;
-            }
-            if (it.ntok == 0u) continue;
-            const uint32_t have = (uint32_t)s.pages.size(), last = (uint32_t)((end - 1u) / page);
-            if (last >= max_pages) { // (a pool of fewer pages than its longest sequence would need)
-                set_error("rows [%u, %llu) need more pages than the pool has", it.pos, (unsigned long long)end);
-                return MKV_ERR_NOMEM;
-            }
-            for (uint32_t j = it.pos / page; j <= last && j < have; j++)
-                if (refs[s.pages[j]] > 1u && refs[s.pages[j]] - left[s.pages[j]] > 1u) {
-                    left[s.pages[j]]++;
-                    fresh++;
-                }
-            if (last >= have) fresh += last + 1u - have;
-            grow_room(s.pages, last + 1u);
-        }
+        // Pages that an item of this call leaves to their other holders count one holder less for the items behind it. refs is put back
+        // before anything is decided.
+        left.clear();
+        const mkv_status st = plan(layer, items, n, fresh);
+        for (uint32_t p : left) refs[p]++;
+        if (st != MKV_OK) return st;
         if (fresh > free_pages.size()) {
             set_error("%llu pages are wanted, %u are free", (unsigned long long)fresh, free_pages.size());
             return MKV_ERR_NOMEM;
@@ -306,17 +282,65 @@ class PageBook {
   private:
     FreeSet free_pages, free_seqs;
     std::vector<uint32_t> refs; // sequences that have the page
+    std::vector<uint32_t> left; // of write()
     uint64_t clock = 0;
 
     static void grow_room(std::vector<uint32_t> &v, size_t n) {
         if (n > v.capacity()) v.reserve(std::max(n, 2u * v.capacity()));
     }
-    void open(uint32_t s, uint32_t len, std::vector<uint32_t> &written) {
-        Seq &q = seqs[s];
-        q.live = true;
-        q.len = len;
-        q.pages.clear();
-        q.written.swap(written);
+    void open(uint32_t s, uint32_t len) {
+        seqs[s].live = true;
+        seqs[s].len = len;
+        seqs[s].pages.clear();
+    }
+    // The checks of write(); `fresh`: the pages that it needs.
+    mkv_status plan(int layer, const mkv_seq_rows *items, int n, uint64_t &fresh) {
+        for (int i = 0; i < n; i++) {
+            const mkv_seq_rows &it = items[i];
+            mkv_status st = need(it.seq);
+            if (st != MKV_OK) return st;
+            Seq &s = seqs[it.seq];
+            if (s.stamp == clock) {
+                set_error("sequence %u is named twice", it.seq);
+                return MKV_ERR_INVALID;
+            }
+            s.stamp = clock;
+            const uint64_t end = (uint64_t)it.pos + it.ntok;
+            if (end > max_tokens) {
+                set_error("rows [%u, %llu) do not fit a sequence of %llu", it.pos, (unsigned long long)end, (unsigned long long)max_tokens);
+                return MKV_ERR_CAPACITY;
+            }
+            if (it.pos > s.written[(size_t)layer]) {
+                set_error("sequence %u has %u rows in layer %d: a write at %u would leave a gap", it.seq, s.written[(size_t)layer], layer, it.pos);
+                return MKV_ERR_STATE;
+            }
+            if (it.ntok == 0u) continue;
+            const uint32_t have = (uint32_t)s.pages.size(), last = (uint32_t)((end - 1u) / page);
+            if (last >= max_pages) { // (a pool of fewer pages than its longest sequence would need)
+                set_error("rows [%u, %llu) need more pages than the pool has", it.pos, (unsigned long long)end);
+                return MKV_ERR_NOMEM;
+            }
+            for (uint32_t j = it.pos / page; j <= last && j < have; j++) {
+                const uint32_t p = s.pages[j];
+                if (refs[p] == 1u) continue;
+                try {
+                    left.push_back(p);
+                } catch (const std::bad_alloc &) {
+                    set_error("out of host memory");
+                    return MKV_ERR_NOMEM;
+                }
+                refs[p]--;
+                fresh++;
+            }
+            if (last >= have) fresh += last + 1u - have;
+            try {
+                grow_room(s.pages, last + 1u);
+            } catch (const std::bad_alloc &) {
+                set_error("out of host memory");
+                return MKV_ERR_NOMEM;
+            }
+        }
+        return MKV_OK;
     }
     uint32_t take_page() {
         const uint32_t p = free_pages.take();

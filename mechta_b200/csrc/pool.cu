@@ -8,51 +8,30 @@
 
 namespace mkv {
 
-// ---- page tables -------------------------------------------------------------------------------------------------
-// The changes travel in the parameter space: no staging memory whose reuse a captured launch would have to survive.
-constexpr uint32_t TABLE_OPS = 320;
-struct TableOps {
-    uint32_t n;
-    TableOp op[TABLE_OPS];
+// ---- what the books ask for --------------------------------------------------------------------------------------
+// Changes of the page tables and copies of pages, in one launch: both lists travel in the parameter space (no staging memory whose reuse
+// a captured launch would have to survive), and copies read pages by their numbers, so their order does not matter. Copies are two
+// bytes of traffic for each byte and nothing to compute: HBM-bound (30,011 tokens of ten layers copied and compacted: 2.46 GB in
+// 375 us, the rate of a plain copy). A block copies 16 KB of one page, of K or V of one layer, four 16-byte loads of a thread in flight.
+constexpr uint32_t BOOK_ENTRIES = 160;
+struct BookArgs {
+    uint32_t n_copies, n_ops;
+    PageCopy c[BOOK_ENTRIES];
+    TableOp op[BOOK_ENTRIES];
 };
-static_assert(sizeof(TableOps) <= 4000, "kernel parameters");
-
-__global__ void __launch_bounds__(128) table_kernel(const __grid_constant__ TableOps ops, uint32_t *__restrict__ table) {
-    ptx::pdl_wait();
-    ptx::pdl_launch_dependents();
-    const TableOp &o = ops.op[blockIdx.x];
-    const uint32_t n = o.n & ~TableOp::COPY;
-    for (uint32_t i = threadIdx.x; i < n; i += 128u) table[o.dst + i] = (o.n & TableOp::COPY) ? table[o.val + i] : o.val + i;
-}
-
-mkv_status launch_table_ops(Pool *p) {
-    std::vector<TableOp> &ops = p->book.ops;
-    for (size_t i = 0; p->ctx && i < ops.size(); i += TABLE_OPS) {
-        TableOps t;
-        t.n = (uint32_t)std::min<size_t>(TABLE_OPS, ops.size() - i);
-        std::copy_n(ops.begin() + (long)i, t.n, t.op);
-        PdlLaunch l(p->ctx, dim3(t.n), 128);
-        MKV_CUDA(cudaLaunchKernelEx(&l.cfg, table_kernel, t, p->table));
-        p->ctx->launches++;
-    }
-    ops.clear();
-    return MKV_OK;
-}
-
-// ---- page copies -------------------------------------------------------------------------------------------------
-// Two bytes of traffic for each byte copied and nothing to compute: HBM-bound. A block copies 16 KB of one page, of K or V of one
-// layer, four 16-byte loads of a thread in flight.
-constexpr uint32_t PAGE_COPIES = 320;
-struct PageCopies {
-    uint32_t n;
-    PageCopy c[PAGE_COPIES];
-};
-static_assert(sizeof(PageCopies) <= 4000, "kernel parameters");
+static_assert(sizeof(BookArgs) <= 4000, "kernel parameters");
 
 __global__ void __launch_bounds__(256)
-page_copy_kernel(const __grid_constant__ PageCopies list, char *__restrict__ mem, size_t layer_bytes, size_t page_bytes, uint32_t row_bytes) {
+books_kernel(const __grid_constant__ BookArgs list, char *__restrict__ mem, size_t layer_bytes, size_t page_bytes, uint32_t row_bytes, uint32_t *__restrict__ table) {
     ptx::pdl_wait();
     ptx::pdl_launch_dependents();
+    if (blockIdx.y >= list.n_copies) {
+        if (blockIdx.x != 0u || blockIdx.z != 0u) return;
+        const TableOp &o = list.op[blockIdx.y - list.n_copies];
+        const uint32_t n = o.n & ~TableOp::COPY;
+        for (uint32_t i = threadIdx.x; i < n; i += 256u) table[o.dst + i] = (o.n & TableOp::COPY) ? table[o.val + i] : o.val + i;
+        return;
+    }
     const PageCopy &c = list.c[blockIdx.y];
     const uint32_t bytes = c.rows * row_bytes; // (a page is at most 256 rows of 64 heads of 256 f32: 16 MB)
     char *base = mem + (size_t)blockIdx.z * layer_bytes;
@@ -68,27 +47,28 @@ page_copy_kernel(const __grid_constant__ PageCopies list, char *__restrict__ mem
         if (at + 4096u * i < bytes) *reinterpret_cast<uint4 *>(dst + at + 4096u * i) = v[i];
 }
 
-mkv_status launch_page_copies(Pool *p) {
+// Launches what is in the lists and clears them.
+static mkv_status follow_books(Pool *p) {
     std::vector<PageCopy> &cs = p->book.copies;
-    for (size_t i = 0; p->ctx && i < cs.size(); i += PAGE_COPIES) {
-        PageCopies t;
-        t.n = (uint32_t)std::min<size_t>(PAGE_COPIES, cs.size() - i);
-        std::copy_n(cs.begin() + (long)i, t.n, t.c);
+    std::vector<TableOp> &ops = p->book.ops;
+    for (size_t i = 0, j = 0; i < cs.size() || j < ops.size();) {
+        BookArgs t;
+        t.n_copies = (uint32_t)std::min<size_t>(BOOK_ENTRIES, cs.size() - i);
+        t.n_ops = (uint32_t)std::min<size_t>(BOOK_ENTRIES, ops.size() - j);
+        std::copy_n(cs.begin() + (long)i, t.n_copies, t.c);
+        std::copy_n(ops.begin() + (long)j, t.n_ops, t.op);
+        i += t.n_copies;
+        j += t.n_ops;
         uint32_t rows = 0;
-        for (uint32_t k = 0; k < t.n; k++) rows = std::max(rows, t.c[k].rows);
-        const unsigned chunks = (unsigned)((rows * p->row_bytes + 16383u) / 16384u);
-        PdlLaunch l(p->ctx, dim3(chunks, t.n, 2u * (unsigned)p->desc.n_layers), 256);
-        MKV_CUDA(cudaLaunchKernelEx(&l.cfg, page_copy_kernel, t, p->mem, p->layer_bytes, p->page_bytes, (uint32_t)p->row_bytes));
+        for (uint32_t k = 0; k < t.n_copies; k++) rows = std::max(rows, t.c[k].rows);
+        const unsigned chunks = (unsigned)std::max<size_t>(1u, (rows * p->row_bytes + 16383u) / 16384u);
+        PdlLaunch l(p->ctx, dim3(chunks, t.n_copies + t.n_ops, t.n_copies ? 2u * (unsigned)p->desc.n_layers : 1u), 256);
+        MKV_CUDA(cudaLaunchKernelEx(&l.cfg, books_kernel, t, p->mem, p->layer_bytes, p->page_bytes, (uint32_t)p->row_bytes, p->table));
         p->ctx->launches++;
     }
     cs.clear();
+    ops.clear();
     return MKV_OK;
-}
-
-// What the books ask for: copies read pages by their numbers, so their order among the table's changes does not matter.
-static mkv_status follow_books(Pool *p) {
-    mkv_status st = launch_page_copies(p);
-    return st == MKV_OK ? launch_table_ops(p) : st;
 }
 
 // ---- new rows ----------------------------------------------------------------------------------------------------

@@ -33,8 +33,6 @@ struct PoolAttn {
     uint32_t window;
     const float *sinks;
 };
-mkv_status launch_table_ops(Pool *p);   // and clears the list
-mkv_status launch_page_copies(Pool *p); // and clears the list
 mkv_status launch_pool_write(Pool *p, int layer, const mkv_seq_rows *items, int n, const PoolWrite &w);
 mkv_status launch_pool_attn(Pool *p, int layer, const mkv_seq_rows *items, int n, const PoolAttn &a);
 mkv_status pool_attn_setup(Pool *p);    // scratch, kernel attributes
