@@ -310,7 +310,8 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         const uint32_t lane_addr = (32u * q4) << 16;
         constexpr uint32_t HD = DIM / 2; // dims of Q and O of a thread
         float *red = reinterpret_cast<float *>(smem + Z::OFF_RED);
-        const uint32_t group = plan.group, tok = row / group, head = row - tok * group, bar_pair = 1u + q4;
+        const uint32_t group = plan.group, inv_group = 65536u / group + 1u, tok = row * inv_group >> 16, head = row - tok * group; // (rows < 128, groups <= 64)
+        const uint32_t bar_pair = 1u + q4;
         auto arrive = [&](uint32_t bar) { // one arrival per warp, after all its lanes
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
@@ -334,7 +335,7 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             const __half *src = g.q + (int64_t)(plan.seq[sg.seq].row + sg.it.tok0) * g.q_stride + (size_t)sg.kvh * group * DIM + (half * CPR + lane % CPR) * 8u;
 #pragma unroll
             for (uint32_t i = 0; i < QB; i++) {
-                const uint32_t r = 32u * q4 + (b * QB + i) * RPI + lane / CPR, t = r / group;
+                const uint32_t r = 32u * q4 + (b * QB + i) * RPI + lane / CPR, t = r * inv_group >> 16;
                 qv[i] = make_uint4(0u, 0u, 0u, 0u);
                 if (r < rows) qv[i] = __ldg(reinterpret_cast<const uint4 *>(src + (int64_t)t * g.q_stride + (r - t * group) * DIM));
             }
@@ -417,15 +418,17 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                         const uint32_t r = idx / (DIM / 8u);
                         *v_chunk(r < z0 ? r : r - z0 + z1, idx % (DIM / 8u)) = make_uint4(0u, 0u, 0u, 0u);
                     }
+                    bool found = false;
                     for (uint32_t idx = st; idx < (p0 - z0 + z1 - p1) * (DIM / 8u); idx += 256u) {
                         const uint32_t i = idx / (DIM / 8u), r = i < p0 - z0 ? z0 + i : i - (p0 - z0) + p1;
                         const uint4 v = *v_chunk(r, idx % (DIM / 8u));
-                        if (half2_not_finite(v.x) || half2_not_finite(v.y) || half2_not_finite(v.z) || half2_not_finite(v.w))
+                        if (half2_not_finite(v.x) || half2_not_finite(v.y) || half2_not_finite(v.z) || half2_not_finite(v.w)) {
                             atomicOr(&sh->bad[t & 1u][r >> 5], 1u << (r & 31u));
+                            found = true;
+                        }
                     }
-                    if (it.ntok > 1u) { // (else all its rows see the same keys)
-                        named_bar_sync(5, 256);
-                        bad_any = (sh->bad[t & 1u][0] | sh->bad[t & 1u][1] | sh->bad[t & 1u][2] | sh->bad[t & 1u][3]) != 0u;
+                    if (p0 - z0 + z1 - p1 != 0u) {
+                        bad_any = named_bar_or(5, 256, found);
                         for (uint32_t idx = st; bad_any && idx < PA_KEYS * (DIM / 8u); idx += 256u) {
                             const uint32_t r = idx / (DIM / 8u);
                             if (sh->bad[t & 1u][r >> 5] >> (r & 31u) & 1u) *v_chunk(r, idx % (DIM / 8u)) = make_uint4(0u, 0u, 0u, 0u);
@@ -438,13 +441,16 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                     // work in base-2 exponents: e^(s scale - m) = 2^(s C - m2), C = scale log2(e)
                     float mt[4] = {NEG_BIG, NEG_BIG, NEG_BIG, NEG_BIG};
                     if (edge) {
-                        __syncwarp(); // (a branch: most tiles have no masked keys)
+                        // the keys of this half that the row sees, a bit each
                         const uint32_t k = key0 + 64u * half;
+                        auto upto = [&](uint32_t key) { return key <= k ? 0ull : key >= k + 64u ? ~0ull : (1ull << (key - k)) - 1ull; };
+                        const uint64_t see = upto(vis) & ~upto(klo);
+                        const uint32_t bits[2] = {(uint32_t)see, (uint32_t)(see >> 32)};
 #pragma unroll
                         for (int h = 0; h < 2; h++)
 #pragma unroll
                             for (int c = 0; c < 32; c++)
-                                if (k + 32u * h + c < klo || k + 32u * h + c >= vis) sr[h][c] = 0xff800000u; // -infinity
+                                if (!(bits[h] & (1u << c))) sr[h][c] = 0xff800000u; // -infinity
                     }
 #pragma unroll
                     for (int h = 0; h < 2; h++)
@@ -536,24 +542,41 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                     float den = l_all;
                     if (g.sinks && real) den += exp2f(g.sinks[sg.kvh * group + head] * PA_LOG2E - (m_ref > NEG_TEST ? m_ref : 0.0f));
                     const float inv = 1.0f / den;
-                    __half *dst = g.out + (int64_t)(sq.row + it.tok0 + tok) * g.out_stride + (size_t)(sg.kvh * group + head) * DIM + HD * half;
+                    // A lane has 64 bytes of its row at a time. Four lanes exchange them, so that each has 16 bytes of each of their four rows and
+                    // a store of the warp touches eight lines instead of 32.
+                    const uint32_t q = lane & 3u;
+                    __half *dst[4];
+#pragma unroll
+                    for (uint32_t i = 0; i < 4u; i++) {
+                        const uint32_t r = (row & ~3u) + i, t = r * inv_group >> 16;
+                        dst[i] = r < rows ? g.out + (int64_t)(sq.row + it.tok0 + t) * g.out_stride + (size_t)(sg.kvh * group + (r - t * group)) * DIM + HD * half + 8u * q : nullptr;
+                    }
 #pragma unroll 1
                     for (uint32_t c0 = 0; c0 < HD; c0 += 32u) {
                         uint32_t orow[32];
                         tmem_ld32(tmem + lane_addr + HD * half + c0, orow);
                         tmem_wait_ld();
-                        if (real) {
+                        uint32_t w[4][4]; // [16-byte chunk][word]
 #pragma unroll
-                            for (int c = 0; c < 32; c += 8) {
-                                uint32_t w[4];
+                        for (int c = 0; c < 32; c += 2) {
+                            const __half2 h2 = __floats2half2_rn(seen ? __uint_as_float(orow[c]) * inv : 0.0f, seen ? __uint_as_float(orow[c + 1]) * inv : 0.0f);
+                            w[c >> 3][(c >> 1) & 3] = *reinterpret_cast<const uint32_t *>(&h2);
+                        }
+#pragma unroll
+                        for (uint32_t m = 1u; m <= 2u; m <<= 1) // chunk and lane change places, a bit of their numbers at a time
+#pragma unroll
+                            for (uint32_t c = 0; c < 4u; c++) {
+                                if (c & m) continue;
 #pragma unroll
                                 for (int e = 0; e < 4; e++) {
-                                    const __half2 h2 = __floats2half2_rn(seen ? __uint_as_float(orow[c + 2 * e]) * inv : 0.0f, seen ? __uint_as_float(orow[c + 2 * e + 1]) * inv : 0.0f);
-                                    w[e] = *reinterpret_cast<const uint32_t *>(&h2);
+                                    const uint32_t got = __shfl_xor_sync(0xffffffffu, (q & m) ? w[c][e] : w[c | m][e], m);
+                                    if (q & m) w[c][e] = got;
+                                    else w[c | m][e] = got;
                                 }
-                                *reinterpret_cast<uint4 *>(dst + c0 + c) = make_uint4(w[0], w[1], w[2], w[3]);
                             }
-                        }
+#pragma unroll
+                        for (uint32_t i = 0; i < 4u; i++)
+                            if (dst[i]) *reinterpret_cast<uint4 *>(dst[i] + c0) = make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]);
                     }
                 } else {
                     // a part: maximum, sum and O as they are, for the merge
