@@ -73,7 +73,8 @@ static mkv_status follow_books(Pool *p) {
 
 // ---- new rows ----------------------------------------------------------------------------------------------------
 // K and V of the new tokens into their pages, K rotated on the way, one rounding to the pool's type. Bound by HBM for prefill blocks
-// and by the launch for steps. A block takes one token at a time: cosines and sines once, then its heads of K and of V.
+// and by the launch for steps. A block takes as many tokens as its threads have units for (two units of 8 values a thread; tokens of very
+// many heads are spread over several blocks); the loads are in flight while the tokens' cosines and sines are computed.
 constexpr uint32_t WRITE_ITEMS = 120;
 struct WriteItems {
     uint32_t n;
@@ -87,48 +88,71 @@ struct WriteArgs {
     const uint32_t *pages;
     size_t page_bytes, row_bytes;
     uint32_t page_shift, kv_heads, head_dim, units, row0; // units of a K head; row0: packed row of the launch's first
+    uint32_t tokens;                                      // of a block
 };
 static_assert(sizeof(WriteItems) + sizeof(WriteArgs) + sizeof(RopeTab) <= 4000, "kernel parameters");
+
+constexpr uint32_t WRITE_PER = 2, WRITE_TOKENS = 16; // units of a thread, most tokens of a block
 
 template <int MODE, class TI, class TO>
 __global__ void __launch_bounds__(256)
 pool_write_kernel(const __grid_constant__ WriteItems items, const __grid_constant__ WriteArgs g, const __grid_constant__ RopeTab tab) {
-    __shared__ float2 cs[MKV_ROPE_MAX_DIMS / 2];
+    extern __shared__ float2 cs[]; // [tokens][pairs]
+    __shared__ uint32_t pos_s[WRITE_TOKENS];
+    __shared__ size_t at_s[WRITE_TOKENS];
     ptx::pdl_wait();
     ptx::pdl_launch_dependents();
-    const uint32_t r = blockIdx.x;
-    uint32_t i = 0, end = items.n; // the item with row[i] <= r < row[i + 1]
-    while (i + 1u < end) {
-        const uint32_t mid = (i + end) / 2u;
-        if (items.row[mid] <= r) i = mid;
-        else end = mid;
-    }
-    const uint32_t p = items.pos[i] + (r - items.row[i]);
-    const uint32_t page = g.pages[items.table[i] + (p >> g.page_shift)];
-    const size_t at = (size_t)page * g.page_bytes + (size_t)(p & ((1u << g.page_shift) - 1u)) * g.row_bytes;
-    const TI *k = static_cast<const TI *>(g.k) + (int64_t)(g.row0 + r) * g.k_stride;
-    const TI *v = static_cast<const TI *>(g.v) + (int64_t)(g.row0 + r) * g.v_stride;
-    TO *kd = reinterpret_cast<TO *>(g.kpages + at), *vd = reinterpret_cast<TO *>(g.vpages + at);
-    for (uint32_t j = threadIdx.x; j < tab.pairs; j += 256u) cs[j] = rope_cs(tab, j, (int32_t)p);
-    __syncthreads();
-    const uint32_t nk = g.kv_heads * g.units, nv = g.kv_heads * g.head_dim / 8u;
-    for (uint32_t j = threadIdx.x; j < nk + nv; j += 256u) {
-        float a[8], b[8];
-        if (j < nk) {
-            const uint32_t head = j / g.units, u = j % g.units;
-            rope_load<MODE>(k + head * g.head_dim, u, tab.pairs, tab.interleaved, a, b);
-            rope_store<MODE>(kd + head * g.head_dim, u, tab.pairs, tab.interleaved, cs, a, b);
+    const uint32_t row0 = blockIdx.x * g.tokens, n = min(g.tokens, items.row[items.n] - row0);
+    const uint32_t nk = g.kv_heads * g.units, nv = g.kv_heads * g.head_dim / 8u, units = nk + nv;
+    float a[WRITE_PER][8], b[WRITE_PER][8];
+    uint32_t tok[WRITE_PER], unit[WRITE_PER];
+#pragma unroll
+    for (uint32_t w = 0; w < WRITE_PER; w++) {
+        const uint32_t idx = (blockIdx.y * WRITE_PER + w) * 256u + threadIdx.x;
+        tok[w] = idx / units;
+        unit[w] = idx % units;
+        if (tok[w] >= n) continue;
+        if (unit[w] < nk) {
+            const uint32_t head = unit[w] / g.units, u = unit[w] % g.units;
+            rope_load<MODE>(static_cast<const TI *>(g.k) + (int64_t)(g.row0 + row0 + tok[w]) * g.k_stride + head * g.head_dim, u, tab.pairs, tab.interleaved, a[w], b[w]);
         } else {
-            const uint32_t e = 8u * (j - nk);
-            if constexpr (MODE == ROPE_ANY) load8<false>(v + e, a);
-            else load8<true>(v + e, a);
-            store8<true>(vd + e, a);
+            const TI *v = static_cast<const TI *>(g.v) + (int64_t)(g.row0 + row0 + tok[w]) * g.v_stride + 8u * (unit[w] - nk);
+            if constexpr (MODE == ROPE_ANY) load8<false>(v, a[w]);
+            else load8<true>(v, a[w]);
+        }
+    }
+    if (threadIdx.x < n) { // where the token's rows go
+        const uint32_t r = row0 + threadIdx.x;
+        uint32_t i = 0, end = items.n; // the item with row[i] <= r < row[i + 1]
+        while (i + 1u < end) {
+            const uint32_t mid = (i + end) / 2u;
+            if (items.row[mid] <= r) i = mid;
+            else end = mid;
+        }
+        const uint32_t p = items.pos[i] + (r - items.row[i]);
+        pos_s[threadIdx.x] = p;
+        at_s[threadIdx.x] = (size_t)g.pages[items.table[i] + (p >> g.page_shift)] * g.page_bytes + (size_t)(p & ((1u << g.page_shift) - 1u)) * g.row_bytes;
+    }
+    __syncthreads();
+    if (tab.pairs) {
+        for (uint32_t j = threadIdx.x; j < n * tab.pairs; j += 256u) cs[j] = rope_cs(tab, j % tab.pairs, (int32_t)pos_s[j / tab.pairs]);
+        __syncthreads();
+    }
+#pragma unroll
+    for (uint32_t w = 0; w < WRITE_PER; w++) {
+        if (tok[w] >= n) continue;
+        if (unit[w] < nk) {
+            const uint32_t head = unit[w] / g.units, u = unit[w] % g.units;
+            rope_store<MODE>(reinterpret_cast<TO *>(g.kpages + at_s[tok[w]]) + head * g.head_dim, u, tab.pairs, tab.interleaved, cs + tok[w] * tab.pairs, a[w], b[w]);
+        } else {
+            store8<true>(reinterpret_cast<TO *>(g.vpages + at_s[tok[w]]) + 8u * (unit[w] - nk), a[w]);
         }
     }
 }
 
 template <class TI, class TO> static mkv_status launch_write(Ctx *ctx, int mode, uint32_t rows, const WriteItems &it, const WriteArgs &g, const RopeTab &tab) {
-    PdlLaunch l(ctx, dim3(rows), 256);
+    const uint32_t units = g.kv_heads * (g.units + g.head_dim / 8u), per = 256u * WRITE_PER;
+    PdlLaunch l(ctx, dim3((rows + g.tokens - 1u) / g.tokens, (g.tokens * units + per - 1u) / per), 256, (size_t)g.tokens * tab.pairs * sizeof(float2));
     switch (mode) {
     case ROPE_COPY: MKV_CUDA(cudaLaunchKernelEx(&l.cfg, pool_write_kernel<ROPE_COPY, TI, TO>, it, g, tab)); break;
     case ROPE_HALF8: MKV_CUDA(cudaLaunchKernelEx(&l.cfg, pool_write_kernel<ROPE_HALF8, TI, TO>, it, g, tab)); break;
@@ -171,7 +195,9 @@ mkv_status launch_pool_write(Pool *p, int layer, const mkv_seq_rows *items, int 
                 it.n++;
             }
         if (it.n == 0u) break;
-        const uint32_t rows = it.row[it.n];
+        const uint32_t rows = it.row[it.n], token_units = g.kv_heads * (g.units + g.head_dim / 8u);
+        // few rows: a block each, for the latency; many: blocks that are full
+        g.tokens = rows < 2u * (uint32_t)p->ctx->sm_count ? 1u : std::max(1u, std::min(WRITE_TOKENS, 256u * WRITE_PER / token_units));
         const bool o16 = p->desc.fmt == MKV_F16;
         mkv_status st;
         if (w.fmt == MKV_F16)

@@ -340,10 +340,14 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 if (r < rows) qv[i] = __ldg(reinterpret_cast<const uint4 *>(src + (int64_t)t * g.q_stride + (r - t * group) * DIM));
             }
         };
+        bool clean = false; // this quarter's rows in shared memory are zeros
         auto put_q = [&](const PlanSegment &sg) { // the first batch has been fetched
             const uint32_t c = half * CPR + lane % CPR; // chunk of the row
+            // (rows that no segment uses are zeros too: products of nothing draw less power, and the clock is bound by that)
+            const bool rows = 32u * q4 < sg.it.ntok * group, write = rows || !clean;
+            clean = !rows;
 #pragma unroll 1
-            for (uint32_t b = 0; b < CPR / QB && 32u * q4 < sg.it.ntok * group; b++) {
+            for (uint32_t b = 0; b < CPR / QB && write; b++) {
                 if (b > 0u) fetch_q(sg, b);
 #pragma unroll
                 for (uint32_t i = 0; i < QB; i++)
