@@ -12,11 +12,10 @@
 //
 // Conversion in place: TMA brings a tile as blocks of [64 keys][32 dims] (rows of 128 bytes, 128-byte swizzle); two lanes read the 256
 // bytes that a key has in two neighbouring blocks and write its 64 hi values into the first block's row and its 64 lo values into the
-// second's, so a tile needs no second buffer. The scale of a tile (K and V each their own) is the one in front's as long as the
-// tile's largest finite value then lies in [2^8, 2^15); otherwise the tile is converted once more, from global memory, with its own
-// scale: no f32 value overflows, and what is lost of a value is 2^-23 of it, or 2^-33 of the tile's
-// largest. Values that are not finite are zero in the
-// operands; their keys are noted, and the softmax threads add their share with ordinary arithmetic for the rows that see them. Keys
+// second's, so a tile needs no second buffer. The scale of a tile (K and V each their own) is the one in front's as long as each
+// converter warp's largest value then lies in [2^8, 2^15) or is zero; otherwise, and where a value is not finite, the tile is converted
+// once more, from global memory, with its own scale: no f32 value overflows, and what is lost of a value is 2^-23 of it, or 2^-33 of
+// the tile's largest. Values that are not finite are zero in the operands; their keys are noted, and the softmax threads add their share with ordinary arithmetic for the rows that see them. Keys
 // that no token of the item sees are zero as well, whatever lies in their rows.
 //
 // Bound by HBM for few rows (a 64-key tile of 256 dims is 128 KB, 5,600 clocks of an SM's share of 6.4 TB/s, and about 2,600 of
@@ -179,6 +178,141 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
 
     // The units of the CTA's T tiles in ring order, whatever segment they belong to: K(0), then K(t + 1) and V(t) for each t. In front of
     // K(t) are t + max(t - 1, 0) tiles of K and V, in front of V(t) min(t + 2, T) + t.
+    // ---------------- converters: a warp has 16 keys of every unit, a lane one of a key's two blocks ----------------
+    auto converter = [&]() {
+        const uint32_t cw = warp - 4u, key_in = 16u * cw + (lane >> 1), j = lane & 1u;
+        // chunk of the block's row that x[i] holds: in an order in which a key's two lanes meet no bank together
+        auto chunk = [&](uint32_t i) { return i ^ (4u * j); };
+        PbRing<PB_NST> at;
+        struct Tile {
+            uint32_t key0, lo, hi, table, kvh;
+        };
+        PbStream ts(plan);
+        auto take = [&](const Tile &last) -> Tile { // the stream's tile, which follows `last`; the stream moves on
+            const PlanItem &it = ts.sg.it;
+            Tile t = {(it.tile0 + ts.tile) * PF_KEYS32, last.lo, last.hi, last.table, last.kvh};
+            if (ts.first()) t = {t.key0, it.lo, it.hi, plan.seq[ts.sg.seq].table, ts.sg.kvh};
+            ts.next();
+            return t;
+        };
+        float k_scale = 1.0f, v_scale = 1.0f;
+        auto convert = [&](bool v, const Tile &tl, uint32_t note) {
+            const uint32_t key = tl.key0 + key_in;
+            const bool in = key >= tl.lo && key < tl.hi, whole = tl.key0 >= tl.lo && tl.key0 + PF_KEYS32 <= tl.hi;
+            const PbRing<PB_NST> begin = at;
+            float amax = 0.0f;
+            bool odd = false; // a value of this lane's is not finite
+            float s = v ? v_scale : k_scale;
+            auto fetch = [&](uint32_t slot, float4 (&x)[8]) { // this lane's values of a unit
+                const uint8_t *u = smem + slot * PB_UNIT + j * PB_BLK;
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; i++) x[i] = *reinterpret_cast<const float4 *>(u + swz128(key_in, chunk(i)));
+            };
+            auto put = [&](uint32_t slot, const float4 (&x)[8]) { // to hi and lo
+                uint8_t *u = smem + slot * PB_UNIT;
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; i += 2u) {
+                    const float y[8] = {x[i].x, x[i].y, x[i].z, x[i].w, x[i + 1].x, x[i + 1].y, x[i + 1].z, x[i + 1].w};
+                    uint4 hi, lo;
+                    split8(y, s, hi, lo);
+                    const uint32_t at_row = swz128(key_in, 4u * j + (chunk(i) >> 1));
+                    *reinterpret_cast<uint4 *>(u + at_row) = hi;
+                    *reinterpret_cast<uint4 *>(u + PB_BLK + at_row) = lo;
+                }
+            };
+            auto look = [&](float4 (&x)[8]) { // amax; odd
+                if (!whole && !in) // (keys that no token of the item sees)
+#pragma unroll
+                    for (uint32_t i = 0; i < 8u; i++) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                uint64_t z[2] = {0ull, 0ull}; // 0 * x is a NaN where x is not finite
+                float top[2] = {amax, 0.0f};
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; i++) {
+                    top[i & 1u] = max3(top[i & 1u], fabsf(x[i].x), fabsf(x[i].y));
+                    top[i & 1u] = max3(top[i & 1u], fabsf(x[i].z), fabsf(x[i].w));
+                    z[i & 1u] = fma2(pack2(x[i].x, x[i].y), 0ull, z[i & 1u]);
+                    z[i & 1u] = fma2(pack2(x[i].z, x[i].w), 0ull, z[i & 1u]);
+                }
+                amax = fmaxf(top[0], top[1]);
+                float z0, z1;
+                unpack2(add2(z[0], z[1]), z0, z1);
+                odd = odd || z0 + z1 != 0.0f;
+            };
+            pb_wait(bar_full + 8u * begin.s, begin.turn, sh, g.status);
+            __syncwarp();
+#pragma unroll 1
+            for (uint32_t h = 0; h < NU; h++) {
+                float4 x[8];
+                fetch(begin.s + h, x);
+                __syncwarp(); // both lanes of a key have read its rows
+                look(x);
+                put(begin.s + h, x);
+            }
+            at.next(NU);
+            // The scale fits if each warp's largest value lies well inside f16's range under it. Otherwise, and where values are not finite, once
+            // more from global memory: the tile's largest finite value, then its values with the scale that this gives, the others as zeros.
+            amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
+            if (named_bar_or(3, 128, odd || (amax != 0.0f && !(amax * s >= 256.0f && amax * s < 32768.0f)))) {
+                const float *src = v ? g.vpages : g.kpages;
+                if (in) {
+                    const size_t page = __ldg(g.pages + tl.table + (key >> g.page_shift));
+                    src += ((page << g.page_shift) + (key & ((1u << g.page_shift) - 1u))) * g.row_floats + (size_t)tl.kvh * DIM + 32u * j;
+                }
+                auto again = [&](uint32_t h, float4 (&x)[8]) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 8u; i++) {
+                        x[i] = in ? *reinterpret_cast<const float4 *>(src + 64u * h + 4u * chunk(i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        float *e = &x[i].x;
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            if (!is_finite_bits(__float_as_uint(e[k]))) e[k] = 0.0f;
+                    }
+                };
+                amax = 0.0f;
+#pragma unroll 1
+                for (uint32_t h = 0; h < NU; h++) {
+                    float4 x[8];
+                    again(h, x);
+#pragma unroll
+                    for (uint32_t i = 0; i < 8u; i++) amax = fmaxf(amax, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
+                }
+                amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
+                if (lane == 0) sh->amax[cw] = __float_as_uint(amax);
+                named_bar_sync(3, 128);
+                uint32_t most = 0u;
+                for (uint32_t i = 0; i < 4u; i++) most = max(most, sh->amax[i]);
+                s = most ? __uint_as_float(scale_bits(most)) : 1.0f;
+                (v ? v_scale : k_scale) = s;
+#pragma unroll 1
+                for (uint32_t h = 0; h < NU; h++) {
+                    float4 x[8];
+                    again(h, x);
+                    put(begin.s + h, x);
+                }
+                named_bar_sync(3, 128); // amax[] has been read
+            }
+            const uint32_t odds = __ballot_sync(0xffffffffu, odd);
+            if (lane == 0) {
+                uint32_t m = 0u;
+                if (odds)
+                    for (uint32_t i = 0; i < 16u; i++) m |= (odds >> (2u * i) & 3u) ? 1u << i : 0u;
+                sh->odd[v ? 1 : 0][note % PB_NOTES][cw] = (uint16_t)m;
+                if (cw == 0u) sh->unscale[v ? 1 : 0][note % PB_NOTES] = __uint_as_float((254u << 23) - __float_as_uint(s)); // 1 / s, s being a power of two
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_conv + 8u * begin.s); // (of the tile's first unit, for all)
+        };
+        // A wait that runs out makes all later ones return at once; the warps go through the same barriers all the same.
+        Tile cur = take(Tile{});
+        convert(false, cur, 0u);
+        for (uint32_t t = 0; t < total; t++) {
+            const Tile ahead = ts.more ? take(cur) : cur;
+            if (t + 1u < total) convert(false, ahead, t + 1u);
+            convert(true, cur, t);
+            cur = ahead;
+        }
+    };
     if (warp < 4u) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
         if (warp == 0 || warp == 3u) {
@@ -205,12 +339,11 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 return t;
             };
             auto load = [&](const CUtensorMap *map, const Tile &t) -> bool { // the units of one K or V tile
-                const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, t.row != ~0u));
+                const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, t.row != ~0u)), bar = bar_full + 8u * at.s; // (of the first unit, for all)
 #pragma unroll 1
                 for (uint32_t h = 0; h < NU; h++, u++, at.next()) {
-                    const uint32_t bar = bar_full + 8u * at.s;
                     if (u >= PB_NST && !__all_sync(0xffffffffu, pb_wait(bar_empty + 8u * at.s, at.turn ^ 1u, sh, g.status))) return false;
-                    if (lane == 0) mbar_expect_tx(bar, boxes * box_rows * 128u);
+                    if (h == 0u && lane == 0) mbar_expect_tx(bar, NU * boxes * box_rows * 128u);
                     __syncwarp();
                     if (t.row != ~0u)
                         tma_load_2d(smem_base + at.s * PB_UNIT + cb * PB_BLK + rb * box_rows * 128u, map, t.x + (int)(64u * h), (int)t.row, bar);
@@ -242,10 +375,10 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                     }
                     if (t >= 2u) ok = ok && pb_wait(bar_s_free + 8u * (t & 1u), ((t >> 1) - 1u) & 1u, sh, g.status);
                     const uint32_t d = tmem + PB_COL_S + 64u * (t & 1u);
+                    ok = ok && pb_wait(bar_conv + 8u * at.s, at.turn, sh, g.status);
+                    tc_fence_after();
 #pragma unroll
                     for (uint32_t h = 0; h < NU; h++) {
-                        ok = ok && pb_wait(bar_conv + 8u * at.s, at.turn, sh, g.status);
-                        tc_fence_after();
                         const uint64_t kd = k_desc + at.s * (PB_UNIT >> 4);
 #pragma unroll
                         for (uint32_t ks = 0; ks < 8u; ks++) // 16 dims an MMA, hi and lo
@@ -269,8 +402,8 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 bool ok = true;
                 for (uint32_t t = 0; ok && t < total; t++) {
                     const uint32_t s0 = at.s;
-#pragma unroll
-                    for (uint32_t h = 0; h < NU; h++, at.next()) ok = ok && pb_wait(bar_conv + 8u * at.s, at.turn, sh, g.status);
+                    ok = ok && pb_wait(bar_conv + 8u * s0, at.turn, sh, g.status);
+                    at.next(NU);
                     ok = ok && pb_wait(bar_p_full, t & 1u, sh, g.status);
                     tc_fence_after();
                     const uint64_t vd = v_desc + s0 * (PB_UNIT >> 4);
@@ -285,135 +418,10 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             }
         }
     } else if (warp < 8u) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-        // ---------------- converters: a warp has 16 keys of every unit, a lane one of a key's two blocks ----------------
-        const uint32_t cw = warp - 4u, key_in = 16u * cw + (lane >> 1), j = lane & 1u;
-        PbRing<PB_NST> at;
-        struct Tile {
-            uint32_t key0, lo, hi, table, kvh;
-        };
-        PbStream ts(plan);
-        auto take = [&]() -> Tile { // the stream's tile; the stream moves on
-            const PlanItem &it = ts.sg.it;
-            const Tile t = {(it.tile0 + ts.tile) * PF_KEYS32, it.lo, it.hi, plan.seq[ts.sg.seq].table, ts.sg.kvh};
-            ts.next();
-            return t;
-        };
-        float k_scale = 1.0f, v_scale = 1.0f;
-        auto convert = [&](bool v, const Tile &tl, uint32_t note) {
-            const uint32_t key = tl.key0 + key_in;
-            const bool in = key >= tl.lo && key < tl.hi, whole = tl.key0 >= tl.lo && tl.key0 + PF_KEYS32 <= tl.hi;
-            const PbRing<PB_NST> begin = at;
-            float amax = 0.0f;
-            bool odd = false; // a value of this lane's is not finite
-            float s = v ? v_scale : k_scale;
-            // 32 values of this lane, x[i] = chunk i ^ 4 j of 4, to hi and lo
-            auto put = [&](uint32_t slot, float4 (&x)[8]) {
-                uint8_t *u = smem + slot * PB_UNIT;
-#pragma unroll
-                for (uint32_t i = 0; i < 8u; i += 2u) {
-                    const float y[8] = {x[i].x, x[i].y, x[i].z, x[i].w, x[i + 1].x, x[i + 1].y, x[i + 1].z, x[i + 1].w};
-                    uint4 hi, lo;
-                    split8(y, s, hi, lo);
-                    const uint32_t at_row = swz128(key_in, 4u * j + ((i ^ (4u * j)) >> 1));
-                    *reinterpret_cast<uint4 *>(u + at_row) = hi;
-                    *reinterpret_cast<uint4 *>(u + PB_BLK + at_row) = lo;
-                }
-            };
-            auto fix = [&](float4 (&x)[8]) { // values that are not finite to zero (rare)
-#pragma unroll
-                for (uint32_t i = 0; i < 8u; i++) {
-                    float *e = &x[i].x;
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        if (!is_finite_bits(__float_as_uint(e[k]))) e[k] = 0.0f;
-                }
-            };
-#pragma unroll 1
-            for (uint32_t h = 0; h < NU; h++, at.next()) {
-                pb_wait(bar_full + 8u * at.s, at.turn, sh, g.status);
-                __syncwarp();
-                const uint8_t *u = smem + at.s * PB_UNIT + j * PB_BLK;
-                float4 x[8];
-#pragma unroll
-                for (uint32_t i = 0; i < 8u; i++) x[i] = *reinterpret_cast<const float4 *>(u + swz128(key_in, i ^ (4u * j))); // (so that a key's two lanes meet no bank together)
-                if (!whole && !in) // (keys that no token of the item sees)
-#pragma unroll
-                    for (uint32_t i = 0; i < 8u; i++) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                uint64_t z = 0ull; // 0 * x is a NaN where x is not finite
-                float top = 0.0f;
-#pragma unroll
-                for (uint32_t i = 0; i < 8u; i++) {
-                    top = max3(top, fabsf(x[i].x), fabsf(x[i].y));
-                    top = max3(top, fabsf(x[i].z), fabsf(x[i].w));
-                    z = fma2(pack2(x[i].x, x[i].y), 0ull, z);
-                    z = fma2(pack2(x[i].z, x[i].w), 0ull, z);
-                }
-                float z0, z1;
-                unpack2(z, z0, z1);
-                if (__any_sync(0xffffffffu, z0 + z1 != 0.0f)) { // (also: both lanes of a key have read its rows)
-                    if (z0 + z1 != 0.0f) odd = true;
-                    fix(x);
-                    top = 0.0f;
-#pragma unroll
-                    for (uint32_t i = 0; i < 8u; i++) top = fmaxf(top, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
-                }
-                amax = fmaxf(amax, top);
-                put(at.s, x);
-            }
-            // The scale fits if each warp's largest value lies well inside f16's range under it; otherwise all look for the tile's largest.
-            amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
-            if (named_bar_or(3, 128, amax != 0.0f && !(amax * s >= 256.0f && amax * s < 32768.0f))) {
-                if (lane == 0) sh->amax[cw] = __float_as_uint(amax);
-                named_bar_sync(3, 128);
-                const uint32_t most = max(max(sh->amax[0], sh->amax[1]), max(sh->amax[2], sh->amax[3]));
-                const float big = __uint_as_float(most) * s;
-                if (!(big >= 256.0f && big < 32768.0f)) { // once more, from global memory, with the tile's own scale
-                    s = __uint_as_float(scale_bits(most));
-                    (v ? v_scale : k_scale) = s;
-                    PbRing<PB_NST> a2 = begin;
-                    const float *src = v ? g.vpages : g.kpages;
-                    if (in) {
-                        const size_t page = __ldg(g.pages + tl.table + (key >> g.page_shift));
-                        src += ((page << g.page_shift) + (key & ((1u << g.page_shift) - 1u))) * g.row_floats + (size_t)tl.kvh * DIM + 32u * j;
-                    }
-#pragma unroll 1
-                    for (uint32_t h = 0; h < NU; h++, a2.next()) {
-                        float4 x[8];
-#pragma unroll
-                        for (uint32_t i = 0; i < 8u; i++) x[i] = in ? *reinterpret_cast<const float4 *>(src + 64u * h + 4u * (i ^ (4u * j))) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        fix(x);
-                        put(a2.s, x);
-                    }
-                }
-                named_bar_sync(3, 128); // amax[] has been read
-            }
-            const uint32_t odds = __ballot_sync(0xffffffffu, odd);
-            if (lane == 0) {
-                uint32_t m = 0u;
-                if (odds)
-                    for (uint32_t i = 0; i < 16u; i++) m |= (odds >> (2u * i) & 3u) ? 1u << i : 0u;
-                sh->odd[v ? 1 : 0][note % PB_NOTES][cw] = (uint16_t)m;
-                if (cw == 0u) sh->unscale[v ? 1 : 0][note % PB_NOTES] = 1.0f / s;
-            }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) {
-                PbRing<PB_NST> a2 = begin;
-                for (uint32_t h = 0; h < NU; h++, a2.next()) mbar_arrive(bar_conv + 8u * a2.s);
-            }
-        };
-        // A wait that runs out makes all later ones return at once; the warps go through the same barriers all the same.
-        Tile cur = take();
-        convert(false, cur, 0u);
-        for (uint32_t t = 0; t < total; t++) {
-            const Tile ahead = ts.more ? take() : cur;
-            if (t + 1u < total) convert(false, ahead, t + 1u);
-            convert(true, cur, t);
-            cur = ahead;
-        }
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        converter();
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;"); // 128 x 48 + 128 x 64 + 256 x 200 = the launch's 512 x 128
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;"); // 128 x 48 + 128 x 80 + 256 x 192 = the launch's 512 x 128
         // ---------------- softmax ----------------
         const uint32_t q4 = warp & 3u, half = (warp - 8u) >> 2;
         const uint32_t lane_addr = (32u * q4) << 16;
