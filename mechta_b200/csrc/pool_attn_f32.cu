@@ -15,8 +15,9 @@
 // second's, so a tile needs no second buffer. The scale of a tile (K and V each their own) is the one in front's as long as each
 // converter warp's largest value then lies in [2^8, 2^15) or is zero; otherwise, and where a value is not finite, the tile is converted
 // once more, from global memory, with its own scale: no f32 value overflows, and what is lost of a value is 2^-23 of it, or 2^-33 of
-// the tile's largest. Values that are not finite are zero in the operands; their keys are noted, and the softmax threads add their share with ordinary arithmetic for the rows that see them. Keys
-// that no token of the item sees are zero as well, whatever lies in their rows.
+// the tile's largest. Values that are not finite are zero in the operands; their keys are noted, and the softmax threads add their
+// share with ordinary arithmetic for the rows that see them. Keys that no token of the item sees are zero as well, whatever lies in
+// their rows.
 //
 // Bound by HBM for few rows (a 64-key tile of 256 dims is 128 KB, 5,600 clocks of an SM's share of 6.4 TB/s, and about 2,600 of
 // products), by the chain softmax - products - fold for long blocks.
@@ -39,8 +40,9 @@ constexpr uint32_t PB_COL_S = 256, PB_COL_Q = 384;
 constexpr uint32_t PB_BLK = 8192;          // [64 keys][32 dims] f32, then [64 keys][64 dims] f16
 constexpr uint32_t PB_UNIT = 2 * PB_BLK;   // 64 dims of a tile
 constexpr uint32_t PB_NST = 12;            // units of the ring: a multiple of a tile's, so that a tile lies in one piece
-constexpr uint32_t PB_OFF_P = PB_NST * PB_UNIT; // P' [128 rows][64 keys] f16; also where S'[64 + r] changes hands
-constexpr uint32_t PB_OFF_RED = PB_OFF_P + 16384; // [2 halves][64 rows] floats, [64 rows] rescale factors, [64 rows] reference maxima
+constexpr uint32_t PB_PBUF = 16384;             // P' [128 rows][64 keys] f16; also where S'[64 + r] changes hands
+constexpr uint32_t PB_OFF_P = PB_NST * PB_UNIT; // two of them, in turn
+constexpr uint32_t PB_OFF_RED = PB_OFF_P + 2 * PB_PBUF; // [2 halves][64 rows] floats, [64 rows] rescale factors, [64 rows] reference maxima
 constexpr uint32_t PB_OFF_BAR = PB_OFF_RED + 1024;
 constexpr uint32_t PB_NBAR = 3 * PB_NST + 7; // full[NST], empty[NST], conv[NST], s_full[2], s_free[2], p_full, pv_done, q_full
 constexpr uint32_t PB_OFF_MISC = PB_OFF_BAR + PB_NBAR * 8;
@@ -409,7 +411,7 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                     const uint64_t vd = v_desc + s0 * (PB_UNIT >> 4);
 #pragma unroll
                     for (uint32_t ks = 0; ks < 8u; ks++) // 16 keys an MMA, hi and lo
-                        tc_mma_f16(tmem, p_desc + (((ks >> 1) * 32u) >> 4), vd + (((ks & 1u) * PB_BLK + (ks >> 1) * 2048u) >> 4), IDESC, ks > 0 ? 1u : 0u);
+                        tc_mma_f16(tmem, p_desc + (((t & 1u) * PB_PBUF + (ks >> 1) * 32u) >> 4), vd + (((ks & 1u) * PB_BLK + (ks >> 1) * 2048u) >> 4), IDESC, ks > 0 ? 1u : 0u);
 #pragma unroll
                     for (uint32_t h = 0; h < NU; h++) tc_commit(bar_empty + 8u * (s0 + h));
                     tc_commit(bar_pv_done);
@@ -441,7 +443,8 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             tc_fence_after();
         };
         // where a thread of row r and this half has its 32 scores or weights in the P' buffer: chunk c of 8 (0..3 in row r, 4..7 in row 64 + r)
-        auto p_chunk = [&](uint32_t c) { return smem + PB_OFF_P + swz128(row + (c >> 2) * 64u, 4u * half + (c & 3u)); };
+        uint8_t *p_buf = smem + PB_OFF_P; // of the tile
+        auto p_chunk = [&](uint32_t c) { return p_buf + swz128(row + (c >> 2) * 64u, 4u * half + (c & 3u)); };
         // Q' of a segment: the row's hi or lo parts, half of the dims, scaled by a power of two of the row's own
         auto load_q = [&](const PlanSegment &sg) -> float {
             const uint32_t rows = sg.it.ntok * group;
@@ -522,8 +525,8 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             const uint32_t end = t0 + (sg.b - sg.a);
 #pragma unroll
             for (uint32_t d = 0; d < HD; d++) O[d] = 0.0f;
-            // O = O * cf + O' of tile t (its weights are against m, as cf is)
-            auto fold = [&](uint32_t t) {
+            // O = O * cf + O' of tile t; its weights are against m, as cf is
+            auto fold = [&](uint32_t t, float m, float cf) {
                 wait(bar_pv_done, t & 1u);
                 const uint64_t odd = *reinterpret_cast<const uint64_t *>(sh->odd[1][t % PB_NOTES]);
                 if (odd != 0ull && hi) { // values of V that are not finite: w v for the rows that see them, added to O' where it lies (rare)
@@ -558,10 +561,8 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             };
             for (uint32_t t = t0; t < end; t++) {
                 const uint32_t key0 = (it.tile0 + sg.a + (t - t0)) * PF_KEYS32;
-                if (t > t0) { // (in front of the scores, so that the registers suffice; also: P' of the tile in front has been multiplied)
-                    if (active) fold(t - 1u);
-                    else wait(bar_pv_done, (t - 1u) & 1u);
-                }
+                p_buf = smem + PB_OFF_P + (t & 1u) * PB_PBUF; // (free: the product of two tiles in front has been folded)
+                const float m_last = m, cf_last = cf;
                 wait(bar_s_full + 8u * (t & 1u), (t >> 1) & 1u);
                 // The half row's 32 scores stay in the P' buffer (keys 8 c .. 8 c + 3 in chunk c, the next four in chunk 4 + c, where their weights go
                 // in the end): the registers are O's.
@@ -650,13 +651,18 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                     named_bar_sync(bar_group, 128);
                     if (!hi) cf = cf_s[row];
                 }
-                arrive(bar_p_full);
+                if (t > t0) { // behind the tile's scores, so that they and the product of the tile in front run together
+                    if (active) fold(t - 1u, m_last, cf_last);
+                    else wait(bar_pv_done, (t - 1u) & 1u);
+                }
+                tc_fence_before();
+                arrive(bar_p_full); // P' is there, and O' is free
             }
             // ---------------- end of the segment ----------------
             more = walk.next(nx);
             if (more) q_next = load_q(nx); // the segment's scores were all there: its Q' may go
             if (active) {
-                fold(end - 1u);
+                fold(end - 1u, m, cf);
                 if (hi) red[64u * half + row] = l;
                 named_bar_sync(bar_group, 128); // (P' is free too: its last products have completed)
                 const float l_all = red[row] + red[64u + row];
