@@ -281,7 +281,7 @@ void mkv_rope_destroy(mkv_rope *r);
 mkv_status mkv_rope_freqs(const mkv_rope *r, double *freqs_host, double *m_host);
 /* y = rotated x for ntok tokens of `heads` heads. backward != 0: the transposed map (angles negated, the same m), which takes
  * the gradient of y to the gradient of x. x and y may be f16 or f32 each, and may be the same memory with the same strides and
- * type (any other overlap is refused). Strides in elements; 0 = dense ([ntok][heads][head_dim]). A head's dims are contiguous. */
+ * type; any other overlap is refused (slices of one buffer, whose tokens lie beside each other, do not overlap). Strides in elements; 0 = dense ([ntok][heads][head_dim]). A head's dims are contiguous. */
 typedef struct {
     const void *x_dev;
     void *y_dev;
@@ -359,7 +359,7 @@ mkv_status mkv_pool_write(mkv_pool *p, int layer, const mkv_seq_rows *items, int
  * blocks together): token t of an item sees first_pos <= key <= pos + t, and with a window key > pos + t - window. The rows must be
  * there (pos + ntok <= the layer's valid rows). A row that sees no key gets zeros.
  * q, out: the pool's type, [tokens of all items, in their order][q_heads][head_dim], token strides in elements (0 = dense; multiples of
- * 16 bytes), 16-byte aligned. scale 0 = 1 / sqrt(head_dim). sinks_dev: [q_heads] logits that join the softmax's maximum and sum and
+ * 16 bytes), 16-byte aligned, not overlapping. scale 0 = 1 / sqrt(head_dim). sinks_dev: [q_heads] logits that join the softmax's maximum and sum and
  * never the output, or NULL. f16 pools: weights are rounded to f16 for the tensor cores (2^-11 of each), everything else is
  * summed in f32; f32 pools: f32-grade throughout. */
 typedef struct {

@@ -231,6 +231,18 @@ struct DeviceScope {
     explicit DeviceScope(Ctx *ctx);
     ~DeviceScope();
 };
+// Rows of `bytes` bytes, `stride` bytes apart, for finding blocks that overlap. Rows that lie between the other block's rows (slices of one
+// buffer, the strides being the same) do not.
+struct RowSpan {
+    uintptr_t at;
+    uint64_t rows, stride, bytes;
+    bool meets(const RowSpan &o) const {
+        if (at >= o.at + (o.rows - 1u) * o.stride + o.bytes || o.at >= at + (rows - 1u) * stride + bytes) return false;
+        if (stride != o.stride || bytes > stride || o.bytes > stride) return true;
+        const uint64_t d = o.at >= at ? (o.at - at) % stride : (stride - (at - o.at) % stride) % stride; // o's rows start this far behind a row
+        return d < bytes || d + o.bytes > stride;
+    }
+};
 // One holder of the ctx (a cache, a pool) less; frees a ctx that was destroyed before its last holder.
 void ctx_release(Ctx *ctx);
 // Tensor map of a [rows][cols] buffer, boxes of 128 bytes x box_rows rows with the 128-byte swizzle.

@@ -47,7 +47,7 @@ books_kernel(const __grid_constant__ BookArgs list, char *__restrict__ mem, size
         if (at + 4096u * i < bytes) *reinterpret_cast<uint4 *>(dst + at + 4096u * i) = v[i];
 }
 
-// Launches what is in the lists and clears them.
+// Launches what is in the lists and clears them; after an error they stay, for the next call.
 static mkv_status follow_books(Pool *p) {
     std::vector<PageCopy> &cs = p->book.copies;
     std::vector<TableOp> &ops = p->book.ops;
@@ -245,7 +245,8 @@ template <class F> static mkv_status change(Pool *p, const F &body) {
     }
     DeviceScope dev(p->ctx);
     if (dev.status != MKV_OK) return dev.status;
-    const mkv_status st = body();
+    mkv_status st = follow_books(p); // (what an earlier call could not launch: entries of one launch do not depend on each other)
+    if (st == MKV_OK) st = body();
     return st == MKV_OK ? follow_books(p) : st;
 }
 
@@ -510,12 +511,18 @@ mkv_status mkv_attn_pool(mkv_pool *h, int layer, const mkv_seq_rows *items, int 
         set_error("q and out must be given and 16-byte aligned, sinks 4-byte aligned");
         return MKV_ERR_INVALID;
     }
+    const uint64_t q_row = (uint64_t)dense * p->elem;
+    if (rows > 0 && RowSpan{(uintptr_t)a.q, rows, (uint64_t)a.q_stride * p->elem, q_row}.meets({(uintptr_t)a.out, rows, (uint64_t)a.out_stride * p->elem, q_row})) {
+        set_error("q and out overlap");
+        return MKV_ERR_INVALID;
+    }
     if (!p->ctx) return no_rows();
     if (rows == 0) return MKV_OK;
     DeviceScope dev(p->ctx);
     if (dev.status != MKV_OK) return dev.status;
     return guarded([&]() -> mkv_status {
-        mkv_status s = prof_begin(p->ctx);
+        mkv_status s = follow_books(p); // (what an earlier call could not launch)
+        if (s == MKV_OK) s = prof_begin(p->ctx);
         if (s == MKV_OK) s = launch_pool_attn(p, layer, items, n, a);
         return s == MKV_OK ? prof_end(p->ctx) : s;
     });

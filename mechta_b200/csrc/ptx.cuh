@@ -280,7 +280,6 @@ __device__ __forceinline__ void tc_commit2(uint32_t bar) {
                  : "memory");
 }
 __device__ __forceinline__ void named_bar_sync(uint32_t id, uint32_t threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-__device__ __forceinline__ void named_bar_arrive(uint32_t id, uint32_t threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 __device__ __forceinline__ bool named_bar_or(uint32_t id, uint32_t threads, bool x) {
     uint32_t r;
     asm volatile(

@@ -84,15 +84,6 @@ template <class TI, class TO> static mkv_status launch_rope(Ctx *ctx, int mode, 
     return MKV_OK;
 }
 
-// First and one-past-last byte of a strided [ntok][heads][head_dim] block
-struct Span {
-    uintptr_t lo, hi;
-};
-static Span span_of(const void *p, uint32_t ntok, uint32_t heads, uint32_t head_dim, int64_t ts, int64_t hs, size_t elem) {
-    const uint64_t last = (uint64_t)(ntok - 1u) * (uint64_t)ts + (uint64_t)(heads - 1u) * (uint64_t)hs + head_dim;
-    return {(uintptr_t)p, (uintptr_t)p + last * elem};
-}
-
 } // namespace mkv
 
 using namespace mkv;
@@ -225,14 +216,14 @@ mkv_status mkv_rope_apply(mkv_ctx *h, const mkv_rope *r, const mkv_rope_rows *in
         set_error("rope: misaligned pointer");
         return MKV_ERR_INVALID;
     }
-    const Span sx = span_of(g.x, in->ntok, in->heads, in->head_dim, g.xt, g.xh, xe), sy = span_of(g.y, in->ntok, in->heads, in->head_dim, g.yt, g.yh, ye);
+    const RowSpan sx = {(uintptr_t)g.x, in->ntok, (uint64_t)g.xt * xe, ((uint64_t)(H - 1) * (uint64_t)g.xh + (uint64_t)D) * xe};
+    const RowSpan sy = {(uintptr_t)g.y, in->ntok, (uint64_t)g.yt * ye, ((uint64_t)(H - 1) * (uint64_t)g.yh + (uint64_t)D) * ye};
     const bool same = g.x == g.y && xe == ye && (in->ntok == 1 || g.xt == g.yt) && (H == 1 || g.xh == g.yh);
-    if (!same && sx.lo < sy.hi && sy.lo < sx.hi) {
+    if (!same && sx.meets(sy)) {
         set_error("rope: x and y overlap without being the same memory in the same layout and type");
         return MKV_ERR_INVALID;
     }
-    const uintptr_t ps = (uintptr_t)g.pos;
-    if (ps < sy.hi && sy.lo < ps + 4ull * in->ntok) {
+    if (sy.meets({(uintptr_t)g.pos, in->ntok, 4u, 4u})) {
         set_error("rope: y overlaps the positions");
         return MKV_ERR_INVALID;
     }

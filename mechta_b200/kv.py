@@ -352,7 +352,7 @@ class KvPool:
                  q_heads: int = HQ, kv_heads: int = HKV, head_dim: int = D):
         self._h = C.c_void_p()
         self.ctx, self.fmt, self.n_layers, self.n_pages, self.page_tokens = ctx, KvFormat(fmt), n_layers, n_pages, page_tokens
-        self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim
+        self.q_heads, self.kv_heads, self.head_dim, self.max_seqs = q_heads, kv_heads, head_dim, max_seqs
         for v in (n_pages, page_tokens, max_seqs, max_tokens):
             _need(0 <= v < 2**32, f"{v} is no size")
         d = _lib.PoolDesc(int(fmt), n_layers, n_pages, page_tokens, max_seqs, max_tokens, q_heads, kv_heads, head_dim)
@@ -374,7 +374,7 @@ class KvPool:
 
     def fork(self, seq: int, length: int | None = None, n: int = 1, copy: bool = False) -> list[int]:
         """n sequences that begin with the first `length` rows of `seq` (all of them by default), on the same pages or on copies."""
-        _need(0 < n < 2**31, f"fork of {n} sequences")
+        _need(0 < n <= self.max_seqs, f"fork of {n} sequences: 1 to {self.max_seqs}")
         kids = (C.c_uint32 * n)()
         check(_lib.lib().mkv_seq_fork(self._h, seq, self.length(seq) if length is None else length, int(copy), n, kids))
         return list(kids)

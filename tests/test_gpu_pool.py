@@ -594,3 +594,102 @@ def test_context_outlives_and_launches_count(ctx):
     with pytest.raises(_lib.MkvError) as e:
         kv.KvPool(ctx, F16, 256, 2**24, 64, 1, 1000)  # 256 TB
     assert e.value.status == _lib.ERR_NOMEM
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_slices_of_one_buffer(ctx, fmt):
+    """q, its rotation and the output as slices of one [tokens][heads] buffer, beside rows that stay."""
+    pool, ids, g = scattered(ctx, fmt, [300, 77], 32, 61)
+    dt = pool.fmt.torch_dtype
+    buf = randn(g, 40, 50, 256, dtype=dt)
+    keep = buf.clone()
+    items = [(ids[0], 0, 263, 37), (ids[1], 0, 74, 3)]
+    pos = torch.tensor([*range(263, 300), 74, 75, 76], device="cuda", dtype=torch.int32)
+    rope = kv.Rope(ctx, 128, layout="interleaved")
+    rope.apply(buf[:, :16], pos, buf[:, 17:33])
+    f, m = rope.freqs()
+    assert ((buf[:, 17:33].double() - rotate64(keep[:, :16], pos, f, m, "interleaved")).abs() <= rope_bound(keep[:, :16], 128, m, dt, "interleaved")).all()
+    want, mag, qk, top = attn64(pool, items, buf[:, 17:33])
+    pool.attn(0, items, buf[:, 17:33], buf[:, 34:])
+    assert ((buf[:, 34:].double() - want).abs() <= attn_bound(fmt, want, mag, qk, top)).all()
+    for s in (slice(0, 17), slice(33, 34)):
+        assert torch.equal(buf[:, s], keep[:, s])
+    pool.close()
+
+
+@pytest.mark.parametrize("fmt,page", [(F16, 256), (F32, 16)])
+def test_rows_beyond_four_gigabytes(ctx, fmt, page):
+    """Pages whose bytes, and f32 pages whose rows times their length, pass 32 bits: written, read, shared, copied and moved."""
+    row = 2 * 256 * (2 if fmt == F16 else 4)
+    low = 2**32 // row + 5 * page
+    pool = kv.KvPool(ctx, fmt, 1, low // page + 150, page, 8, low + 1000)
+    g = gen(71)
+    front, a = pool.create(), pool.create()
+    pool.set_len(front, low)
+    k, v = randn(g, 700, 2, 256), randn(g, 700, 2, 256)
+    pool.write(0, [(a, 0, 0, 700)], k, v)
+    assert pool.pages(a).min() >= low // page
+    dt = pool.fmt.torch_dtype
+    for x, y in zip(rows_of(pool, a), (k, v)):
+        assert torch.equal(x, y.to(dt))
+    b, c = pool.fork(a, 693)[0], pool.fork(a, 690, copy=True)[0]
+    pool.write(0, [(b, 0, 693, 2)], v[:2], k[:2])
+    q = randn(g, 30, 16, 256, dtype=dt)
+    items = [(a, 0, 680, 20), (b, 3, 688, 7), (c, 0, 687, 3)]
+    first = check_attn(pool, items, q)
+    pool.truncate(front, 100)
+    assert pool.compact() > 0 and pool.pages(a).max() < 150
+    assert torch.equal(check_attn(pool, items, q), first)
+    pool.close()
+
+
+def test_two_streams_at_once(ctx):
+    """Pools of contexts on streams of their own, with calls of both in flight together and another stream current."""
+    main = torch.cuda.current_stream()
+    sides = []
+    for i, fmt in enumerate((F16, F32, F16)):
+        stream = torch.cuda.Stream()
+        c = kv.KvContext(0, stream)
+        with torch.cuda.stream(stream):
+            pool, ids, g = scattered(c, fmt, [9000, 500, 64], 64, 80 + i)
+            q = randn(g, 72, 16, 256, dtype=pool.fmt.torch_dtype)
+        stream.synchronize()
+        sides.append((stream, c, pool, [(ids[0], 0, 8999, 1), (ids[1], 0, 430, 70), (ids[2], 0, 63, 1)], q, kv.Rope(c)))
+    main.synchronize()
+    outs = [[torch.full_like(s[4], math.nan) for _ in range(20)] for s in sides]
+    turned = [torch.empty_like(s[4]) for s in sides]
+    pos = torch.arange(72, device="cuda", dtype=torch.int32)
+    main.synchronize()
+    for r in range(20):
+        for (_, _, pool, items, q, rope), out, t in zip(sides, outs, turned):
+            rope.apply(q, pos, t)
+            pool.attn(0, items, t, out[r])
+    for (stream, c, pool, items, q, rope), out, t in zip(sides, outs, turned):
+        stream.synchronize()
+        want, mag, qk, top = attn64(pool, items, t)
+        bound = attn_bound(pool.fmt, want, mag, qk, top)
+        for o in out:
+            assert ((o.double() - want).abs() <= bound).all()
+        pool.close()
+        c.close()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("heads,rot,layout", [((64, 64, 256), 6, "half"), ((64, 1, 256), 256, "interleaved"), ((64, 64, 64), 64, "half")])
+def test_most_heads(ctx, fmt, heads, rot, layout):
+    """The most KV heads and the most query heads of one, from rows at odd addresses."""
+    hq, hkv, dim = heads
+    pool, ids, g = scattered(ctx, fmt, [0, 130], 64, 90, heads=heads)
+    rope = kv.Rope(ctx, rot, layout=layout)
+    f, m = rope.freqs()
+    k, v = (randn(g, 5, hkv * dim + 1)[:, 1:].unflatten(1, (hkv, dim)) for _ in range(2))
+    pool.write(0, [(ids[0], 0, 0, 2), (ids[1], 0, 130, 3)], k, v, rope)
+    pos = torch.tensor([0, 1, 130, 131, 132], device="cuda", dtype=torch.int32)
+    want, bound = rotate64(k, pos, f, m, layout), rope_bound(k, rot, m, pool.fmt.torch_dtype, layout)
+    for s, at in ((ids[0], slice(0, 2)), (ids[1], slice(2, 5))):
+        gk, gv = rows_of(pool, s)
+        n = at.stop - at.start
+        assert ((gk[-n:].double() - want[at]).abs() <= bound[at]).all() and torch.equal(gv[-n:], v[at].to(gv.dtype))
+    q = randn(g, 6, hq, dim, dtype=pool.fmt.torch_dtype)
+    check_attn(pool, [(ids[0], 0, 1, 1), (ids[1], 0, 128, 5)], q)
+    pool.close()

@@ -289,3 +289,37 @@ def test_ropes_that_are_refused():
     assert apply(n=0, x=0, y=0)[0] == _lib.OK
     with pytest.raises(_lib.MkvError):
         kv.Rope(None).apply(torch.zeros(1, 1, 64), torch.zeros(1, dtype=torch.int32), torch.zeros(1, 1, 64))
+
+
+def test_blocks_that_overlap():
+    """Slices of one buffer lie beside each other; anything else that shares bytes is refused."""
+    import ctypes as C
+    L = _lib.lib()
+    r = kv.Rope(None, 64)
+    buf = np.zeros((5, 6, 64), np.float32)  # [tokens][heads]
+    pos = np.zeros(5, np.int32)
+
+    def apply(x_head, y_head, heads, xt=384, yt=384, n=5, yf=1):
+        rows = _lib.RopeRows(buf.ctypes.data + 256 * x_head, buf.ctypes.data + 256 * y_head, 1, yf, n, heads, 64, xt, 0, yt, 0, pos.ctypes.data, 0)
+        assert L.mkv_rope_apply(None, r._h, C.byref(rows)) == _lib.ERR_INVALID
+        return L.mkv_last_error().decode() == "null ctx"  # nothing wrong but the missing context
+
+    assert apply(0, 0, 3) and apply(0, 3, 3) and apply(3, 0, 3) and apply(5, 0, 1) and apply(4, 2, 2, n=4) and apply(0, 0, 6)
+    assert apply(8, 0, 2, n=3) and apply(9, 5, 1, n=3)            # a token further on, beside the rows
+    assert not apply(0, 3, 2, yf=0)                               # (f16: the token strides in bytes differ)
+    assert not apply(0, 2, 3) and not apply(2, 0, 3) and not apply(0, 6, 3, n=4) and not apply(7, 0, 2, n=3) and not apply(4, 0, 3)
+    assert not apply(0, 3, 3, yt=448, n=4) and not apply(0, 3, 3, xt=192, n=3)
+    p = pool()
+    a = p.create()
+    p.set_len(a, 30)
+    wide = torch.zeros(4, 32, 256, dtype=torch.float16)
+
+    def attn(q, out):
+        return status(p.attn, 0, [(a, 0, 26, 4)], q, out)
+
+    assert attn(wide[:, :16], wide[:, 16:]) == _lib.ERR_UNSUPPORTED and attn(wide[:, 16:], wide[:, :16]) == _lib.ERR_UNSUPPORTED
+    assert attn(wide[:, :16], wide[:, :16]) == _lib.ERR_INVALID and attn(wide[:, :16], wide[:, 15:31]) == _lib.ERR_INVALID
+    flat = torch.zeros(8, 16, 256, dtype=torch.float16)
+    assert attn(flat[:4], flat[4:]) == _lib.ERR_UNSUPPORTED and attn(flat[:4], flat[1:5]) == _lib.ERR_INVALID
+    with pytest.raises(_lib.MkvError):
+        p.fork(a, n=2**31 - 1)
