@@ -75,6 +75,7 @@ static mkv_status follow_books(Pool *p) {
 // K and V of the new tokens into their pages, K rotated on the way, one rounding to the pool's type. Bound by HBM for prefill blocks
 // and by the launch for steps. A block takes as many tokens as its threads have units for (two units of 8 values a thread; tokens of very
 // many heads are spread over several blocks); the loads are in flight while the tokens' cosines and sines are computed.
+// Measured: 7,682 rows of four f32 heads of 128 (63 MB) in 14.8 us, 4.3 TB/s; 128 rows of two f16 heads of 256 3.1 us.
 constexpr uint32_t WRITE_ITEMS = 120;
 struct WriteItems {
     uint32_t n;
@@ -196,7 +197,8 @@ mkv_status launch_pool_write(Pool *p, int layer, const mkv_seq_rows *items, int 
             }
         if (it.n == 0u) break;
         const uint32_t rows = it.row[it.n], token_units = g.kv_heads * (g.units + g.head_dim / 8u);
-        // few rows: a block each, for the latency; many: blocks that are full
+        // few rows: a block each, for the latency (128 rows: 3.1 us, in full blocks 3.7); many: blocks that are full (7,682 rows: 14.8 us, in
+        // blocks of one row 18.3)
         g.tokens = rows < 2u * (uint32_t)p->ctx->sm_count ? 1u : std::max(1u, std::min(WRITE_TOKENS, 256u * WRITE_PER / token_units));
         const bool o16 = p->desc.fmt == MKV_F16;
         mkv_status st;

@@ -68,7 +68,8 @@ bool pool_plan(const Pool *p, const mkv_seq_rows *items, int n, int &i, uint32_t
 
 // ---- the merge of split items --------------------------------------------------------------------------------------
 // out = sum_s e^(m_s - M) O_s / (sum_s e^(m_s - M) l_s + e^(sink - M)) over an item's parts. A few dozen L2 accesses of a thread one after
-// the other are all there is to it, so the parts of a row are spread over up to 16 groups of threads, which meet in shared memory.
+// the other are all there is to it, so the parts of a row are spread over up to 16 groups of threads, which meet in shared memory (one
+// token over 4,096, 32 parts: the whole call takes 12.1 us, with one group 19.5, with blocks of 256 threads in place of 1,024 12.5).
 struct MergeArgs {
     const float *scratch, *sinks;
     void *out;
@@ -200,6 +201,8 @@ mkv_status pool_attn_setup(Pool *p) {
 
 mkv_status launch_pool_attn(Pool *p, int layer, const mkv_seq_rows *items, int n, const PoolAttn &a) {
     const bool f16 = p->desc.fmt == MKV_F16;
+    // What a segment costs beside its tiles, measured with 0, 2 and 4 tiles: ragged blocks under a window of 513 in f16 110, 73 and 89 us;
+    // f32 blocks 464, 449 and 452; long histories hardly care (32 sessions in f16 338, 340 and 339; eight in f32 181, 173 and 167).
     const PlanCost cost = f16 ? PlanCost{128u, 128u, 2u} : PlanCost{64u, 64u, 2u};
     PoolPlan plan;
     MergeList merge;

@@ -19,8 +19,10 @@
 // share with ordinary arithmetic for the rows that see them. Keys that no token of the item sees are zero as well, whatever lies in
 // their rows.
 //
-// Bound by HBM for few rows (a 64-key tile of 256 dims is 128 KB, 5,600 clocks of an SM's share of 6.4 TB/s, and about 2,600 of
-// products), by the chain softmax - products - fold for long blocks.
+// Bound by the converters: a K or V tile of 64 KB takes its four warps 3,500 to 4,700 clocks (a unit's chain wait - load - split - store
+// is about 800, whatever its share of a warp), so a tile of 256 dims about 9,000, where HBM would take 5,600 and the products take
+// 2,600. More converter warps make each chain longer by as much: eight measured the same. Eight sessions of up to 32,000 tokens
+// (533 MB) take 172 us, 3.1 TB/s; blocks of 300 to 512 tokens over up to 4,096 (46 GFLOP, three f16 products each) 446 us.
 //
 // Roles (512 threads, four warpgroups whose register budgets are set with setmaxnreg): warps 0 and 3 = TMA producers, warp 1 =
 // issues S' and owns the TMEM, warp 2 = issues O', warps 4..7 = converters, warps 8..15 = softmax and owners of O: two threads per TMEM
