@@ -44,7 +44,7 @@ constexpr uint32_t PB_UNIT = 2 * PB_BLK;   // 64 dims of a tile
 constexpr uint32_t PB_NST = 12;            // units of the ring: a multiple of a tile's, so that a tile lies in one piece
 constexpr uint32_t PB_PBUF = 16384;             // P' [128 rows][64 keys] f16; also where S'[64 + r] changes hands
 constexpr uint32_t PB_OFF_P = PB_NST * PB_UNIT; // two of them, in turn
-constexpr uint32_t PB_OFF_RED = PB_OFF_P + 2 * PB_PBUF; // [2 halves][64 rows] floats, [64 rows] rescale factors, [64 rows] reference maxima
+constexpr uint32_t PB_OFF_RED = PB_OFF_P + 2 * PB_PBUF; // [2 halves][64 rows] floats, [64 rows] rescale factors, [64 rows] scales of Q'
 constexpr uint32_t PB_OFF_BAR = PB_OFF_RED + 1024;
 constexpr uint32_t PB_NBAR = 3 * PB_NST + 7; // full[NST], empty[NST], conv[NST], s_full[2], s_free[2], p_full, pv_done, q_full
 constexpr uint32_t PB_OFF_MISC = PB_OFF_BAR + PB_NBAR * 8;
@@ -242,8 +242,26 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 unpack2(add2(z[0], z[1]), z0, z1);
                 odd = odd || z0 + z1 != 0.0f;
             };
+            auto tile_scale = [&]() -> float { // of the largest of all warps' amax
+                const uint32_t mine = __reduce_max_sync(0xffffffffu, __float_as_uint(amax));
+                if (lane == 0) sh->amax[cw] = mine;
+                named_bar_sync(3, 128); // (there is another in front of the next use of amax[])
+                uint32_t most = 0u;
+                for (uint32_t i = 0; i < 4u; i++) most = max(most, sh->amax[i]);
+                return most ? __uint_as_float(scale_bits(most)) : 1.0f;
+            };
             pb_wait(bar_full + 8u * begin.s, begin.turn, sh, g.status);
             __syncwarp();
+            if (note == 0u) { // the first tile has no scale in front of it: its largest value gives it
+#pragma unroll 1
+                for (uint32_t h = 0; h < NU; h++) {
+                    float4 x[8];
+                    fetch(begin.s + h, x);
+                    look(x);
+                }
+                s = (v ? v_scale : k_scale) = tile_scale();
+                amax = 0.0f;
+            }
 #pragma unroll 1
             for (uint32_t h = 0; h < NU; h++) {
                 float4 x[8];
@@ -280,13 +298,7 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
 #pragma unroll
                     for (uint32_t i = 0; i < 8u; i++) amax = fmaxf(amax, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
                 }
-                amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
-                if (lane == 0) sh->amax[cw] = __float_as_uint(amax);
-                named_bar_sync(3, 128);
-                uint32_t most = 0u;
-                for (uint32_t i = 0; i < 4u; i++) most = max(most, sh->amax[i]);
-                s = most ? __uint_as_float(scale_bits(most)) : 1.0f;
-                (v ? v_scale : k_scale) = s;
+                s = (v ? v_scale : k_scale) = tile_scale();
 #pragma unroll 1
                 for (uint32_t h = 0; h < NU; h++) {
                     float4 x[8];
@@ -354,8 +366,9 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 }
                 return true;
             };
-            Tile cur = look_up(), ahead = look_up();
+            Tile cur = look_up();
             bool ok = load(&kmap, cur);
+            Tile ahead = look_up();
             while (ok && cur.is) {
                 const Tile later = look_up(); // (its page is there when its turn comes)
                 if (ahead.is) ok = load(&kmap, ahead);
@@ -432,8 +445,9 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         const bool hi = q4 < 2u;                             // this lane has a row's hi parts, else its lo parts
         const uint32_t row = 32u * (q4 & 1u) + lane;         // the row, 0 .. 63
         const uint32_t bar_group = 1u + (q4 & 1u);           // the four warps that have these 32 rows
+        const uint32_t own = (q4 >> 1) + 2u * half;          // this warp's number among them
         constexpr uint32_t HD = DIM / 2;                     // dims of Q' and O of a thread
-        float *red = reinterpret_cast<float *>(smem + PB_OFF_RED), *cf_s = red + 128;
+        float *red = reinterpret_cast<float *>(smem + PB_OFF_RED), *cf_s = red + 128, *q_s = red + 192;
         const uint32_t group = plan.group, tok = row / group, head = row - tok * group;
         auto arrive = [&](uint32_t bar) { // one arrival per warp, after all its lanes
             __syncwarp();
@@ -447,51 +461,78 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         // where a thread of row r and this half has its 32 scores or weights in the P' buffer: chunk c of 8 (0..3 in row r, 4..7 in row 64 + r)
         uint8_t *p_buf = smem + PB_OFF_P; // of the tile
         auto p_chunk = [&](uint32_t c) { return p_buf + swz128(row + (c >> 2) * 64u, 4u * half + (c & 3u)); };
-        // Q' of a segment: the row's hi or lo parts, half of the dims, scaled by a power of two of the row's own
-        auto load_q = [&](const PlanSegment &sg) -> float {
+        // Q' of a segment, scaled by a power of two of each row's own (its inverse is returned). Four threads fetch a row, 16 of every 64 dims
+        // each; the hi and lo parts change hands in `stage` (a P' buffer that no product reads), 64 dims at a time, and go to the tensor memory
+        // from the threads that have the lanes.
+        auto load_q = [&](const PlanSegment &sg, uint8_t *stage) -> float {
             const uint32_t rows = sg.it.ntok * group;
             float unscale = 1.0f;
             if (32u * (q4 & 1u) < rows) {
-                const float *src = g.q + (int64_t)(plan.seq[sg.seq].row + sg.it.tok0 + tok) * g.q_stride + (size_t)(sg.kvh * group + head) * DIM + HD * half;
-                const bool real = row < rows;
+                const uint32_t fr = 32u * (q4 & 1u) + 8u * own + (lane >> 2), j = lane & 3u, ftok = fr / group;
+                const bool there = fr < rows;
+                const float *src = g.q + (int64_t)(plan.seq[sg.seq].row + sg.it.tok0 + ftok) * g.q_stride + (size_t)(sg.kvh * group + fr - ftok * group) * DIM + 16u * j;
+                auto fetch = [&](uint32_t c, float4 (&x)[4]) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 4u; i++) x[i] = there ? __ldg(reinterpret_cast<const float4 *>(src + 64u * c + 4u * i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                };
                 uint32_t amax = 0u;
-                if (real)
-#pragma unroll 4
-                    for (uint32_t d = 0; d < HD; d += 4u) {
-                        const uint4 a = __ldg(reinterpret_cast<const uint4 *>(src + d));
+#pragma unroll
+                for (uint32_t c = 0; c < NU; c += 2u) {
+                    float4 x[2][4];
+                    fetch(c, x[0]);
+                    if (c + 1u < NU) fetch(c + 1u, x[1]);
+#pragma unroll
+                    for (uint32_t k = 0; k < 2u && c + k < NU; k++)
+#pragma unroll
+                        for (uint32_t i = 0; i < 4u; i++) {
+                            const float *e = &x[k][i].x;
+#pragma unroll
+                            for (int n = 0; n < 4; n++) {
+                                const uint32_t b = __float_as_uint(e[n]) & 0x7fffffffu;
+                                amax = max(amax, b < 0x7f800000u ? b : 0u);
+                            }
+                        }
+                }
+                amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                const float s = amax ? __uint_as_float(scale_bits(amax)) : 1.0f;
+                if (j == 0u) q_s[fr] = 1.0f / s;
+                float4 x[4];
+                fetch(0, x);
+#pragma unroll
+                for (uint32_t c = 0; c < NU; c++) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 2u; i++) {
+                        const float4 u = x[2 * i], w = x[2 * i + 1];
+                        const float y[8] = {u.x * s, u.y * s, u.z * s, u.w * s, w.x * s, w.y * s, w.z * s, w.w * s};
+                        uint32_t h4[4], l4[4];
 #pragma unroll
                         for (uint32_t e = 0; e < 4u; e++) {
-                            const uint32_t b = e == 0 ? a.x : e == 1 ? a.y : e == 2 ? a.z : a.w;
-                            if (is_finite_bits(b)) amax = max(amax, b & 0x7fffffffu);
+                            const __half2 h = __floats2half2_rn(y[2 * e], y[2 * e + 1]);
+                            const float2 f = __half22float2(h);
+                            const __half2 l = __floats2half2_rn(isfinite(f.x) ? y[2 * e] - f.x : 0.0f, isfinite(f.y) ? y[2 * e + 1] - f.y : 0.0f);
+                            h4[e] = *reinterpret_cast<const uint32_t *>(&h);
+                            l4[e] = *reinterpret_cast<const uint32_t *>(&l);
                         }
+                        *reinterpret_cast<uint4 *>(stage + swz128(fr, 2u * j + i)) = make_uint4(h4[0], h4[1], h4[2], h4[3]);
+                        *reinterpret_cast<uint4 *>(stage + swz128(64u + fr, 2u * j + i)) = make_uint4(l4[0], l4[1], l4[2], l4[3]);
                     }
-                red[64u * half + row] = __uint_as_float(amax); // (hi and lo threads write the same)
-                named_bar_sync(bar_group, 128);
-                amax = max(__float_as_uint(red[row]), __float_as_uint(red[64u + row]));
-                const float s = amax ? __uint_as_float(scale_bits(amax)) : 1.0f;
-                unscale = 1.0f / s;
-#pragma unroll 1
-                for (uint32_t d = 0; d < HD; d += 32u) {
+                    if (c + 1u < NU) fetch(c + 1u, x);
+                    named_bar_sync(bar_group, 128);
                     uint32_t w[16];
 #pragma unroll
-                    for (uint32_t i = 0; i < 8u; i++) {
-                        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (real) a = __ldg(reinterpret_cast<const float4 *>(src + d + 4u * i));
-                        const float x[4] = {a.x * s, a.y * s, a.z * s, a.w * s};
-#pragma unroll
-                        for (uint32_t e = 0; e < 4u; e += 2u) {
-                            __half2 h = __floats2half2_rn(x[e], x[e + 1]);
-                            if (!hi) {
-                                const float2 f = __half22float2(h);
-                                h = __floats2half2_rn(isfinite(f.x) ? x[e] - f.x : 0.0f, isfinite(f.y) ? x[e + 1] - f.y : 0.0f);
-                            }
-                            w[2 * i + (e >> 1)] = *reinterpret_cast<const uint32_t *>(&h);
-                        }
+                    for (uint32_t i = 0; i < 4u; i++) {
+                        const uint4 v = *reinterpret_cast<const uint4 *>(stage + swz128(row + (hi ? 0u : 64u), 4u * half + i));
+                        w[4 * i] = v.x;
+                        w[4 * i + 1] = v.y;
+                        w[4 * i + 2] = v.z;
+                        w[4 * i + 3] = v.w;
                     }
-                    tmem_st16(tmem + lane_addr + PB_COL_Q + (HD * half + d) / 2u, w);
+                    tmem_st16(tmem + lane_addr + PB_COL_Q + 32u * c + 16u * half, w);
+                    if (c == 0u) unscale = q_s[row];
+                    named_bar_sync(bar_group, 128); // the stage is free
                 }
                 tmem_wait_st();
-                named_bar_sync(bar_group, 128); // red[] is free
             }
             tc_fence_before();
             arrive(bar_q_full);
@@ -509,7 +550,7 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         PlanWalk walk(plan, blockIdx.x, PF_KEYS32);
         PlanSegment sg, nx;
         bool more = walk.next(sg);
-        float q_unscale = load_q(sg), q_next = 1.0f;
+        float q_unscale = load_q(sg, smem + PB_OFF_P), q_next = 1.0f;
         while (more) {
             const PlanItem it = sg.it;
             const PlanSeq &sq = plan.seq[sg.seq];
@@ -662,42 +703,52 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             }
             // ---------------- end of the segment ----------------
             more = walk.next(nx);
-            if (more) q_next = load_q(nx); // the segment's scores were all there: its Q' may go
+            if (more) q_next = load_q(nx, smem + PB_OFF_P + (end & 1u) * PB_PBUF); // the segment's scores were all there: its Q' may go
             if (active) {
                 fold(end - 1u, m, cf);
                 if (hi) red[64u * half + row] = l;
                 named_bar_sync(bar_group, 128); // (P' is free too: its last products have completed)
                 const float l_all = red[row] + red[64u + row];
                 const bool seen = real && klo < vis;
-                float inv = 0.0f;
-                float *dst = nullptr;
+                float inv = 1.0f;
+                float *part = nullptr; // a part: maximum, sum and O as they are, for the merge
                 if (sg.whole) {
                     float den = l_all;
                     if (g.sinks && real) den += exp2f(g.sinks[sg.kvh * group + head] * PB_LOG2E - (m > NEG_TEST ? m : 0.0f));
                     inv = 1.0f / den;
-                    dst = g.out + (int64_t)(sq.row + it.tok0 + tok) * g.out_stride + (size_t)(sg.kvh * group + head) * DIM + HD * half;
-                } else { // a part: maximum, sum and O as they are, for the merge
-                    float *ps = g.scratch + part_slot(blockIdx.x, sg.part) * part_floats(DIM);
-                    inv = 1.0f;
-                    dst = ps + (size_t)row * DIM + HD * half;
-                    if (hi && half == 0u && real) *reinterpret_cast<float2 *>(ps + 128u * DIM + 2u * row) = make_float2(m, seen ? l_all : -1.0f);
+                } else {
+                    part = g.scratch + part_slot(blockIdx.x, sg.part) * part_floats(DIM);
+                    if (hi && half == 0u && real) *reinterpret_cast<float2 *>(part + 128u * DIM + 2u * row) = make_float2(m, seen ? l_all : -1.0f);
                 }
+                // The row's hi and lo parts meet in the P' buffers, in turn, 32 dims of each half at a time; all threads store, 128 bytes of a row
+                // side by side.
 #pragma unroll
-                for (uint32_t c0 = 0; c0 < HD; c0 += 32u) { // the row's hi and lo parts meet, 32 dims at a time
+                for (uint32_t c0 = 0; c0 < HD; c0 += 32u) {
+                    p_buf = smem + PB_OFF_P + ((c0 >> 5) & 1u) * PB_PBUF;
                     if (!hi)
 #pragma unroll
                         for (uint32_t c = 0; c < 8u; c++) *reinterpret_cast<float4 *>(p_chunk(c)) = make_float4(O[c0 + 4 * c], O[c0 + 4 * c + 1], O[c0 + 4 * c + 2], O[c0 + 4 * c + 3]);
                     named_bar_sync(bar_group, 128);
-                    if (hi && real)
+                    if (hi)
 #pragma unroll
                         for (uint32_t c = 0; c < 8u; c++) {
                             const float4 x = *reinterpret_cast<const float4 *>(p_chunk(c));
-                            *reinterpret_cast<float4 *>(dst + c0 + 4u * c) =
+                            *reinterpret_cast<float4 *>(p_chunk(c)) =
                                 seen ? make_float4((O[c0 + 4 * c] + x.x) * inv, (O[c0 + 4 * c + 1] + x.y) * inv, (O[c0 + 4 * c + 2] + x.z) * inv, (O[c0 + 4 * c + 3] + x.w) * inv)
                                      : make_float4(0.f, 0.f, 0.f, 0.f);
                         }
                     named_bar_sync(bar_group, 128);
+#pragma unroll
+                    for (uint32_t i = 0; i < 4u; i++) {
+                        const uint32_t r = 32u * (q4 & 1u) + 8u * i + 2u * own + (lane >> 4), h = (lane >> 3) & 1u, c = lane & 7u, r_tok = r / group;
+                        if (r >= rows) continue;
+                        const uint32_t d = HD * h + c0 + 4u * c;
+                        float *dst = part ? part + (size_t)r * DIM + d
+                                          : g.out + (int64_t)(sq.row + it.tok0 + r_tok) * g.out_stride + (size_t)(sg.kvh * group + r - r_tok * group) * DIM + d;
+                        *reinterpret_cast<float4 *>(dst) = *reinterpret_cast<const float4 *>(p_buf + swz128(r + (c >> 2) * 64u, 4u * h + (c & 3u)));
+                    }
                 }
+                named_bar_sync(bar_group, 128); // the buffers are free
             } else {
                 wait(bar_pv_done, (end - 1u) & 1u);
             }
