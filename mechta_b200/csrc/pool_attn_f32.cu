@@ -28,6 +28,8 @@
 // issues S' and owns the TMEM, warp 2 = issues O', warps 4..7 = converters, warps 8..15 = softmax and owners of O: two threads per TMEM
 // lane, 32 of a tile's keys and half of the dims each. TMEM: O' = columns 0 .. DIM - 1, S' = 256 .. 319 and 320 .. 383, Q' = 384 ...
 // Every wait is bounded; TMEM is freed on every path.
+#include <type_traits>
+
 #include "pool_plan.cuh"
 #include "ptx.cuh"
 
@@ -252,14 +254,11 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             };
             pb_wait(bar_full + 8u * begin.s, begin.turn, sh, g.status);
             __syncwarp();
-            if (note == 0u) { // the first tile has no scale in front of it: its largest value gives it
-#pragma unroll 1
-                for (uint32_t h = 0; h < NU; h++) {
-                    float4 x[8];
-                    fetch(begin.s + h, x);
-                    look(x);
-                }
-                s = (v ? v_scale : k_scale) = tile_scale();
+            if (note == 0u) { // the first tile has no scale in front of it: the largest value of its first 64 dims gives it, to [2^11, 2^12)
+                float4 x[8];
+                fetch(begin.s, x);
+                look(x);
+                s = (v ? v_scale : k_scale) = 0.25f * tile_scale();
                 amax = 0.0f;
             }
 #pragma unroll 1
@@ -463,8 +462,10 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         auto p_chunk = [&](uint32_t c) { return p_buf + swz128(row + (c >> 2) * 64u, 4u * half + (c & 3u)); };
         // Q' of a segment, scaled by a power of two of each row's own (its inverse is returned). Four threads fetch a row, 16 of every 64 dims
         // each; the hi and lo parts change hands in `stage` (a P' buffer that no product reads), 64 dims at a time, and go to the tensor memory
-        // from the threads that have the lanes.
-        auto load_q = [&](const PlanSegment &sg, uint8_t *stage) -> float {
+        // from the threads that have the lanes. The first segment's values stay in registers between the search for the largest one and
+        // the split; later ones are read twice, since the registers are O's.
+        auto load_q = [&](const PlanSegment &sg, uint8_t *stage, auto first) -> float {
+            constexpr bool FIRST = decltype(first)::value;
             const uint32_t rows = sg.it.ntok * group;
             float unscale = 1.0f;
             if (32u * (q4 & 1u) < rows) {
@@ -476,34 +477,44 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                     for (uint32_t i = 0; i < 4u; i++) x[i] = there ? __ldg(reinterpret_cast<const float4 *>(src + 64u * c + 4u * i)) : make_float4(0.f, 0.f, 0.f, 0.f);
                 };
                 uint32_t amax = 0u;
+                auto look = [&](const float4 (&x)[4]) {
 #pragma unroll
-                for (uint32_t c = 0; c < NU; c += 2u) {
-                    float4 x[2][4];
-                    fetch(c, x[0]);
-                    if (c + 1u < NU) fetch(c + 1u, x[1]);
+                    for (uint32_t i = 0; i < 4u; i++) {
+                        const float e[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
-                    for (uint32_t k = 0; k < 2u && c + k < NU; k++)
-#pragma unroll
-                        for (uint32_t i = 0; i < 4u; i++) {
-                            const float *e = &x[k][i].x;
-#pragma unroll
-                            for (int n = 0; n < 4; n++) {
-                                const uint32_t b = __float_as_uint(e[n]) & 0x7fffffffu;
-                                amax = max(amax, b < 0x7f800000u ? b : 0u);
-                            }
+                        for (int n = 0; n < 4; n++) {
+                            const uint32_t b = __float_as_uint(e[n]) & 0x7fffffffu;
+                            amax = max(amax, b < 0x7f800000u ? b : 0u);
                         }
+                    }
+                };
+                float4 x[FIRST ? NU : 2u][4];
+                if constexpr (FIRST) {
+#pragma unroll
+                    for (uint32_t c = 0; c < NU; c++) fetch(c, x[c]);
+#pragma unroll
+                    for (uint32_t c = 0; c < NU; c++) look(x[c]);
+                } else {
+#pragma unroll
+                    for (uint32_t c = 0; c < NU; c += 2u) {
+                        fetch(c, x[0]);
+                        if (c + 1u < NU) fetch(c + 1u, x[1]);
+                        look(x[0]);
+                        if (c + 1u < NU) look(x[1]);
+                    }
+                    fetch(0, x[0]);
                 }
                 amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
                 amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
                 const float s = amax ? __uint_as_float(scale_bits(amax)) : 1.0f;
                 if (j == 0u) q_s[fr] = 1.0f / s;
-                float4 x[4];
-                fetch(0, x);
 #pragma unroll
                 for (uint32_t c = 0; c < NU; c++) {
+                    const float4(&y4)[4] = x[FIRST ? c : c & 1u];
+                    if (!FIRST && c + 1u < NU) fetch(c + 1u, x[(c + 1u) & 1u]);
 #pragma unroll
                     for (uint32_t i = 0; i < 2u; i++) {
-                        const float4 u = x[2 * i], w = x[2 * i + 1];
+                        const float4 u = y4[2 * i], w = y4[2 * i + 1];
                         const float y[8] = {u.x * s, u.y * s, u.z * s, u.w * s, w.x * s, w.y * s, w.z * s, w.w * s};
                         uint32_t h4[4], l4[4];
 #pragma unroll
@@ -517,7 +528,6 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                         *reinterpret_cast<uint4 *>(stage + swz128(fr, 2u * j + i)) = make_uint4(h4[0], h4[1], h4[2], h4[3]);
                         *reinterpret_cast<uint4 *>(stage + swz128(64u + fr, 2u * j + i)) = make_uint4(l4[0], l4[1], l4[2], l4[3]);
                     }
-                    if (c + 1u < NU) fetch(c + 1u, x);
                     named_bar_sync(bar_group, 128);
                     uint32_t w[16];
 #pragma unroll
@@ -550,7 +560,7 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         PlanWalk walk(plan, blockIdx.x, PF_KEYS32);
         PlanSegment sg, nx;
         bool more = walk.next(sg);
-        float q_unscale = load_q(sg, smem + PB_OFF_P), q_next = 1.0f;
+        float q_unscale = load_q(sg, smem + PB_OFF_P, std::true_type{}), q_next = 1.0f;
         while (more) {
             const PlanItem it = sg.it;
             const PlanSeq &sq = plan.seq[sg.seq];
@@ -703,7 +713,7 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             }
             // ---------------- end of the segment ----------------
             more = walk.next(nx);
-            if (more) q_next = load_q(nx, smem + PB_OFF_P + (end & 1u) * PB_PBUF); // the segment's scores were all there: its Q' may go
+            if (more) q_next = load_q(nx, smem + PB_OFF_P + (end & 1u) * PB_PBUF, std::false_type{}); // the segment's scores were all there: its Q' may go
             if (active) {
                 fold(end - 1u, m, cf);
                 if (hi) red[64u * half + row] = l;
