@@ -718,44 +718,62 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 fold(end - 1u, m, cf);
                 if (hi) red[64u * half + row] = l;
                 named_bar_sync(bar_group, 128); // (P' is free too: its last products have completed)
-                const float l_all = red[row] + red[64u + row];
-                const bool seen = real && klo < vis;
-                float inv = 1.0f;
                 float *part = nullptr; // a part: maximum, sum and O as they are, for the merge
-                if (sg.whole) {
-                    float den = l_all;
-                    if (g.sinks && real) den += exp2f(g.sinks[sg.kvh * group + head] * PB_LOG2E - (m > NEG_TEST ? m : 0.0f));
-                    inv = 1.0f / den;
-                } else {
-                    part = g.scratch + part_slot(blockIdx.x, sg.part) * part_floats(DIM);
-                    if (hi && half == 0u && real) *reinterpret_cast<float2 *>(part + 128u * DIM + 2u * row) = make_float2(m, seen ? l_all : -1.0f);
+                if (!sg.whole) part = g.scratch + part_slot(blockIdx.x, sg.part) * part_floats(DIM);
+                float inv = 0.0f;
+                if (hi) {
+                    const float l_all = red[row] + red[64u + row];
+                    const bool seen = real && klo < vis;
+                    if (sg.whole) {
+                        float den = l_all;
+                        if (g.sinks && real) den += exp2f(g.sinks[sg.kvh * group + head] * PB_LOG2E - (m > NEG_TEST ? m : 0.0f));
+                        if (seen) inv = 1.0f / den; // (otherwise O is zero, and stays so)
+                    } else {
+                        inv = 1.0f;
+                        if (half == 0u && real) *reinterpret_cast<float2 *>(part + 128u * DIM + 2u * row) = make_float2(m, seen ? l_all : -1.0f);
+                    }
+                    if (half == 0u) cf_s[row] = inv;
                 }
-                // The row's hi and lo parts meet in the P' buffers, in turn, 32 dims of each half at a time; all threads store, 128 bytes of a row
-                // side by side.
+                // The row's hi and lo parts meet in the P' buffers, in turn, 32 dims of each half at a time: the one thread adds up the first 16, the
+                // other the rest. All threads store, 128 bytes of a row side by side.
+                float *dst[4]; // of the four rows of this thread that are stored
+#pragma unroll
+                for (uint32_t i = 0; i < 4u; i++) {
+                    const uint32_t r = 32u * (q4 & 1u) + 8u * i + 2u * own + (lane >> 4), r_tok = r / group;
+                    dst[i] = (part ? part + (size_t)r * DIM
+                                   : g.out + (int64_t)(sq.row + it.tok0 + r_tok) * g.out_stride + (size_t)(sg.kvh * group + r - r_tok * group) * DIM) +
+                             HD * (lane >> 3 & 1u) + 4u * (lane & 7u);
+                }
 #pragma unroll
                 for (uint32_t c0 = 0; c0 < HD; c0 += 32u) {
                     p_buf = smem + PB_OFF_P + ((c0 >> 5) & 1u) * PB_PBUF;
-                    if (!hi)
+                    auto give = [&](auto from) { // 16 dims
+                        constexpr uint32_t F = decltype(from)::value;
 #pragma unroll
-                        for (uint32_t c = 0; c < 8u; c++) *reinterpret_cast<float4 *>(p_chunk(c)) = make_float4(O[c0 + 4 * c], O[c0 + 4 * c + 1], O[c0 + 4 * c + 2], O[c0 + 4 * c + 3]);
-                    named_bar_sync(bar_group, 128);
-                    if (hi)
+                        for (uint32_t c = 0; c < 4u; c++)
+                            *reinterpret_cast<float4 *>(p_chunk(F / 4u + c)) = make_float4(O[c0 + F + 4 * c], O[c0 + F + 4 * c + 1], O[c0 + F + 4 * c + 2], O[c0 + F + 4 * c + 3]);
+                    };
+                    auto sum = [&](auto from) {
+                        constexpr uint32_t F = decltype(from)::value;
 #pragma unroll
-                        for (uint32_t c = 0; c < 8u; c++) {
-                            const float4 x = *reinterpret_cast<const float4 *>(p_chunk(c));
-                            *reinterpret_cast<float4 *>(p_chunk(c)) =
-                                seen ? make_float4((O[c0 + 4 * c] + x.x) * inv, (O[c0 + 4 * c + 1] + x.y) * inv, (O[c0 + 4 * c + 2] + x.z) * inv, (O[c0 + 4 * c + 3] + x.w) * inv)
-                                     : make_float4(0.f, 0.f, 0.f, 0.f);
+                        for (uint32_t c = 0; c < 4u; c++) {
+                            const float4 x = *reinterpret_cast<const float4 *>(p_chunk(F / 4u + c));
+                            *reinterpret_cast<float4 *>(p_chunk(F / 4u + c)) = make_float4((O[c0 + F + 4 * c] + x.x) * inv, (O[c0 + F + 4 * c + 1] + x.y) * inv,
+                                                                                          (O[c0 + F + 4 * c + 2] + x.z) * inv, (O[c0 + F + 4 * c + 3] + x.w) * inv);
                         }
+                    };
+                    if (hi) give(std::integral_constant<uint32_t, 16>{});
+                    else give(std::integral_constant<uint32_t, 0>{});
+                    named_bar_sync(bar_group, 128);
+                    if (c0 == 0u) inv = cf_s[row];
+                    if (hi) sum(std::integral_constant<uint32_t, 0>{});
+                    else sum(std::integral_constant<uint32_t, 16>{});
                     named_bar_sync(bar_group, 128);
 #pragma unroll
                     for (uint32_t i = 0; i < 4u; i++) {
-                        const uint32_t r = 32u * (q4 & 1u) + 8u * i + 2u * own + (lane >> 4), h = (lane >> 3) & 1u, c = lane & 7u, r_tok = r / group;
-                        if (r >= rows) continue;
-                        const uint32_t d = HD * h + c0 + 4u * c;
-                        float *dst = part ? part + (size_t)r * DIM + d
-                                          : g.out + (int64_t)(sq.row + it.tok0 + r_tok) * g.out_stride + (size_t)(sg.kvh * group + r - r_tok * group) * DIM + d;
-                        *reinterpret_cast<float4 *>(dst) = *reinterpret_cast<const float4 *>(p_buf + swz128(r + (c >> 2) * 64u, 4u * h + (c & 3u)));
+                        const uint32_t r = 32u * (q4 & 1u) + 8u * i + 2u * own + (lane >> 4), c = lane & 7u;
+                        const float4 x = *reinterpret_cast<const float4 *>(p_buf + swz128(r + (c >> 2) * 64u, 4u * (lane >> 3 & 1u) + (c & 3u)));
+                        if (r < rows) *reinterpret_cast<float4 *>(dst[i] + c0) = x;
                     }
                 }
                 named_bar_sync(bar_group, 128); // the buffers are free
