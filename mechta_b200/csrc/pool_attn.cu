@@ -69,7 +69,8 @@ bool pool_plan(const Pool *p, const mkv_seq_rows *items, int n, int &i, uint32_t
 // ---- the merge of split items --------------------------------------------------------------------------------------
 // out = sum_s e^(m_s - M) O_s / (sum_s e^(m_s - M) l_s + e^(sink - M)) over an item's parts. A few dozen L2 accesses of a thread one after
 // the other are all there is to it, so the parts of a row are spread over up to 16 groups of threads, which meet in shared memory (one
-// token over 4,096, 32 parts: the whole call takes 12.1 us, with one group 19.5, with blocks of 256 threads in place of 1,024 12.5).
+// token over 4,096, 32 parts of 8 rows: the whole call takes 12.2 us, with one group 19.5), as long as all threads fit the GPU at once (24
+// items of 5 to 9 parts of up to 128 rows: 19.7 us with one group, with two, in blocks of 1,024 threads, 24.1).
 struct MergeArgs {
     const float *scratch, *sinks;
     void *out;
@@ -160,10 +161,11 @@ template <class T, int DIM> static mkv_status launch_merge(Pool *p, const MergeL
         parts = std::max<uint32_t>(parts, list.item[i].parts);
         rows = std::max(rows, list.item[i].ntok * list.group);
     }
-    const uint32_t threads = parts > 4u ? 1024u : 256u, slots = threads / (DIM / 4);
     MergeArgs g = {p->scratch, a.sinks, a.out, a.out_stride, 1u};
-    while (g.groups < slots && g.groups < 16u && 4u * g.groups < parts) g.groups *= 2u;
-    const uint32_t rpb = slots / g.groups;
+    // as many groups as the parts keep busy, while all threads fit the GPU at once
+    constexpr uint32_t L = DIM / 4;
+    while (g.groups < 16u && 4u * g.groups < parts && (uint64_t)list.n * rows * L * 2u * g.groups <= 2048ull * (uint32_t)p->ctx->sm_count) g.groups *= 2u;
+    const uint32_t threads = std::max(256u, g.groups * L), rpb = threads / L / g.groups;
     PdlLaunch l(p->ctx, dim3((rows + rpb - 1u) / rpb, list.n), threads);
     MKV_CUDA(cudaLaunchKernelEx(&l.cfg, pool_merge_kernel<T, DIM>, list, g));
     p->ctx->launches++;
