@@ -46,8 +46,8 @@ constexpr uint32_t PB_UNIT = 2 * PB_BLK;   // 64 dims of a tile
 constexpr uint32_t PB_NST = 12;            // units of the ring: a multiple of a tile's, so that a tile lies in one piece
 constexpr uint32_t PB_PBUF = 16384;             // P' [128 rows][64 keys] f16; also where S'[64 + r] changes hands
 constexpr uint32_t PB_OFF_P = PB_NST * PB_UNIT; // two of them, in turn
-constexpr uint32_t PB_OFF_RED = PB_OFF_P + 2 * PB_PBUF; // [2 halves][64 rows] floats, [64 rows] rescale factors, [64 rows] scales of Q'
-constexpr uint32_t PB_OFF_BAR = PB_OFF_RED + 1024;
+constexpr uint32_t PB_OFF_RED = PB_OFF_P + 2 * PB_PBUF; // [4 quarters of a tile's keys][64 rows] floats, [64 rows] scales of Q'
+constexpr uint32_t PB_OFF_BAR = PB_OFF_RED + 1280;
 constexpr uint32_t PB_NBAR = 3 * PB_NST + 7; // full[NST], empty[NST], conv[NST], s_full[2], s_free[2], p_full, pv_done, q_full
 constexpr uint32_t PB_OFF_MISC = PB_OFF_BAR + PB_NBAR * 8;
 constexpr uint32_t PB_NOTES = 16;          // tiles whose scale and notes are kept: more than the ring holds
@@ -445,8 +445,9 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         const uint32_t row = 32u * (q4 & 1u) + lane;         // the row, 0 .. 63
         const uint32_t bar_group = 1u + (q4 & 1u);           // the four warps that have these 32 rows
         const uint32_t own = (q4 >> 1) + 2u * half;          // this warp's number among them
+        const uint32_t e = hi ? 0u : 1u;
         constexpr uint32_t HD = DIM / 2;                     // dims of Q' and O of a thread
-        float *red = reinterpret_cast<float *>(smem + PB_OFF_RED), *cf_s = red + 128, *q_s = red + 192;
+        float *red = reinterpret_cast<float *>(smem + PB_OFF_RED), *q_s = red + 256;
         const uint32_t group = plan.group, tok = row / group, head = row - tok * group;
         auto arrive = [&](uint32_t bar) { // one arrival per warp, after all its lanes
             __syncwarp();
@@ -617,92 +618,75 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 p_buf = smem + PB_OFF_P + (t & 1u) * PB_PBUF; // (free: the product of two tiles in front has been folded)
                 const float m_last = m, cf_last = cf;
                 wait(bar_s_full + 8u * (t & 1u), (t >> 1) & 1u);
-                // The half row's 32 scores stay in the P' buffer (keys 8 c .. 8 c + 3 in chunk c, the next four in chunk 4 + c, where their weights go
-                // in the end): the registers are O's.
+                // A half row's 32 scores: the thread with the hi parts' products takes the first 16, the other the rest; the other 16 of each change
+                // hands in the P' buffer.
                 const uint32_t s_col = tmem + lane_addr + PB_COL_S + 64u * (t & 1u) + 32u * half;
-                auto s_chunk = [&](uint32_t g4) { return p_chunk((g4 >> 1) + 4u * (g4 & 1u)); };
+                uint32_t w[16];
                 if (active) {
-                    if (!hi) {
-                        uint32_t w[32];
-                        tmem_ld32(s_col, w);
-                        tmem_wait_ld();
+                    tmem_ld16(s_col + 16u * (1u - e), w);
+                    tmem_wait_ld();
 #pragma unroll
-                        for (uint32_t c = 0; c < 8u; c++) *reinterpret_cast<uint4 *>(s_chunk(c)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
-                    }
-                    named_bar_sync(bar_group, 128);
-                    if (hi) {
-                        const float f = g.scale2 * (q_unscale * sh->unscale[0][t % PB_NOTES]);
-                        const uint32_t k0 = key0 + 32u * half, odd = *reinterpret_cast<const uint32_t *>(&sh->odd[0][t % PB_NOTES][2u * half]);
-                        const bool edge = key0 < it.all_lo || key0 + PF_KEYS32 > it.all_hi || !real;
-                        // the keys of this half that the row sees, a bit each; not those with values that are not finite
-                        uint32_t see = 0xffffffffu;
-                        if (edge) {
-                            const uint32_t a = klo > k0 ? min(klo - k0, 32u) : 0u, e = vis > k0 ? min(vis - k0, 32u) : 0u;
-                            see = (uint32_t)((1ull << e) - 1ull) & ~(uint32_t)((1ull << a) - 1ull);
-                        }
-                        const uint32_t plain = see & odd;
-                        see &= ~odd;
-                        float mx = NEG_BIG;
-#pragma unroll
-                        for (uint32_t h = 0; h < 2u; h++) {
-                            uint32_t w[16];
-                            tmem_ld16(s_col + 16u * h, w);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (uint32_t c = 0; c < 4u; c++) {
-                                float4 x = *reinterpret_cast<const float4 *>(s_chunk(4u * h + c));
-                                x.x = (__uint_as_float(w[4 * c]) + x.x) * f;
-                                x.y = (__uint_as_float(w[4 * c + 1]) + x.y) * f;
-                                x.z = (__uint_as_float(w[4 * c + 2]) + x.z) * f;
-                                x.w = (__uint_as_float(w[4 * c + 3]) + x.w) * f;
-                                if (see != 0xffffffffu) {
-                                    const uint32_t b = see >> (16u * h + 4u * c);
-                                    x = make_float4(b & 1u ? x.x : -INFINITY, b & 2u ? x.y : -INFINITY, b & 4u ? x.z : -INFINITY, b & 8u ? x.w : -INFINITY);
-                                }
-                                mx = max3(max3(mx, x.x, x.y), x.z, x.w);
-                                *reinterpret_cast<float4 *>(s_chunk(4u * h + c)) = x;
-                            }
-                        }
-#pragma unroll 1
-                        for (uint32_t left = plain; left != 0u; left &= left - 1u) { // (rare)
-                            const uint32_t r = (uint32_t)__ffs((int)left) - 1u;
-                            const float x = plain_score(q_row, k_row(g.kpages, k0 + r));
-                            mx = fmaxf(mx, x);
-                            reinterpret_cast<float *>(s_chunk(r >> 2))[r & 3u] = x;
-                        }
-                        red[64u * half + row] = mx;
-                    }
+                    for (uint32_t c = 0; c < 4u; c++) *reinterpret_cast<uint4 *>(p_chunk(4u * (1u - e) + c)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+                    tmem_ld16(s_col + 16u * e, w);
+                    tmem_wait_ld();
                 }
                 tc_fence_before();
                 arrive(bar_s_free + 8u * (t & 1u));
                 if (active) {
                     named_bar_sync(bar_group, 128);
-                    if (hi) {
-                        const float m_new = max3(m, red[row], red[64u + row]);
-                        cf = m > NEG_TEST ? exp2f(m - m_new) : 0.0f; // (O and l are zero until the first key)
-                        m = m_new;
-                        if (half == 0u) cf_s[row] = cf;
-                        const float neg_m = m > NEG_TEST ? -m : 0.0f;
-                        float sum = 0.0f;
-#pragma unroll
-                        for (uint32_t c = 0; c < 4u; c++) {
-                            const float4 u = *reinterpret_cast<const float4 *>(p_chunk(c)), v = *reinterpret_cast<const float4 *>(p_chunk(4u + c));
-                            float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-#pragma unroll
-                            for (uint32_t e = 0; e < 8u; e++) {
-                                x[e] = ex2(x[e] + neg_m);
-                                sum += x[e];
-                            }
-                            uint4 a, b;
-                            split8(x, 16384.0f, a, b); // 2^14: f16's smallest step is then 2^-38 of the largest weight
-                            *reinterpret_cast<uint4 *>(p_chunk(c)) = a;
-                            *reinterpret_cast<uint4 *>(p_chunk(4u + c)) = b;
-                        }
-                        l = fmaf(l, cf, sum);
-                        fence_proxy_async();
+                    const float f = g.scale2 * (q_unscale * sh->unscale[0][t % PB_NOTES]);
+                    const uint32_t k0 = key0 + 32u * half + 16u * e, odd = sh->odd[0][t % PB_NOTES][2u * half + e];
+                    // the keys of this thread that the row sees, a bit each; not those with values that are not finite
+                    uint32_t see = 0xffffu;
+                    if (key0 < it.all_lo || key0 + PF_KEYS32 > it.all_hi || !real) {
+                        const uint32_t a = klo > k0 ? min(klo - k0, 16u) : 0u, b = vis > k0 ? min(vis - k0, 16u) : 0u;
+                        see = ((1u << b) - 1u) & ~((1u << a) - 1u);
                     }
+                    const uint32_t plain = see & odd;
+                    see &= ~odd;
+                    float x[16], mx = NEG_BIG;
+#pragma unroll
+                    for (uint32_t c = 0; c < 4u; c++) {
+                        const float4 y = *reinterpret_cast<const float4 *>(p_chunk(4u * e + c));
+                        const float o[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                        for (uint32_t n = 0; n < 4u; n++) x[4 * c + n] = (__uint_as_float(w[4 * c + n]) + o[n]) * f;
+                    }
+                    if (see != 0xffffu)
+#pragma unroll
+                        for (uint32_t c = 0; c < 16u; c++) x[c] = see >> c & 1u ? x[c] : -INFINITY;
+#pragma unroll 1
+                    for (uint32_t left = plain; left != 0u; left &= left - 1u) { // (rare)
+                        const uint32_t r = (uint32_t)__ffs((int)left) - 1u;
+                        const float y = plain_score(q_row, k_row(g.kpages, k0 + r));
+#pragma unroll
+                        for (uint32_t c = 0; c < 16u; c++)
+                            if (c == r) x[c] = y;
+                    }
+#pragma unroll
+                    for (uint32_t c = 0; c < 16u; c += 2u) mx = max3(mx, x[c], x[c + 1]);
+                    red[64u * (2u * half + e) + row] = mx;
                     named_bar_sync(bar_group, 128);
-                    if (!hi) cf = cf_s[row];
+                    const float m_new = max3(max3(m, red[row], red[64u + row]), red[128u + row], red[192u + row]);
+                    cf = m > NEG_TEST ? exp2f(m - m_new) : 0.0f; // (O and l are zero until the first key)
+                    m = m_new;
+                    const float neg_m = m > NEG_TEST ? -m : 0.0f;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (uint32_t c = 0; c < 2u; c++) {
+                        float y[8];
+#pragma unroll
+                        for (uint32_t n = 0; n < 8u; n++) {
+                            y[n] = ex2(x[8 * c + n] + neg_m);
+                            sum += y[n];
+                        }
+                        uint4 a, b;
+                        split8(y, 16384.0f, a, b); // 2^14: f16's smallest step is then 2^-38 of the largest weight
+                        *reinterpret_cast<uint4 *>(p_chunk(2u * e + c)) = a;
+                        *reinterpret_cast<uint4 *>(p_chunk(4u + 2u * e + c)) = b;
+                    }
+                    l = fmaf(l, cf, sum);
+                    fence_proxy_async();
                 }
                 if (t > t0) { // behind the tile's scores, so that they and the product of the tile in front run together
                     if (active) fold(t - 1u, m_last, cf_last);
@@ -716,23 +700,19 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             if (more) q_next = load_q(nx, smem + PB_OFF_P + (end & 1u) * PB_PBUF, std::false_type{}); // the segment's scores were all there: its Q' may go
             if (active) {
                 fold(end - 1u, m, cf);
-                if (hi) red[64u * half + row] = l;
+                red[64u * (2u * half + e) + row] = l;
                 named_bar_sync(bar_group, 128); // (P' is free too: its last products have completed)
+                const float l_all = (red[row] + red[64u + row]) + (red[128u + row] + red[192u + row]);
+                const bool seen = real && klo < vis;
                 float *part = nullptr; // a part: maximum, sum and O as they are, for the merge
-                if (!sg.whole) part = g.scratch + part_slot(blockIdx.x, sg.part) * part_floats(DIM);
-                float inv = 0.0f;
-                if (hi) {
-                    const float l_all = red[row] + red[64u + row];
-                    const bool seen = real && klo < vis;
-                    if (sg.whole) {
-                        float den = l_all;
-                        if (g.sinks && real) den += exp2f(g.sinks[sg.kvh * group + head] * PB_LOG2E - (m > NEG_TEST ? m : 0.0f));
-                        if (seen) inv = 1.0f / den; // (otherwise O is zero, and stays so)
-                    } else {
-                        inv = 1.0f;
-                        if (half == 0u && real) *reinterpret_cast<float2 *>(part + 128u * DIM + 2u * row) = make_float2(m, seen ? l_all : -1.0f);
-                    }
-                    if (half == 0u) cf_s[row] = inv;
+                float inv = 1.0f;
+                if (sg.whole) {
+                    float den = l_all;
+                    if (g.sinks && real) den += exp2f(g.sinks[sg.kvh * group + head] * PB_LOG2E - (m > NEG_TEST ? m : 0.0f));
+                    inv = seen ? 1.0f / den : 0.0f; // (O is zero then, and stays so)
+                } else {
+                    part = g.scratch + part_slot(blockIdx.x, sg.part) * part_floats(DIM);
+                    if (hi && half == 0u && real) *reinterpret_cast<float2 *>(part + 128u * DIM + 2u * row) = make_float2(m, seen ? l_all : -1.0f);
                 }
                 // The row's hi and lo parts meet in the P' buffers, in turn, 32 dims of each half at a time: the one thread adds up the first 16, the
                 // other the rest. All threads store, 128 bytes of a row side by side.
@@ -765,7 +745,6 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                     if (hi) give(std::integral_constant<uint32_t, 16>{});
                     else give(std::integral_constant<uint32_t, 0>{});
                     named_bar_sync(bar_group, 128);
-                    if (c0 == 0u) inv = cf_s[row];
                     if (hi) sum(std::integral_constant<uint32_t, 0>{});
                     else sum(std::integral_constant<uint32_t, 16>{});
                     named_bar_sync(bar_group, 128);
