@@ -393,16 +393,17 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                     const uint32_t d = tmem + PB_COL_S + 64u * (t & 1u);
                     ok = ok && pb_wait(bar_conv + 8u * at.s, at.turn, sh, g.status);
                     tc_fence_after();
+                    // All of K lo first: what a step truncates is 2^-24 of the sum so far, and that is small until K hi comes in.
 #pragma unroll
-                    for (uint32_t h = 0; h < NU; h++) {
-                        const uint64_t kd = k_desc + at.s * (PB_UNIT >> 4);
+                    for (uint32_t n = 0; n < 2u * NU; n++) {
+                        const uint32_t h = n % NU;
+                        const uint64_t kd = k_desc + (at.s + h) * (PB_UNIT >> 4) + (n < NU ? PB_BLK >> 4 : 0u);
 #pragma unroll
-                        for (uint32_t ks = 0; ks < 8u; ks++) // 16 dims an MMA, hi and lo
-                            tc_mma_f16_ta(d, tmem + PB_COL_Q + 32u * h + 8u * (ks >> 1), kd + (((ks & 1u) * PB_BLK + (ks >> 1) * 32u) >> 4), IDESC,
-                                          (h > 0 || ks > 0) ? 1u : 0u);
-                        tc_commit(bar_empty + 8u * at.s);
-                        at.next();
+                        for (uint32_t ks = 0; ks < 4u; ks++) // 16 dims an MMA
+                            tc_mma_f16_ta(d, tmem + PB_COL_Q + 32u * h + 8u * ks, kd + ((ks * 32u) >> 4), IDESC, (n > 0 || ks > 0) ? 1u : 0u);
+                        if (n >= NU) tc_commit(bar_empty + 8u * (at.s + h));
                     }
+                    at.next(NU);
                     tc_commit(bar_s_full + 8u * (t & 1u));
                     if (t > 0u) at.next(NU); // over a tile of V
                     ts.next();
@@ -424,8 +425,9 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                     tc_fence_after();
                     const uint64_t vd = v_desc + s0 * (PB_UNIT >> 4);
 #pragma unroll
-                    for (uint32_t ks = 0; ks < 8u; ks++) // 16 keys an MMA, hi and lo
-                        tc_mma_f16(tmem, p_desc + (((t & 1u) * PB_PBUF + (ks >> 1) * 32u) >> 4), vd + (((ks & 1u) * PB_BLK + (ks >> 1) * 2048u) >> 4), IDESC, ks > 0 ? 1u : 0u);
+                    for (uint32_t ks = 0; ks < 8u; ks++) // 16 keys an MMA, V lo first
+                        tc_mma_f16(tmem, p_desc + (((t & 1u) * PB_PBUF + (ks & 3u) * 32u) >> 4), vd + (((ks < 4u ? PB_BLK : 0u) + (ks & 3u) * 2048u) >> 4), IDESC,
+                                   ks > 0 ? 1u : 0u);
 #pragma unroll
                     for (uint32_t h = 0; h < NU; h++) tc_commit(bar_empty + 8u * (s0 + h));
                     tc_commit(bar_pv_done);
