@@ -204,8 +204,14 @@ mkv_status pool_attn_setup(Pool *p) {
 mkv_status launch_pool_attn(Pool *p, int layer, const mkv_seq_rows *items, int n, const PoolAttn &a) {
     const bool f16 = p->desc.fmt == MKV_F16;
     // What a segment costs beside its tiles, measured with 0, 2 and 4 tiles: ragged blocks under a window of 513 in f16 110, 73 and 89 us;
-    // f32 blocks 464, 449 and 452; long histories hardly care (32 sessions in f16 338, 340 and 339; eight in f32 181, 173 and 167).
-    const PlanCost cost = f16 ? PlanCost{128u, 128u, 2u} : PlanCost{64u, 64u, 2u};
+    // f32 blocks (with 1, 2 and 4) 440, 432 and 440; long histories hardly care (32 sessions in f16 338, 340 and 339; eight in f32 171, 168 and
+    // 165).
+    PlanCost cost = f16 ? PlanCost{128u, 128u, 2u} : PlanCost{64u, 64u, 2u};
+    if (!f16) { // items of at most 32 rows have a form of the kernel of their own (PB_FEW)
+        uint32_t most = 0;
+        for (int i = 0; i < n; i++) most = std::max(most, items[i].ntok);
+        if ((uint64_t)most * (uint32_t)(p->desc.q_heads / p->desc.kv_heads) <= 32u) cost.rows = 32u;
+    }
     PoolPlan plan;
     MergeList merge;
     uint32_t rows = 0;

@@ -19,14 +19,17 @@
 // share with ordinary arithmetic for the rows that see them. Keys that no token of the item sees are zero as well, whatever lies in
 // their rows.
 //
-// Bound by the converters: a K or V tile of 64 KB takes its four warps 3,500 to 4,700 clocks (a unit's chain wait - load - split - store
-// is about 800, whatever its share of a warp), so a tile of 256 dims about 9,000, where HBM would take 5,600 and the products take
-// 2,600. More converter warps make each chain longer by as much: eight measured the same. Eight sessions of up to 32,000 tokens
-// (533 MB) take 172 us, 3.1 TB/s; blocks of 300 to 512 tokens over up to 4,096 (46 GFLOP, three f16 products each) 446 us.
+// Bound by the time that a tile stays in the ring: a K or V tile of 64 KB lands about 3,000 clocks after its load was issued, its four
+// converter warps take 3,500 to 4,500 (a unit's chain load - split - store is about 800, whatever a warp's share of it; eight warps on a
+// tile measured the same), products and their waits the rest, and shared memory holds three. Eight sessions of up to 32,000 tokens (533 MB)
+// take 154 us, 3.5 TB/s; blocks of 300 to 512 tokens over up to 4,096 (46 GFLOP, three f16 products each) 405 us.
+//
+// Where every item has at most 32 rows (decode steps, drafts; FEW) the four warps that would have rows 32 .. 63 are a second team of
+// converters, the first one takes K and it takes V: nine sessions with heads of 128 88 us, with one team 96; heads of 256 154 and 157.
 //
 // Roles (512 threads, four warpgroups whose register budgets are set with setmaxnreg): warps 0 and 3 = TMA producers, warp 1 =
 // issues S' and owns the TMEM, warp 2 = issues O', warps 4..7 = converters, warps 8..15 = softmax and owners of O: two threads per TMEM
-// lane, 32 of a tile's keys and half of the dims each. TMEM: O' = columns 0 .. DIM - 1, S' = 256 .. 319 and 320 .. 383, Q' = 384 ...
+// lane, half of the dims each, and of a row's four threads 16 of a tile's keys each. TMEM: O' = columns 0 .. DIM - 1, S' = 256 .. 319 and 320 .. 383, Q' = 384 ...
 // Every wait is bounded; TMEM is freed on every path.
 #include <type_traits>
 
@@ -36,7 +39,7 @@
 namespace mkv {
 using namespace ptx;
 
-constexpr uint32_t PF_KEYS32 = 64;
+constexpr uint32_t PF_KEYS32 = 64, PB_FEW = 32;
 constexpr int PB_THREADS = 512;
 constexpr long long PB_WAIT_LIMIT = 2000000000ll;
 constexpr float PB_LOG2E = 1.4426950408889634f;
@@ -48,14 +51,15 @@ constexpr uint32_t PB_PBUF = 16384;             // P' [128 rows][64 keys] f16; a
 constexpr uint32_t PB_OFF_P = PB_NST * PB_UNIT; // two of them, in turn
 constexpr uint32_t PB_OFF_RED = PB_OFF_P + 2 * PB_PBUF; // [4 quarters of a tile's keys][64 rows] floats, [64 rows] scales of Q'
 constexpr uint32_t PB_OFF_BAR = PB_OFF_RED + 1280;
-constexpr uint32_t PB_NBAR = 3 * PB_NST + 7; // full[NST], empty[NST], conv[NST], s_full[2], s_free[2], p_full, pv_done, q_full
+constexpr uint32_t PB_KINDS = 8;           // K tiles, and V tiles, that the ring cannot hold at one time: barriers of each kind
+constexpr uint32_t PB_NBAR = PB_NST + 4 * PB_KINDS + 7; // empty[NST], full[2][KINDS], conv[2][KINDS], s_full[2], s_free[2], p_full, pv_done, q_full
 constexpr uint32_t PB_OFF_MISC = PB_OFF_BAR + PB_NBAR * 8;
-constexpr uint32_t PB_NOTES = 16;          // tiles whose scale and notes are kept: more than the ring holds
+constexpr uint32_t PB_NOTES = 8;           // tiles whose scale and notes are kept: more than the ring holds
 
 struct PbShared {
     uint32_t tmem_base;
     volatile uint32_t abort;
-    uint32_t amax[4];                 // of each converter warp
+    uint32_t amax[2][4];              // [team][converter warp]
     float unscale[2][PB_NOTES];       // [K, V][tile]
     uint16_t odd[2][PB_NOTES][4];     // keys with a value that is not finite, 16 of each converter warp
 };
@@ -143,33 +147,36 @@ __device__ __forceinline__ void split8(const float (&x)[8], float s, uint4 &hi, 
     lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
-template <int DIM>
+template <int DIM, bool FEW>
 __global__ void __launch_bounds__(PB_THREADS, 1)
 pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PoolPlan plan,
                      const __grid_constant__ PbArgs g) {
-    constexpr uint32_t NU = DIM / 64; // units of a tile
+    constexpr uint32_t NU = DIM / 64;       // units of a tile
+    constexpr uint32_t SOFT = FEW ? 4 : 8;  // softmax warps
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *smem = smem_raw + (smem_base - smem_u32(smem_raw));
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t bar0 = smem_base + PB_OFF_BAR;
-    const uint32_t bar_full = bar0, bar_empty = bar0 + 8u * PB_NST, bar_conv = bar0 + 16u * PB_NST, bar_s_full = bar0 + 24u * PB_NST;
+    const uint32_t bar_empty = bar0, bar_full = bar0 + 8u * PB_NST, bar_conv = bar_full + 16u * PB_KINDS, bar_s_full = bar_conv + 16u * PB_KINDS;
     const uint32_t bar_s_free = bar_s_full + 16u, bar_p_full = bar_s_free + 16u, bar_pv_done = bar_p_full + 8u, bar_q_full = bar_pv_done + 8u;
+    // full and conv: of K or V tile t. (Not of a slot of the ring: who waits for K tiles alone would miss a slot's phases for V.)
+    auto of_tile = [](bool v, uint32_t t) { return 8u * ((v ? PB_KINDS : 0u) + t % PB_KINDS); };
     PbShared *sh = reinterpret_cast<PbShared *>(smem + PB_OFF_MISC);
 
     if (tid == 0) {
-        for (uint32_t s = 0; s < PB_NST; s++) {
+        for (uint32_t s = 0; s < PB_NST; s++) mbar_init(bar_empty + 8u * s, 1);
+        for (uint32_t s = 0; s < 2u * PB_KINDS; s++) {
             mbar_init(bar_full + 8u * s, 2); // one arrival per producer
-            mbar_init(bar_empty + 8u * s, 1);
             mbar_init(bar_conv + 8u * s, 4); // one arrival per converter warp
         }
         for (uint32_t s = 0; s < 2u; s++) {
             mbar_init(bar_s_full + 8u * s, 1);
-            mbar_init(bar_s_free + 8u * s, 8); // one arrival per softmax warp
+            mbar_init(bar_s_free + 8u * s, SOFT); // one arrival per softmax warp
         }
-        mbar_init(bar_p_full, 8);
+        mbar_init(bar_p_full, SOFT);
         mbar_init(bar_pv_done, 1);
-        mbar_init(bar_q_full, 8);
+        mbar_init(bar_q_full, SOFT);
         sh->abort = 0;
         fence_barrier_init();
         fence_proxy_async();
@@ -185,8 +192,9 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     // The units of the CTA's T tiles in ring order, whatever segment they belong to: K(0), then K(t + 1) and V(t) for each t. In front of
     // K(t) are t + max(t - 1, 0) tiles of K and V, in front of V(t) min(t + 2, T) + t.
     // ---------------- converters: a warp has 16 keys of every unit, a lane one of a key's two blocks ----------------
-    auto converter = [&]() {
-        const uint32_t cw = warp - 4u, key_in = 16u * cw + (lane >> 1), j = lane & 1u;
+    // One team of four warps for K and V, or one for each.
+    auto converter = [&](bool k_tiles, bool v_tiles, uint32_t cw) {
+        const uint32_t team = k_tiles ? 0u : 1u, bar_team = 3u + team, key_in = 16u * cw + (lane >> 1), j = lane & 1u;
         // chunk of the block's row that x[i] holds: in an order in which a key's two lanes meet no bank together
         auto chunk = [&](uint32_t i) { return i ^ (4u * j); };
         PbRing<PB_NST> at;
@@ -246,13 +254,13 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             };
             auto tile_scale = [&]() -> float { // of the largest of all warps' amax
                 const uint32_t mine = __reduce_max_sync(0xffffffffu, __float_as_uint(amax));
-                if (lane == 0) sh->amax[cw] = mine;
-                named_bar_sync(3, 128); // (there is another in front of the next use of amax[])
+                if (lane == 0) sh->amax[team][cw] = mine;
+                named_bar_sync(bar_team, 128); // (there is another in front of the next use of amax[])
                 uint32_t most = 0u;
-                for (uint32_t i = 0; i < 4u; i++) most = max(most, sh->amax[i]);
+                for (uint32_t i = 0; i < 4u; i++) most = max(most, sh->amax[team][i]);
                 return most ? __uint_as_float(scale_bits(most)) : 1.0f;
             };
-            pb_wait(bar_full + 8u * begin.s, begin.turn, sh, g.status);
+            pb_wait(bar_full + of_tile(v, note), (note / PB_KINDS) & 1u, sh, g.status);
             __syncwarp();
             if (note == 0u) { // the first tile has no scale in front of it: the largest value of its first 64 dims gives it, to [2^11, 2^12)
                 float4 x[8];
@@ -273,7 +281,7 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             // The scale fits if each warp's largest value lies well inside f16's range under it. Otherwise, and where values are not finite, once
             // more from global memory: the tile's largest finite value, then its values with the scale that this gives, the others as zeros.
             amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
-            if (named_bar_or(3, 128, odd || (amax != 0.0f && !(amax * s >= 256.0f && amax * s < 32768.0f)))) {
+            if (named_bar_or(bar_team, 128, odd || (amax != 0.0f && !(amax * s >= 256.0f && amax * s < 32768.0f)))) {
                 const float *src = v ? g.vpages : g.kpages;
                 if (in) {
                     const size_t page = __ldg(g.pages + tl.table + (key >> g.page_shift));
@@ -304,7 +312,7 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                     again(h, x);
                     put(begin.s + h, x);
                 }
-                named_bar_sync(3, 128); // amax[] has been read
+                named_bar_sync(bar_team, 128); // amax[] has been read
             }
             const uint32_t odds = __ballot_sync(0xffffffffu, odd);
             if (lane == 0) {
@@ -316,15 +324,20 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             }
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar_conv + 8u * begin.s); // (of the tile's first unit, for all)
+            if (lane == 0) mbar_arrive(bar_conv + of_tile(v, note));
         };
         // A wait that runs out makes all later ones return at once; the warps go through the same barriers all the same.
         Tile cur = take(Tile{});
-        convert(false, cur, 0u);
+        if (k_tiles) convert(false, cur, 0u);
+        else at.next(NU);
         for (uint32_t t = 0; t < total; t++) {
             const Tile ahead = ts.more ? take(cur) : cur;
-            if (t + 1u < total) convert(false, ahead, t + 1u);
-            convert(true, cur, t);
+            if (t + 1u < total) {
+                if (k_tiles) convert(false, ahead, t + 1u);
+                else at.next(NU);
+            }
+            if (v_tiles) convert(true, cur, t);
+            else at.next(NU);
             cur = ahead;
         }
     };
@@ -353,25 +366,25 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 if (t.is) ts.next();
                 return t;
             };
-            auto load = [&](const CUtensorMap *map, const Tile &t) -> bool { // the units of one K or V tile
-                const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, t.row != ~0u)), bar = bar_full + 8u * at.s; // (of the first unit, for all)
+            auto load = [&](bool v, const Tile &t, uint32_t n) -> bool { // the units of K or V tile n
+                const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, t.row != ~0u)), bar = bar_full + of_tile(v, n);
 #pragma unroll 1
                 for (uint32_t h = 0; h < NU; h++, u++, at.next()) {
                     if (u >= PB_NST && !__all_sync(0xffffffffu, pb_wait(bar_empty + 8u * at.s, at.turn ^ 1u, sh, g.status))) return false;
                     if (h == 0u && lane == 0) mbar_expect_tx(bar, NU * boxes * box_rows * 128u);
                     __syncwarp();
                     if (t.row != ~0u)
-                        tma_load_2d(smem_base + at.s * PB_UNIT + cb * PB_BLK + rb * box_rows * 128u, map, t.x + (int)(64u * h), (int)t.row, bar);
+                        tma_load_2d(smem_base + at.s * PB_UNIT + cb * PB_BLK + rb * box_rows * 128u, v ? &vmap : &kmap, t.x + (int)(64u * h), (int)t.row, bar);
                 }
                 return true;
             };
             Tile cur = look_up();
-            bool ok = load(&kmap, cur);
+            bool ok = load(false, cur, 0u);
             Tile ahead = look_up();
-            while (ok && cur.is) {
+            for (uint32_t t = 0; ok && cur.is; t++) {
                 const Tile later = look_up(); // (its page is there when its turn comes)
-                if (ahead.is) ok = load(&kmap, ahead);
-                ok = ok && load(&vmap, cur);
+                if (ahead.is) ok = load(false, ahead, t + 1u);
+                ok = ok && load(true, cur, t);
                 cur = ahead;
                 ahead = later;
             }
@@ -391,7 +404,7 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                     }
                     if (t >= 2u) ok = ok && pb_wait(bar_s_free + 8u * (t & 1u), ((t >> 1) - 1u) & 1u, sh, g.status);
                     const uint32_t d = tmem + PB_COL_S + 64u * (t & 1u);
-                    ok = ok && pb_wait(bar_conv + 8u * at.s, at.turn, sh, g.status);
+                    ok = ok && pb_wait(bar_conv + of_tile(false, t), (t / PB_KINDS) & 1u, sh, g.status);
                     tc_fence_after();
                     // All of K lo first: what a step truncates is 2^-24 of the sum so far, and that is small until K hi comes in.
 #pragma unroll
@@ -419,7 +432,7 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 bool ok = true;
                 for (uint32_t t = 0; ok && t < total; t++) {
                     const uint32_t s0 = at.s;
-                    ok = ok && pb_wait(bar_conv + 8u * s0, at.turn, sh, g.status);
+                    ok = ok && pb_wait(bar_conv + of_tile(true, t), (t / PB_KINDS) & 1u, sh, g.status);
                     at.next(NU);
                     ok = ok && pb_wait(bar_p_full, t & 1u, sh, g.status);
                     tc_fence_after();
@@ -437,9 +450,20 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         }
     } else if (warp < 8u) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-        converter();
+        converter(true, !FEW, warp - 4u);
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 192;"); // 128 x 48 + 128 x 80 + 256 x 192 = the launch's 512 x 128
+        if (FEW && (warp & 1u)) {
+            // the lanes of rows 32 .. 63, which no item has: zeros, so that their products draw less power
+            const uint32_t z[16] = {};
+            const uint32_t q4 = warp & 3u, half = (warp - 8u) >> 2;
+            for (uint32_t c = 0; c < DIM / 4u; c += 16u) tmem_st16(tmem + ((32u * q4) << 16) + PB_COL_Q + DIM / 4u * half + c, z);
+            tmem_wait_st();
+            for (uint32_t c = 0; c < 8u; c++) *reinterpret_cast<uint4 *>(smem + PB_OFF_P + half * PB_PBUF + swz128(32u * q4 + lane, c)) = make_uint4(0u, 0u, 0u, 0u);
+            fence_proxy_async();
+            tc_fence_before();
+            converter(false, true, (warp - 8u) >> 1);
+        } else {
         // ---------------- softmax ----------------
         const uint32_t q4 = warp & 3u, half = (warp - 8u) >> 2;
         const uint32_t lane_addr = (32u * q4) << 16;
@@ -765,6 +789,7 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             t0 = end;
             sg = nx;
         }
+        }
     }
 
     // ---------------- teardown ----------------
@@ -783,7 +808,10 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
 
 template <int DIM> static mkv_status launch_dim(Pool *p, int layer, const PoolPlan &plan, const PbArgs &g) {
     PdlLaunch l(p->ctx, dim3(plan.ctas), PB_THREADS, PB_SMEM);
-    MKV_CUDA(cudaLaunchKernelEx(&l.cfg, pool_attn_f32_kernel<DIM>, p->maps[2 * (size_t)layer], p->maps[2 * (size_t)layer + 1], plan, g));
+    if (plan.block * plan.group <= PB_FEW)
+        MKV_CUDA(cudaLaunchKernelEx(&l.cfg, pool_attn_f32_kernel<DIM, true>, p->maps[2 * (size_t)layer], p->maps[2 * (size_t)layer + 1], plan, g));
+    else
+        MKV_CUDA(cudaLaunchKernelEx(&l.cfg, pool_attn_f32_kernel<DIM, false>, p->maps[2 * (size_t)layer], p->maps[2 * (size_t)layer + 1], plan, g));
     p->ctx->launches++;
     return MKV_OK;
 }
@@ -810,11 +838,15 @@ mkv_status launch_pool_attn_f32(Pool *p, int layer, const PoolPlan &plan, const 
     }
 }
 
-mkv_status pool_attn_f32_setup(Pool *) {
-    MKV_CUDA(cudaFuncSetAttribute(pool_attn_f32_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PB_SMEM));
-    MKV_CUDA(cudaFuncSetAttribute(pool_attn_f32_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PB_SMEM));
-    MKV_CUDA(cudaFuncSetAttribute(pool_attn_f32_kernel<256>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PB_SMEM));
+template <int DIM> static mkv_status setup_dim() {
+    MKV_CUDA(cudaFuncSetAttribute(pool_attn_f32_kernel<DIM, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PB_SMEM));
+    MKV_CUDA(cudaFuncSetAttribute(pool_attn_f32_kernel<DIM, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PB_SMEM));
     return MKV_OK;
+}
+mkv_status pool_attn_f32_setup(Pool *) {
+    mkv_status st = setup_dim<64>();
+    if (st == MKV_OK) st = setup_dim<128>();
+    return st == MKV_OK ? setup_dim<256>() : st;
 }
 
 } // namespace mkv
