@@ -207,10 +207,10 @@ mkv_status launch_pool_attn(Pool *p, int layer, const mkv_seq_rows *items, int n
     // f32 blocks (with 1, 2 and 4) 440, 432 and 440; long histories hardly care (32 sessions in f16 338, 340 and 339; eight in f32 171, 168 and
     // 165).
     PlanCost cost = f16 ? PlanCost{128u, 128u, 2u} : PlanCost{64u, 64u, 2u};
-    if (!f16) { // items of at most 32 rows have a form of the kernel of their own (PB_FEW)
+    if (!f16) { // items of at most 32 rows have a form of the kernel of their own
         uint32_t most = 0;
         for (int i = 0; i < n; i++) most = std::max(most, items[i].ntok);
-        if ((uint64_t)most * (uint32_t)(p->desc.q_heads / p->desc.kv_heads) <= 32u) cost.rows = 32u;
+        if ((uint64_t)most * (uint32_t)(p->desc.q_heads / p->desc.kv_heads) <= PLAN_FEW) cost.rows = PLAN_FEW;
     }
     PoolPlan plan;
     MergeList merge;

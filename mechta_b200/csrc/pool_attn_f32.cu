@@ -39,7 +39,7 @@
 namespace mkv {
 using namespace ptx;
 
-constexpr uint32_t PF_KEYS32 = 64, PB_FEW = 32;
+constexpr uint32_t PF_KEYS32 = 64;
 constexpr int PB_THREADS = 512;
 constexpr long long PB_WAIT_LIMIT = 2000000000ll;
 constexpr float PB_LOG2E = 1.4426950408889634f;
@@ -808,7 +808,7 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
 
 template <int DIM> static mkv_status launch_dim(Pool *p, int layer, const PoolPlan &plan, const PbArgs &g) {
     PdlLaunch l(p->ctx, dim3(plan.ctas), PB_THREADS, PB_SMEM);
-    if (plan.block * plan.group <= PB_FEW)
+    if (plan.block * plan.group <= PLAN_FEW)
         MKV_CUDA(cudaLaunchKernelEx(&l.cfg, pool_attn_f32_kernel<DIM, true>, p->maps[2 * (size_t)layer], p->maps[2 * (size_t)layer + 1], plan, g));
     else
         MKV_CUDA(cudaLaunchKernelEx(&l.cfg, pool_attn_f32_kernel<DIM, false>, p->maps[2 * (size_t)layer], p->maps[2 * (size_t)layer + 1], plan, g));

@@ -14,6 +14,7 @@ namespace mkv {
 
 constexpr uint32_t PLAN_SEQS = 128; // sequences of one launch
 constexpr uint32_t PLAN_CTAS = 160;
+constexpr uint32_t PLAN_FEW = 32; // rows of an item up to which the f32 kernel has a form of its own
 
 struct PlanSeq {
     uint32_t table, first, pos, ntok, row; // first entry of the page table; first key seen; ...; packed tokens in front
