@@ -169,3 +169,63 @@ impl<'c> KvCache<'c> {
 impl Drop for KvCache<'_> {
     fn drop(&mut self) { unsafe { sys::mkv_cache_destroy(self.raw) } }
 }
+
+/// Rotary positions: layouts, partial dims and the frequency scalings of mkv_rope_desc. Host data only.
+pub struct Rope { raw: *mut sys::mkv_rope }
+
+impl Rope {
+    pub fn new(desc: &sys::mkv_rope_desc) -> Result<Self, KvError> {
+        let mut raw = ptr::null_mut();
+        check(unsafe { sys::mkv_rope_create(desc, &mut raw) })?;
+        Ok(Rope { raw })
+    }
+    /// `rows` holds device addresses of the caller's buffers.
+    pub fn apply(&self, ctx: &KvContext, rows: &sys::mkv_rope_rows) -> Result<(), KvError> { check(unsafe { sys::mkv_rope_apply(ctx.raw, self.raw, rows) }) }
+}
+
+impl Drop for Rope {
+    fn drop(&mut self) { unsafe { sys::mkv_rope_destroy(self.raw) } }
+}
+
+/// Pages of K and V rows for many sequences. Sequences are small numbers, used again after `free`.
+pub struct KvPool<'c> { raw: *mut sys::mkv_pool, _ctx: PhantomData<&'c KvContext> }
+
+impl<'c> KvPool<'c> {
+    pub fn new(ctx: &'c KvContext, desc: &sys::mkv_pool_desc) -> Result<Self, KvError> {
+        let mut raw = ptr::null_mut();
+        check(unsafe { sys::mkv_pool_create(ctx.raw, desc, &mut raw) })?;
+        Ok(KvPool { raw, _ctx: PhantomData })
+    }
+    pub fn free_pages(&self) -> u32 { unsafe { sys::mkv_pool_free_pages(self.raw) } }
+    pub fn create(&mut self) -> Result<u32, KvError> {
+        let mut seq = 0u32;
+        check(unsafe { sys::mkv_seq_create(self.raw, &mut seq) })?;
+        Ok(seq)
+    }
+    /// `n` sequences that begin with the first `len` rows of `seq`, on its pages or on copies.
+    pub fn fork(&mut self, seq: u32, len: u32, copy: bool, n: usize) -> Result<Vec<u32>, KvError> {
+        let mut kids = vec![0u32; n];
+        check(unsafe { sys::mkv_seq_fork(self.raw, seq, len, copy as c_int, n as c_int, kids.as_mut_ptr()) })?;
+        Ok(kids)
+    }
+    pub fn free(&mut self, seqs: &[u32]) -> Result<(), KvError> { check(unsafe { sys::mkv_seq_free(self.raw, seqs.as_ptr(), seqs.len() as c_int) }) }
+    pub fn truncate(&mut self, seq: u32, len: u32) -> Result<(), KvError> { check(unsafe { sys::mkv_seq_truncate(self.raw, seq, len) }) }
+    pub fn set_len(&mut self, seq: u32, len: u32) -> Result<(), KvError> { check(unsafe { sys::mkv_seq_set_len(self.raw, seq, len) }) }
+    pub fn len(&self, seq: u32) -> u32 { unsafe { sys::mkv_seq_len(self.raw, seq) } }
+    pub fn compact(&mut self) -> Result<u32, KvError> {
+        let mut moved = 0u32;
+        check(unsafe { sys::mkv_pool_compact(self.raw, &mut moved) })?;
+        Ok(moved)
+    }
+    /// New rows of `items` in one layer. `rows.rope` (may be NULL) is that of a live `Rope`.
+    pub fn write(&mut self, layer: i32, items: &[sys::mkv_seq_rows], rows: &sys::mkv_pool_rows) -> Result<(), KvError> {
+        check(unsafe { sys::mkv_pool_write(self.raw, layer as c_int, items.as_ptr(), items.len() as c_int, rows) })
+    }
+    pub fn attn(&mut self, layer: i32, items: &[sys::mkv_seq_rows], args: &sys::mkv_pool_attn) -> Result<(), KvError> {
+        check(unsafe { sys::mkv_attn_pool(self.raw, layer as c_int, items.as_ptr(), items.len() as c_int, args) })
+    }
+}
+
+impl Drop for KvPool<'_> {
+    fn drop(&mut self) { unsafe { sys::mkv_pool_destroy(self.raw) } }
+}
