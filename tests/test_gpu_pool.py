@@ -693,3 +693,32 @@ def test_most_heads(ctx, fmt, heads, rot, layout):
     q = randn(g, 6, hq, dim, dtype=pool.fmt.torch_dtype)
     check_attn(pool, [(ids[0], 0, 1, 1), (ids[1], 0, 128, 5)], q)
     pool.close()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("heads,front", [((16, 2, 256), 0.0), ((16, 2, 256), 2.0**-9), ((16, 2, 256), 2.0**9), ((32, 4, 128), 2.0**9), ((6, 2, 64), 1.0)])
+@pytest.mark.parametrize("news", [(1, 2, 3), (70, 1, 33)])
+def test_magnitudes_that_jump(ctx, fmt, heads, front, news):
+    """Rows whose size changes from one stretch of keys to the next, the first 64 dims of another size than the rest: scales that are kept,
+    left and found again, with few rows and with many."""
+    hq, hkv, dim = heads
+    lens = [500, 64, 333]
+    pool, ids, g = scattered(ctx, fmt, lens, 16, 101, heads=heads)
+    sizes = [1.0, 2.0**-8, 2.0**-8, 2.0**4, 0.0, 1.0] if fmt == F16 else [1.0, 2.0**-40, 2.0**-12, 2.0**6, 0.0, 2.0**-100, 1.0]
+    for t, most in zip(pool.buffer_tensors(0), (1.0, 2.0**5 if fmt == F16 else 2.0**60)):
+        for i, n in zip(ids, lens):
+            pages = torch.from_numpy(pool.pages(i).astype(np.int64)).cuda()
+            at = torch.arange(len(pages) * 16, device="cuda")
+            size = torch.tensor(sizes, device="cuda")[(at // 83) % len(sizes)] * most
+            rows = torch.randn(len(pages) * 16, hkv, dim, device="cuda", generator=g) * size[:, None, None]
+            rows[..., :64] *= front
+            t[pages] = rows.to(t.dtype).view(len(pages), 16, hkv, dim)
+    q = randn(g, sum(news), hq, dim, dtype=pool.fmt.torch_dtype) * 2.0**-6
+    items = [(i, 0, n - m, m) for i, n, m in zip(ids, lens, news)]
+    got = run_attn(pool, items, q)
+    want, mag, qk, top = attn64(pool, items, q)
+    # The largest f16 rows are infinite: what the formula makes of those has to come out as well, or NaN in place of an infinity: scores are
+    # hundreds apart here, a weight below 2^-149 (e^-104) is zero in 32 bits, and zero times an infinity is NaN.
+    same = (got == want) | (got.isnan() & ~want.isfinite())
+    assert (((got.double() - want).abs() <= attn_bound(fmt, want, mag, qk, top)) | same).all()
+    pool.close()
