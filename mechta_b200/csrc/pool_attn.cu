@@ -46,12 +46,17 @@ bool pool_plan(const Pool *p, const mkv_seq_rows *items, int n, int &i, uint32_t
     plan.block = cost.rows / plan.group;
     plan.window = window;
     uint64_t total = 0, count = 0;
+    uint32_t longest = 0;
     for (; i < n && plan.nseq < PLAN_SEQS; i++) {
         if (items[i].ntok == 0u) continue;
         PlanSeq &s = plan.seq[plan.nseq];
         s = {items[i].seq * p->book.max_pages, items[i].first_pos, items[i].pos, items[i].ntok, rows};
         uint64_t tiles = 0, blocks = 0;
-        for (; blocks * plan.block < s.ntok; blocks++) tiles += plan_item(s, window, plan.block, (uint32_t)blocks, cost.keys).tiles;
+        for (; blocks * plan.block < s.ntok; blocks++) {
+            const uint32_t t = plan_item(s, window, plan.block, (uint32_t)blocks, cost.keys).tiles;
+            tiles += t;
+            longest = std::max(longest, t);
+        }
         if (total + tiles * plan.kv_heads > 0x7fffffffull && plan.nseq > 0u) break; // (one sequence alone stays below: mkv_attn_pool refuses more)
         total += tiles * plan.kv_heads;
         count += blocks * plan.kv_heads;
@@ -62,6 +67,7 @@ bool pool_plan(const Pool *p, const mkv_seq_rows *items, int n, int &i, uint32_t
     const uint32_t sms = std::min<uint32_t>((uint32_t)p->ctx->sm_count, PLAN_CTAS);
     // the least that could do, and a little more as often as it takes
     uint64_t budget = std::max<uint64_t>((total + count * cost.segment + sms - 1u) / sms, cost.segment + 1u);
+    if (longest <= cost.whole) budget = std::max<uint64_t>(budget, cost.segment + longest); // nothing is split
     while (!plan_cut(plan, merge, cost, sms, budget)) budget += budget / 32u + 1u;
     return true;
 }
@@ -206,7 +212,9 @@ mkv_status launch_pool_attn(Pool *p, int layer, const mkv_seq_rows *items, int n
     // What a segment costs beside its tiles, measured with 0, 2 and 4 tiles: ragged blocks under a window of 513 in f16 110, 73 and 89 us;
     // f32 blocks (with 1, 2 and 4) 440, 432 and 440; long histories hardly care (32 sessions in f16 338, 340 and 339; eight in f32 171, 168 and
     // 165).
-    PlanCost cost = f16 ? PlanCost{128u, 128u, 2u} : PlanCost{64u, 64u, 2u};
+    // Where all items have at most two tiles, a second tile in a row is sooner done than a merge (windows of 23 in f16 heads of 128 11.6 us,
+    // split 15.0; in f32 11.5 and 12.7), but not in f32 with heads of 256 (20.7 us, split 16.8).
+    PlanCost cost = f16 ? PlanCost{128u, 128u, 2u, 2u} : PlanCost{64u, 64u, 2u, p->desc.head_dim == 256 ? 1u : 2u};
     if (!f16) { // items of at most 32 rows have a form of the kernel of their own
         uint32_t most = 0;
         for (int i = 0; i < n; i++) most = std::max(most, items[i].ntok);

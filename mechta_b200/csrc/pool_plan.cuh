@@ -113,6 +113,7 @@ struct PlanCost {
     uint32_t rows;    // of an item: query heads of a KV head times tokens
     uint32_t keys;    // of a tile
     uint32_t segment; // in tiles
+    uint32_t whole;   // tiles of an item up to which it is not worth a merge
 };
 bool pool_plan(const Pool *p, const mkv_seq_rows *items, int n, int &i, uint32_t &rows, uint32_t window, const PlanCost &cost, PoolPlan &plan, MergeList &merge);
 
