@@ -50,6 +50,16 @@ class FreeSet {
         bits[x / 64u] &= ~(1ull << (x % 64u));
         count--;
     }
+    // Calls f for the numbers in [a, b) that are free, or that are not, in ascending order, until it returns false.
+    template <class F> void each(uint32_t a, uint32_t b, bool free, const F &f) const {
+        for (size_t w = a / 64u; w * 64u < b; w++) {
+            uint64_t x = free ? bits[w] : ~bits[w];
+            if (w == a / 64u) x &= ~0ull << (a % 64u);
+            if ((w + 1u) * 64u > b) x &= (1ull << (b % 64u)) - 1ull;
+            for (; x; x &= x - 1ull)
+                if (!f((uint32_t)(w * 64u) + (uint32_t)__builtin_ctzll(x))) return;
+        }
+    }
     void give(uint32_t x) {
         bits[x / 64u] |= 1ull << (x % 64u);
         low = std::min<size_t>(low, x / 64u);
@@ -249,12 +259,12 @@ class PageBook {
 
     mkv_status compact(uint32_t *moved) {
         const uint32_t used = n_pages - free_pages.size();
+        if (moved) *moved = 0u;
+        if (used == n_pages || free_pages.lowest() >= used) return MKV_OK; // the pages in use are the lowest
         std::vector<uint32_t> src, dst;
-        for (uint32_t p = used; p < n_pages; p++)
-            if (!free_pages.has(p)) src.push_back(p);
+        free_pages.each(used, n_pages, false, [&](uint32_t p) { return src.push_back(p), true; });
         dst.reserve(src.size());
-        for (uint32_t p = 0; p < used && dst.size() < src.size(); p++)
-            if (free_pages.has(p)) dst.push_back(p);
+        free_pages.each(0u, used, true, [&](uint32_t p) { return dst.push_back(p), dst.size() < src.size(); });
         size_t entries = 0;
         for (const Seq &s : seqs)
             for (uint32_t p : s.pages) entries += p >= used;
@@ -356,10 +366,10 @@ class PageBook {
     }
     void shrink(uint32_t s, uint32_t want) {
         std::vector<uint32_t> &v = seqs[s].pages;
-        while (v.size() > want) {
-            if (--refs[v.back()] == 0u) free_pages.give(v.back());
-            v.pop_back();
-        }
+        if (v.size() <= want) return;
+        for (size_t j = want; j < v.size(); j++)
+            if (--refs[v[j]] == 0u) free_pages.give(v[j]);
+        v.resize(want);
     }
     void cut(uint32_t s, uint32_t len) {
         shrink(s, pages_of(len));

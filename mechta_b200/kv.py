@@ -359,39 +359,47 @@ class KvPool:
         L = _lib.lib()
         check(L.mkv_pool_create(ctx._h if ctx is not None else None, C.byref(d), C.byref(self._h)))
         self._dtype, self._device = self.fmt.torch_dtype, ctx.device if ctx is not None else -1
-        self._write, self._attn = L.mkv_pool_write, L.mkv_attn_pool
+        self._write, self._attn, self._lib = L.mkv_pool_write, L.mkv_attn_pool, L
+        self._out = C.c_uint32()  # where calls put a number
+        self._out_ref = C.byref(self._out)
 
     # -- bookkeeping
     @property
     def free_pages(self) -> int:
-        return int(_lib.lib().mkv_pool_free_pages(self._h))
+        return self._lib.mkv_pool_free_pages(self._h)
 
     def create(self) -> int:
         """An empty sequence."""
-        s = C.c_uint32()
-        check(_lib.lib().mkv_seq_create(self._h, C.byref(s)))
-        return s.value
+        check(self._lib.mkv_seq_create(self._h, self._out_ref))
+        return self._out.value
 
     def fork(self, seq: int, length: int | None = None, n: int = 1, copy: bool = False) -> list[int]:
         """n sequences that begin with the first `length` rows of `seq` (all of them by default), on the same pages or on copies."""
         _need(0 < n <= self.max_seqs, f"fork of {n} sequences: 1 to {self.max_seqs}")
+        if n == 1:
+            check(self._lib.mkv_seq_fork(self._h, seq, self.length(seq) if length is None else length, copy, 1, self._out_ref))
+            return [self._out.value]
         kids = (C.c_uint32 * n)()
-        check(_lib.lib().mkv_seq_fork(self._h, seq, self.length(seq) if length is None else length, int(copy), n, kids))
-        return list(kids)
+        check(self._lib.mkv_seq_fork(self._h, seq, self.length(seq) if length is None else length, copy, n, kids))
+        return kids[:]
 
     def free(self, seqs) -> None:
-        a = np.ascontiguousarray(seqs, np.uint32).reshape(-1)
-        check(_lib.lib().mkv_seq_free(self._h, a.ctypes.data, a.size))
+        if type(seqs) is list and {*map(type, seqs)} <= {int}:
+            a, n = (C.c_uint32 * len(seqs))(*seqs), len(seqs)
+        else:
+            held = np.ascontiguousarray(seqs, np.uint32).reshape(-1)
+            a, n = held.ctypes.data, held.size
+        check(self._lib.mkv_seq_free(self._h, a, n))
 
     def truncate(self, seq: int, length: int) -> None:
-        check(_lib.lib().mkv_seq_truncate(self._h, seq, length))
+        check(self._lib.mkv_seq_truncate(self._h, seq, length))
 
     def set_len(self, seq: int, length: int) -> None:
         """Declares rows valid that the host fills itself (buffer_tensors), in all layers."""
-        check(_lib.lib().mkv_seq_set_len(self._h, seq, length))
+        check(self._lib.mkv_seq_set_len(self._h, seq, length))
 
     def length(self, seq: int) -> int:
-        return int(_lib.lib().mkv_seq_len(self._h, seq))
+        return self._lib.mkv_seq_len(self._h, seq)
 
     def pages(self, seq: int) -> np.ndarray:
         n = C.c_uint32()
@@ -402,9 +410,8 @@ class KvPool:
 
     def compact(self) -> int:
         """Moves the pages in use together; returns how many moved."""
-        n = C.c_uint32()
-        check(_lib.lib().mkv_pool_compact(self._h, C.byref(n)))
-        return n.value
+        check(self._lib.mkv_pool_compact(self._h, self._out_ref))
+        return self._out.value
 
     # -- rows
     def buffers(self, layer: int) -> tuple[int, int]:
