@@ -5,6 +5,7 @@
 // token: its cosines and sines (one product in f64 and one sincospi a pair) are computed once, in shared memory, while the block's
 // loads of x are in flight. Measured: 8,192 tokens of 32 heads of 128 f32 dims (268 MB) in 42.6 us, 6.3 TB/s, 98% of a plain copy's rate;
 // the queries of a four-token step 2.3 us.
+#include <algorithm>
 #include <cmath>
 #include <new>
 
@@ -15,14 +16,15 @@
 namespace mkv {
 
 RopeTab rope_tab(const mkv_rope *r, bool backward) {
-    RopeTab t = {};
+    RopeTab t;
     t.m = 1.0f;
+    t.pairs = t.interleaved = 0u;
     t.sign = backward ? -1.0f : 1.0f;
     if (!r) return t;
     t.m = (float)r->m;
     t.pairs = (uint32_t)r->desc.dims / 2u;
     t.interleaved = r->desc.layout == MKV_ROPE_INTERLEAVED;
-    for (uint32_t i = 0; i < t.pairs; i++) t.turns[i] = r->freq[i] / 6.283185307179586476925286766559;
+    std::copy_n(r->turns, t.pairs, t.turns);
     return t;
 }
 
@@ -148,6 +150,7 @@ mkv_status mkv_rope_create(const mkv_rope_desc *d, mkv_rope **out) {
             f = f / s * (1.0 - keep) + f * keep;
         }
         r->freq[i] = f;
+        r->turns[i] = f / 6.283185307179586476925286766559;
     }
     *out = r;
     return MKV_OK;

@@ -5,7 +5,8 @@
 
 struct mkv_rope {
     mkv_rope_desc desc;
-    double freq[MKV_ROPE_MAX_DIMS / 2]; // radians per position
+    double freq[MKV_ROPE_MAX_DIMS / 2];  // radians per position
+    double turns[MKV_ROPE_MAX_DIMS / 2]; // whole turns per position
     double m;                           // factor on cosine and sine
 };
 
