@@ -274,16 +274,20 @@ def _need(ok, text: str) -> None:
 
 
 def _fmt_of(t: torch.Tensor) -> int:
-    if t.dtype is torch.float16:
-        return _lib.F16
-    _need(t.dtype is torch.float32, f"{t.dtype}: must be float16 or float32")
-    return _lib.F32
+    if t.dtype is torch.float32:
+        return _lib.F32
+    if t.dtype is not torch.float16:
+        _need(False, f"{t.dtype}: must be float16 or float32")
+    return _lib.F16
 
 
 def _block(t: torch.Tensor, device: int, what: str) -> tuple[tuple, int, int]:
-    """Shape, token and head stride (0 where there is one token or head) of a [tokens][heads][dims] tensor on `device` whose dims are
-    contiguous and whose tokens and heads are not broadcast."""
-    shape, stride = t.shape, t.stride()
+    """Shape, token and head stride (0 where they are dense, or where there is one token or head) of a [tokens][heads][dims] tensor on
+    `device` whose dims are contiguous and whose tokens and heads are not broadcast."""
+    shape = t.shape
+    if len(shape) == 3 and t.is_contiguous() and (device < 0 or t.get_device() == device):
+        return shape, 0, 0
+    stride = t.stride()
     if len(shape) != 3 or (stride[2] != 1 and shape[2] > 1 and 0 not in shape):
         _need(False, f"{what} must be [tokens][heads][dims] with contiguous dims")
     ts, hs = (stride[0] if shape[0] > 1 else 0), (stride[1] if shape[1] > 1 else 0)
@@ -430,38 +434,38 @@ class KvPool:
         shape, ts, hs = _block(t, self._device, what)
         if shape != (rows, heads, self.head_dim):
             _need(False, f"{what} is {tuple(shape)}, the items want {(rows, heads, self.head_dim)}")
-        if heads > 1 and rows > 0 and hs != self.head_dim:
+        if heads > 1 and rows > 0 and hs not in (0, self.head_dim):
             _need(False, f"{what}: a token's heads must be contiguous")
         return ts
 
     @staticmethod
-    def _items(items) -> tuple[np.ndarray, int, int, int]:
-        """The items as an array, its address, their number, their tokens."""
+    def _items(items) -> tuple[bytes, int, int]:
+        """The items as the library takes them, their number, their tokens."""
         a = items
-        if not (type(a) is np.ndarray and a.dtype == np.uint32 and a.flags.c_contiguous):
+        if not (type(a) is np.ndarray and a.dtype == np.uint32):
             a = np.ascontiguousarray(items, np.uint32)
         if a.ndim != 2 or a.shape[1] != 4:
             _need(a.size == 0, "items are rows of (sequence, first_pos, pos, ntok)")
             a = a.reshape(0, 4)
         n = len(a)
         rows = sum(a[:, 3].tolist()) if n <= 64 else int(a[:, 3].sum(dtype=np.int64))
-        return a, a.__array_interface__["data"][0], n, rows
+        return a.tobytes(), n, rows  # (a copy in rows' order, sooner made than an array's address is asked for)
 
     def write(self, layer: int, items, k: torch.Tensor, v: torch.Tensor, rope: Rope | None = None) -> None:
         """New rows of the items' sequences in one layer; k, v f32 or f16 [tokens of all items][kv_heads][head_dim]. rope rotates k at
         the rows' positions."""
-        a, at, n, rows = self._items(items)
+        a, n, rows = self._items(items)
         if k.dtype is not v.dtype:
             _need(False, "k and v must have one type")
         r = _lib.PoolRows(k.data_ptr(), v.data_ptr(), _fmt_of(k), self._rows(k, self.kv_heads, rows, "k"), self._rows(v, self.kv_heads, rows, "v"),
                           rope._h if rope is not None else None)
-        check(self._write(self._h, layer, at, n, C.byref(r)))
+        check(self._write(self._h, layer, a, n, C.byref(r)))
 
     def attn(self, layer: int, items, q: torch.Tensor, out: torch.Tensor, window: int = 0, sinks: torch.Tensor | None = None,
              scale: float = 0.0) -> None:
         """Attention of the items' tokens over their sequences; q, out in the pool's type, [tokens of all items][q_heads][head_dim].
         scale 0 = 1 / sqrt(head_dim); sinks f32 [q_heads]."""
-        a, at, n, rows = self._items(items)
+        a, n, rows = self._items(items)
         if q.dtype is not self._dtype or out.dtype is not self._dtype:
             _need(False, f"q and out must be {self._dtype}")
         if not 0 <= window < 2**32:
@@ -471,7 +475,7 @@ class KvPool:
             _need(sinks.get_device() == self._device, "sinks must be where the pool is")
         r = _lib.PoolAttn(q.data_ptr(), out.data_ptr(), self._rows(q, self.q_heads, rows, "q"), self._rows(out, self.q_heads, rows, "out"), scale,
                           window, sinks.data_ptr() if sinks is not None else None)
-        check(self._attn(self._h, layer, at, n, C.byref(r)))
+        check(self._attn(self._h, layer, a, n, C.byref(r)))
 
     def close(self) -> None:
         if self._h:
