@@ -69,8 +69,9 @@ struct PaShared {
     uint32_t tmem_base;
     volatile uint32_t abort;
     volatile uint32_t keep; // 1 + the tile whose products are added to O although it is its segment's first
-    uint32_t bad[2][4];     // [tile parity]: keys of the tile whose V row is not finite and that not every token sees
+    uint32_t bad[3][4];     // [tile's S buffer]: keys of the tile whose V row is not finite and that not every token sees
 };
+static_assert(sizeof(PaShared) <= 64, "OFF_MISC");
 
 struct PaArgs {
     const __half *q;
@@ -162,7 +163,7 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         mbar_init(bar_q_full, 8);
         sh->abort = 0;
         sh->keep = 0;
-        for (int i = 0; i < 8; i++) sh->bad[i >> 2][i & 3] = 0;
+        for (int i = 0; i < 12; i++) sh->bad[i >> 2][i & 3] = 0;
         fence_barrier_init();
         fence_proxy_async();
     }
@@ -432,7 +433,7 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                         const uint32_t i = idx / (DIM / 8u), r = i < p0 - z0 ? z0 + i : i - (p0 - z0) + p1;
                         const uint4 v = *v_chunk(r, idx % (DIM / 8u));
                         if (half2_not_finite(v.x) || half2_not_finite(v.y) || half2_not_finite(v.z) || half2_not_finite(v.w)) {
-                            atomicOr(&sh->bad[t & 1u][r >> 5], 1u << (r & 31u));
+                            atomicOr(&sh->bad[buf.s][r >> 5], 1u << (r & 31u));
                             found = true;
                         }
                     }
@@ -440,7 +441,7 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                         bad_any = named_bar_or(5, 256, found);
                         for (uint32_t idx = st; bad_any && idx < PA_KEYS * (DIM / 8u); idx += 256u) {
                             const uint32_t r = idx / (DIM / 8u);
-                            if (sh->bad[t & 1u][r >> 5] >> (r & 31u) & 1u) *v_chunk(r, idx % (DIM / 8u)) = make_uint4(0u, 0u, 0u, 0u);
+                            if (sh->bad[buf.s][r >> 5] >> (r & 31u) & 1u) *v_chunk(r, idx % (DIM / 8u)) = make_uint4(0u, 0u, 0u, 0u);
                         }
                     }
                     fence_proxy_async();
@@ -516,7 +517,7 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                             // rows of V that are not finite, zero in shared memory: w v for the tokens that see them
                             for (uint32_t r = 0; bad_any && r < PA_KEYS; r++) {
                                 const uint32_t key = key0 + r;
-                                if (!(sh->bad[t & 1u][r >> 5] >> (r & 31u) & 1u) || !real || key < klo || key >= vis) continue;
+                                if (!(sh->bad[buf.s][r >> 5] >> (r & 31u) & 1u) || !real || key < klo || key >= vis) continue;
                                 const size_t page = g.pages[sq.table + (key >> g.page_shift)], off = key & ((1u << g.page_shift) - 1u);
                                 const __half *v = reinterpret_cast<const __half *>(g.vpages + ((page << g.page_shift) + off) * g.row_bytes) + (size_t)sg.kvh * DIM + c0;
                                 const __half *k = reinterpret_cast<const __half *>(g.kpages + ((page << g.page_shift) + off) * g.row_bytes) + (size_t)sg.kvh * DIM;
@@ -533,7 +534,8 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 }
                 if (bad_any) {
                     named_bar_sync(5, 256);
-                    if (st < 4u) sh->bad[t & 1u][st] = 0u; // (used again two tiles on, behind this tile's p_full)
+                    // Noted again NBUF tiles on: those scores are behind this tile's product, which is behind the p_full of the warp that clears.
+                    if (st < 4u) sh->bad[buf.s][st] = 0u;
                     if (t == t0 && st == 0u) sh->keep = t + 1u; // what was put into O stays
                 }
                 owed = bar_p_full + 8u * buf.s;

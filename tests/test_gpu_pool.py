@@ -722,3 +722,30 @@ def test_magnitudes_that_jump(ctx, fmt, heads, front, news):
     same = (got == want) | (got.isnan() & ~want.isfinite())
     assert (((got.double() - want).abs() <= attn_bound(fmt, want, mag, qk, top)) | same).all()
     pool.close()
+
+
+@pytest.mark.parametrize("heads", [(6, 2, 64), (12, 4, 128), (6, 2, 256)])
+def test_values_that_are_not_finite_on_both_sides_of_a_whole_tile(ctx, heads):
+    """An item of three tiles of 128 keys: a window's lower edge, a tile that every token sees, the diagonal, with a V row that is not finite in
+    both partly seen tiles. What the first one noted must not meet what the third one notes; many items at one time, several calls."""
+    pos, ntok, window = 128 * 3 + 40, 42, 250        # keys 175 .. 465 in tiles 1, 2, 3; all tokens see 216 .. 424
+    low, high = 178, 444                             # seen by tokens 0 .. 3, and by 20 ..
+    n = 150
+    pool, ids, g = scattered(ctx, F16, [pos + ntok] * n, 32, 7, heads=heads, spare=0)
+    q = randn(g, n * ntok, heads[0], heads[2], dtype=torch.float16)
+    items = [(i, 0, pos, ntok) for i in ids]
+    k, v = pool.buffer_tensors(0)
+    at = torch.from_numpy(np.array([pool.pages(i)[[low // 32, high // 32]] for i in ids], np.int64)).cuda()
+    v[at[:, 0], low % 32], v[at[:, 1], high % 32] = 0.5, 0.5
+    want, mag, qk, top = attn64(pool, items, q, window=window)
+    bound = attn_bound(F16, want, mag, qk, top)
+    v[at[:, 0], low % 32, :, 3], v[at[:, 1], high % 32, :, 5] = math.nan, math.inf
+    bad = torch.zeros(n, ntok, heads[0], heads[2], device="cuda", dtype=torch.bool)
+    bad[:, :4, :, 3] = True
+    bad[:, 20:, :, 5] = True
+    bad = bad.view_as(q)
+    for _ in range(5):
+        got = run_attn(pool, items, q, window=window)
+        assert torch.equal(~torch.isfinite(got), bad)
+        assert ((got.double() - want).abs() <= bound)[~bad].all()
+    pool.close()
