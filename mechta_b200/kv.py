@@ -457,6 +457,8 @@ class KvPool:
         a, n, rows = self._items(items)
         if k.dtype is not v.dtype:
             _need(False, "k and v must have one type")
+        if rope is not None and not rope._h:
+            _need(False, "rope is closed")  # (a null handle would mean: k is rotated already)
         r = _lib.PoolRows(k.data_ptr(), v.data_ptr(), _fmt_of(k), self._rows(k, self.kv_heads, rows, "k"), self._rows(v, self.kv_heads, rows, "v"),
                           rope._h if rope is not None else None)
         check(self._write(self._h, layer, a, n, C.byref(r)))

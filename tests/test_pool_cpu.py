@@ -323,3 +323,14 @@ def test_blocks_that_overlap():
     assert attn(flat[:4], flat[4:]) == _lib.ERR_UNSUPPORTED and attn(flat[:4], flat[1:5]) == _lib.ERR_INVALID
     with pytest.raises(_lib.MkvError):
         p.fork(a, n=2**31 - 1)
+
+
+def test_a_closed_rope_is_not_taken_for_rotated_rows():
+    p = pool()
+    a = p.create()
+    rope, k = kv.Rope(None, 64), torch.zeros(4, 2, 256)
+    assert status(p.write, 0, [(a, 0, 0, 4)], k, k, rope) == _lib.ERR_UNSUPPORTED  # nothing wrong but the missing device
+    rope.close()
+    assert status(p.write, 0, [(a, 0, 0, 4)], k, k, rope) == _lib.ERR_INVALID
+    assert status(rope.freqs) == _lib.ERR_INVALID
+    p.close()
