@@ -359,6 +359,7 @@ class KvPool:
         self.q_heads, self.kv_heads, self.head_dim, self.max_seqs = q_heads, kv_heads, head_dim, max_seqs
         for v in (n_pages, page_tokens, max_seqs, max_tokens):
             _need(0 <= v < 2**32, f"{v} is no size")
+        _need(ctx is None or ctx._h, "the context is closed")  # (a null handle would make a pool of the bookkeeping alone)
         d = _lib.PoolDesc(int(fmt), n_layers, n_pages, page_tokens, max_seqs, max_tokens, q_heads, kv_heads, head_dim)
         L = _lib.lib()
         check(L.mkv_pool_create(ctx._h if ctx is not None else None, C.byref(d), C.byref(self._h)))

@@ -1,5 +1,6 @@
 """The pool's bookkeeping and the argument checks of the paged operators, without a device: pages, forks, copy on write, compaction
 against a plain model; every refusal leaves the books as they were."""
+import ctypes as C
 import math
 import random
 
@@ -334,3 +335,9 @@ def test_a_closed_rope_is_not_taken_for_rotated_rows():
     assert status(p.write, 0, [(a, 0, 0, 4)], k, k, rope) == _lib.ERR_INVALID
     assert status(rope.freqs) == _lib.ERR_INVALID
     p.close()
+
+
+def test_a_closed_context_makes_no_pool():
+    ctx = kv.KvContext.__new__(kv.KvContext)  # as close() leaves it
+    ctx._h, ctx.device, ctx.stream = C.c_void_p(), 0, None
+    assert status(kv.KvPool, ctx, kv.KvFormat.F16, 1, 4, 16, 2, 64) == _lib.ERR_INVALID
