@@ -273,6 +273,24 @@ def _need(ok, text: str) -> None:
         raise MkvError(_lib.ERR_INVALID, text)
 
 
+def _u32(*numbers: int) -> None:
+    """Refuses what ctypes would cut to 32 bits."""
+    for v in numbers:
+        if not 0 <= v < 2**32:
+            _need(False, f"{v}: must lie between 0 and 2^32 - 1")
+
+
+def _u32_array(numbers) -> np.ndarray:
+    """Whole numbers as uint32; refuses those that a cast would cut or round."""
+    a = np.asarray(numbers)
+    if a.dtype.kind not in "iu" and a.size:
+        _need(False, f"{a.dtype}: must be whole numbers from 0 to 2^32 - 1")
+    wide = a.astype(np.uint64)  # (a negative one is above 2^63)
+    if (wide >> np.uint64(32)).any():
+        _need(False, "numbers must lie between 0 and 2^32 - 1")
+    return wide.astype(np.uint32)
+
+
 def _fmt_of(t: torch.Tensor) -> int:
     if t.dtype is torch.float32:
         return _lib.F32
@@ -311,6 +329,7 @@ class Rope:
         _need(layout in self.LAYOUTS, f"layout {layout!r}: one of {sorted(self.LAYOUTS)}")
         _need(scaling in self.SCALINGS, f"scaling {scaling!r}: one of {sorted(self.SCALINGS)}")
         self.ctx, self.dims = ctx, int(dims)
+        _need(0 <= self.dims < 2**31, f"{dims} rotated dims")
         d = _lib.RopeDesc(self.dims, self.LAYOUTS[layout], self.SCALINGS[scaling], base, factor, original, slow, fast)
         check(_lib.lib().mkv_rope_create(C.byref(d), C.byref(self._h)))
         self._apply = _lib.lib().mkv_rope_apply
@@ -331,6 +350,8 @@ class Rope:
         if shape != out_shape:
             _need(False, f"x is {tuple(shape)}, out {tuple(out_shape)}")
         n, heads, dim = shape
+        if max(shape) >= 2**31:
+            _need(False, f"x is {tuple(shape)}: at most 2^31 - 1 of each")
         if positions.dtype is not torch.int32 or positions.shape != (n,) or not positions.is_contiguous() or positions.get_device() != ctx.device:
             _need(False, f"positions must be contiguous int32 [tokens] on cuda:{ctx.device}")
         r = _lib.RopeRows(x.data_ptr(), out.data_ptr(), _fmt_of(x), _fmt_of(out), n, heads, dim, xt, xh, yt, yh, positions.data_ptr(), backward)
@@ -357,8 +378,9 @@ class KvPool:
         self._h = C.c_void_p()
         self.ctx, self.fmt, self.n_layers, self.n_pages, self.page_tokens = ctx, KvFormat(fmt), n_layers, n_pages, page_tokens
         self.q_heads, self.kv_heads, self.head_dim, self.max_seqs = q_heads, kv_heads, head_dim, max_seqs
-        for v in (n_pages, page_tokens, max_seqs, max_tokens):
-            _need(0 <= v < 2**32, f"{v} is no size")
+        _u32(n_pages, page_tokens, max_seqs, max_tokens)
+        for v in (n_layers, q_heads, kv_heads, head_dim):
+            _need(0 <= v < 2**31, f"{v} is no size")
         _need(ctx is None or ctx._h, "the context is closed")  # (a null handle would make a pool of the bookkeeping alone)
         d = _lib.PoolDesc(int(fmt), n_layers, n_pages, page_tokens, max_seqs, max_tokens, q_heads, kv_heads, head_dim)
         L = _lib.lib()
@@ -381,32 +403,40 @@ class KvPool:
     def fork(self, seq: int, length: int | None = None, n: int = 1, copy: bool = False) -> list[int]:
         """n sequences that begin with the first `length` rows of `seq` (all of them by default), on the same pages or on copies."""
         _need(0 < n <= self.max_seqs, f"fork of {n} sequences: 1 to {self.max_seqs}")
+        if length is None:
+            length = self.length(seq)
+        _u32(seq, length)
         if n == 1:
-            check(self._lib.mkv_seq_fork(self._h, seq, self.length(seq) if length is None else length, copy, 1, self._out_ref))
+            check(self._lib.mkv_seq_fork(self._h, seq, length, copy, 1, self._out_ref))
             return [self._out.value]
         kids = (C.c_uint32 * n)()
-        check(self._lib.mkv_seq_fork(self._h, seq, self.length(seq) if length is None else length, copy, n, kids))
+        check(self._lib.mkv_seq_fork(self._h, seq, length, copy, n, kids))
         return kids[:]
 
     def free(self, seqs) -> None:
         if type(seqs) is list and {*map(type, seqs)} <= {int}:
+            _u32(*seqs)
             a, n = (C.c_uint32 * len(seqs))(*seqs), len(seqs)
         else:
-            held = np.ascontiguousarray(seqs, np.uint32).reshape(-1)
+            held = _u32_array(seqs).reshape(-1)
             a, n = held.ctypes.data, held.size
         check(self._lib.mkv_seq_free(self._h, a, n))
 
     def truncate(self, seq: int, length: int) -> None:
+        _u32(seq, length)
         check(self._lib.mkv_seq_truncate(self._h, seq, length))
 
     def set_len(self, seq: int, length: int) -> None:
         """Declares rows valid that the host fills itself (buffer_tensors), in all layers."""
+        _u32(seq, length)
         check(self._lib.mkv_seq_set_len(self._h, seq, length))
 
     def length(self, seq: int) -> int:
+        _u32(seq)
         return self._lib.mkv_seq_len(self._h, seq)
 
     def pages(self, seq: int) -> np.ndarray:
+        _u32(seq)
         n = C.c_uint32()
         check(_lib.lib().mkv_seq_pages(self._h, seq, None, 0, C.byref(n)))
         a = np.empty(n.value, np.uint32)
@@ -419,7 +449,12 @@ class KvPool:
         return self._out.value
 
     # -- rows
+    def _layer(self, layer: int) -> None:
+        if not 0 <= layer < self.n_layers:
+            _need(False, f"layer {layer} outside [0, {self.n_layers})")
+
     def buffers(self, layer: int) -> tuple[int, int]:
+        self._layer(layer)
         k, v = C.c_void_p(), C.c_void_p()
         check(_lib.lib().mkv_pool_buffers(self._h, layer, C.byref(k), C.byref(v)))
         return k.value, v.value
@@ -444,7 +479,7 @@ class KvPool:
         """The items as the library takes them, their number, their tokens."""
         a = items
         if not (type(a) is np.ndarray and a.dtype == np.uint32):
-            a = np.ascontiguousarray(items, np.uint32)
+            a = _u32_array(items)
         if a.ndim != 2 or a.shape[1] != 4:
             _need(a.size == 0, "items are rows of (sequence, first_pos, pos, ntok)")
             a = a.reshape(0, 4)
@@ -455,6 +490,7 @@ class KvPool:
     def write(self, layer: int, items, k: torch.Tensor, v: torch.Tensor, rope: Rope | None = None) -> None:
         """New rows of the items' sequences in one layer; k, v f32 or f16 [tokens of all items][kv_heads][head_dim]. rope rotates k at
         the rows' positions."""
+        self._layer(layer)
         a, n, rows = self._items(items)
         if k.dtype is not v.dtype:
             _need(False, "k and v must have one type")
@@ -468,6 +504,7 @@ class KvPool:
              scale: float = 0.0) -> None:
         """Attention of the items' tokens over their sequences; q, out in the pool's type, [tokens of all items][q_heads][head_dim].
         scale 0 = 1 / sqrt(head_dim); sinks f32 [q_heads]."""
+        self._layer(layer)
         a, n, rows = self._items(items)
         if q.dtype is not self._dtype or out.dtype is not self._dtype:
             _need(False, f"q and out must be {self._dtype}")

@@ -341,3 +341,41 @@ def test_a_closed_context_makes_no_pool():
     ctx = kv.KvContext.__new__(kv.KvContext)  # as close() leaves it
     ctx._h, ctx.device, ctx.stream = C.c_void_p(), 0, None
     assert status(kv.KvPool, ctx, kv.KvFormat.F16, 1, 4, 16, 2, 64) == _lib.ERR_INVALID
+
+
+def test_numbers_beyond_32_bits_are_refused():
+    """Sequences, lengths, layers, sizes and items, as Python numbers and as arrays of other types: none is cut to 32 bits or to a whole number."""
+    p, I = pool(), _lib.ERR_INVALID
+    a = p.create()
+    p.set_len(a, 30)
+    far = 2**32
+    for seqs in ([far + a], [-1], (far + a,), np.array([far + a]), np.array([-far + a]), np.array([a + 0.0]), [a, far], [a + 0.5], [2**64 + a]):
+        assert status(p.free, seqs) == I, seqs
+    assert status(p.truncate, a, far) == I and status(p.truncate, far + a, 0) == I and status(p.truncate, a, -far) == I
+    assert status(p.set_len, a, far + 40) == I and status(p.set_len, far + a, 40) == I
+    assert status(p.fork, a, far + 7) == I and status(p.fork, far + a, 7) == I and status(p.fork, far + a) == I and status(p.fork, a, far + 7, 3) == I
+    assert status(p.length, far + a) == I and status(p.pages, far + a) == I and status(p.buffers, far) == I
+    k, q = torch.zeros(4, 2, 256), torch.zeros(4, 16, 256, dtype=torch.float16)
+    good = [a, 0, 26, 4]
+    for at in range(4):
+        for off in (far, -far, 0.5, 2**64):
+            row = list(good)
+            row[at] += off
+            for items in ([tuple(row)], np.array([row])):
+                assert status(p.write, 0, items, k, k) == I, items
+                assert status(p.attn, 0, items, q, q.clone()) == I, items
+    for items in ([tuple(good)], np.array([good]), np.array([good], np.int32), np.array([good], np.uint32), np.array([good], np.uint64)):
+        assert status(p.write, 0, items, k, k) == status(p.attn, 0, items, q, q.clone()) == _lib.ERR_UNSUPPORTED  # nothing wrong but the missing device
+    assert status(p.write, far, [good], k, k) == I and status(p.attn, far, [good], q, q.clone()) == I
+    for kw in (dict(layers=far + 2), dict(n_pages=far + 40), dict(kv_heads=far + 2), dict(q_heads=far + 16), dict(head_dim=far + 64), dict(longest=far + 400)):
+        assert status(pool, **kw) == I, kw
+    assert status(kv.Rope, None, far + 64) == I
+    ctx = kv.KvContext.__new__(kv.KvContext)
+    ctx._h, ctx.device, ctx.stream = C.c_void_p(), -1, None
+    x = torch.empty(far + 5, 1, 64, device="meta")
+    with pytest.raises(_lib.MkvError, match="at most 2"):
+        kv.Rope(ctx, 64).apply(x, torch.empty(far + 5, dtype=torch.int32, device="meta"), x)
+    assert p.length(a) == 30 and p.free_pages == 38
+    p.free(np.array([a]))
+    assert p.free_pages == 40
+    p.close()
