@@ -135,7 +135,8 @@ __global__ void __launch_bounds__(1024) pool_merge_kernel(const __grid_constant_
     const float sink = g.sinks ? g.sinks[head] * 1.4426950408889634f : NEG_BIG;
     float Mr = sink;
     for (uint32_t k = 0; k < g.groups; k++) Mr = fmaxf(Mr, ml_s[slot + k].x);
-    float den = sink > NEG_TEST ? exp2f(sink - Mr) : 0.0f;
+    // (the difference of two infinities is no number: a sink of infinity takes everything; one of NaN makes the row NaN)
+    float den = sink <= NEG_TEST ? 0.0f : sink == Mr ? 1.0f : exp2f(sink - Mr);
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
     seen = true;
     for (uint32_t k = 0; k < g.groups; k++) {

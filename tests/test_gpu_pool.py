@@ -749,3 +749,22 @@ def test_values_that_are_not_finite_on_both_sides_of_a_whole_tile(ctx, heads):
         assert torch.equal(~torch.isfinite(got), bad)
         assert ((got.double() - want).abs() <= bound)[~bad].all()
     pool.close()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("length", [30, 5000])
+def test_sinks_that_are_not_finite(ctx, fmt, length):
+    """In an item that is whole and in one that is split: a sink of infinity (and one that is infinite in base-2 exponents) leaves nothing of the
+    keys, one of NaN makes its head's rows NaN, those of minus infinity and of the lowest value are none."""
+    pool, ids, g = scattered(ctx, fmt, [length], 64, 13)
+    q = randn(g, 1, 16, 256, dtype=pool.fmt.torch_dtype)
+    items = [(ids[0], 0, length - 1, 1)]
+    sinks = torch.zeros(16, device="cuda")
+    sinks[:5] = torch.tensor([math.inf, 3e38, math.nan, -math.inf, torch.finfo(torch.float32).min])
+    got = run_attn(pool, items, q, sinks=sinks)
+    assert (got[:, :2] == 0).all() and got[:, 2].isnan().all()
+    plain = sinks.clone()
+    plain[:3], plain[3:5] = 0.0, -1e4  # (as good as none, and finite in the formula)
+    want, mag, qk, top = attn64(pool, items, q, sinks=plain)
+    assert ((got.double() - want).abs() <= attn_bound(fmt, want, mag, qk, top))[:, 3:].all()
+    pool.close()
