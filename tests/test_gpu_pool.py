@@ -768,3 +768,24 @@ def test_sinks_that_are_not_finite(ctx, fmt, length):
     want, mag, qk, top = attn64(pool, items, q, sinks=plain)
     assert ((got.double() - want).abs() <= attn_bound(fmt, want, mag, qk, top))[:, 3:].all()
     pool.close()
+
+
+@pytest.mark.parametrize("heads,n,times", [((8, 1, 64), 65536, 1), ((16, 2, 256), 65536, 1), ((8, 1, 64), 16384, 200), ((16, 2, 256), 16384, 100)])
+@pytest.mark.parametrize("below", [12.0, 17.4, 19.0])
+def test_a_key_above_a_long_flat_tail(ctx, heads, n, times, below):
+    """One key, and all others `below` nats under it with values of one sign: what the tail adds up to comes out, in split and in whole items. Its
+    weights are all rounded alike: by 2^-11 of themselves, or half a step of what f16 holds below 2^-14, 2^-25, of weights that are at least 2^7 times those
+    against the row's largest; the output by 2^-11 once more."""
+    pool, ids, g = scattered(ctx, F16, [n], 64, 3, heads=heads)
+    k, v = pool.buffer_tensors(0)
+    pages = torch.from_numpy(pool.pages(ids[0]).astype(np.int64)).cuda()
+    k[pages], v[pages] = 0.0, 1.0
+    k[pages[0], 0], v[pages[0], 0] = below / heads[2], 0.0
+    q = torch.ones(1, heads[0], heads[2], device="cuda", dtype=torch.float16)
+    items = [(ids[0], 0, n - 1, 1)] * times
+    got = run_attn(pool, items, q.expand(len(items), -1, -1).contiguous(), scale=1.0)
+    want, mag, qk, top = attn64(pool, items[:1], q, scale=1.0)
+    off = (got.double() - want).abs()
+    bound = want * (2.0**-10 + 2 * qk * 2.0**-20 + 2.0**-18) + n * 2.0**-32 + 2.0**-25
+    assert (off <= bound).all(), f"{float(got.min())} to {float(got.max())} for {float(want.min())}"
+    pool.close()
