@@ -361,7 +361,7 @@ mkv_status mkv_pool_write(mkv_pool *p, int layer, const mkv_seq_rows *items, int
  * q, out: the pool's type, [tokens of all items, in their order][q_heads][head_dim], token strides in elements (0 = dense; multiples of
  * 16 bytes), 16-byte aligned, not overlapping. scale 0 = 1 / sqrt(head_dim). sinks_dev: [q_heads] logits that join the softmax's maximum and sum and
  * never the output, or NULL. f16 pools: weights are rounded to f16 for the tensor cores (by 2^-11 of themselves, or by 2^-32 of the row's
- * largest where that is more), everything else is summed in f32; f32 pools: f32-grade throughout (values are taken as two f16 parts, 22 bits; one below 2^-33 of the largest value of its
+ * largest where that is more; the softmax's sum is that of the rounded ones), everything else is summed in f32; f32 pools: f32-grade throughout (values are taken as two f16 parts, 22 bits; one below 2^-33 of the largest value of its
  * 64 rows, or of its query, counts as nothing). */
 typedef struct {
     const void *q_dev;

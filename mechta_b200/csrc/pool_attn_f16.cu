@@ -7,7 +7,9 @@
 //   P = 2^(S - reference) as f16, back into the columns of S (base-2 exponents throughout)
 //   O += P V    A = P (tensor memory), B = the V tile as TMA left it (N-major)
 // One pass: the reference of a row lies PA_BIAS2 = 7 below its maximum at the time, and moves only when a tile exceeds that maximum by more
-// than PA_LAZY2 = 8 (then O is rescaled); sums are kept in f32. Weights stay below 2^15 (f16 ends at 65,504) and are rounded by 2^-11 of
+// than PA_LAZY2 = 8 (then O is rescaled); sums are kept in f32, those of the weights over what f16 has of them, so that an output is a true mean of
+// the values: the weights are cut to 11 bits in front of both (one operation each, 62.3 us where the case below takes 61.4 with sums of other
+// weights; taken back from f16 they cost 64.5). Weights stay below 2^15 (f16 ends at 65,504) and are rounded by 2^-11 of
 // themselves down to 2^-21 of the row's largest, by 2^-32 of that below (with the reference at the maximum itself it was 2^-25, and 65,536 keys at
 // 2^-25 of one, 0.2% of the sum, were lost). 8 is as seldom exceeded as more would be (ragged blocks under a window with 6, 8, 10 and 11.5: 63.8, 61.4,
 // 61.3 and 61.0 us); scores of N(0, 1) grow by about 4 behind their first tile.
@@ -77,6 +79,10 @@ struct PaShared {
     uint32_t bad[3][4];     // [tile's S buffer]: keys of the tile whose V row is not finite and that not every token sees
 };
 static_assert(sizeof(PaShared) <= 64, "OFF_MISC");
+
+// The 11 bits of a weight that f16 has. Of a weight times 1 + 2^-11, that is the weight to within 2^-11 of itself.
+__device__ __forceinline__ float pa_cut(float w) { return __uint_as_float(__float_as_uint(w) & 0xffffe000u); }
+constexpr float PA_HALF2 = 7.04269e-4f; // log2(1 + 2^-11): m_ref is so much smaller than what weights and their sums stand for
 
 struct PaArgs {
     const __half *q;
@@ -472,7 +478,7 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
 #pragma unroll
                         for (int c = 0; c < 32; c += 2) mt[(c >> 1) & 3] = max3(mt[(c >> 1) & 3], __uint_as_float(sr[h][c]), __uint_as_float(sr[h][c + 1]));
                     float mx = max3(fmaxf(mt[0], mt[1]), mt[2], mt[3]);
-                    mx = mx > NEG_TEST ? mx * g.scale2 - PA_BIAS2 : NEG_BIG; // the reference that this half row's tile asks for
+                    mx = mx > NEG_TEST ? mx * g.scale2 - (PA_BIAS2 + PA_HALF2) : NEG_BIG; // the reference that this half row's tile asks for
                     // It moves for the first tile with a key and when the tile exceeds it by more than PA_LAZY2. The two warps that share these 32
                     // rows vote; only then they exchange maxima.
                     float cf = 1.0f;
@@ -496,8 +502,8 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                         for (int c = 0; c < 32; c += 2) {
                             float x0, x1;
                             unpack2(fma2(pack2(__uint_as_float(sr[h][c]), __uint_as_float(sr[h][c + 1])), c2, m2), x0, x1);
-                            x0 = ex2(x0);
-                            x1 = ex2(x1);
+                            x0 = pa_cut(ex2(x0));
+                            x1 = pa_cut(ex2(x1));
                             sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], pack2(x0, x1));
                             const __half2 hp = __floats2half2_rn(x0, x1);
                             ph[c >> 1] = *reinterpret_cast<const uint32_t *>(&hp);
@@ -529,7 +535,7 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                                 const __half *q = g.q + (int64_t)(sq.row + it.tok0 + tok) * g.q_stride + (size_t)(sg.kvh * group + head) * DIM;
                                 float s = 0.0f;
                                 for (int d = 0; d < DIM; d++) s = fmaf(__half2float(q[d]), __half2float(k[d]), s);
-                                const float w = exp2f(fmaf(s, g.scale2, neg_m));
+                                const float w = pa_cut(exp2f(fmaf(s, g.scale2, neg_m)));
 #pragma unroll
                                 for (int c = 0; c < 32; c++) orow[c] = __float_as_uint(fmaf(w, __half2float(v[c]), __uint_as_float(orow[c])));
                             }
@@ -573,7 +579,7 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 if (sg.whole) {
                     // out[token][head][:] = O / (l + sink)
                     float den = l_all;
-                    if (g.sinks && real) den += exp2f(g.sinks[sg.kvh * group + head] * PA_LOG2E - (m_ref > NEG_TEST ? m_ref : 0.0f));
+                    if (g.sinks && real) den += exp2f(g.sinks[sg.kvh * group + head] * PA_LOG2E - (m_ref > NEG_TEST ? m_ref + PA_HALF2 : 0.0f));
                     const float inv = 1.0f / den;
                     __half *dst[4];
 #pragma unroll
@@ -600,7 +606,7 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 } else {
                     // a part: maximum, sum and O as they are, for the merge
                     float *ps = g.scratch + part_slot(blockIdx.x, sg.part) * part_floats(DIM);
-                    if (half == 0u && real) *reinterpret_cast<float2 *>(ps + 128u * DIM + 2u * row) = make_float2(m_ref, seen ? l_all : -1.0f);
+                    if (half == 0u && real) *reinterpret_cast<float2 *>(ps + 128u * DIM + 2u * row) = make_float2(m_ref > NEG_TEST ? m_ref + PA_HALF2 : NEG_BIG, seen ? l_all : -1.0f);
                     // The exchange pays where many rows are stored (six blocks of up to 109 tokens of six heads: the call takes 14.1 us, without it
                     // 17.3); one token's rows are few lines either way, and sooner stored as they are (12.1 us, with it 13.2).
                     const bool many = rows > 32u;

@@ -789,3 +789,20 @@ def test_a_key_above_a_long_flat_tail(ctx, heads, n, times, below):
     bound = want * (2.0**-10 + 2 * qk * 2.0**-20 + 2.0**-18) + n * 2.0**-32 + 2.0**-25
     assert (off <= bound).all(), f"{float(got.min())} to {float(got.max())} for {float(want.min())}"
     pool.close()
+
+
+@pytest.mark.parametrize("heads", [(16, 2, 256), (12, 4, 128), (8, 1, 64)])
+@pytest.mark.parametrize("value", [1.0, -0.0078125])
+def test_equal_values_come_out_as_they_are(ctx, heads, value):
+    """A mean of equal values is that value whatever the weights: the sums run over the weights as the products take them. (Both are f32 sums of
+    the same f16 numbers, off by 2^-15 at most here, and the nearest other output is 2^-11 away.) Few keys, many, split rows, windows."""
+    n = 3001
+    pool, ids, g = scattered(ctx, F16, [n, 700], 64, 4, heads=heads)
+    pool.buffer_tensors(0)[1].fill_(value)
+    q = randn(g, 102, heads[0], heads[2], dtype=torch.float16)
+    for scale in (0.3, 0.06, 1.0):
+        for first, window in ((0, 0), (n - 100, 0), (n - 3, 0), (0, 130), (0, 3)):
+            got = run_attn(pool, [(ids[0], first, n - 2, 2), (ids[1], max(first - n + 700, 0), 600, 100)], q, scale=scale, window=window)
+            assert ((got == value) | ((got == 0).all(-1, keepdim=True))).all()
+            assert (got[1] == value).all() and (got[-1] == value).all()
+    pool.close()
