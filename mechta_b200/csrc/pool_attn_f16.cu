@@ -400,7 +400,8 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             const bool real = row < rows;
             const uint32_t vis = real ? sq.pos + it.tok0 + tok + 1u : 0u; // this row sees klo <= key < vis
             const uint32_t klo = real ? plan_lowest(sq, plan.window, it.tok0 + tok) : 0u;
-            float m_ref = NEG_BIG, l = 0.0f; // l: this thread's keys only
+            // Weights are 2^(s C - m_ref), m_ref = m_raw C - PA_BIAS2 - PA_HALF2 for the score m_raw of a key. l: this thread's keys only.
+            float m_raw = NEG_BIG, m_ref = 0.0f, l = 0.0f;
             const uint32_t end = t0 + (sg.b - sg.a);
             more = walk.next(nx);
             for (uint32_t t = t0; t < end; t++, buf.next()) {
@@ -478,21 +479,31 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
 #pragma unroll
                         for (int c = 0; c < 32; c += 2) mt[(c >> 1) & 3] = max3(mt[(c >> 1) & 3], __uint_as_float(sr[h][c]), __uint_as_float(sr[h][c + 1]));
                     float mx = max3(fmaxf(mt[0], mt[1]), mt[2], mt[3]);
-                    mx = mx > NEG_TEST ? mx * g.scale2 - (PA_BIAS2 + PA_HALF2) : NEG_BIG; // the reference that this half row's tile asks for
-                    // It moves for the first tile with a key and when the tile exceeds it by more than PA_LAZY2. The two warps that share these 32
-                    // rows vote; only then they exchange maxima.
+                    // The reference moves for the first tile with a key and when the tile exceeds it by more than PA_LAZY2. The two warps that share
+                    // these 32 rows vote; only then they exchange maxima.
                     float cf = 1.0f;
-                    if (pair_bar_or(bar_pair, mx > NEG_TEST && (m_ref < NEG_TEST || mx > m_ref + PA_LAZY2))) {
+                    auto moves = [&]() { return mx > NEG_TEST && (m_raw < NEG_TEST || (mx - m_raw) * g.scale2 > PA_LAZY2); };
+                    if (pair_bar_or(bar_pair, moves())) {
                         red[128u * half + row] = mx;
                         pair_bar_sync(bar_pair);
                         mx = fmaxf(mx, red[128u * (half ^ 1u) + row]);
-                        if (mx > NEG_TEST && (m_ref < NEG_TEST || mx > m_ref + PA_LAZY2)) {
-                            const float m_new = fmaxf(m_ref, mx);
-                            cf = m_ref > NEG_TEST ? exp2f(m_ref - m_new) : 1.0f;
-                            m_ref = m_new;
+                        if (moves()) {
+                            cf = m_raw > NEG_TEST ? exp2f((m_raw - mx) * g.scale2) : 1.0f;
+                            m_raw = mx;
+                            m_ref = mx * g.scale2 - (PA_BIAS2 + PA_HALF2);
                         }
                     }
-                    const float neg_m = m_ref > NEG_TEST ? -m_ref : 0.0f;
+                    float neg_m = -m_ref;
+                    // Half a step of m_ref is 2^-5 at 2^20, but with the scores of rows that are thousands long it would take weights out of f16's
+                    // range; there the difference of the scores comes first.
+                    const bool far = fabsf(m_ref) > 1048576.0f;
+                    if (far) {
+                        neg_m = PA_BIAS2 + PA_HALF2;
+#pragma unroll
+                        for (int h = 0; h < 2; h++)
+#pragma unroll
+                            for (int c = 0; c < 32; c++) sr[h][c] = __float_as_uint(__uint_as_float(sr[h][c]) - m_raw);
+                    }
                     const uint64_t c2 = pack2(g.scale2, g.scale2), m2 = pack2(neg_m, neg_m);
                     uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
@@ -535,7 +546,7 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                                 const __half *q = g.q + (int64_t)(sq.row + it.tok0 + tok) * g.q_stride + (size_t)(sg.kvh * group + head) * DIM;
                                 float s = 0.0f;
                                 for (int d = 0; d < DIM; d++) s = fmaf(__half2float(q[d]), __half2float(k[d]), s);
-                                const float w = pa_cut(exp2f(fmaf(s, g.scale2, neg_m)));
+                                const float w = pa_cut(exp2f(fmaf(far ? s - m_raw : s, g.scale2, neg_m)));
 #pragma unroll
                                 for (int c = 0; c < 32; c++) orow[c] = __float_as_uint(fmaf(w, __half2float(v[c]), __uint_as_float(orow[c])));
                             }
@@ -579,7 +590,7 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 if (sg.whole) {
                     // out[token][head][:] = O / (l + sink)
                     float den = l_all;
-                    if (g.sinks && real) den += exp2f(g.sinks[sg.kvh * group + head] * PA_LOG2E - (m_ref > NEG_TEST ? m_ref + PA_HALF2 : 0.0f));
+                    if (g.sinks && real) den += exp2f(g.sinks[sg.kvh * group + head] * PA_LOG2E - (m_ref + PA_HALF2));
                     const float inv = 1.0f / den;
                     __half *dst[4];
 #pragma unroll
@@ -606,7 +617,7 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 } else {
                     // a part: maximum, sum and O as they are, for the merge
                     float *ps = g.scratch + part_slot(blockIdx.x, sg.part) * part_floats(DIM);
-                    if (half == 0u && real) *reinterpret_cast<float2 *>(ps + 128u * DIM + 2u * row) = make_float2(m_ref > NEG_TEST ? m_ref + PA_HALF2 : NEG_BIG, seen ? l_all : -1.0f);
+                    if (half == 0u && real) *reinterpret_cast<float2 *>(ps + 128u * DIM + 2u * row) = make_float2(m_raw > NEG_TEST ? m_ref + PA_HALF2 : NEG_BIG, seen ? l_all : -1.0f);
                     // The exchange pays where many rows are stored (six blocks of up to 109 tokens of six heads: the call takes 14.1 us, without it
                     // 17.3); one token's rows are few lines either way, and sooner stored as they are (12.1 us, with it 13.2).
                     const bool many = rows > 32u;

@@ -806,3 +806,22 @@ def test_equal_values_come_out_as_they_are(ctx, heads, value):
             assert ((got == value) | ((got == 0).all(-1, keepdim=True))).all()
             assert (got[1] == value).all() and (got[-1] == value).all()
     pool.close()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("heads", [(16, 2, 256), (12, 4, 128), (4, 4, 64)])
+@pytest.mark.parametrize("size", [2.0**7, 2.0**13, 2.0**15])
+def test_scores_of_very_long_rows(ctx, fmt, heads, size):
+    """Queries and keys of +size and -size: products and sums are exact, different scores are at least 2^10 apart, so a row is the mean of the
+    values whose keys tie for its maximum (their weights are equal), rounded once, however large the scores are."""
+    lens, news = [5, 700, 9000], [5, 40, 2]
+    pool, ids, g = scattered(ctx, fmt, lens, 64, 17, heads=heads)
+    k = pool.buffer_tensors(0)[0]
+    k.copy_(k.sign() * size + (k == 0) * size)
+    q = ((randn(g, sum(news), heads[0], heads[2]) > 0).float() * 2 - 1).mul_(size).to(k.dtype)
+    items = [(i, 0, n - m, m) for i, n, m in zip(ids, lens, news)]
+    for window in (0, 300):
+        got = run_attn(pool, items, q, window=window)
+        want, mag, *_ = attn64(pool, items, q, window=window)
+        assert ((got.double() - want).abs() <= mag * 2.0**-18 + want.abs() * 2.0**-11 + 2.0**-25).all()
+    pool.close()
