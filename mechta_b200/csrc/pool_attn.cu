@@ -64,7 +64,7 @@ bool pool_plan(const Pool *p, const mkv_seq_rows *items, int n, int &i, uint32_t
         rows += s.ntok;
     }
     if (plan.nseq == 0u) return false;
-    const uint32_t sms = std::min<uint32_t>((uint32_t)p->ctx->sm_count, PLAN_CTAS);
+    const uint32_t sms = (uint32_t)pool_attn_ctas(p);
     // the least that could do, and a little more as often as it takes
     uint64_t budget = std::max<uint64_t>((total + count * cost.segment + sms - 1u) / sms, cost.segment + 1u);
     if (longest <= cost.whole) budget = std::max<uint64_t>(budget, cost.segment + longest); // nothing is split
@@ -190,7 +190,7 @@ mkv_status launch_pool_merge(Pool *p, const MergeList &list, const PoolAttn &a) 
 
 mkv_status pool_attn_setup(Pool *p) {
     const bool f16 = p->desc.fmt == MKV_F16;
-    const size_t bytes = 2u * (size_t)std::min<uint32_t>((uint32_t)p->ctx->sm_count, PLAN_CTAS) * part_floats((uint32_t)p->desc.head_dim) * sizeof(float);
+    const size_t bytes = pool_attn_ctas(p) * (2u * part_floats((uint32_t)p->desc.head_dim) + (f16 ? 128u * (size_t)p->desc.head_dim : 0u)) * sizeof(float);
     if (cudaMalloc(reinterpret_cast<void **>(&p->scratch), bytes) != cudaSuccess) {
         cudaGetLastError();
         set_error("out of device memory for %zu bytes of scratch", bytes);

@@ -13,6 +13,10 @@
 // themselves down to 2^-21 of the row's largest, by 2^-32 of that below (with the reference at the maximum itself it was 2^-25, and 65,536 keys at
 // 2^-25 of one, 0.2% of the sum, were lost). 8 is as seldom exceeded as more would be (ragged blocks under a window with 6, 8, 10 and 11.5: 63.8, 61.4,
 // 61.3 and 61.0 us); scores of N(0, 1) grow by about 4 behind their first tile.
+// The tensor core's f32 sums truncate, all in one direction: about 2^-23.3 of O for each 16 keys (values of one sign over 300,000 keys came out 1.0e-3
+// too small). So every 48 tiles (4.2e-5 by then, a sixth of an output's smallest half step) O is added, with rounding, to what its thread has of it
+// in global memory, and starts again; the segment's end adds the two. The long block below takes 1,239 us where it took 1,204 without, every 32
+// tiles 1,280, every 64 1,232: what it costs is the wait for the product in front.
 // TMEM: O = columns 0 .. DIM - 1, then two (DIM = 256) or three S buffers of 128 columns, so that the scores of the next tiles are there when
 // a tile's softmax begins.
 //
@@ -47,6 +51,7 @@ constexpr uint32_t PA_KEYS = 128;
 constexpr int PA_THREADS = 384;
 constexpr uint32_t PA_SOFTMAX_TID0 = 128;
 constexpr long long PA_WAIT_LIMIT = 2000000000ll;
+constexpr uint32_t PA_FOLD = 48; // tiles whose products are added up in tensor memory
 constexpr float PA_LOG2E = 1.4426950408889634f;
 constexpr float PA_BIAS2 = 7.0f; // a row's reference lies so far below its maximum, in base-2 exponents,
 constexpr float PA_LAZY2 = 8.0f; // and moves when a tile exceeds that maximum by more than this
@@ -93,6 +98,7 @@ struct PaArgs {
     const char *vpages;
     const float *sinks;
     float *scratch;
+    float *fold; // of a CTA [DIM / 8][256 threads][4]: O of the tiles that were folded
     uint32_t *status;
     size_t row_bytes;
     float scale2; // scale * log2(e)
@@ -402,6 +408,21 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             const uint32_t klo = real ? plan_lowest(sq, plan.window, it.tok0 + tok) : 0u;
             // Weights are 2^(s C - m_ref), m_ref = m_raw C - PA_BIAS2 - PA_HALF2 for the score m_raw of a key. l: this thread's keys only.
             float m_raw = NEG_BIG, m_ref = 0.0f, l = 0.0f;
+            float m_fold = NEG_BIG; // m_raw of what has been folded
+            // this thread's 16-byte piece i of it
+            auto folded = [&](uint32_t i) { return reinterpret_cast<float4 *>(g.fold) + ((blockIdx.x * (DIM / 8u) + i) * 256u + threadIdx.x - PA_SOFTMAX_TID0); };
+            auto add_folded = [&](uint32_t (&o)[32], uint32_t c0) { // o: 32 dims from c0 on of this thread's
+                if (!(m_fold > NEG_TEST)) return; // (none yet, or no key seen)
+                const float f = exp2f((m_fold - m_raw) * g.scale2);
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; i++) {
+                    const float4 x = __ldcg(folded(c0 / 4u + i));
+                    o[4 * i] = __float_as_uint(fmaf(x.x, f, __uint_as_float(o[4 * i])));
+                    o[4 * i + 1] = __float_as_uint(fmaf(x.y, f, __uint_as_float(o[4 * i + 1])));
+                    o[4 * i + 2] = __float_as_uint(fmaf(x.z, f, __uint_as_float(o[4 * i + 2])));
+                    o[4 * i + 3] = __float_as_uint(fmaf(x.w, f, __uint_as_float(o[4 * i + 3])));
+                }
+            };
             const uint32_t end = t0 + (sg.b - sg.a);
             more = walk.next(nx);
             for (uint32_t t = t0; t < end; t++, buf.next()) {
@@ -525,8 +546,10 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                     unpack2(add2(sum[0], sum[1]), s0, s1);
                     l = l * cf + (s0 + s1);
                     const bool moved = t > t0 && __any_sync(0xffffffffu, cf != 1.0f);
-                    if (moved || bad_any) { // this warp's rows of O (rare)
+                    const bool fold = t > t0 && (t - t0) % PA_FOLD == 0u;
+                    if (moved || bad_any || fold) { // this warp's rows of O (rare)
                         if (t > t0) wait_pv(t - 1u);
+                        const bool adds = m_fold > NEG_TEST && m_fold == m_raw; // (each piece has one thread, and the order of its additions)
 #pragma unroll 1
                         for (uint32_t c0 = HD * half; c0 < HD * half + HD; c0 += 32u) {
                             uint32_t orow[32];
@@ -536,6 +559,19 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                             }
 #pragma unroll
                             for (int c = 0; c < 32; c++) orow[c] = t > t0 ? __float_as_uint(__uint_as_float(orow[c]) * cf) : 0u;
+                            if (fold) { // O goes on from zero
+                                if (!adds) add_folded(orow, c0 - HD * half);
+#pragma unroll
+                                for (uint32_t i = 0; i < 8u; i++) {
+                                    const float4 x = make_float4(__uint_as_float(orow[4 * i]), __uint_as_float(orow[4 * i + 1]), __uint_as_float(orow[4 * i + 2]),
+                                                                 __uint_as_float(orow[4 * i + 3]));
+                                    float4 *to = folded((c0 - HD * half) / 4u + i);
+                                    if (adds) red_add4(to, x);
+                                    else *to = x;
+                                }
+#pragma unroll
+                                for (int c = 0; c < 32; c++) orow[c] = 0u;
+                            }
                             // rows of V that are not finite, zero in shared memory: w v for the tokens that see them
                             for (uint32_t r = 0; bad_any && r < PA_KEYS; r++) {
                                 const uint32_t key = key0 + r;
@@ -552,6 +588,7 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                             }
                             tmem_st32(tmem + lane_addr + c0, orow);
                         }
+                        if (fold) m_fold = m_raw;
                     }
                 }
                 if (bad_any) {
@@ -603,6 +640,7 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                         uint32_t orow[32];
                         tmem_ld32(tmem + lane_addr + HD * half + c0, orow);
                         tmem_wait_ld();
+                        add_folded(orow, c0);
                         uint32_t w[4][4]; // [16-byte chunk][word]
 #pragma unroll
                         for (int c = 0; c < 32; c += 2) {
@@ -627,6 +665,7 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                         uint32_t orow[32];
                         tmem_ld32(tmem + lane_addr + HD * half + c0, orow);
                         tmem_wait_ld();
+                        add_folded(orow, c0);
                         if (!many) {
                             if (real)
 #pragma unroll
@@ -685,6 +724,7 @@ mkv_status launch_pool_attn_f16(Pool *p, int layer, const PoolPlan &plan, const 
     g.vpages = p->layer_ptr(layer, 1);
     g.sinks = a.sinks;
     g.scratch = p->scratch;
+    g.fold = p->scratch + 2u * pool_attn_ctas(p) * part_floats((uint32_t)p->desc.head_dim);
     g.status = p->ctx->dev_status;
     g.row_bytes = p->row_bytes;
     g.scale2 = a.scale * PA_LOG2E;

@@ -117,9 +117,12 @@ struct PlanCost {
 };
 bool pool_plan(const Pool *p, const mkv_seq_rows *items, int n, int &i, uint32_t &rows, uint32_t window, const PlanCost &cost, PoolPlan &plan, MergeList &merge);
 
-// The floats of a part in scratch memory: [128 rows][dim], then [128 rows][maximum, sum]; two parts a CTA
+// The floats of a part in scratch memory: [128 rows][dim], then [128 rows][maximum, sum]; two parts a CTA. Behind those of all CTAs the f16 kernel
+// has another [128 rows][dim] for each.
 __host__ __device__ inline size_t part_floats(uint32_t dim) { return 128u * (size_t)(dim + 2u); }
 __host__ __device__ inline size_t part_slot(uint32_t cta, uint32_t part) { return 2u * (size_t)cta + part; }
+
+inline size_t pool_attn_ctas(const Pool *p) { return std::min<uint32_t>((uint32_t)p->ctx->sm_count, PLAN_CTAS); }
 
 mkv_status launch_pool_merge(Pool *p, const MergeList &merge, const PoolAttn &a);
 mkv_status pool_attn_f16_setup(Pool *);

@@ -825,3 +825,61 @@ def test_scores_of_very_long_rows(ctx, fmt, heads, size):
         want, mag, *_ = attn64(pool, items, q, window=window)
         assert ((got.double() - want).abs() <= mag * 2.0**-18 + want.abs() * 2.0**-11 + 2.0**-25).all()
     pool.close()
+
+
+@pytest.mark.parametrize("heads,n,ntok", [((64, 1, 64), 300000, 300), ((16, 2, 256), 200000, 600)])
+def test_values_of_one_sign_over_a_long_history(ctx, heads, n, ntok):
+    """Sums over hundreds of thousands of keys do not drift. The tensor core's sums truncate; a step of 16 keys loses up to 2^-23 of the
+    sum in the end (an ulp of the present sum, twice, which is half the last one on average), 2^-15 + 2^-16 over the 384 steps that it adds up before
+    they are put aside. What else an output is off by is a rounding each of weights, sums and output, which has no direction."""
+    pool, ids, g = scattered(ctx, F16, [n], 256, 6, heads=heads, spare=0)
+    v = pool.buffer_tensors(0)[1]
+    v.uniform_(0.5, 1.5, generator=g)
+    v.mul_(torch.linspace(1.0, 1.9, heads[2], device="cuda").half())
+    q = randn(g, ntok, heads[0], heads[2], dtype=torch.float16)
+    got = run_attn(pool, [(ids[0], 0, n - ntok, ntok)], q)
+    last = 8192 // (heads[0] * heads[2])
+    want = attn64(pool, [(ids[0], 0, n - last, last)], q[-last:])[0]
+    drift = float(((got[-last:].double() - want) / want).mean())
+    assert abs(drift) <= 2.0**-15 + 2.0**-16, drift
+    pool.close()
+
+
+@pytest.mark.parametrize("heads", [(16, 2, 256), (12, 4, 128), (4, 4, 64)])
+@pytest.mark.parametrize("keys", ["flat", "rising", "falling", "jumping"])
+def test_histories_of_many_tiles(ctx, heads, keys):
+    """Segments of 130 to 500 tiles, whole and cut, with references that stay, rise tile by tile, fall behind or jump late; windows, sinks, values
+    that are not finite in the last, partly seen tile, with which a new sum of outputs starts (144 and 192 whole tiles in front)."""
+    hq, hkv, dim = heads
+    ntok = min(16, 128 // (hq // hkv))
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    for tiles, times in ((144, sms // hkv), (192, sms // hkv), (300, 5 + 2 * sms // hkv)):
+        n = 128 * tiles + 100
+        pool, ids, g = scattered(ctx, F16, [n], 128, tiles, heads=heads, spare=0)
+        k, v = pool.buffer_tensors(0)
+        pages = torch.from_numpy(pool.pages(ids[0]).astype(np.int64)).cuda()
+        ramp = torch.linspace(0, 30, len(pages) * 128, device="cuda")
+        along = {"flat": 0 * ramp, "rising": ramp, "falling": 30 - ramp, "jumping": torch.where(ramp > 29.9, 25.0, 0.0) + torch.where(ramp > 20, 9.0, 0.0)}[keys]
+        k[pages, :, :, 0] = along.view(len(pages), 128, 1).half()
+        q = randn(g, ntok, hq, dim, dtype=torch.float16)
+        q[..., 0] = dim**0.5 if keys != "flat" else 0.5
+        many = q.repeat(times, 1, 1)
+        sinks = randn(g, hq)
+        for window, first, s in ((0, 0, None), (n - 900, 0, sinks), (0, 5000, sinks)):
+            items = [(ids[0], first, n - ntok, ntok)]
+            got = run_attn(pool, items * times, many, window=window, sinks=s).view(times, ntok, hq, dim)
+            want, mag, qk, top = attn64(pool, items, q, window=window, sinks=s)
+            assert ((got.double() - want).abs() <= attn_bound(F16, want, mag, qk, top)).all(), (tiles, window, first)
+        at = (int(pages[-1]), 100 - ntok + 3)  # the row of token 3
+        items = [(ids[0], 0, n - ntok, ntok)]
+        clean = run_attn(pool, items * times, many).view(times, ntok, hq, dim)
+        want, mag, qk, top = attn64(pool, items, q)  # (the other dims and tokens stay as they are)
+        v[at][:, 1], v[at][:, 2] = math.nan, math.inf
+        got = run_attn(pool, items * times, many).view(times, ntok, hq, dim)
+        bad = torch.zeros_like(got, dtype=torch.bool)
+        bad[:, 3:, :, 1:3] = True
+        assert torch.equal(~torch.isfinite(got), bad)
+        assert torch.equal(got[:, :3], clean[:, :3])
+        bound = attn_bound(F16, want, mag, qk, top) + 2.0**-11 * mag  # (that key's weight and the row's sum have roundings of their own)
+        assert ((got.double() - want).abs() <= bound)[~bad].all()
+        pool.close()
