@@ -71,7 +71,7 @@ class PageBook {
   public:
     struct Seq {
         bool live = false;
-        uint32_t len = 0;
+        uint32_t len = 0, before = 0;  // before: len in front of the last write
         uint64_t stamp = 0;            // the last call that named the sequence, to find one that is named twice
         std::vector<uint32_t> pages;
         std::vector<uint32_t> written; // per layer: rows [0, written) are there
@@ -228,6 +228,7 @@ class PageBook {
             const mkv_seq_rows &it = items[i];
             if (it.ntok == 0u) continue;
             Seq &s = seqs[it.seq];
+            s.before = s.len;
             const uint32_t have = (uint32_t)s.pages.size(), last = (it.pos + it.ntok - 1u) / page;
             bool own = true;
             for (uint32_t j = it.pos / page; j <= last && j < have; j++) {
@@ -255,6 +256,17 @@ class PageBook {
             s.written[(size_t)layer] = end;
         }
         return MKV_OK;
+    }
+
+    // The rows of the last write() did not get to the device: they do not count. (What else it did stays: pages taken or copied are the
+    // sequences' own, rows behind the new ones are forgotten.)
+    void not_written(int layer, const mkv_seq_rows *items, int n) {
+        for (int i = 0; i < n; i++) {
+            if (items[i].ntok == 0u) continue;
+            Seq &s = seqs[items[i].seq];
+            s.written[(size_t)layer] = std::min(s.written[(size_t)layer], items[i].pos);
+            if (s.len > s.before) cut(items[i].seq, s.before);
+        }
     }
 
     mkv_status compact(uint32_t *moved) {

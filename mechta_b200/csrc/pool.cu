@@ -237,8 +237,8 @@ static mkv_status need_pool(const void *p) {
     return MKV_ERR_INVALID;
 }
 
-// A change of the books and what follows it on the device.
-template <class F> static mkv_status change(Pool *p, const F &body) {
+// A change of the books and what follows it on the device; `undo` takes the change back when that could not be launched.
+template <class F, class U> static mkv_status change(Pool *p, const F &body, const U &undo) {
     if (!p->ctx) {
         const mkv_status st = body();
         p->book.ops.clear();
@@ -249,7 +249,13 @@ template <class F> static mkv_status change(Pool *p, const F &body) {
     if (dev.status != MKV_OK) return dev.status;
     mkv_status st = follow_books(p); // (what an earlier call could not launch: entries of one launch do not depend on each other)
     if (st == MKV_OK) st = body();
-    return st == MKV_OK ? follow_books(p) : st;
+    if (st != MKV_OK) return st;
+    st = follow_books(p);
+    if (st != MKV_OK) undo();
+    return st;
+}
+template <class F> static mkv_status change(Pool *p, const F &body) {
+    return change(p, body, [] {}); // (the next call makes up for it)
 }
 
 static mkv_status check_items(const Pool *p, int layer, const mkv_seq_rows *items, int n, uint64_t *rows) {
@@ -395,7 +401,7 @@ mkv_status mkv_seq_create(mkv_pool *h, uint32_t *seq) {
 mkv_status mkv_seq_fork(mkv_pool *h, uint32_t seq, uint32_t len, int copy, int n, uint32_t *children) {
     if (need_pool(h) != MKV_OK || need_pool(children) != MKV_OK) return MKV_ERR_INVALID;
     Pool *p = pool_of(h);
-    return guarded([&] { return change(p, [&] { return p->book.fork(seq, len, copy != 0, n, children); }); });
+    return guarded([&] { return change(p, [&] { return p->book.fork(seq, len, copy != 0, n, children); }, [&] { p->book.free_all(children, n); }); });
 }
 
 mkv_status mkv_seq_free(mkv_pool *h, const uint32_t *seqs, int n) {
@@ -467,11 +473,13 @@ mkv_status mkv_pool_write(mkv_pool *h, int layer, const mkv_seq_rows *items, int
             const mkv_status checked = p->book.write(layer, items, n, true);
             return checked == MKV_OK ? no_rows() : checked;
         }
-        mkv_status st2 = change(p, [&] { return p->book.write(layer, items, n, false); });
+        auto undo = [&] { p->book.not_written(layer, items, n); };
+        mkv_status st2 = change(p, [&] { return p->book.write(layer, items, n, false); }, undo);
         if (st2 != MKV_OK || rows == 0) return st2;
         DeviceScope dev(p->ctx);
-        if (dev.status != MKV_OK) return dev.status;
-        return launch_pool_write(p, layer, items, n, w);
+        st2 = dev.status != MKV_OK ? dev.status : launch_pool_write(p, layer, items, n, w);
+        if (st2 != MKV_OK) undo();
+        return st2;
     });
 }
 

@@ -2,6 +2,7 @@
 over pages. Needs a B200.
 
 Tolerances follow from the roundings (a half step is eps / 2 of the value): see `attn_bound` and the comments beside each test."""
+import ctypes as C
 import math
 
 import numpy as np
@@ -883,3 +884,79 @@ def test_histories_of_many_tiles(ctx, heads, keys):
         bound = attn_bound(F16, want, mag, qk, top) + 2.0**-11 * mag  # (that key's weight and the row's sum have roundings of their own)
         assert ((got.double() - want).abs() <= bound)[~bad].all()
         pool.close()
+
+
+class failing_launches:
+    """Launches on the stream return an error: the driver refuses a call that may not be captured and with it all that follows in that capture. Nothing
+    reaches the GPU meanwhile."""
+
+    def __init__(self, stream):
+        self.cu, self.stream = C.CDLL("libcuda.so.1"), C.c_void_p(stream.cuda_stream)
+
+    def __enter__(self):
+        assert self.cu.cuStreamBeginCapture_v2(self.stream, 2) == 0  # 2: relaxed
+        assert self.cu.cuStreamSynchronize(self.stream) == 900       # unsupported in a capture, which is invalid from now on
+
+    def __exit__(self, *_):
+        graph = C.c_void_p()
+        assert self.cu.cuStreamEndCapture(self.stream, C.byref(graph)) == 901 and not graph
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_writes_and_forks_that_do_not_reach_the_device(ctx, fmt):
+    """After an error of a launch the rows that it should have written are not there, forks are not made, and the call can be repeated."""
+    stream = torch.cuda.Stream()
+    c2 = kv.KvContext(0, stream)
+    with torch.cuda.stream(stream):
+        page = 16
+        pool, ids, g = scattered(c2, fmt, [40, 20, 33], page, 19, layers=2, spare=30, longest=400)
+        a, b, c = ids
+        d = pool.fork(b)[0]
+        dt = pool.fmt.torch_dtype
+        k, v, q = randn(g, 50, 2, 256), randn(g, 50, 2, 256), randn(g, 50, 16, 256, dtype=dt)
+        out = torch.empty_like(q)
+        before = {s: [[t.clone() for t in rows_of(pool, s, l)] for l in range(2)] for s in (a, b, c, d)}
+        free = pool.free_pages
+        stream.synchronize()
+
+        def fails(call, *args, **kw):
+            with failing_launches(stream), pytest.raises(_lib.MkvError) as e:
+                call(*args, **kw)
+            assert e.value.status == _lib.ERR_CUDA
+
+        def refused(items):
+            with pytest.raises(_lib.MkvError) as e:
+                pool.attn(1, items, q[:1], out[:1])
+            assert e.value.status == _lib.ERR_STATE
+
+        fails(pool.write, 1, [(a, 0, 40, 3)], k[:3], v[:3])                       # rows on a page that is there
+        refused([(a, 0, 40, 1)])
+        assert pool.length(a) == 40 and pool.free_pages == free
+        fails(pool.write, 1, [(a, 0, 40, 30), (b, 0, 20, 4), (c, 0, 10, 2)], k[:36], v[:36])  # new pages, a copied page, rows in front of the end
+        for s, n in ((a, 40), (b, 20), (c, 10)):
+            refused([(s, 0, n, 1)])
+            assert pool.length(s) == (12 if s == c else n)
+        assert pool.free_pages == free + 2 - 1  # (c gave two pages back, b has one of its own now)
+        for copy in (False, True):
+            pool.set_len(a, 40)  # (what the failed call left for the device gets there)
+            fails(pool.fork, a, 40, 3, copy)
+            assert pool.free_pages == free + 1
+        assert pool.create() == d + 1
+        pool.free([d + 1])
+        items = [(a, 0, 40, 30), (b, 0, 20, 4), (c, 0, 10, 2)]
+        pool.write(1, items, k[:36], v[:36])
+        pool.attn(1, items, q[:36], out[:36])
+        want, mag, qk, top = attn64(pool, items, q[:36], layer=1)
+        assert ((out[:36].double() - want).abs() <= attn_bound(fmt, want, mag, qk, top)).all()
+        for (s, _, p, n), at in zip(items, (0, 30, 34)):
+            for l in range(2):
+                for got, old, new in zip(rows_of(pool, s, l), before[s][l], (k, v)):
+                    assert torch.equal(got[:p], old[:p])
+                    if l == 1:
+                        assert torch.equal(got[p:], new[at:at + n].to(dt))
+        for l in range(2):
+            for got, old in zip(rows_of(pool, d, l), before[d][l]):
+                assert torch.equal(got, old)
+        stream.synchronize()
+        pool.close()
+    c2.close()
