@@ -281,7 +281,8 @@ void mkv_rope_destroy(mkv_rope *r);
 mkv_status mkv_rope_freqs(const mkv_rope *r, double *freqs_host, double *m_host);
 /* y = rotated x for ntok tokens of `heads` heads. backward != 0: the transposed map (angles negated, the same m), which takes
  * the gradient of y to the gradient of x. x and y may be f16 or f32 each, and may be the same memory with the same strides and
- * type; any other overlap is refused (slices of one buffer, whose tokens lie beside each other, do not overlap). Strides in elements; 0 = dense ([ntok][heads][head_dim]). A head's dims are contiguous. */
+ * type; any other overlap is refused (slices of one buffer do not overlap, whether their tokens or their heads lie beside each other). Strides in
+ * elements; 0 = dense ([ntok][heads][head_dim]). A head's dims are contiguous. */
 typedef struct {
     const void *x_dev;
     void *y_dev;

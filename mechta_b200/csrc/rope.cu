@@ -222,8 +222,15 @@ mkv_status mkv_rope_apply(mkv_ctx *h, const mkv_rope *r, const mkv_rope_rows *in
     }
     const RowSpan sx = {(uintptr_t)g.x, in->ntok, (uint64_t)g.xt * xe, ((uint64_t)(H - 1) * (uint64_t)g.xh + (uint64_t)D) * xe};
     const RowSpan sy = {(uintptr_t)g.y, in->ntok, (uint64_t)g.yt * ye, ((uint64_t)(H - 1) * (uint64_t)g.yh + (uint64_t)D) * ye};
+    // Slices of every head (a query beside its gate) lie between one another's: where one of the two strides is a multiple of the other, all
+    // heads of all tokens are among rows at the smaller one.
+    auto all_heads = [&](const void *at, int64_t t, int64_t h, size_t e) {
+        const int64_t s = H == 1 ? t : in->ntok == 1 ? h : std::min(t, h), span = (int64_t)(in->ntok - 1u) * t + (H - 1) * h;
+        if (s < 1 || t % s != 0 || h % s != 0) return RowSpan{(uintptr_t)at, 1u, 1u, (uint64_t)(span + D) * e}; // (all of it)
+        return RowSpan{(uintptr_t)at, (uint64_t)(span / s) + 1u, (uint64_t)s * e, (uint64_t)D * e};
+    };
     const bool same = g.x == g.y && xe == ye && (in->ntok == 1 || g.xt == g.yt) && (H == 1 || g.xh == g.yh);
-    if (!same && sx.meets(sy)) {
+    if (!same && sx.meets(sy) && all_heads(g.x, g.xt, g.xh, xe).meets(all_heads(g.y, g.yt, g.yh, ye))) {
         set_error("rope: x and y overlap without being the same memory in the same layout and type");
         return MKV_ERR_INVALID;
     }

@@ -379,3 +379,23 @@ def test_numbers_beyond_32_bits_are_refused():
     p.free(np.array([a]))
     assert p.free_pages == 40
     p.close()
+
+
+def test_slices_of_every_head_do_not_overlap():
+    """x and y in one buffer, each a part of every head, in both orders of tokens and heads; parts that share a value are refused."""
+    L = _lib.lib()
+    r = kv.Rope(None, 64)
+    buf = np.zeros((5, 6, 200), np.float32)
+    pos = np.zeros(5, np.int32)
+
+    def apply(x, y, dim=64, n=5, heads=6, xt=1200, yt=1200, xh=200, yh=200, yf=1):
+        rows = _lib.RopeRows(buf.ctypes.data + 4 * x, buf.ctypes.data + 4 * y, 1, yf, n, heads, dim, xt, xh, yt, yh, pos.ctypes.data, 0)
+        assert L.mkv_rope_apply(None, r._h, C.byref(rows)) == _lib.ERR_INVALID
+        return L.mkv_last_error().decode() == "null ctx"  # nothing wrong but the missing context
+
+    assert apply(0, 64) and apply(64, 0) and apply(0, 136) and apply(136, 0) and apply(0, 100, dim=100) and apply(0, 64, n=1)
+    assert apply(0, 64, xt=200, yt=200, xh=1200, yh=1200, n=6, heads=5) and not apply(0, 63, xt=200, yt=200, xh=1200, yh=1200, n=6, heads=5)
+    assert apply(0, 264, n=4) and apply(200, 64, n=4, heads=5)  # a head further on, another part of it
+    assert not apply(0, 63) and not apply(63, 0) and not apply(0, 137, dim=64, n=4) and not apply(0, 100, dim=101)
+    assert not apply(0, 64, yh=208, yt=1248, n=4) and not apply(0, 64, yf=0, n=2)
+    assert not apply(0, 200) and not apply(0, 1200, n=4)
