@@ -159,10 +159,10 @@ class _State:
 
 
 @functools.lru_cache(maxsize=None)
-def _context(stream):
-    """A host program has one context for all its pools."""
+def _context(device, stream):
+    """A host program has one context for all its pools on a device and stream (which the context keeps, so that its handle stays its own)."""
     from mechta_b200 import kv
-    return kv.KvContext(torch.cuda.current_device(), torch.cuda.current_stream())
+    return kv.KvContext(device, torch.cuda.current_stream())
 
 
 def _rope(s, case):
@@ -204,7 +204,7 @@ def prepare(case, seed):
         return torch.randn(*shape, device="cuda", generator=g)
 
     if own:
-        s.ctx = _context(torch.cuda.current_stream().cuda_stream)
+        s.ctx = _context(torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream)
     if s.kind == "rope":
         n, heads, dim = case["tokens"], case["heads"], case["dim"]
         x = normal(n, heads, 2 * dim if case["gated"] else dim).to(_dtype(case["src"]))
