@@ -7,12 +7,11 @@
 //   P = 2^(S - reference) as f16, back into the columns of S (base-2 exponents throughout)
 //   O += P V    A = P (tensor memory), B = the V tile as TMA left it (N-major)
 // One pass: the reference of a row lies PA_BIAS2 = 7 below its maximum at the time, and moves only when a tile exceeds that maximum by more
-// than PA_LAZY2 = 8 (then O is rescaled); sums are kept in f32, those of the weights over what f16 has of them, so that an output is a true mean of
-// the values: the weights are cut to 11 bits in front of both (one operation each, 62.3 us where the case below takes 61.4 with sums of other
-// weights; taken back from f16 they cost 64.5). Weights stay below 2^15 (f16 ends at 65,504) and are rounded by 2^-11 of
-// themselves down to 2^-21 of the row's largest, by 2^-32 of that below (with the reference at the maximum itself it was 2^-25, and 65,536 keys at
-// 2^-25 of one, 0.2% of the sum, were lost). 8 is as seldom exceeded as more would be (ragged blocks under a window with 6, 8, 10 and 11.5: 63.8, 61.4,
-// 61.3 and 61.0 us); scores of N(0, 1) grow by about 4 behind their first tile.
+// than PA_LAZY2 = 8 (then O is rescaled). Weights stay below 2^15 (f16 ends at 65,504) and are rounded by 2^-11 of themselves down to 2^-21 of the
+// row's largest, by 2^-32 of that below (with the reference at the maximum itself it was 2^-25, and 65,536 keys at 2^-25 of one, 0.2% of the sum,
+// were lost). 8 is as seldom exceeded as more would be (ragged blocks under a window with 6, 8, 10 and 11.5: 63.8, 61.4, 61.3 and 61.0 us); scores
+// of N(0, 1) grow by about 4 behind their first tile. Sums are kept in f32, and those of the weights run over the rounded ones, so that an output is
+// a true mean of the values (the same blocks 63.4 us, 61.4 with sums of the weights in front of their rounding).
 // The tensor core's f32 sums truncate, all in one direction: about 2^-23.3 of O for each 16 keys (values of one sign over 300,000 keys came out 1.0e-3
 // too small). So every 48 tiles (4.2e-5 by then, a sixth of an output's smallest half step) O is added, with rounding, to what its thread has of it
 // in global memory, and starts again; the segment's end adds the two. The long block below takes 1,239 us where it took 1,204 without, every 32
@@ -84,10 +83,6 @@ struct PaShared {
     uint32_t bad[3][4];     // [tile's S buffer]: keys of the tile whose V row is not finite and that not every token sees
 };
 static_assert(sizeof(PaShared) <= 64, "OFF_MISC");
-
-// The 11 bits of a weight that f16 has. Of a weight times 1 + 2^-11, that is the weight to within 2^-11 of itself.
-__device__ __forceinline__ float pa_cut(float w) { return __uint_as_float(__float_as_uint(w) & 0xffffe000u); }
-constexpr float PA_HALF2 = 7.04269e-4f; // log2(1 + 2^-11): m_ref is so much smaller than what weights and their sums stand for
 
 struct PaArgs {
     const __half *q;
@@ -406,7 +401,7 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             const bool real = row < rows;
             const uint32_t vis = real ? sq.pos + it.tok0 + tok + 1u : 0u; // this row sees klo <= key < vis
             const uint32_t klo = real ? plan_lowest(sq, plan.window, it.tok0 + tok) : 0u;
-            // Weights are 2^(s C - m_ref), m_ref = m_raw C - PA_BIAS2 - PA_HALF2 for the score m_raw of a key. l: this thread's keys only.
+            // Weights are 2^(s C - m_ref), m_ref = m_raw C - PA_BIAS2 for the score m_raw of a key. l: this thread's keys only.
             float m_raw = NEG_BIG, m_ref = 0.0f, l = 0.0f;
             float m_fold = NEG_BIG; // m_raw of what has been folded
             // this thread's 16-byte piece i of it
@@ -511,7 +506,7 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                         if (moves()) {
                             cf = m_raw > NEG_TEST ? exp2f((m_raw - mx) * g.scale2) : 1.0f;
                             m_raw = mx;
-                            m_ref = mx * g.scale2 - (PA_BIAS2 + PA_HALF2);
+                            m_ref = mx * g.scale2 - PA_BIAS2;
                         }
                     }
                     float neg_m = -m_ref;
@@ -519,14 +514,14 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                     // range; there the difference of the scores comes first.
                     const bool far = fabsf(m_ref) > 1048576.0f;
                     if (far) {
-                        neg_m = PA_BIAS2 + PA_HALF2;
+                        neg_m = PA_BIAS2;
 #pragma unroll
                         for (int h = 0; h < 2; h++)
 #pragma unroll
                             for (int c = 0; c < 32; c++) sr[h][c] = __float_as_uint(__uint_as_float(sr[h][c]) - m_raw);
                     }
                     const uint64_t c2 = pack2(g.scale2, g.scale2), m2 = pack2(neg_m, neg_m);
-                    uint64_t sum[2] = {0ull, 0ull};
+                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f}; // of the weights as the products take them
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         uint32_t ph[16]; // 32 weights as f16 pairs
@@ -534,17 +529,13 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                         for (int c = 0; c < 32; c += 2) {
                             float x0, x1;
                             unpack2(fma2(pack2(__uint_as_float(sr[h][c]), __uint_as_float(sr[h][c + 1])), c2, m2), x0, x1);
-                            x0 = pa_cut(ex2(x0));
-                            x1 = pa_cut(ex2(x1));
-                            sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], pack2(x0, x1));
-                            const __half2 hp = __floats2half2_rn(x0, x1);
+                            const __half2 hp = __floats2half2_rn(ex2(x0), ex2(x1));
                             ph[c >> 1] = *reinterpret_cast<const uint32_t *>(&hp);
+                            add_f16x2(sum[c & 2], sum[(c & 2) + 1], ph[c >> 1]);
                         }
                         tmem_st16(s_col + 16u * h, ph);
                     }
-                    float s0, s1;
-                    unpack2(add2(sum[0], sum[1]), s0, s1);
-                    l = l * cf + (s0 + s1);
+                    l = l * cf + ((sum[0] + sum[2]) + (sum[1] + sum[3]));
                     const bool moved = t > t0 && __any_sync(0xffffffffu, cf != 1.0f);
                     const bool fold = t > t0 && (t - t0) % PA_FOLD == 0u;
                     if (moved || bad_any || fold) { // this warp's rows of O (rare)
@@ -582,7 +573,7 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                                 const __half *q = g.q + (int64_t)(sq.row + it.tok0 + tok) * g.q_stride + (size_t)(sg.kvh * group + head) * DIM;
                                 float s = 0.0f;
                                 for (int d = 0; d < DIM; d++) s = fmaf(__half2float(q[d]), __half2float(k[d]), s);
-                                const float w = pa_cut(exp2f(fmaf(far ? s - m_raw : s, g.scale2, neg_m)));
+                                const float w = __half2float(__float2half_rn(exp2f(fmaf(far ? s - m_raw : s, g.scale2, neg_m))));
 #pragma unroll
                                 for (int c = 0; c < 32; c++) orow[c] = __float_as_uint(fmaf(w, __half2float(v[c]), __uint_as_float(orow[c])));
                             }
@@ -627,7 +618,7 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 if (sg.whole) {
                     // out[token][head][:] = O / (l + sink)
                     float den = l_all;
-                    if (g.sinks && real) den += exp2f(g.sinks[sg.kvh * group + head] * PA_LOG2E - (m_ref + PA_HALF2));
+                    if (g.sinks && real) den += exp2f(g.sinks[sg.kvh * group + head] * PA_LOG2E - m_ref);
                     const float inv = 1.0f / den;
                     __half *dst[4];
 #pragma unroll
@@ -655,7 +646,7 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 } else {
                     // a part: maximum, sum and O as they are, for the merge
                     float *ps = g.scratch + part_slot(blockIdx.x, sg.part) * part_floats(DIM);
-                    if (half == 0u && real) *reinterpret_cast<float2 *>(ps + 128u * DIM + 2u * row) = make_float2(m_raw > NEG_TEST ? m_ref + PA_HALF2 : NEG_BIG, seen ? l_all : -1.0f);
+                    if (half == 0u && real) *reinterpret_cast<float2 *>(ps + 128u * DIM + 2u * row) = make_float2(m_raw > NEG_TEST ? m_ref : NEG_BIG, seen ? l_all : -1.0f);
                     // The exchange pays where many rows are stored (six blocks of up to 109 tokens of six heads: the call takes 14.1 us, without it
                     // 17.3); one token's rows are few lines either way, and sooner stored as they are (12.1 us, with it 13.2).
                     const bool many = rows > 32u;

@@ -151,6 +151,15 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+// lo += the low f16 of w, hi += the high one
+__device__ __forceinline__ void add_f16x2(float &lo, float &hi, uint32_t w) {
+    asm("{\n\t.reg .f16 a, b;\n\t"
+        "mov.b32 {a, b}, %2;\n\t"
+        "add.rn.f32.f16 %0, a, %0;\n\t"
+        "add.rn.f32.f16 %1, b, %1;\n\t}"
+        : "+f"(lo), "+f"(hi)
+        : "r"(w));
+}
 // *p += x in global memory, without waiting for it
 __device__ __forceinline__ void red_add4(float4 *p, float4 x) {
     asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(x.x), "f"(x.y), "f"(x.z), "f"(x.w) : "memory");
