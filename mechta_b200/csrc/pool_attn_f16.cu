@@ -184,7 +184,9 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh->tmem_base;
-    pdl_wait(); // nothing global is touched before the kernel in front has finished
+    // Nothing global is touched before the kernel in front has finished. This kernel has begun before that, so what that one may have written (page
+    // tables, rotated queries) is not read-only for it, and no load takes the read-only path.
+    pdl_wait();
     pdl_launch_dependents();
 
     // The units of the CTA's T tiles in ring order, whatever segment they belong to: K(0) .. K(LEAD - 1), then K(t + LEAD) and V(t) for
@@ -212,7 +214,7 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             const uint32_t *pages = g.pages + plan.seq[ts.sg.seq].table;
             auto row = [&](bool mine, uint32_t key) {
                 if (!mine || key + box_rows <= it.lo || key >= it.hi) return ~0u;
-                return (__ldg(pages + (key >> g.page_shift)) << g.page_shift) + (key & (page_tokens - 1u));
+                return (pages[key >> g.page_shift] << g.page_shift) + (key & (page_tokens - 1u));
             };
             t.k_row = row(t.is && cb < Z::BOXES, key0 + rb * box_rows);
 #pragma unroll
@@ -355,7 +357,7 @@ pool_attn_f16_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             for (uint32_t i = 0; i < QB; i++) {
                 const uint32_t r = 32u * q4 + (b * QB + i) * RPI + lane / CPR, t = r * inv_group >> 16;
                 qv[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (r < rows) qv[i] = __ldg(reinterpret_cast<const uint4 *>(src + (int64_t)t * g.q_stride + (r - t * group) * DIM));
+                if (r < rows) qv[i] = *reinterpret_cast<const uint4 *>(src + (int64_t)t * g.q_stride + (r - t * group) * DIM);
             }
         };
         bool clean = false; // this quarter's rows in shared memory are zeros

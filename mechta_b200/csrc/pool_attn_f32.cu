@@ -186,7 +186,9 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh->tmem_base, total = plan.start[blockIdx.x].tiles;
-    pdl_wait(); // nothing global is touched before the kernel in front has finished
+    // Nothing global is touched before the kernel in front has finished. This kernel has begun before that, so what that one may have written (page
+    // tables, rotated queries) is not read-only for it, and no load takes the read-only path.
+    pdl_wait();
     pdl_launch_dependents();
 
     // The units of the CTA's T tiles in ring order, whatever segment they belong to: K(0), then K(t + 1) and V(t) for each t. In front of
@@ -284,7 +286,7 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             if (named_bar_or(bar_team, 128, odd || (amax != 0.0f && !(amax * s >= 256.0f && amax * s < 32768.0f)))) {
                 const float *src = v ? g.vpages : g.kpages;
                 if (in) {
-                    const size_t page = __ldg(g.pages + tl.table + (key >> g.page_shift));
+                    const size_t page = __ldcg(g.pages + tl.table + (key >> g.page_shift));
                     src += ((page << g.page_shift) + (key & ((1u << g.page_shift) - 1u))) * g.row_floats + (size_t)tl.kvh * DIM + 32u * j;
                 }
                 auto again = [&](uint32_t h, float4 (&x)[8]) {
@@ -362,7 +364,7 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 const PlanItem &it = ts.sg.it;
                 const uint32_t key = (it.tile0 + ts.tile) * PF_KEYS32 + rb * box_rows;
                 if (t.is && cb < 2u && key + box_rows > it.lo && key < it.hi)
-                    t.row = (__ldg(g.pages + plan.seq[ts.sg.seq].table + (key >> g.page_shift)) << g.page_shift) + (key & (page_tokens - 1u));
+                    t.row = (__ldcg(g.pages + plan.seq[ts.sg.seq].table + (key >> g.page_shift)) << g.page_shift) + (key & (page_tokens - 1u));
                 if (t.is) ts.next();
                 return t;
             };
@@ -501,7 +503,7 @@ pool_attn_f32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 const float *src = g.q + (int64_t)(plan.seq[sg.seq].row + sg.it.tok0 + ftok) * g.q_stride + (size_t)(sg.kvh * group + fr - ftok * group) * DIM + 16u * j;
                 auto fetch = [&](uint32_t c, float4 (&x)[4]) {
 #pragma unroll
-                    for (uint32_t i = 0; i < 4u; i++) x[i] = there ? __ldg(reinterpret_cast<const float4 *>(src + 64u * c + 4u * i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (uint32_t i = 0; i < 4u; i++) x[i] = there ? __ldcg(reinterpret_cast<const float4 *>(src + 64u * c + 4u * i)) : make_float4(0.f, 0.f, 0.f, 0.f);
                 };
                 uint32_t amax = 0u;
                 auto look = [&](const float4 (&x)[4]) {

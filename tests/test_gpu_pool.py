@@ -960,3 +960,37 @@ def test_writes_and_forks_that_do_not_reach_the_device(ctx, fmt):
         stream.synchronize()
         pool.close()
     c2.close()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_tables_that_change_right_in_front_of_the_attention(ctx, fmt):
+    """Tables of 2 entries, sixteen sequences in 128 bytes, copied from one another and read by the next launch, over and over: every row is the
+    value of the pages that its sequence has now."""
+    hq, hkv, dim, n = 4, 4, 64, 60
+    pool = kv.KvPool(ctx, fmt, 1, 200, 16, n + 4, 32, hq, hkv, dim)
+    k, v = pool.buffer_tensors(0)
+    k.zero_()
+    v.copy_(torch.arange(200, device="cuda").view(200, 1, 1, 1).expand_as(v))
+    parents = [pool.create() for _ in range(4)]
+    for p in parents:
+        pool.set_len(p, 16)
+    q = torch.ones(n, hq, dim, device="cuda", dtype=pool.fmt.torch_dtype)
+    outs, wants = [], []
+    for r in range(100):
+        kids = [c for p in (parents[r % 4:] + parents[:r % 4]) for c in pool.fork(p, n=n // 4)]
+        out = torch.full_like(q, math.nan)
+        pool.attn(0, [(c, 0, 15, 1) for c in kids], q, out)
+        outs.append(out)
+        wants.append([float(pool.pages(c)[0]) for c in kids])
+        pool.free(kids[::-1] if r % 3 else kids)
+        if r % 5 == 0:  # the parents' pages change as well
+            pool.free(parents)
+            hold = pool.create()
+            pool.set_len(hold, 16 + r % 17)
+            parents = [pool.create() for _ in range(4)]
+            for p in parents[::-1]:
+                pool.set_len(p, 16)
+            pool.free([hold])
+    for out, want in zip(outs, wants):
+        assert (out == torch.tensor(want, device="cuda")[:, None, None]).all()
+    pool.close()
