@@ -347,8 +347,11 @@ mkv_status mkv_seq_pages(const mkv_pool *p, uint32_t seq, uint32_t *pages_host, 
 mkv_status mkv_pool_compact(mkv_pool *p, uint32_t *moved_out);
 /* New rows of n sequences (each at most once) in one layer, by mkv_append's rule: pos may not lie beyond the rows the layer has;
  * afterwards the sequence ends at pos + ntok (rows behind are forgotten) and the layer's rows are valid up to there. Takes missing
- * pages and copies shared ones (all layers) as needed: MKV_ERR_NOMEM, with nothing changed, when they do not suffice.
- * k, v: f32 or f16 [ntok of all items, in their order][kv_heads][head_dim], token strides in elements (0 = dense).
+ * pages and copies shared ones (all layers) as needed: MKV_ERR_NOMEM, with nothing changed, when they do not suffice. An item without tokens
+ * leaves its sequence as it is. What other layers have on a shared page from pos on is not copied and counts no longer: fork between steps,
+ * not between the layers of one.
+ * k, v: f32 or f16 [ntok of all items, in their order][kv_heads][head_dim], token strides in elements (0 = dense); not rows
+ * that the call writes.
  * rope: rotates K at the rows' positions (dims <= head_dim); NULL when K is already rotated. */
 typedef struct {
     const void *k_dev;
@@ -364,8 +367,9 @@ mkv_status mkv_pool_write(mkv_pool *p, int layer, const mkv_seq_rows *items, int
  * q, out: the pool's type, [tokens of all items, in their order][q_heads][head_dim], token strides in elements (0 = dense; multiples of
  * 16 bytes), 16-byte aligned, not overlapping. scale 0 = 1 / sqrt(head_dim). sinks_dev: [q_heads] logits that join the softmax's maximum and sum and
  * never the output, or NULL. f16 pools: weights are rounded to f16 for the tensor cores (by 2^-11 of themselves, or by 2^-32 of the row's
- * largest where that is more; the softmax's sum is that of the rounded ones), everything else is summed in f32; f32 pools: f32-grade throughout (values are taken as two f16 parts, 22 bits; one below 2^-33 of the largest value of its
- * 64 rows, or of its query, counts as nothing). */
+ * largest where that is more; the softmax's sum is that of the rounded ones), everything else is summed in f32; f32 pools:
+ * f32-grade throughout (values are taken as two f16 parts, 22 bits; one below 2^-33 of the largest value of its 64 rows, or of its query, counts
+ * as nothing). Values are summed up before the division: the keys seen times the largest |v| has to stay within f32. */
 typedef struct {
     const void *q_dev;
     void *out_dev;

@@ -12,8 +12,8 @@ struct Pool {
     size_t elem = 2, row_bytes = 0, page_bytes = 0, layer_bytes = 0; // layer_bytes: the K (or V) pages of one layer
     char *mem = nullptr;                                            // [layer][K, V][page][row]
     uint32_t *table = nullptr;                                      // [max_seqs][max_pages]
-    float *scratch = nullptr;                                       // partials of split work of the attention
-    std::vector<CUtensorMap> maps;                                  // [layer][K, V] (f16)
+    float *scratch = nullptr;                                       // of the attention: parts of split work, folded outputs (pool_plan.cuh)
+    std::vector<CUtensorMap> maps;                                  // [layer][K, V]
     explicit Pool(const mkv_pool_desc &d) : desc(d), book(d.n_pages, d.page_tokens, d.max_seqs, d.max_tokens, d.n_layers) {}
     char *layer_ptr(int layer, int kv) const { return mem + (2u * (size_t)layer + (size_t)kv) * layer_bytes; }
 };

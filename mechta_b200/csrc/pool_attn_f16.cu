@@ -32,9 +32,9 @@
 // only some of its tokens see are searched; one that is not finite is zeroed too and its share added to the rows that see it
 // with ordinary arithmetic.
 //
-// Bound by HBM for few rows (32 sessions of up to 65,536 tokens, 2.18 GB: 339 us, 6.4 TB/s, the rate of a plain copy), by the chain of
-// softmax and products for long blocks (2,048 tokens over 32,768: 1.13 TFLOP in 1.2 ms, 0.93 PFLOP/s: under load the GPU's power limit
-// takes part of the clock), by the segments' latencies for small work: about 6 us from the start to the last store of a CTA with one
+// Bound by HBM for few rows (32 sessions of up to 65,536 tokens, 2.18 GB: 345 us in a burst, 6.3 TB/s, and 366 to 390 one after the other, where the
+// GPU's power limit takes part of the clock), by the chain of softmax and products for long blocks (2,048 tokens over 32,768: 1.13 TFLOP in
+// 1.1 ms in a burst, 1.23 ms one after the other, 0.92 PFLOP/s), by the segments' latencies for small work: about 6 us from the start to the last store of a CTA with one
 // tile, of which the page lookup and the first tile's way take 2, softmax and products 3, the part's stores 1; the merge is 3 more.
 //
 // Roles (384 threads, three warpgroups whose register budgets are set with setmaxnreg): warps 0 and 3 = TMA producers, warp 1 = issues

@@ -107,14 +107,14 @@ struct MergeList {
     MergeItem item[PLAN_CTAS];
 };
 
-// Plans one launch over the items [i, n) that it takes (i is moved on); rows: packed tokens in front of them, moved on too.
-// Returns false when no item with tokens is left.
 struct PlanCost {
     uint32_t rows;    // of an item: query heads of a KV head times tokens
     uint32_t keys;    // of a tile
     uint32_t segment; // in tiles
     uint32_t whole;   // tiles of an item up to which it is not worth a merge
 };
+// Plans one launch over the items [i, n) that it takes (i is moved on); rows: packed tokens in front of them, moved on too.
+// Returns false when no item with tokens is left.
 bool pool_plan(const Pool *p, const mkv_seq_rows *items, int n, int &i, uint32_t &rows, uint32_t window, const PlanCost &cost, PoolPlan &plan, MergeList &merge);
 
 // The floats of a part in scratch memory: [128 rows][dim], then [128 rows][maximum, sum]; two parts a CTA. Behind those of all CTAs the f16 kernel

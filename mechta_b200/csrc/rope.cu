@@ -32,7 +32,7 @@ struct RopeArgs {
     const void *x;
     void *y;
     const int32_t *pos;
-    uint32_t heads, head_dim, units; // units of a head
+    uint32_t heads, units; // units of a head
     int64_t xt, xh, yt, yh;
 };
 
@@ -189,7 +189,6 @@ mkv_status mkv_rope_apply(mkv_ctx *h, const mkv_rope *r, const mkv_rope_rows *in
     g.y = in->y_dev;
     g.pos = in->pos_dev;
     g.heads = in->heads;
-    g.head_dim = in->head_dim;
     const int64_t dense = (int64_t)in->heads * in->head_dim;
     g.xh = in->x_head_stride ? in->x_head_stride : in->head_dim;
     g.yh = in->y_head_stride ? in->y_head_stride : in->head_dim;

@@ -1,5 +1,5 @@
 // Rotary positions: the host's frequency table, which travels in the kernel's parameter space, and the device code that rotates
-// one head, shared by the operator of its own (rope.cu) and the writer of paged rows (pool_write.cu).
+// one head, shared by the operator of its own (rope.cu) and the writer of paged rows (pool.cu).
 #pragma once
 #include "internal.cuh"
 
