@@ -47,10 +47,7 @@ books_kernel(const __grid_constant__ BookArgs list, char *__restrict__ mem, size
         if (at + 4096u * i < bytes) *reinterpret_cast<uint4 *>(dst + at + 4096u * i) = v[i];
 }
 
-// Launches what is in the lists and clears them; after an error they stay, for the next call.
-static mkv_status follow_books(Pool *p) {
-    std::vector<PageCopy> &cs = p->book.copies;
-    std::vector<TableOp> &ops = p->book.ops;
+static mkv_status launch_books(Pool *p, const std::vector<PageCopy> &cs, const std::vector<TableOp> &ops) {
     for (size_t i = 0, j = 0; i < cs.size() || j < ops.size();) {
         BookArgs t;
         t.n_copies = (uint32_t)std::min<size_t>(BOOK_ENTRIES, cs.size() - i);
@@ -66,6 +63,37 @@ static mkv_status follow_books(Pool *p) {
         MKV_CUDA(cudaLaunchKernelEx(&l.cfg, books_kernel, t, p->mem, p->layer_bytes, p->page_bytes, (uint32_t)p->row_bytes, p->table));
         p->ctx->launches++;
     }
+    return MKV_OK;
+}
+
+// Launches what is in the lists and clears them; after an error they stay, for the next call. In a capture the launches are only recorded: the
+// pages are the sequences' own from now on, but the graph may never run, and rows written through a table that still has others would be written
+// to other sequences' pages. So the lists are kept, and the first call outside a capture does all of it (again, where the graph has run:
+// tables and pages are as it left them, so that changes nothing). Another capture may not begin before: its graph would either go without, or
+// repeat with each replay what belongs to other sequences.
+static mkv_status follow_books(Pool *p) {
+    std::vector<PageCopy> &cs = p->book.copies;
+    std::vector<TableOp> &ops = p->book.ops;
+    if (cs.empty() && ops.empty() && p->recorded.empty()) return MKV_OK;
+    cudaStreamCaptureStatus status;
+    unsigned long long id = 0;
+    MKV_CUDA(cudaStreamGetCaptureInfo(p->ctx->stream, &status, &id));
+    if (status == cudaStreamCaptureStatusNone) id = 0;
+    if (id != p->capture && id != 0 && !p->recorded.empty()) {
+        set_error("an earlier capture changed pages: a call outside a capture has to come first");
+        return MKV_ERR_STATE;
+    }
+    if (id == 0)
+        for (const BookWork &w : p->recorded) {
+            const mkv_status st = launch_books(p, w.copies, w.ops);
+            if (st != MKV_OK) return st;
+        }
+    if (id == 0) p->recorded.clear();
+    p->capture = id;
+    if (id != 0 && !(cs.empty() && ops.empty())) p->recorded.reserve(p->recorded.size() + 1u);
+    const mkv_status st = launch_books(p, cs, ops);
+    if (st != MKV_OK) return st;
+    if (id != 0 && !(cs.empty() && ops.empty())) p->recorded.push_back({std::move(cs), std::move(ops)});
     cs.clear();
     ops.clear();
     return MKV_OK;

@@ -994,3 +994,65 @@ def test_tables_that_change_right_in_front_of_the_attention(ctx, fmt):
     for out, want in zip(outs, wants):
         assert (out == torch.tensor(want, device="cuda")[:, None, None]).all()
     pool.close()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_a_capture_that_takes_pages_and_never_runs(ctx, fmt):
+    """The step is captured, its graph dropped (or run), and the step made again without a capture: its rows lie on the sequences' own pages, those
+    of all other sequences are as they were. A second capture before any other call is refused; the first one's later calls are not."""
+    stream = torch.cuda.Stream()
+    c2 = kv.KvContext(0, stream)
+    dt = kv.KvFormat(fmt).torch_dtype
+    for runs in (0, 1, 2):
+        with torch.cuda.stream(stream):
+            pool, ids, g = scattered(c2, fmt, [64, 48, 40], 16, 23, spare=30, longest=400)
+            a, b, c = ids
+            d = pool.fork(c)[0]  # (shares c's last page)
+            x, q = [randn(g, 6, 2, 256) for _ in range(2)], randn(g, 6, 16, 256, dtype=dt)
+            out = torch.empty_like(q)
+            before = {s: [t.clone() for t in rows_of(pool, s)] for s in (a, b, c, d)}
+            items = [(a, 0, 64, 2), (b, 0, 48, 1), (d, 0, 40, 3)]  # two new pages, a copied one
+
+            def step():
+                pool.write(0, items, *x)
+                pool.attn(0, items, q, out)
+
+            stream.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                step()
+                more = pool.fork(a, 64)[0]
+                pool.write(0, [(more, 0, 64, 1)], x[0][:1], x[1][:1])
+            for r in range(runs):
+                graph.replay()
+                replayed = out.clone()
+            if not runs:
+                second = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(second, stream=stream):
+                    out.zero_()
+                    for call in (step, lambda: pool.fork(a), lambda: pool.attn(0, items, q, out)):
+                        with pytest.raises(_lib.MkvError) as e:
+                            call()
+                        assert e.value.status == _lib.ERR_STATE
+                stream.synchronize()
+                del graph, second
+            step()
+            if runs:
+                assert torch.equal(out, replayed)
+                del graph
+            want, mag, qk, top = attn64(pool, items, q)
+            assert ((out.double() - want).abs() <= attn_bound(fmt, want, mag, qk, top)).all()
+            pool.write(0, [(more, 0, 64, 1)], x[0][5:], x[1][5:])
+            for s, p, at, n in ((a, 64, 0, 2), (b, 48, 2, 1), (c, 40, 0, 0), (d, 40, 3, 3), (more, 64, 5, 1)):
+                for got, old, new in zip(rows_of(pool, s), before[s if s != more else a], x):
+                    assert torch.equal(got[:p], old[:p]) and torch.equal(got[p:], new[at:at + n].to(dt))
+            stream.synchronize()
+            third = torch.cuda.CUDAGraph()  # (all that was recorded is done: another capture may change pages)
+            with torch.cuda.graph(third, stream=stream):
+                pool.write(0, [(c, 0, 40, 1)], x[0][:1], x[1][:1])
+            third.replay()
+            assert torch.equal(rows_of(pool, c)[0][40], x[0][0].to(dt)) and torch.equal(rows_of(pool, d)[0][40], x[0][3].to(dt))
+            stream.synchronize()
+            del third
+            pool.close()
+    c2.close()
