@@ -7,8 +7,10 @@ libmechta_kv through ctypes with raw pointers.
 """
 from __future__ import annotations
 
+import array
 import ctypes as C
 import enum
+import itertools
 from dataclasses import dataclass
 
 import numpy as np
@@ -275,20 +277,19 @@ def _need(ok, text: str) -> None:
 
 def _u32(*numbers: int) -> None:
     """Refuses what ctypes would cut to 32 bits."""
-    for v in numbers:
-        if not 0 <= v < 2**32:
-            _need(False, f"{v}: must lie between 0 and 2^32 - 1")
+    if min(numbers) < 0 or max(numbers) >= 2**32:
+        _need(False, f"{numbers}: must lie between 0 and 2^32 - 1")
 
 
 def _u32_array(numbers) -> np.ndarray:
     """Whole numbers as uint32; refuses those that a cast would cut or round."""
-    a = np.asarray(numbers)
+    a = np.ascontiguousarray(numbers)
     if a.dtype.kind not in "iu" and a.size:
         _need(False, f"{a.dtype}: must be whole numbers from 0 to 2^32 - 1")
-    wide = a.astype(np.uint64)  # (a negative one is above 2^63)
-    if (wide >> np.uint64(32)).any():
+    words = a.astype(np.int64, copy=False).view(np.uint32)  # the low half of each number, then the high half
+    if words[..., 1::2].any():
         _need(False, "numbers must lie between 0 and 2^32 - 1")
-    return wide.astype(np.uint32)
+    return words[..., ::2]
 
 
 def _fmt_of(t: torch.Tensor) -> int:
@@ -405,7 +406,8 @@ class KvPool:
         _need(0 < n <= self.max_seqs, f"fork of {n} sequences: 1 to {self.max_seqs}")
         if length is None:
             length = self.length(seq)
-        _u32(seq, length)
+        if not (0 <= seq < 2**32 and 0 <= length < 2**32):
+            _u32(seq, length)
         if n == 1:
             check(self._lib.mkv_seq_fork(self._h, seq, length, copy, 1, self._out_ref))
             return [self._out.value]
@@ -415,15 +417,17 @@ class KvPool:
 
     def free(self, seqs) -> None:
         if type(seqs) is list and {*map(type, seqs)} <= {int}:
-            _u32(*seqs)
+            if seqs:
+                _u32(*seqs)
             a, n = (C.c_uint32 * len(seqs))(*seqs), len(seqs)
         else:
-            held = _u32_array(seqs).reshape(-1)
+            held = np.ascontiguousarray(_u32_array(seqs)).reshape(-1)
             a, n = held.ctypes.data, held.size
         check(self._lib.mkv_seq_free(self._h, a, n))
 
     def truncate(self, seq: int, length: int) -> None:
-        _u32(seq, length)
+        if not (0 <= seq < 2**32 and 0 <= length < 2**32):
+            _u32(seq, length)
         check(self._lib.mkv_seq_truncate(self._h, seq, length))
 
     def set_len(self, seq: int, length: int) -> None:
@@ -432,11 +436,12 @@ class KvPool:
         check(self._lib.mkv_seq_set_len(self._h, seq, length))
 
     def length(self, seq: int) -> int:
-        _u32(seq)
+        if not 0 <= seq < 2**32:
+            _u32(seq, seq)
         return self._lib.mkv_seq_len(self._h, seq)
 
     def pages(self, seq: int) -> np.ndarray:
-        _u32(seq)
+        _u32(seq, seq)
         n = C.c_uint32()
         check(_lib.lib().mkv_seq_pages(self._h, seq, None, 0, C.byref(n)))
         a = np.empty(n.value, np.uint32)
@@ -478,6 +483,14 @@ class KvPool:
     def _items(items) -> tuple[bytes, int, int]:
         """The items as the library takes them, their number, their tokens."""
         a = items
+        if type(a) is list and a:
+            try:
+                if {*map(len, a)} != {4}:
+                    _need(False, "items are rows of (sequence, first_pos, pos, ntok)")
+                a = array.array("I", itertools.chain.from_iterable(a))
+            except (TypeError, OverflowError):
+                _need(False, "items must be whole numbers from 0 to 2^32 - 1")
+            return a.tobytes(), len(items), sum(a[3::4])
         if not (type(a) is np.ndarray and a.dtype == np.uint32):
             a = _u32_array(items)
         if a.ndim != 2 or a.shape[1] != 4:
