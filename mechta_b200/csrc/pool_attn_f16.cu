@@ -14,8 +14,8 @@
 // a true mean of the values (the same blocks 63.4 us, 61.4 with sums of the weights in front of their rounding).
 // The tensor core's f32 sums truncate, all in one direction: about 2^-23.3 of O for each 16 keys (values of one sign over 300,000 keys came out 1.0e-3
 // too small). So every 48 tiles (4.2e-5 by then, a sixth of an output's smallest half step) O is added, with rounding, to what its thread has of it
-// in global memory, and starts again; the segment's end adds the two. The long block below takes 1,239 us where it took 1,204 without, every 32
-// tiles 1,280, every 64 1,232: what it costs is the wait for the product in front.
+// in global memory, and starts again; the segment's end adds the two. A fold takes 6,000 clocks, the time that the SM's 128 KB of stores need; the
+// long block below takes 1,232 us where it took 1,195 without, 1,280 with a fold every 32 tiles.
 // TMEM: O = columns 0 .. DIM - 1, then two (DIM = 256) or three S buffers of 128 columns, so that the scores of the next tiles are there when
 // a tile's softmax begins.
 //
@@ -34,8 +34,9 @@
 //
 // Bound by HBM for few rows (32 sessions of up to 65,536 tokens, 2.18 GB: 345 us in a burst, 6.3 TB/s, and 366 to 390 one after the other, where the
 // GPU's power limit takes part of the clock), by the chain of softmax and products for long blocks (2,048 tokens over 32,768: 1.13 TFLOP in
-// 1.1 ms in a burst, 1.23 ms one after the other, 0.92 PFLOP/s), by the segments' latencies for small work: about 6 us from the start to the last store of a CTA with one
-// tile, of which the page lookup and the first tile's way take 2, softmax and products 3, the part's stores 1; the merge is 3 more.
+// 1.1 ms in a burst, 1.23 to 1.27 ms one after the other, 0.9 PFLOP/s), by the segments' latencies for small work: about 6 us from the start to
+// the last store of a CTA with one tile, of which the page lookup and the first tile's way take 2, softmax and products 3, the part's stores 1;
+// the merge is 3 more.
 //
 // Roles (384 threads, three warpgroups whose register budgets are set with setmaxnreg): warps 0 and 3 = TMA producers, warp 1 = issues
 // S = Q K^T and owns the TMEM, warp 2 = issues O += P V, warps 4..11 = softmax. Every wait is bounded; TMEM is

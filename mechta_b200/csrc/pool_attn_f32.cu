@@ -30,7 +30,7 @@
 // Roles (512 threads, four warpgroups whose register budgets are set with setmaxnreg): warps 0 and 3 = TMA producers, warp 1 =
 // issues S' and owns the TMEM, warp 2 = issues O', warps 4..7 = converters, warps 8..15 = softmax and owners of O: two threads per TMEM
 // lane, half of the dims each, and of a row's four threads 16 of a tile's keys each. TMEM: O' = columns 0 .. DIM - 1, S' = 256 .. 319 and 320 .. 383, Q' = 384 ...
-// Every wait is bounded; TMEM is freed on every path.
+// Every wait is bounded; TMEM is freed on every path. With heads of 256 a thread spills 380 to 480 bytes, of 128 about 100.
 #include <type_traits>
 
 #include "pool_plan.cuh"
