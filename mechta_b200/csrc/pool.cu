@@ -66,11 +66,15 @@ static mkv_status launch_books(Pool *p, const std::vector<PageCopy> &cs, const s
     return MKV_OK;
 }
 
+static bool is_capturing(const void *pool) {
+    cudaStreamCaptureStatus status; // (of an invalid capture the launches fail)
+    return cudaStreamIsCapturing(static_cast<const Pool *>(pool)->ctx->stream, &status) == cudaSuccess && status == cudaStreamCaptureStatusActive;
+}
+
 // Launches what is in the lists and clears them; after an error they stay, for the next call. In a capture the launches are only recorded: the
-// pages are the sequences' own from now on, but the graph may never run, and rows written through a table that still has others would be written
-// to other sequences' pages. So the lists are kept, and the first call outside a capture does all of it (again, where the graph has run:
-// tables and pages are as it left them, so that changes nothing). Another capture may not begin before: its graph would either go without, or
-// repeat with each replay what belongs to other sequences.
+// pages are the sequences' own from now on, but the graph may never run, and rows written through a table that still has others would land on
+// other sequences' pages. So the first call outside a capture writes these sequences' tables from the books, whether the graph has run or not.
+// Another capture may not begin before: its graph would go without.
 static mkv_status follow_books(Pool *p) {
     std::vector<PageCopy> &cs = p->book.copies;
     std::vector<TableOp> &ops = p->book.ops;
@@ -79,21 +83,24 @@ static mkv_status follow_books(Pool *p) {
     unsigned long long id = 0;
     MKV_CUDA(cudaStreamGetCaptureInfo(p->ctx->stream, &status, &id));
     if (status == cudaStreamCaptureStatusNone) id = 0;
-    if (id != p->capture && id != 0 && !p->recorded.empty()) {
-        set_error("an earlier capture changed pages: a call outside a capture has to come first");
+    if (!p->recorded.empty() && id == 0) {
+        for (uint32_t s : p->recorded) {
+            const std::vector<uint32_t> &v = p->book.seqs[s].pages; // (pageable memory: read before the call returns)
+            if (p->book.alive(s) && !v.empty())
+                MKV_CUDA(cudaMemcpyAsync(p->table + (size_t)s * p->book.max_pages, v.data(), v.size() * sizeof(uint32_t), cudaMemcpyHostToDevice, p->ctx->stream));
+        }
+        p->recorded.clear();
+    } else if ((!p->recorded.empty() && id != p->capture) || (id != 0 && !cs.empty())) { // (copies: of a call whose launch failed)
+        set_error("an earlier call changed pages: one outside a capture has to come first");
         return MKV_ERR_STATE;
     }
-    if (id == 0)
-        for (const BookWork &w : p->recorded) {
-            const mkv_status st = launch_books(p, w.copies, w.ops);
-            if (st != MKV_OK) return st;
-        }
-    if (id == 0) p->recorded.clear();
     p->capture = id;
-    if (id != 0 && !(cs.empty() && ops.empty())) p->recorded.reserve(p->recorded.size() + 1u);
+    if (id != 0) p->recorded.reserve(p->recorded.size() + ops.size() + p->book.max_seqs); // (nothing may fail behind the launch)
     const mkv_status st = launch_books(p, cs, ops);
     if (st != MKV_OK) return st;
-    if (id != 0 && !(cs.empty() && ops.empty())) p->recorded.push_back({std::move(cs), std::move(ops)});
+    for (size_t i = 0; id != 0 && i < ops.size(); i++) // (a run of entries may go on into the next sequence's table)
+        for (uint32_t s = ops[i].dst / p->book.max_pages; s <= (ops[i].dst + (ops[i].n & ~TableOp::COPY) - 1u) / p->book.max_pages; s++)
+            if (p->recorded.empty() || p->recorded.back() != s) p->recorded.push_back(s);
     cs.clear();
     ops.clear();
     return MKV_OK;
@@ -369,6 +376,8 @@ mkv_status mkv_pool_create(mkv_ctx *h, const mkv_pool_desc *d, mkv_pool **out) {
         }
         p->ctx = ctx;
         ctx->live_caches++;
+        p->book.capturing = is_capturing;
+        p->book.device = p;
         auto fail = [&](mkv_status s) {
             mkv_pool_destroy(reinterpret_cast<mkv_pool *>(p));
             return s;

@@ -5,12 +5,6 @@
 
 namespace mkv {
 
-// What one change of the books asks of the device
-struct BookWork {
-    std::vector<PageCopy> copies;
-    std::vector<TableOp> ops;
-};
-
 struct Pool {
     Ctx *ctx = nullptr; // null: the bookkeeping alone
     mkv_pool_desc desc = {};
@@ -20,8 +14,8 @@ struct Pool {
     uint32_t *table = nullptr;                                      // [max_seqs][max_pages]
     float *scratch = nullptr;                                       // of the attention: parts of split work, folded outputs (pool_plan.cuh)
     std::vector<CUtensorMap> maps;                                  // [layer][K, V]
-    // What was recorded into the capture of that number and may never run
-    std::vector<BookWork> recorded;
+    // Sequences whose tables were changed in the capture of that number, which may never run
+    std::vector<uint32_t> recorded;
     unsigned long long capture = 0;
     explicit Pool(const mkv_pool_desc &d) : desc(d), book(d.n_pages, d.page_tokens, d.max_seqs, d.max_tokens, d.n_layers) {}
     char *layer_ptr(int layer, int kv) const { return mem + (2u * (size_t)layer + (size_t)kv) * layer_bytes; }

@@ -998,30 +998,41 @@ def test_tables_that_change_right_in_front_of_the_attention(ctx, fmt):
 
 @pytest.mark.parametrize("fmt", FMTS)
 def test_a_capture_that_takes_pages_and_never_runs(ctx, fmt):
-    """The step is captured, its graph dropped (or run), and the step made again without a capture: its rows lie on the sequences' own pages, those
-    of all other sequences are as they were. A second capture before any other call is refused; the first one's later calls are not."""
+    """Pages are taken and shared in a capture, its graph dropped (or run), and the step made again without a capture: its rows lie on the sequences'
+    own pages, those of all other sequences are as they were. Copies in a capture, and a second capture before any other call, are refused; the first
+    one's later calls are not."""
     stream = torch.cuda.Stream()
     c2 = kv.KvContext(0, stream)
     dt = kv.KvFormat(fmt).torch_dtype
     for runs in (0, 1, 2):
         with torch.cuda.stream(stream):
-            pool, ids, g = scattered(c2, fmt, [64, 48, 40], 16, 23, spare=30, longest=400)
-            a, b, c = ids
+            pool, ids, g = scattered(c2, fmt, [64, 48, 40, 64], 16, 23, spare=30, longest=400)
+            a, b, c, e = ids
             d = pool.fork(c)[0]  # (shares c's last page)
             x, q = [randn(g, 6, 2, 256) for _ in range(2)], randn(g, 6, 16, 256, dtype=dt)
             out = torch.empty_like(q)
-            before = {s: [t.clone() for t in rows_of(pool, s)] for s in (a, b, c, d)}
-            items = [(a, 0, 64, 2), (b, 0, 48, 1), (d, 0, 40, 3)]  # two new pages, a copied one
+            before = {s: [t.clone() for t in rows_of(pool, s)] for s in (a, b, c, d, e)}
+            items = [(a, 0, 64, 2), (b, 0, 48, 1), (e, 0, 48, 3)]  # two new pages; one in place of a page that is shared by then
 
             def step():
                 pool.write(0, items, *x)
                 pool.attn(0, items, q, out)
 
+            def refused(*calls):
+                books = [pool.free_pages, *(pool.length(i) for i in range(12))]
+                for call in calls:
+                    with pytest.raises(_lib.MkvError) as err:
+                        call()
+                    assert err.value.status == _lib.ERR_STATE
+                assert [pool.free_pages, *(pool.length(i) for i in range(12))] == books
+
             stream.synchronize()
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph, stream=stream):
+                more, kid = pool.fork(a, 64)[0], pool.fork(e)[0]
+                pool.truncate(e, 48)
                 step()
-                more = pool.fork(a, 64)[0]
+                refused(lambda: pool.write(0, [(d, 0, 40, 1)], x[0][:1], x[1][:1]), lambda: pool.fork(b, copy=True), lambda: pool.fork(b, n=2, copy=True))
                 pool.write(0, [(more, 0, 64, 1)], x[0][:1], x[1][:1])
             for r in range(runs):
                 graph.replay()
@@ -1030,10 +1041,7 @@ def test_a_capture_that_takes_pages_and_never_runs(ctx, fmt):
                 second = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(second, stream=stream):
                     out.zero_()
-                    for call in (step, lambda: pool.fork(a), lambda: pool.attn(0, items, q, out)):
-                        with pytest.raises(_lib.MkvError) as e:
-                            call()
-                        assert e.value.status == _lib.ERR_STATE
+                    refused(step, lambda: pool.fork(a), lambda: pool.attn(0, items, q, out))
                 stream.synchronize()
                 del graph, second
             step()
@@ -1042,17 +1050,29 @@ def test_a_capture_that_takes_pages_and_never_runs(ctx, fmt):
                 del graph
             want, mag, qk, top = attn64(pool, items, q)
             assert ((out.double() - want).abs() <= attn_bound(fmt, want, mag, qk, top)).all()
-            pool.write(0, [(more, 0, 64, 1)], x[0][5:], x[1][5:])
-            for s, p, at, n in ((a, 64, 0, 2), (b, 48, 2, 1), (c, 40, 0, 0), (d, 40, 3, 3), (more, 64, 5, 1)):
-                for got, old, new in zip(rows_of(pool, s), before[s if s != more else a], x):
+            pool.write(0, [(more, 0, 64, 1), (d, 0, 40, 1)], x[0][4:], x[1][4:])
+            for s, p, at, n, was in ((a, 64, 0, 2, a), (b, 48, 2, 1, b), (c, 40, 0, 0, c), (d, 40, 5, 1, d), (e, 48, 3, 3, e), (more, 64, 4, 1, a), (kid, 64, 0, 0, e)):
+                assert pool.length(s) == p + n
+                for got, old, new in zip(rows_of(pool, s), before[was], x):
                     assert torch.equal(got[:p], old[:p]) and torch.equal(got[p:], new[at:at + n].to(dt))
+                # by the device's tables: attention to one key gives its value (f32: of two parts, 2^-23 of it, of sums of them, and 2^-33 of its tile's largest)
+                seen = torch.empty(p + n, 16, 256, device="cuda", dtype=dt)
+                pool.attn(0, [(s, i, i, 1) for i in range(p + n)], torch.zeros_like(seen), seen)
+                value = rows_of(pool, s)[1].double()
+                assert ((seen.view(p + n, 2, 8, 256)[:, :, 0].double() - value).abs() <= value.abs() * 2.0**-20 + 8 * 2.0**-33).all()
+            pool.free([more])
             stream.synchronize()
             third = torch.cuda.CUDAGraph()  # (all that was recorded is done: another capture may change pages)
             with torch.cuda.graph(third, stream=stream):
-                pool.write(0, [(c, 0, 40, 1)], x[0][:1], x[1][:1])
+                refused(pool.compact)
+                pool.write(0, [(c, 0, 40, 9)], torch.cat(x)[:9], torch.cat(x)[:9])
             third.replay()
-            assert torch.equal(rows_of(pool, c)[0][40], x[0][0].to(dt)) and torch.equal(rows_of(pool, d)[0][40], x[0][3].to(dt))
+            for i, row in enumerate(torch.cat(x)[:9]):
+                assert torch.equal(rows_of(pool, c)[0][40 + i], row.to(dt))
+            assert torch.equal(rows_of(pool, d)[0][40], x[0][5].to(dt))
             stream.synchronize()
             del third
+            pool.free([a])
+            assert pool.compact() > 0
             pool.close()
     c2.close()
