@@ -305,9 +305,8 @@ mkv_status mkv_rope_apply(mkv_ctx *ctx, const mkv_rope *r, const mkv_rope_rows *
  * and then return MKV_ERR_UNSUPPORTED; all other calls work.
  * What a call does to the bookkeeping is done when it returns; what it does to rows is enqueued on the ctx's stream. A captured
  * launch keeps the pages of its capture: replay it only while its sequences are as they were then, and in the order of the ctx's stream
- * (the calls of a ctx share the scratch of split work). Pages that captured calls took or shared are the sequences' own also when the graph
- * never runs; the pool's next call that needs the device has to be made outside a capture then (MKV_ERR_STATE in another one). A call that would
- * copy pages is refused in a capture (MKV_ERR_STATE). A call that is refused changes nothing. One that fails with MKV_ERR_CUDA leaves no
+ * (the calls of a ctx share the scratch of split work). Pages that captured calls took, copied or shared are the sequences' own also when the
+ * graph never runs; the pool's next call behind the capture that needs the device has to be made outside of one (MKV_ERR_STATE in another one). A call that is refused changes nothing. One that fails with MKV_ERR_CUDA leaves no
  * forks, and none of the rows that it should have written count (the sequence ends where it ended before, or at the new rows' end if that is
  * less; the layer's rows end at pos): it may be repeated. */
 typedef struct mkv_pool mkv_pool;

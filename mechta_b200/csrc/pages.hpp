@@ -82,8 +82,6 @@ class PageBook {
     std::vector<Seq> seqs;
     std::vector<TableOp> ops;
     std::vector<PageCopy> copies;
-    bool (*capturing)(const void *) = nullptr; // whether what follows on the device would only be recorded
-    const void *device = nullptr;
 
     PageBook(uint32_t n_pages_, uint32_t page_, uint32_t max_seqs_, uint32_t max_tokens_, int layers)
         : n_pages(n_pages_), page(page_), max_seqs(max_seqs_), max_tokens(max_tokens_), n_layers(layers), seqs(max_seqs_),
@@ -97,13 +95,6 @@ class PageBook {
         if (alive(s)) return MKV_OK;
         set_error("no sequence %u", s);
         return MKV_ERR_INVALID;
-    }
-
-    // A graph that never runs copies nothing, and one that has run may have changed what it copied from: neither can be made up for.
-    mkv_status may_copy() const {
-        if (!capturing || !capturing(device)) return MKV_OK;
-        set_error("pages cannot be copied in a capture: make the call outside of one first");
-        return MKV_ERR_STATE;
     }
 
     mkv_status create(uint32_t *out) {
@@ -133,7 +124,6 @@ class PageBook {
             set_error("fork of %d sequences: %u sequences and %u pages are free", n, free_seqs.size(), free_pages.size());
             return MKV_ERR_NOMEM;
         }
-        if (copy && np > 0u && (st = may_copy()) != MKV_OK) return st;
         // All that may fail for want of memory comes first; a sequence keeps its vectors' room for the next one of its number.
         for (uint32_t i = 0, c = free_seqs.lowest(); i < (uint32_t)n; i++, c++) {
             while (!free_seqs.has(c)) c++;
@@ -283,8 +273,6 @@ class PageBook {
         const uint32_t used = n_pages - free_pages.size();
         if (moved) *moved = 0u;
         if (used == n_pages || free_pages.lowest() >= used) return MKV_OK; // the pages in use are the lowest
-        const mkv_status st = may_copy();
-        if (st != MKV_OK) return st;
         std::vector<uint32_t> src, dst;
         free_pages.each(used, n_pages, false, [&](uint32_t p) { return src.push_back(p), true; });
         dst.reserve(src.size());
@@ -357,7 +345,6 @@ class PageBook {
             for (uint32_t j = it.pos / page; j <= last && j < have; j++) {
                 const uint32_t p = s.pages[j];
                 if (refs[p] == 1u) continue;
-                if (j * page < it.pos && (st = may_copy()) != MKV_OK) return st;
                 try {
                     left.push_back(p);
                 } catch (const std::bad_alloc &) {

@@ -14,17 +14,23 @@ namespace mkv {
 // bytes of traffic for each byte and nothing to compute: HBM-bound (30,011 tokens of ten layers copied and compacted: 2.46 GB in
 // 375 us, the rate of a plain copy). A block copies 16 KB of one page, of K or V of one layer, four 16-byte loads of a thread in flight.
 constexpr uint32_t BOOK_ENTRIES = 160;
+// RECORDED: notes that the capture has run; MADE_UP: nothing if it has. (Captures are made up for one by one, so the latest number will do, and an
+// older graph that runs again does not take it back.)
+enum { BOOK_NOW = 0, BOOK_RECORDED = 1, BOOK_MADE_UP = 2 };
 struct BookArgs {
-    uint32_t n_copies, n_ops;
+    uint32_t n_copies, n_ops, mode, capture;
     PageCopy c[BOOK_ENTRIES];
     TableOp op[BOOK_ENTRIES];
 };
 static_assert(sizeof(BookArgs) <= 4000, "kernel parameters");
 
 __global__ void __launch_bounds__(256)
-books_kernel(const __grid_constant__ BookArgs list, char *__restrict__ mem, size_t layer_bytes, size_t page_bytes, uint32_t row_bytes, uint32_t *__restrict__ table) {
+books_kernel(const __grid_constant__ BookArgs list, char *__restrict__ mem, size_t layer_bytes, size_t page_bytes, uint32_t row_bytes, uint32_t *__restrict__ table,
+             uint32_t *__restrict__ ran) {
     ptx::pdl_wait();
     ptx::pdl_launch_dependents();
+    if (list.mode == BOOK_MADE_UP && __ldcg(ran) >= list.capture) return;
+    if (list.mode == BOOK_RECORDED && blockIdx.x + blockIdx.y + blockIdx.z + threadIdx.x == 0u) atomicMax(ran, list.capture);
     if (blockIdx.y >= list.n_copies) {
         if (blockIdx.x != 0u || blockIdx.z != 0u) return;
         const TableOp &o = list.op[blockIdx.y - list.n_copies];
@@ -47,9 +53,11 @@ books_kernel(const __grid_constant__ BookArgs list, char *__restrict__ mem, size
         if (at + 4096u * i < bytes) *reinterpret_cast<uint4 *>(dst + at + 4096u * i) = v[i];
 }
 
-static mkv_status launch_books(Pool *p, const std::vector<PageCopy> &cs, const std::vector<TableOp> &ops) {
+static mkv_status launch_books(Pool *p, const std::vector<PageCopy> &cs, const std::vector<TableOp> &ops, uint32_t mode) {
     for (size_t i = 0, j = 0; i < cs.size() || j < ops.size();) {
         BookArgs t;
+        t.mode = mode;
+        t.capture = p->captures;
         t.n_copies = (uint32_t)std::min<size_t>(BOOK_ENTRIES, cs.size() - i);
         t.n_ops = (uint32_t)std::min<size_t>(BOOK_ENTRIES, ops.size() - j);
         std::copy_n(cs.begin() + (long)i, t.n_copies, t.c);
@@ -60,47 +68,44 @@ static mkv_status launch_books(Pool *p, const std::vector<PageCopy> &cs, const s
         for (uint32_t k = 0; k < t.n_copies; k++) rows = std::max(rows, t.c[k].rows);
         const unsigned chunks = (unsigned)std::max<size_t>(1u, (rows * p->row_bytes + 16383u) / 16384u);
         PdlLaunch l(p->ctx, dim3(chunks, t.n_copies + t.n_ops, t.n_copies ? 2u * (unsigned)p->desc.n_layers : 1u), 256);
-        MKV_CUDA(cudaLaunchKernelEx(&l.cfg, books_kernel, t, p->mem, p->layer_bytes, p->page_bytes, (uint32_t)p->row_bytes, p->table));
+        MKV_CUDA(cudaLaunchKernelEx(&l.cfg, books_kernel, t, p->mem, p->layer_bytes, p->page_bytes, (uint32_t)p->row_bytes, p->table, p->table + p->table_entries()));
         p->ctx->launches++;
     }
     return MKV_OK;
 }
 
-static bool is_capturing(const void *pool) {
-    cudaStreamCaptureStatus status; // (of an invalid capture the launches fail)
-    return cudaStreamIsCapturing(static_cast<const Pool *>(pool)->ctx->stream, &status) == cudaSuccess && status == cudaStreamCaptureStatusActive;
-}
-
 // Launches what is in the lists and clears them; after an error they stay, for the next call. In a capture the launches are only recorded: the
 // pages are the sequences' own from now on, but the graph may never run, and rows written through a table that still has others would land on
-// other sequences' pages. So the first call outside a capture writes these sequences' tables from the books, whether the graph has run or not.
-// Another capture may not begin before: its graph would go without.
+// other sequences' pages. So the lists are kept, and the first call outside a capture launches them as work that is left out on the device where the
+// graph has run by then. Another capture may not begin before: its graph would either go without, or repeat what belongs to other sequences.
 static mkv_status follow_books(Pool *p) {
     std::vector<PageCopy> &cs = p->book.copies;
     std::vector<TableOp> &ops = p->book.ops;
-    if (cs.empty() && ops.empty() && p->recorded.empty()) return MKV_OK;
+    const bool any = !cs.empty() || !ops.empty();
+    if (!any && p->recorded.empty()) return MKV_OK;
     cudaStreamCaptureStatus status;
     unsigned long long id = 0;
     MKV_CUDA(cudaStreamGetCaptureInfo(p->ctx->stream, &status, &id));
     if (status == cudaStreamCaptureStatusNone) id = 0;
     if (!p->recorded.empty() && id == 0) {
-        for (uint32_t s : p->recorded) {
-            const std::vector<uint32_t> &v = p->book.seqs[s].pages; // (pageable memory: read before the call returns)
-            if (p->book.alive(s) && !v.empty())
-                MKV_CUDA(cudaMemcpyAsync(p->table + (size_t)s * p->book.max_pages, v.data(), v.size() * sizeof(uint32_t), cudaMemcpyHostToDevice, p->ctx->stream));
+        for (const BookWork &w : p->recorded) {
+            const mkv_status st = launch_books(p, w.copies, w.ops, BOOK_MADE_UP);
+            if (st != MKV_OK) return st;
         }
         p->recorded.clear();
-    } else if ((!p->recorded.empty() && id != p->capture) || (id != 0 && !cs.empty())) { // (copies: of a call whose launch failed)
-        set_error("an earlier call changed pages: one outside a capture has to come first");
+    } else if (!p->recorded.empty() && id != p->capture) {
+        set_error("an earlier capture changed pages: a call outside a capture has to come first");
         return MKV_ERR_STATE;
     }
     p->capture = id;
-    if (id != 0) p->recorded.reserve(p->recorded.size() + ops.size() + p->book.max_seqs); // (nothing may fail behind the launch)
-    const mkv_status st = launch_books(p, cs, ops);
+    if (!any) return MKV_OK;
+    if (id != 0) {
+        p->recorded.reserve(p->recorded.size() + 1u); // (nothing may fail behind the launch)
+        if (p->recorded.empty()) p->captures++;
+    }
+    const mkv_status st = launch_books(p, cs, ops, id != 0 ? BOOK_RECORDED : BOOK_NOW);
     if (st != MKV_OK) return st;
-    for (size_t i = 0; id != 0 && i < ops.size(); i++) // (a run of entries may go on into the next sequence's table)
-        for (uint32_t s = ops[i].dst / p->book.max_pages; s <= (ops[i].dst + (ops[i].n & ~TableOp::COPY) - 1u) / p->book.max_pages; s++)
-            if (p->recorded.empty() || p->recorded.back() != s) p->recorded.push_back(s);
+    if (id != 0) p->recorded.push_back({std::move(cs), std::move(ops)});
     cs.clear();
     ops.clear();
     return MKV_OK;
@@ -376,15 +381,13 @@ mkv_status mkv_pool_create(mkv_ctx *h, const mkv_pool_desc *d, mkv_pool **out) {
         }
         p->ctx = ctx;
         ctx->live_caches++;
-        p->book.capturing = is_capturing;
-        p->book.device = p;
         auto fail = [&](mkv_status s) {
             mkv_pool_destroy(reinterpret_cast<mkv_pool *>(p));
             return s;
         };
         DeviceScope dev(ctx);
         if (dev.status != MKV_OK) return fail(dev.status);
-        const size_t bytes = 2u * (size_t)d->n_layers * p->layer_bytes, tb = (size_t)d->max_seqs * p->book.max_pages * sizeof(uint32_t);
+        const size_t bytes = 2u * (size_t)d->n_layers * p->layer_bytes, tb = (p->table_entries() + 1u) * sizeof(uint32_t);
         if (cudaMalloc(reinterpret_cast<void **>(&p->mem), bytes) != cudaSuccess || cudaMalloc(reinterpret_cast<void **>(&p->table), tb) != cudaSuccess) {
             cudaGetLastError();
             set_error("out of device memory for a pool of %zu bytes", bytes + tb);

@@ -5,6 +5,12 @@
 
 namespace mkv {
 
+// What one change of the books asks of the device
+struct BookWork {
+    std::vector<PageCopy> copies;
+    std::vector<TableOp> ops;
+};
+
 struct Pool {
     Ctx *ctx = nullptr; // null: the bookkeeping alone
     mkv_pool_desc desc = {};
@@ -14,9 +20,12 @@ struct Pool {
     uint32_t *table = nullptr;                                      // [max_seqs][max_pages]
     float *scratch = nullptr;                                       // of the attention: parts of split work, folded outputs (pool_plan.cuh)
     std::vector<CUtensorMap> maps;                                  // [layer][K, V]
-    // Sequences whose tables were changed in the capture of that number, which may never run
-    std::vector<uint32_t> recorded;
+    // What was recorded into the capture of that number and may never run; captures that have recorded anything are counted, and a word behind the
+    // tables on the device has the latest that ran
+    std::vector<BookWork> recorded;
     unsigned long long capture = 0;
+    uint32_t captures = 0;
+    size_t table_entries() const { return (size_t)desc.max_seqs * book.max_pages; }
     explicit Pool(const mkv_pool_desc &d) : desc(d), book(d.n_pages, d.page_tokens, d.max_seqs, d.max_tokens, d.n_layers) {}
     char *layer_ptr(int layer, int kv) const { return mem + (2u * (size_t)layer + (size_t)kv) * layer_bytes; }
 };

@@ -997,82 +997,89 @@ def test_tables_that_change_right_in_front_of_the_attention(ctx, fmt):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
-def test_a_capture_that_takes_pages_and_never_runs(ctx, fmt):
-    """Pages are taken and shared in a capture, its graph dropped (or run), and the step made again without a capture: its rows lie on the sequences'
-    own pages, those of all other sequences are as they were. Copies in a capture, and a second capture before any other call, are refused; the first
-    one's later calls are not."""
+@pytest.mark.parametrize("runs", [0, 1])
+def test_pages_that_change_in_a_capture(ctx, fmt, runs):
+    """Pages are taken, shared, copied and moved in a capture whose graph then runs or is dropped; its writes are made again without a capture. Every
+    sequence has the rows of a twin pool that did the same without captures, by the books and by the device's tables. A second capture before any
+    other call is refused."""
     stream = torch.cuda.Stream()
     c2 = kv.KvContext(0, stream)
     dt = kv.KvFormat(fmt).torch_dtype
-    for runs in (0, 1, 2):
-        with torch.cuda.stream(stream):
-            pool, ids, g = scattered(c2, fmt, [64, 48, 40, 64], 16, 23, spare=30, longest=400)
-            a, b, c, e = ids
-            d = pool.fork(c)[0]  # (shares c's last page)
-            x, q = [randn(g, 6, 2, 256) for _ in range(2)], randn(g, 6, 16, 256, dtype=dt)
-            out = torch.empty_like(q)
-            before = {s: [t.clone() for t in rows_of(pool, s)] for s in (a, b, c, d, e)}
-            items = [(a, 0, 64, 2), (b, 0, 48, 1), (e, 0, 48, 3)]  # two new pages; one in place of a page that is shared by then
+    with torch.cuda.stream(stream):
+        (pool, ids, g), (twin, twin_ids, _) = (scattered(c2, fmt, [64, 48, 40, 64, 100], 16, 23, spare=30, longest=400) for _ in range(2))
+        assert ids == twin_ids
+        a, b, c, e, h = ids
+        x = [randn(g, 9, 2, 256) for _ in range(2)]
+        for p in (pool, twin):
+            assert p.fork(c) == [5]  # (shares c's last page)
 
-            def step():
-                pool.write(0, items, *x)
-                pool.attn(0, items, q, out)
+        def rows(p, s, pos, n, at):
+            p.write(0, [(s, 0, pos, n)], x[0][at:at + n], x[1][at:at + n])
 
-            def refused(*calls):
-                books = [pool.free_pages, *(pool.length(i) for i in range(12))]
-                for call in calls:
+        def change(p, n):
+            """In two parts, so that what the second one finds depends on the first."""
+            if n == 0:
+                p.write(0, [(a, 0, 64, 2), (b, 0, 48, 1), (5, 0, 40, 3)], x[0][:6], x[1][:6])  # two new pages, one copied
+                rows(p, c, 37, 2, 1)                       # over rows that were copied just now
+                kids = [*p.fork(a, 64), *p.fork(e), *p.fork(b, copy=True)]
+                p.truncate(e, 48)
+                rows(p, e, 48, 2, 3)                       # a new page in place of a shared one; the child keeps that
+                rows(p, kids[0], 64, 1, 5)
+            else:
+                p.free([h])
+                assert p.compact() > 0                     # pages that were copied to move on, others take their numbers
+                more = p.create()
+                rows(p, more, 0, 9, 0)
+
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            for n in range(2):
+                change(pool, n)
+        for n in range(2):
+            change(twin, n)
+        if runs:
+            graph.replay()
+        else:
+            second, q = torch.cuda.CUDAGraph(), torch.zeros(1, 16, 256, device="cuda", dtype=dt)
+            stream.synchronize()
+            with torch.cuda.graph(second, stream=stream):
+                free = pool.free_pages
+                for call in (lambda: rows(pool, a, 66, 1, 0), lambda: pool.fork(a), lambda: pool.attn(0, [(a, 0, 0, 1)], q, q + 1), lambda: pool.compact()):
                     with pytest.raises(_lib.MkvError) as err:
                         call()
                     assert err.value.status == _lib.ERR_STATE
-                assert [pool.free_pages, *(pool.length(i) for i in range(12))] == books
-
+                assert pool.free_pages == free and pool.length(a) == 66
             stream.synchronize()
-            graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(graph, stream=stream):
-                more, kid = pool.fork(a, 64)[0], pool.fork(e)[0]
-                pool.truncate(e, 48)
-                step()
-                refused(lambda: pool.write(0, [(d, 0, 40, 1)], x[0][:1], x[1][:1]), lambda: pool.fork(b, copy=True), lambda: pool.fork(b, n=2, copy=True))
-                pool.write(0, [(more, 0, 64, 1)], x[0][:1], x[1][:1])
-            for r in range(runs):
-                graph.replay()
-                replayed = out.clone()
-            if not runs:
-                second = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(second, stream=stream):
-                    out.zero_()
-                    refused(step, lambda: pool.fork(a), lambda: pool.attn(0, items, q, out))
-                stream.synchronize()
-                del graph, second
-            step()
-            if runs:
-                assert torch.equal(out, replayed)
-                del graph
-            want, mag, qk, top = attn64(pool, items, q)
-            assert ((out.double() - want).abs() <= attn_bound(fmt, want, mag, qk, top)).all()
-            pool.write(0, [(more, 0, 64, 1), (d, 0, 40, 1)], x[0][4:], x[1][4:])
-            for s, p, at, n, was in ((a, 64, 0, 2, a), (b, 48, 2, 1, b), (c, 40, 0, 0, c), (d, 40, 5, 1, d), (e, 48, 3, 3, e), (more, 64, 4, 1, a), (kid, 64, 0, 0, e)):
-                assert pool.length(s) == p + n
-                for got, old, new in zip(rows_of(pool, s), before[was], x):
-                    assert torch.equal(got[:p], old[:p]) and torch.equal(got[p:], new[at:at + n].to(dt))
-                # by the device's tables: attention to one key gives its value (f32: of two parts, 2^-23 of it, of sums of them, and 2^-33 of its tile's largest)
-                seen = torch.empty(p + n, 16, 256, device="cuda", dtype=dt)
-                pool.attn(0, [(s, i, i, 1) for i in range(p + n)], torch.zeros_like(seen), seen)
-                value = rows_of(pool, s)[1].double()
-                assert ((seen.view(p + n, 2, 8, 256)[:, :, 0].double() - value).abs() <= value.abs() * 2.0**-20 + 8 * 2.0**-33).all()
-            pool.free([more])
-            stream.synchronize()
-            third = torch.cuda.CUDAGraph()  # (all that was recorded is done: another capture may change pages)
-            with torch.cuda.graph(third, stream=stream):
-                refused(pool.compact)
-                pool.write(0, [(c, 0, 40, 9)], torch.cat(x)[:9], torch.cat(x)[:9])
-            third.replay()
-            for i, row in enumerate(torch.cat(x)[:9]):
-                assert torch.equal(rows_of(pool, c)[0][40 + i], row.to(dt))
-            assert torch.equal(rows_of(pool, d)[0][40], x[0][5].to(dt))
-            stream.synchronize()
-            del third
-            pool.free([a])
-            assert pool.compact() > 0
-            pool.close()
+            del graph, second
+        pool.compact()
+        for p in (pool, twin):  # the writes of the capture once more
+            p.write(0, [(a, 0, 64, 2), (b, 0, 48, 1), (5, 0, 40, 3)], x[0][:6], x[1][:6])
+            p.write(0, [(c, 0, 37, 2)], x[0][1:3], x[1][1:3])
+            rows(p, e, 48, 2, 3)
+            rows(p, 6, 64, 1, 5)
+            rows(p, 8, 48, 1, 2)  # (copied from b behind its write)
+            rows(p, h, 0, 9, 0)  # (the number of the one that was freed)
+        for s in range(9):
+            n = pool.length(s)
+            assert n == twin.length(s) and n > 0 and np.array_equal(pool.pages(s), twin.pages(s))
+            for got, want in zip(rows_of(pool, s), rows_of(twin, s)):
+                assert torch.equal(got, want), s
+            # by the device's tables: attention to one key gives its value (f32: of two parts, 2^-23 of it, of sums of them, and 2^-33 of its tile's largest)
+            seen, value = torch.empty(n, 16, 256, device="cuda", dtype=dt), rows_of(pool, s)[1].double()
+            pool.attn(0, [(s, i, i, 1) for i in range(n)], torch.zeros_like(seen), seen)
+            assert ((seen.view(n, 2, 8, 256)[:, :, 0].double() - value).abs() <= value.abs() * 2.0**-20 + 8 * 2.0**-33).all(), s
+        stream.synchronize()
+        third = torch.cuda.CUDAGraph()  # (all that was recorded is done: another capture may change pages)
+        with torch.cuda.graph(third, stream=stream):
+            rows(pool, c, 39, 9, 0)
+        third.replay()
+        third.replay()
+        assert torch.equal(rows_of(pool, c)[0][39:], x[0].to(dt)) and torch.equal(rows_of(pool, 5)[0], rows_of(twin, 5)[0])
+        stream.synchronize()
+        if runs:
+            del graph
+        del third
+        pool.close()
+        twin.close()
     c2.close()
