@@ -290,7 +290,11 @@ template <class F, class U> static mkv_status change(Pool *p, const F &body, con
     mkv_status st = follow_books(p); // (what an earlier call could not launch: entries of one launch do not depend on each other)
     if (st == MKV_OK) st = body();
     if (st != MKV_OK) return st;
-    st = follow_books(p);
+    try {
+        st = follow_books(p);
+    } catch (const std::bad_alloc &) {
+        st = no_memory();
+    }
     if (st != MKV_OK) undo();
     return st;
 }
